@@ -188,6 +188,143 @@ int ec_flat_search(const float *q, int nq, int topk, int64_t *ids, float *scores
 int ec_flat_search_noalloc(const float *d_x, int64_t n, int d, const float *d_q, int nq,
                            int topk, int64_t *d_ids, float *d_scores, void *stream);
 
+/* ---- operators on device buffers ---------------------------------------------
+ * Rotary positions, causal attention and a paged key / value cache over
+ * caller-owned DEVICE buffers, for hosts that keep a Llama-family model's
+ * activations in HBM (llama.lisp computes them per sequence on the host).
+ * Like ec_flat_search_noalloc they need no ec_init, allocate no device memory
+ * and enqueue on `stream` (a cudaStream_t, NULL = legacy default stream)
+ * without synchronising; a call can be captured into a CUDA graph and
+ * replayed.  The device is that of the buffers (all of one call on one
+ * device); the caller's current device is unchanged.  Shapes, strides and
+ * pointers are checked before anything is launched (EC_EINVAL); what lies in
+ * device memory (offsets, tables, lengths, positions) is checked by the
+ * kernels, which read and write nothing out of range.
+ *
+ * Packed rows: element i of head h of token t lies at p[t * token_stride +
+ * h * head_stride + i] (strides in elements).  Sequence s is the tokens
+ * [cu[s], cu[s + 1]) (int32, ascending from >= 0, empty sequences allowed);
+ * rows behind cu[nseq] are left as they are. */
+
+/* Waits inside the operators' kernels are bounded.  Waits for the current
+ * device, then returns EC_ETIMEOUT (and clears the mark) if one of them gave
+ * up since the last call, in which case that call's outputs are not valid;
+ * else EC_OK. */
+int ec_op_status(void);
+
+/* frequency scalings of ec_rope_table */
+#define EC_ROPE_NONE 0
+#define EC_ROPE_LINEAR 1 /* f / factor                                         */
+#define EC_ROPE_LLAMA3 2 /* by turns in `original` positions: below p0 as linear,
+                          * above p1 unchanged, in between blended             */
+#define EC_ROPE_YARN 3   /* by pair index, between the pairs that turn p0 (fast,
+                          * unchanged) and p1 (slow, as linear) times           */
+
+/* cos_t / sin_t[p * (rot_dim / 2) + i] = amplitude * cos / sin(p * f_i),
+ * f_i = theta^(-2 i / rot_dim) scaled as above; angles in double, rounded once
+ * (llama::init-rope, llama.lisp:124-135).  amplitude 0: 0.1 ln(factor) + 1
+ * for yarn, else 1. */
+int ec_rope_table(float *cos_t, float *sin_t, int64_t positions, int rot_dim, double theta,
+                  int scaling, double factor, double p0, double p1, double original,
+                  double amplitude, void *stream);
+
+/* Turn the first rot_dim elements of every head by the angle of the token's
+ * position (llama.lisp:137-146): pairs (i, i + rot_dim / 2), or (2i, 2i + 1)
+ * when `interleaved`; by the opposite angle when `inverse` (the gradient).
+ * The rest of the head passes through.  x and y: EC_F32 / EC_BF16 / EC_F16
+ * packed rows, y == x in place (else they must not overlap); one call takes
+ * query and key heads that follow each other in a row.  A token with a
+ * negative position is left out (its y unchanged); a position past the table
+ * gives NaN. */
+int ec_rope(const void *x, int64_t x_token, int64_t x_head, void *y, int64_t y_token,
+            int64_t y_head, int dtype, int64_t tokens, int heads, int head_dim, int rot_dim,
+            int interleaved, int inverse, const int32_t *pos, const float *cos_t,
+            const float *sin_t, int64_t positions, void *stream);
+
+/* Causal attention of packed prompts (llama::layer-forward, llama.lisp:255-271):
+ * out[t, h] = sum over keys j <= t of t's sequence of
+ * softmax_j(scale * q[t, h] . k[j, h / group]) * v[j, h / group], group =
+ * q_heads / kv_heads.  EC_BF16 or EC_F16, head_dim a multiple of 8 up to 128,
+ * all pointers 16-byte aligned and strides multiples of 8; scale 0 means
+ * 1 / sqrt(head_dim).  lse (NULL or [tokens][q_heads]) receives the natural
+ * log of the softmax's denominator.  Sums and statistics are fp32,
+ * probabilities are rounded to the inputs' type for the product with v.  A
+ * NaN or infinity in a sequence's keys or values reaches no other sequence. */
+int ec_attn_prompt(const void *q, int64_t q_token, int64_t q_head, const void *k,
+                   int64_t k_token, int64_t k_head, const void *v, int64_t v_token,
+                   int64_t v_head, void *out, int64_t o_token, int64_t o_head, float *lse,
+                   int dtype, int64_t tokens, int q_heads, int kv_heads, int head_dim,
+                   const int32_t *cu, int nseq, float scale, void *stream);
+
+/* status[0] of the page operations; anything but EC_KV_OK: nothing changed */
+#define EC_KV_OK 0
+#define EC_KV_FULL 1 /* status[1] pages needed, fewer are free                  */
+#define EC_KV_BAD 2  /* a slot out of range or named twice, a negative or too long
+                      * length, a fork into a slot in use or from one it fills  */
+
+/* Bytes of the scratch (`work`) of a cache's page operations. */
+int64_t ec_kv_work_size(int pages, int slots);
+
+/* Describe a paged cache in the caller's device memory: k and v
+ * [layers][pages][page_size][heads][head_dim] (EC_BF16 or EC_F16, page_size
+ * 16, 32, 64 or 128), tables[slots][table_width] (page of tokens
+ * [j * page_size, (j + 1) * page_size) of a slot), lens[slots], refs[pages]
+ * (slots that hold a page, 0 = free).  An empty cache has lens and refs 0.
+ * The handle keeps the description only; calls on one cache are ordered by
+ * the caller's streams. */
+int ec_kv_open(void *k, void *v, int dtype, int layers, int pages, int page_size, int heads,
+               int head_dim, int32_t *tables, int slots, int table_width, int32_t *lens,
+               int32_t *refs, void *work, int64_t work_bytes, int *handle);
+int ec_kv_close(int handle);
+
+/* Make room for add[i] more tokens in slots[i] (distinct), as a whole or not
+ * at all: lens grows by add, new pages are the lowest free ones, in the order
+ * of the list.  status: int32[2] on the device, {code, pages taken}. */
+int ec_kv_reserve(int handle, const int32_t *slots, const int32_t *add, int n, int32_t *status,
+                  void *stream);
+
+/* Make the empty slots dst[i] (distinct) copies of src[i]: whole pages are
+ * shared, a partly filled last page is copied, in every layer, to a page of
+ * its own (the lowest free ones, in the order of the list). */
+int ec_kv_fork(int handle, const int32_t *src, const int32_t *dst, int n, int32_t *status,
+               void *stream);
+
+/* Empty the slots (distinct; an empty one is no error): pages that no other
+ * slot holds become free (status[1] of them). */
+int ec_kv_free(int handle, const int32_t *slots, int n, int32_t *status, void *stream);
+
+/* Move the pages in use to the front: the r-th lowest page in use that lies
+ * at or above their number moves to the r-th lowest free one below it, in
+ * every layer, and the tables follow.  status[1]: pages moved. */
+int ec_kv_compact(int handle, int32_t *status, void *stream);
+
+/* Write the packed rows k and v into one layer: sequence s is the last
+ * cu[s + 1] - cu[s] tokens of slots[s] (NULL: slot s), whose room has been
+ * reserved.  A token whose page is not in the table is left out. */
+int ec_kv_write(int handle, int layer, const void *k, int64_t k_token, int64_t k_head,
+                const void *v, int64_t v_token, int64_t v_head, int64_t tokens,
+                const int32_t *cu, const int32_t *slots, int nseq, void *stream);
+
+/* Bytes of the scratch (`work`) of ec_attn_cached for up to `tokens` new
+ * tokens of `nseq` sequences.  It must be zero before its first use, belongs
+ * to one call at a time (calls in order on one stream may share it, two that
+ * may run at once may not) and is left ready for the next call. */
+int64_t ec_attn_cached_work_size(int handle, int64_t tokens, int q_heads, int nseq, int max_new);
+
+/* Attention of new tokens over their slot's pages, the tokens' own keys and
+ * values included: the queries of sequence s are the last cu[s + 1] - cu[s]
+ * positions of slots[s] (NULL: slot s; a slot may be named twice), each sees
+ * every position up to its own.  From one token per sequence to whole
+ * prompts; max_new: the longest sequence (a hint for the split of the work).
+ * A query that sees nothing (more tokens than the slot holds) gives 0 and an
+ * lse of -infinity.  A page that is not in [0, pages) reads as zeros; what a
+ * page holds behind its slot's length is not used.  Otherwise as
+ * ec_attn_prompt. */
+int ec_attn_cached(int handle, int layer, const void *q, int64_t q_token, int64_t q_head,
+                   void *out, int64_t o_token, int64_t o_head, float *lse, int64_t tokens,
+                   int q_heads, const int32_t *cu, const int32_t *slots, int nseq, int max_new,
+                   float scale, void *work, int64_t work_bytes, void *stream);
+
 /* ---- index files (no reference counterpart in C; the formats are the
  * reference's, with the dimension passed in instead of the constant 384 of
  * ann.lisp:19 / kb.lisp:23 / embed.lisp:83) --------------------------------- */

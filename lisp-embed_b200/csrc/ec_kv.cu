@@ -1,0 +1,552 @@
+// ec_kv.cu -- pages of a key / value cache: reserve, fork, free, compact and
+// write, on caller-owned device buffers.
+//
+// A slot's tokens lie in pages of page_size rows; tables[slot][j] is the page
+// of its tokens [j * page_size, (j + 1) * page_size), lens[slot] its length
+// and refs[page] the number of slots that hold a page (0: free).  Whole pages
+// can be shared; a partly filled last page belongs to one slot, so writing
+// behind lens[slot] never touches another slot's rows.
+//
+// Every request is planned by one CTA (its lists are short and pages are given
+// out in a fixed order, the lowest free page first, so the state after a call
+// does not depend on timing); what moves many bytes runs on a grid that reads
+// the plan.  A request either happens as a whole or changes nothing: status[0]
+// says which, and every index read from the device is checked before use.
+#include <algorithm>
+#include <map>
+#include <mutex>
+
+#include "ec_ops.h"
+
+namespace ec {
+
+namespace {
+std::mutex g_kv_mu;
+std::map<int, std::shared_ptr<const KvCache>> g_kv;
+int g_kv_next = 1;
+}  // namespace
+
+std::shared_ptr<const KvCache> kv_find(int handle) {
+  std::lock_guard<std::mutex> lk(g_kv_mu);
+  auto it = g_kv.find(handle);
+  if (it == g_kv.end()) {
+    set_error(EC_EINVAL, "unknown cache handle %d", handle);
+    return nullptr;
+  }
+  return it->second;
+}
+
+namespace {
+
+constexpr int kPlanThreads = 1024;
+
+// scratch: [0, pages) pages handed out or holes, [pages, 2 pages) new page of
+// a moved page, then one claim per slot, then the plan's scalars
+struct Plan {
+  int32_t *list, *map, *claim, *scalars;
+  __host__ __device__ explicit Plan(const KvCache& c)
+      : list(c.work), map(c.work + c.pages), claim(c.work + 2 * static_cast<int64_t>(c.pages)),
+        scalars(c.work + 2 * static_cast<int64_t>(c.pages) + c.slots) {}
+};
+constexpr int kPlanScalars = 16;
+
+__device__ __forceinline__ int pages_of(int len, int page) { return (len + page - 1) / page; }
+
+// exclusive prefix sum of v over the CTA (kPlanThreads threads), total in sum
+__device__ __forceinline__ int block_scan(int v, int& sum) {
+  __shared__ int part[32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int x = v;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, d);
+    if (lane >= d) x += y;
+  }
+  if (lane == 31) part[warp] = x;
+  __syncthreads();
+  if (warp == 0) {
+    int p = part[lane];
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, p, d);
+      if (lane >= d) p += y;
+    }
+    part[lane] = p;
+  }
+  __syncthreads();
+  sum = part[31];
+  const int before = (warp ? part[warp - 1] : 0) + x - v;
+  __syncthreads();
+  return before;
+}
+
+// The `need` lowest free pages into list; false if there are fewer.
+__device__ bool find_free(const KvCache& c, int32_t* list, int64_t need) {
+  int64_t got = 0;
+  for (int p0 = 0; p0 < c.pages && got < need; p0 += kPlanThreads * 4) {
+    int free_[4], n = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int p = p0 + threadIdx.x * 4 + i;
+      free_[i] = p < c.pages && c.refs[p] == 0;
+      n += free_[i];
+    }
+    int sum;
+    int64_t r = got + block_scan(n, sum);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (free_[i]) {
+        if (r < need) list[r] = p0 + threadIdx.x * 4 + i;
+        ++r;
+      }
+    got += sum;
+  }
+  __syncthreads();
+  return got >= need;
+}
+
+// Whether slots[0..n) are slots and no two are the same.  A slot is claimed by
+// the index that names it; whoever does not find its own claim is a second.
+__device__ bool claim_slots(const KvCache& c, int32_t* claim, const int32_t* slots, int n) {
+  bool bad = false;
+  for (int i = threadIdx.x; i < n; i += kPlanThreads) {
+    const int s = slots[i];
+    if (s < 0 || s >= c.slots) bad = true;
+    else claim[s] = i;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += kPlanThreads) {
+    const int s = slots[i];
+    if (s >= 0 && s < c.slots && claim[s] != i) bad = true;
+  }
+  return !__syncthreads_or(bad);
+}
+
+__device__ __forceinline__ bool bad_len(const KvCache& c, int len) {
+  return len < 0 || len > static_cast<int64_t>(c.width) * c.page_size;
+}
+
+// ---------------------------------------------------------------- reserve --
+__global__ void __launch_bounds__(kPlanThreads) kv_reserve_kernel(const KvCache c, const int32_t* slots,
+                                                                  const int32_t* add, int n, int32_t* status) {
+  const Plan plan(c);
+  bool ok = claim_slots(c, plan.claim, slots, n);
+  bool bad = false;
+  if (ok)
+    for (int i = threadIdx.x; i < n; i += kPlanThreads) {
+      const int len = c.lens[slots[i]];
+      bad |= bad_len(c, len) || add[i] < 0 ||
+             static_cast<int64_t>(len) + add[i] > static_cast<int64_t>(c.width) * c.page_size;
+    }
+  if (__syncthreads_or(bad || !ok)) {
+    if (threadIdx.x == 0) status[0] = EC_KV_BAD, status[1] = 0;
+    return;
+  }
+  int64_t need = 0;
+  for (int i0 = 0; i0 < n; i0 += kPlanThreads) {
+    const int i = i0 + threadIdx.x;
+    int v = 0;
+    if (i < n) {
+      const int len = c.lens[slots[i]];
+      v = pages_of(len + add[i], c.page_size) - pages_of(len, c.page_size);
+      v = min(v, c.pages + 1);  // at most 2^20 + 1: the sum over a CTA fits 32 bits
+    }
+    int sum;
+    block_scan(v, sum);
+    need += sum;
+  }
+  if (need > c.pages || !find_free(c, plan.list, need)) {
+    if (threadIdx.x == 0) status[0] = EC_KV_FULL, status[1] = static_cast<int32_t>(min(need, int64_t(INT32_MAX)));
+    return;
+  }
+  int at = 0;
+  for (int i0 = 0; i0 < n; i0 += kPlanThreads) {
+    const int i = i0 + threadIdx.x;
+    int have = 0, v = 0, s = 0, len = 0;
+    if (i < n) {
+      s = slots[i];
+      len = c.lens[s];
+      have = pages_of(len, c.page_size);
+      v = pages_of(len + add[i], c.page_size) - have;
+    }
+    int sum;
+    const int off = at + block_scan(v, sum);
+    for (int j = 0; j < v; ++j) {
+      const int p = plan.list[off + j];
+      c.tables[static_cast<int64_t>(s) * c.width + have + j] = p;
+      c.refs[p] = 1;
+    }
+    if (i < n) c.lens[s] = len + add[i];
+    at += sum;
+  }
+  if (threadIdx.x == 0) status[0] = EC_KV_OK, status[1] = static_cast<int32_t>(need);
+}
+
+// ------------------------------------------------------------------- fork --
+// the copy of every source's partly filled page goes to list[rank]
+__global__ void __launch_bounds__(kPlanThreads) kv_fork_plan_kernel(const KvCache c, const int32_t* src,
+                                                                    const int32_t* dst, int n, int32_t* status) {
+  const Plan plan(c);
+  const bool ok = claim_slots(c, plan.claim, dst, n);
+  bool bad = false;
+  if (ok)
+    for (int i = threadIdx.x; i < n; i += kPlanThreads) {
+      const int s = src[i];
+      if (s < 0 || s >= c.slots) {
+        bad = true;
+        continue;
+      }
+      // a source that is itself filled by this call
+      const int by = plan.claim[s];
+      bad |= by >= 0 && by < n && dst[by] == s;
+      bad |= bad_len(c, c.lens[s]) || c.lens[dst[i]] != 0;
+    }
+  if (__syncthreads_or(bad || !ok)) {
+    if (threadIdx.x == 0) status[0] = EC_KV_BAD, status[1] = 0, plan.scalars[0] = 0;
+    return;
+  }
+  int need = 0;
+  for (int i0 = 0; i0 < n; i0 += kPlanThreads) {
+    const int i = i0 + threadIdx.x;
+    int sum;
+    block_scan(i < n && c.lens[src[i]] % c.page_size ? 1 : 0, sum);
+    need += sum;
+  }
+  if (need > c.pages || !find_free(c, plan.list, need)) {
+    if (threadIdx.x == 0) status[0] = EC_KV_FULL, status[1] = need, plan.scalars[0] = 0;
+    return;
+  }
+  // the copy's page is the destination's last one; the rest follows
+  int at = 0;
+  for (int i0 = 0; i0 < n; i0 += kPlanThreads) {
+    const int i = i0 + threadIdx.x;
+    const int len = i < n ? c.lens[src[i]] : 0;
+    const int v = len % c.page_size ? 1 : 0;
+    int sum;
+    const int off = at + block_scan(v, sum);
+    if (v) {
+      const int p = plan.list[off];
+      c.tables[static_cast<int64_t>(dst[i]) * c.width + len / c.page_size] = p;
+      c.refs[p] = 1;
+    }
+    at += sum;
+  }
+  if (threadIdx.x == 0) status[0] = EC_KV_OK, status[1] = need, plan.scalars[0] = 1;
+}
+
+// rows [0, rows) of page `from` to page `to`, in layer l of the keys (kv 0)
+// or values (kv 1)
+__device__ __forceinline__ void copy_rows(const KvCache& c, int l, int kv, int from, int to, int rows) {
+  const int64_t row = static_cast<int64_t>(c.heads) * c.head_dim / 8;  // 16-byte pieces
+  uint4* base = static_cast<uint4*>(kv ? c.v : c.k) + static_cast<int64_t>(l) * c.pages * c.page_size * row;
+  const uint4* s = base + static_cast<int64_t>(from) * c.page_size * row;
+  uint4* d = base + static_cast<int64_t>(to) * c.page_size * row;
+  const int64_t n = rows * row;
+  for (int64_t i = threadIdx.x; i < n; i += blockDim.x) d[i] = s[i];
+}
+
+// block (i, piece): piece 0 also shares the whole pages of request i
+__global__ void kv_fork_copy_kernel(const KvCache c, const int32_t* src, const int32_t* dst) {
+  const Plan plan(c);
+  if (plan.scalars[0] == 0) return;
+  const int i = blockIdx.x, s = src[i], d = dst[i];
+  const int len = c.lens[s];
+  const int full = len / c.page_size, rest = len % c.page_size;
+  const int32_t* from = c.tables + static_cast<int64_t>(s) * c.width;
+  int32_t* to = c.tables + static_cast<int64_t>(d) * c.width;
+  if (blockIdx.y == 0) {
+    for (int j = threadIdx.x; j < full; j += blockDim.x) {
+      const int p = from[j];
+      to[j] = p;
+      if (p >= 0 && p < c.pages) atomicAdd(&c.refs[p], 1);
+    }
+    if (threadIdx.x == 0) c.lens[d] = len;
+  }
+  if (rest && from[full] >= 0 && from[full] < c.pages)
+    for (int l = blockIdx.y; l < 2 * c.layers; l += gridDim.y) copy_rows(c, l >> 1, l & 1, from[full], to[full], rest);
+}
+
+// ------------------------------------------------------------------- free --
+__global__ void __launch_bounds__(kPlanThreads) kv_free_plan_kernel(const KvCache c, const int32_t* slots, int n,
+                                                                    int32_t* status) {
+  const Plan plan(c);
+  const bool ok = claim_slots(c, plan.claim, slots, n);
+  bool bad = false;
+  if (ok)
+    for (int i = threadIdx.x; i < n; i += kPlanThreads) bad |= bad_len(c, c.lens[slots[i]]);
+  bad = __syncthreads_or(bad || !ok);
+  if (threadIdx.x == 0) status[0] = bad ? EC_KV_BAD : EC_KV_OK, status[1] = 0, plan.scalars[0] = !bad;
+}
+
+// block per slot: its pages let go, its row of the table cleared
+__global__ void kv_free_kernel(const KvCache c, const int32_t* slots, int32_t* status) {
+  const Plan plan(c);
+  if (plan.scalars[0] == 0) return;
+  const int s = slots[blockIdx.x];
+  const int np = pages_of(c.lens[s], c.page_size);
+  __syncthreads();
+  int32_t* row = c.tables + static_cast<int64_t>(s) * c.width;
+  int gone = 0;
+  for (int j = threadIdx.x; j < c.width; j += blockDim.x) {
+    const int p = row[j];
+    if (j < np && p >= 0 && p < c.pages) gone += atomicSub(&c.refs[p], 1) == 1;
+    row[j] = -1;
+  }
+  gone = __reduce_add_sync(0xffffffffu, gone);
+  if ((threadIdx.x & 31) == 0 && gone) atomicAdd(&status[1], gone);
+  if (threadIdx.x == 0) c.lens[s] = 0;
+}
+
+// ---------------------------------------------------------------- compact --
+// list[r]: the r-th hole below the number of live pages; map[p]: the hole
+// that live page p above it moves to; scalars: {live, moves}
+__global__ void __launch_bounds__(kPlanThreads) kv_compact_plan_kernel(const KvCache c, int32_t* status) {
+  const Plan plan(c);
+  int live = 0;
+  for (int p0 = 0; p0 < c.pages; p0 += kPlanThreads * 4) {
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int p = p0 + threadIdx.x * 4 + i;
+      n += p < c.pages && c.refs[p] > 0;
+    }
+    int sum;
+    block_scan(n, sum);
+    live += sum;
+  }
+  int holes = 0;
+  for (int p0 = 0; p0 < live; p0 += kPlanThreads) {
+    const int p = p0 + threadIdx.x;
+    const int v = p < live && c.refs[p] <= 0;
+    int sum;
+    const int r = holes + block_scan(v, sum);
+    if (v) plan.list[r] = p;
+    holes += sum;
+  }
+  __syncthreads();
+  int moves = 0;
+  for (int p0 = live; p0 < c.pages && moves < holes; p0 += kPlanThreads) {
+    const int p = p0 + threadIdx.x;
+    const int v = p < c.pages && c.refs[p] > 0;
+    int sum;
+    const int r = moves + block_scan(v, sum);
+    if (v) {
+      const int to = plan.list[r];
+      plan.map[p] = to;
+      plan.map[r] = p;  // r < holes <= live <= p: the page that fills hole r
+      c.refs[to] = c.refs[p];
+      c.refs[p] = 0;
+    }
+    moves += sum;
+  }
+  if (threadIdx.x == 0) {
+    plan.scalars[0] = live;
+    plan.scalars[1] = moves;
+    status[0] = EC_KV_OK;
+    status[1] = moves;
+  }
+}
+
+__global__ void kv_compact_copy_kernel(const KvCache c) {
+  const Plan plan(c);
+  const int live = plan.scalars[0], moves = plan.scalars[1];
+  if (moves == 0) return;
+  const int per = 2 * c.layers;
+  for (int64_t w = blockIdx.x; w < static_cast<int64_t>(moves) * per; w += gridDim.x) {
+    const int r = static_cast<int>(w / per), l = static_cast<int>(w % per);
+    copy_rows(c, l >> 1, l & 1, plan.map[r], plan.list[r], c.page_size);
+  }
+  // the tables of the slots in use
+  const int64_t n = static_cast<int64_t>(c.slots) * c.width;
+  for (int64_t e = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; e < n;
+       e += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+    const int p = c.tables[e];
+    if (p < live || p >= c.pages) continue;
+    if (static_cast<int>(e % c.width) < pages_of(c.lens[e / c.width], c.page_size)) c.tables[e] = plan.map[p];
+  }
+}
+
+// ------------------------------------------------------------------ write --
+struct WriteArgs {
+  const uint4 *k, *v;
+  int64_t kt, kh, vt, vh;  // strides in 16-byte pieces
+  int64_t tokens;
+  const int32_t *cu, *slots;
+  int nseq, layer;
+};
+
+// A block takes kWriteTokens tokens: their sequence and place in the cache,
+// then 16-byte pieces of their rows.
+constexpr int kWriteTokens = 8;
+__global__ void kv_write_kernel(const KvCache c, const WriteArgs a) {
+  __shared__ int64_t at[kWriteTokens];  // row in the pool, -1: none
+  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * kWriteTokens;
+  if (threadIdx.x < kWriteTokens) {
+    const int64_t t = t0 + threadIdx.x;
+    int64_t row = -1;
+    if (t < a.tokens) {
+      // last sequence that starts at or before t
+      int lo = 0, hi = a.nseq - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (a.cu[mid] <= t) lo = mid;
+        else hi = mid - 1;
+      }
+      const int64_t end = a.cu[lo + 1];
+      const int s = a.slots ? a.slots[lo] : lo;
+      if (a.cu[lo] <= t && t < end && s >= 0 && s < c.slots) {
+        const int64_t p = c.lens[s] - (end - t);
+        if (p >= 0 && p < static_cast<int64_t>(c.width) * c.page_size) {
+          const int page = c.tables[static_cast<int64_t>(s) * c.width + p / c.page_size];
+          if (page >= 0 && page < c.pages) row = static_cast<int64_t>(page) * c.page_size + p % c.page_size;
+        }
+      }
+    }
+    at[threadIdx.x] = row;
+  }
+  __syncthreads();
+  const int piece = c.head_dim / 8, row = c.heads * piece;
+  const int64_t pool = static_cast<int64_t>(a.layer) * c.pages * c.page_size * row;
+  uint4 *dk = static_cast<uint4*>(c.k) + pool, *dv = static_cast<uint4*>(c.v) + pool;
+  for (int e = threadIdx.x; e < kWriteTokens * row; e += blockDim.x) {
+    const int i = e / row, r = e % row, h = r / piece, x = r % piece;
+    if (at[i] < 0) continue;
+    dk[at[i] * row + r] = a.k[(t0 + i) * a.kt + h * a.kh + x];
+    dv[at[i] * row + r] = a.v[(t0 + i) * a.vt + h * a.vh + x];
+  }
+}
+
+int check_lists(const void* a, const void* b, int n, const void* status) {
+  if (n < 0) return set_error(EC_EINVAL, "negative count");
+  if (!status || (n > 0 && (!a || !b))) return set_error(EC_EINVAL, "a list or the status is NULL");
+  if (!op_aligned(a, 4) || !op_aligned(b, 4) || !op_aligned(status, 4))
+    return set_error(EC_EINVAL, "lists and status must be 4-byte aligned");
+  return EC_OK;
+}
+
+}  // namespace
+}  // namespace ec
+
+using namespace ec;
+
+extern "C" int64_t ec_kv_work_size(int pages, int slots) {
+  clear_error();
+  if (pages < 1 || slots < 1) return set_error(EC_EINVAL, "pages and slots must be positive");
+  return 4 * (2 * static_cast<int64_t>(pages) + slots + kPlanScalars);
+}
+
+extern "C" int ec_kv_open(void* k, void* v, int dtype, int layers, int pages, int page_size, int heads, int head_dim,
+                          int32_t* tables, int slots, int table_width, int32_t* lens, int32_t* refs, void* work,
+                          int64_t work_bytes, int* handle) {
+  clear_error();
+  if (!k || !v || !tables || !lens || !refs || !work || !handle) return set_error(EC_EINVAL, "a cache buffer is NULL");
+  if (dtype != EC_BF16 && dtype != EC_F16) return set_error(EC_EINVAL, "a cache holds bf16 or f16, not dtype %d", dtype);
+  if (layers < 1 || layers > 65536 || pages < 1 || pages > (1 << 20) || slots < 1 || slots > (1 << 24) ||
+      table_width < 1 || table_width > (1 << 24) || heads < 1 || heads > 1024)
+    return set_error(EC_EINVAL, "bad cache shape: %d layers of %d pages, %d heads, %d slots of %d pages", layers, pages,
+                     heads, slots, table_width);
+  if (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128)
+    return set_error(EC_EINVAL, "page_size %d (supported: 16, 32, 64, 128)", page_size);
+  if (head_dim < 8 || head_dim > 128 || head_dim % 8)
+    return set_error(EC_EINVAL, "head_dim %d (supported: multiples of 8 up to 128)", head_dim);
+  if (static_cast<int64_t>(table_width) * page_size > INT32_MAX)
+    return set_error(EC_EINVAL, "a table row of %d pages passes 2^31 tokens", table_width);
+  if (!op_aligned(k, 16) || !op_aligned(v, 16) || !op_aligned(work, 16))
+    return set_error(EC_EINVAL, "pages and work must be 16-byte aligned");
+  if (!op_aligned(tables, 4) || !op_aligned(lens, 4) || !op_aligned(refs, 4))
+    return set_error(EC_EINVAL, "tables, lens and refs must be 4-byte aligned");
+  if (work_bytes < ec_kv_work_size(pages, slots))
+    return set_error(EC_EINVAL, "work holds %lld bytes, the cache needs %lld", static_cast<long long>(work_bytes),
+                     static_cast<long long>(ec_kv_work_size(pages, slots)));
+  auto c = std::make_shared<KvCache>(KvCache{k, v, dtype, layers, pages, page_size, heads, head_dim, tables, slots,
+                                             table_width, lens, refs, static_cast<int32_t*>(work)});
+  std::lock_guard<std::mutex> lk(g_kv_mu);
+  *handle = g_kv_next++;
+  g_kv[*handle] = std::move(c);
+  return EC_OK;
+}
+
+extern "C" int ec_kv_close(int handle) {
+  clear_error();
+  if (!kv_find(handle)) return EC_EINVAL;
+  std::lock_guard<std::mutex> lk(g_kv_mu);
+  g_kv.erase(handle);
+  return EC_OK;
+}
+
+extern "C" int ec_kv_reserve(int handle, const int32_t* slots, const int32_t* add, int n, int32_t* status,
+                             void* stream) {
+  clear_error();
+  auto c = kv_find(handle);
+  if (!c) return EC_EINVAL;
+  if (int rc = check_lists(slots, add, n, status)) return rc;
+  OpDevice dev;
+  if (int rc = dev.enter({c->refs, slots, add, status})) return rc;
+  kv_reserve_kernel<<<1, kPlanThreads, 0, static_cast<cudaStream_t>(stream)>>>(*c, slots, add, n, status);
+  return check_cuda(cudaGetLastError(), "kv reserve");
+}
+
+extern "C" int ec_kv_fork(int handle, const int32_t* src, const int32_t* dst, int n, int32_t* status, void* stream) {
+  clear_error();
+  auto c = kv_find(handle);
+  if (!c) return EC_EINVAL;
+  if (int rc = check_lists(src, dst, n, status)) return rc;
+  OpDevice dev;
+  if (int rc = dev.enter({c->refs, src, dst, status})) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  kv_fork_plan_kernel<<<1, kPlanThreads, 0, st>>>(*c, src, dst, n, status);
+  if (int rc = check_cuda(cudaGetLastError(), "kv fork")) return rc;
+  if (n == 0) return EC_OK;
+  kv_fork_copy_kernel<<<dim3(n, std::min(2 * c->layers, 65535)), 256, 0, st>>>(*c, src, dst);
+  return check_cuda(cudaGetLastError(), "kv fork copy");
+}
+
+extern "C" int ec_kv_free(int handle, const int32_t* slots, int n, int32_t* status, void* stream) {
+  clear_error();
+  auto c = kv_find(handle);
+  if (!c) return EC_EINVAL;
+  if (int rc = check_lists(slots, slots, n, status)) return rc;
+  OpDevice dev;
+  if (int rc = dev.enter({c->refs, slots, status})) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  kv_free_plan_kernel<<<1, kPlanThreads, 0, st>>>(*c, slots, n, status);
+  if (int rc = check_cuda(cudaGetLastError(), "kv free")) return rc;
+  if (n == 0) return EC_OK;
+  kv_free_kernel<<<n, 128, 0, st>>>(*c, slots, status);
+  return check_cuda(cudaGetLastError(), "kv free");
+}
+
+extern "C" int ec_kv_compact(int handle, int32_t* status, void* stream) {
+  clear_error();
+  auto c = kv_find(handle);
+  if (!c) return EC_EINVAL;
+  if (int rc = check_lists(status, status, 0, status)) return rc;
+  OpDevice dev;
+  if (int rc = dev.enter({c->refs, status})) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  kv_compact_plan_kernel<<<1, kPlanThreads, 0, st>>>(*c, status);
+  if (int rc = check_cuda(cudaGetLastError(), "kv compact")) return rc;
+  kv_compact_copy_kernel<<<dev.num_sms() * 8, 256, 0, st>>>(*c);
+  return check_cuda(cudaGetLastError(), "kv compact copy");
+}
+
+extern "C" int ec_kv_write(int handle, int layer, const void* k, int64_t k_token, int64_t k_head, const void* v,
+                           int64_t v_token, int64_t v_head, int64_t tokens, const int32_t* cu, const int32_t* slots,
+                           int nseq, void* stream) {
+  clear_error();
+  auto c = kv_find(handle);
+  if (!c) return EC_EINVAL;
+  if (layer < 0 || layer >= c->layers) return set_error(EC_EINVAL, "layer %d of %d", layer, c->layers);
+  if (tokens < 0 || tokens > INT32_MAX || nseq < 0) return set_error(EC_EINVAL, "bad token or sequence count");
+  if (int rc = op_check_rows("k", {k, k_token, k_head}, tokens, c->heads, c->head_dim)) return rc;
+  if (int rc = op_check_rows("v", {v, v_token, v_head}, tokens, c->heads, c->head_dim)) return rc;
+  if (tokens == 0 || nseq == 0) return EC_OK;
+  if (!cu || !op_aligned(cu, 4) || !op_aligned(slots, 4)) return set_error(EC_EINVAL, "cu is NULL or a list misaligned");
+  OpDevice dev;
+  if (int rc = dev.enter({c->refs, k, v, cu, slots})) return rc;
+  const WriteArgs a{static_cast<const uint4*>(k), static_cast<const uint4*>(v), k_token / 8, k_head / 8, v_token / 8,
+                    v_head / 8, tokens, cu, slots, nseq, layer};
+  const int64_t grid = (tokens + kWriteTokens - 1) / kWriteTokens;
+  kv_write_kernel<<<static_cast<unsigned>(grid), 256, 0, static_cast<cudaStream_t>(stream)>>>(*c, a);
+  return check_cuda(cudaGetLastError(), "kv write");
+}

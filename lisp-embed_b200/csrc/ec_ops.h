@@ -1,0 +1,85 @@
+// ec_ops.h -- what the operators over caller-owned device buffers (rotary
+// positions, prompt and cached attention, the paged cache) share: argument
+// checks, the device of a call, and the description behind a cache handle.
+//
+// Like ec_flat_search_noalloc they need no ec_init, allocate no device memory
+// and only enqueue work on the caller's stream.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <initializer_list>
+#include <memory>
+
+#include "ec_state.h"
+
+namespace ec {
+
+// Makes the device that holds `p` current for one call and puts the caller's
+// device back afterwards: a host that drives several GPUs passes buffers of a
+// device other than the current one.
+class OpDevice {
+ public:
+  // EC_OK, or an error when one of the non-null pointers is not device memory
+  // or lies on another device than the first
+  int enter(std::initializer_list<const void*> ptrs);
+  ~OpDevice();
+  int num_sms() const { return sms_; }
+  int ordinal() const { return dev_; }
+
+ private:
+  int prev_ = -1, dev_ = -1, sms_ = 0;
+};
+
+// element size of EC_F32 / EC_BF16 / EC_F16, 0 for another code
+inline int op_elem_size(int dtype) {
+  return dtype == EC_F32 ? 4 : dtype == EC_BF16 || dtype == EC_F16 ? 2 : 0;
+}
+inline bool op_aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+// Heads of a packed row: element (token, head, i) lies at
+// p[token * token_stride + head * head_stride + i].
+struct OpRows {
+  const void* p;
+  int64_t token, head;
+};
+// checks pointer, 16-byte base and strides (in elements of 2 bytes), and that
+// heads do not overlap
+int op_check_rows(const char* name, const OpRows& r, int64_t tokens, int heads, int head_dim);
+
+// a cache as ec_kv_open describes it; the memory is the caller's
+struct KvCache {
+  void *k, *v;         // [layers][pages][page_size][heads][head_dim]
+  int dtype, layers, pages, page_size, heads, head_dim;
+  int32_t* tables;     // [slots][width]
+  int slots, width;
+  int32_t* lens;       // [slots]
+  int32_t* refs;       // [pages]
+  int32_t* work;       // scratch of the page operations
+};
+// the cache behind a handle (held until the pointer goes away), or nullptr
+// with the error set
+std::shared_ptr<const KvCache> kv_find(int handle);
+
+// ---- attention over packed queries (ec_attn_ops.cu) --------------------------
+struct AttnOp {
+  int dtype, head_dim, q_heads, kv_heads;
+  OpRows q, k, v, out;  // k and v unused with a cache
+  float* lse;           // [tokens][q_heads] or nullptr
+  int64_t tokens;
+  const int32_t* cu;    // [nseq + 1]
+  int nseq;
+  float scale;
+  // keys in a cache (nullptr: the packed rows k and v)
+  const KvCache* cache;
+  int layer;
+  const int32_t* slots;  // [nseq] or nullptr (sequence s is slot s)
+  int max_new;
+  void* work;
+  size_t work_bytes;
+};
+int run_attention(const AttnOp& op, int num_sms, cudaStream_t st);
+size_t attention_work_bytes(const KvCache& c, int64_t tokens, int q_heads, int nseq, int max_new);
+
+}  // namespace ec

@@ -1,0 +1,254 @@
+// ec_rope.cu -- rotary positions on caller-owned device buffers.
+//
+// Pair i of a head is turned by the angle pos * f_i:
+//   y0 = x0 c - x1 s,  y1 = x1 c + x0 s,
+// with (x0, x1) = (x[i], x[i + rot/2]) (halves) or (x[2i], x[2i + 1])
+// (interleaved) of the first `rot` elements; the rest of the head passes
+// through.  The turn is orthogonal, so its gradient is the turn by -angle.
+#include <cuda_fp16.h>
+
+#include <cmath>
+
+#include "ec_ops.h"
+
+namespace ec {
+namespace {
+
+// ------------------------------------------------------------------ table --
+struct TableArgs {
+  float *cos_t, *sin_t;
+  int64_t positions;
+  int half;
+  double theta;
+  int scaling;
+  double factor, p0, p1, original, amplitude;
+};
+
+// frequency of pair i (llama.lisp:124-135 without scaling)
+__device__ double rope_freq(const TableArgs& a, int i) {
+  const double f = pow(a.theta, -static_cast<double>(i) / a.half);
+  const double two_pi = 6.283185307179586476925;
+  if (a.scaling == EC_ROPE_LINEAR) return f / a.factor;
+  if (a.scaling == EC_ROPE_LLAMA3) {
+    // turns within the original context: below p0 scaled, above p1 kept
+    const double keep = fmin(fmax((a.original * f / two_pi - a.p0) / (a.p1 - a.p0), 0.0), 1.0);
+    return (1.0 - keep) * f / a.factor + keep * f;
+  }
+  if (a.scaling == EC_ROPE_YARN) {
+    // pair index at which p0 (fast) / p1 (slow) turns fit the original context
+    const double rot = 2.0 * a.half, lt = 2.0 * log(a.theta);
+    const double low = fmax(floor(rot * log(a.original / (a.p0 * two_pi)) / lt), 0.0);
+    const double high = fmin(ceil(rot * log(a.original / (a.p1 * two_pi)) / lt), rot - 1.0);
+    const double ramp = fmin(fmax((i - low) / fmax(high - low, 1e-3), 0.0), 1.0);
+    return f / a.factor * ramp + f * (1.0 - ramp);
+  }
+  return f;
+}
+
+__global__ void rope_table_kernel(const TableArgs a) {
+  const int64_t n = a.positions * a.half;
+  for (int64_t e = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; e < n;
+       e += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+    double s, c;
+    sincos(static_cast<double>(e / a.half) * rope_freq(a, static_cast<int>(e % a.half)), &s, &c);
+    a.cos_t[e] = static_cast<float>(c * a.amplitude);
+    a.sin_t[e] = static_cast<float>(s * a.amplitude);
+  }
+}
+
+// ------------------------------------------------------------------- turn --
+struct RopeArgs {
+  const void* x;
+  void* y;
+  int64_t xt, xh, yt, yh;  // strides in elements
+  int64_t tokens, positions;
+  int heads, half, tail;   // tail: elements past the turned part (0 in place)
+  int inverse;
+  const int32_t* pos;
+  const float *cos_t, *sin_t;
+};
+
+__device__ __forceinline__ float to_f(float v) { return v; }
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+template <typename T>
+__device__ __forceinline__ T from_f(float v);
+template <>
+__device__ __forceinline__ float from_f<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
+
+template <typename T, int V>
+struct alignas(sizeof(T) * V) Vec {
+  T e[V];
+};
+
+// One thread: V pairs (or V elements of the tail) of one token's head.  The
+// angle's cos and sin are read once for `V` pairs and kept for the heads.
+template <typename T, int V, bool INTER>
+__global__ void rope_kernel(const RopeArgs a, int per_head, int groups, int heads_per) {
+  using VT = Vec<T, V>;
+  using VF = Vec<float, V>;
+  const int64_t n = a.tokens * groups * per_head;
+  for (int64_t e = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; e < n;
+       e += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+    const int c = static_cast<int>(e % per_head);
+    const int64_t tg = e / per_head;
+    const int g = static_cast<int>(tg % groups);
+    const int64_t t = tg / groups;
+    const int32_t p = a.pos[t];
+    if (p < 0) continue;  // a row without a position stays as it is
+    const int h0 = g * heads_per, h1 = min(h0 + heads_per, a.heads);
+    const T* x = static_cast<const T*>(a.x) + t * a.xt;
+    T* y = static_cast<T*>(a.y) + t * a.yt;
+    if (c * V >= a.half) {
+      const int i = 2 * a.half + c * V - a.half;
+      for (int h = h0; h < h1; ++h)
+        *reinterpret_cast<VT*>(y + h * a.yh + i) = *reinterpret_cast<const VT*>(x + h * a.xh + i);
+      continue;
+    }
+    VF co, si;
+    if (p < a.positions) {
+      co = *reinterpret_cast<const VF*>(a.cos_t + static_cast<int64_t>(p) * a.half + c * V);
+      si = *reinterpret_cast<const VF*>(a.sin_t + static_cast<int64_t>(p) * a.half + c * V);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) co.e[i] = si.e[i] = NAN;
+    }
+    if (a.inverse) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) si.e[i] = -si.e[i];
+    }
+    for (int h = h0; h < h1; ++h) {
+      const T* xp = x + h * a.xh + (INTER ? 2 * c * V : c * V);
+      T* yp = y + h * a.yh + (INTER ? 2 * c * V : c * V);
+      const int second = INTER ? V : a.half;
+      VT u = *reinterpret_cast<const VT*>(xp), w = *reinterpret_cast<const VT*>(xp + second), ru, rw;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        if (INTER) {
+          // V consecutive pairs: elements 2i, 2i + 1 of the two vectors
+          if constexpr (V > 1) {
+            const VT& s = 2 * i < V ? u : w;
+            VT& r = 2 * i < V ? ru : rw;
+            const int k = (2 * i) % V;
+            const float x0 = to_f(s.e[k]), x1 = to_f(s.e[k + 1]);
+            r.e[k] = from_f<T>(x0 * co.e[i] - x1 * si.e[i]);
+            r.e[k + 1] = from_f<T>(x1 * co.e[i] + x0 * si.e[i]);
+            continue;
+          }
+        }
+        const float x0 = to_f(u.e[i]), x1 = to_f(w.e[i]);
+        ru.e[i] = from_f<T>(x0 * co.e[i] - x1 * si.e[i]);
+        rw.e[i] = from_f<T>(x1 * co.e[i] + x0 * si.e[i]);
+      }
+      *reinterpret_cast<VT*>(yp) = ru;
+      *reinterpret_cast<VT*>(yp + second) = rw;
+    }
+  }
+}
+
+template <typename T, int V>
+cudaError_t launch_rope(const RopeArgs& a, int interleaved, int num_sms, cudaStream_t st) {
+  const int per_head = (a.half + a.tail) / V;
+  // a head per thread while that does not fill the GPU, then several, so
+  // that the angles are read once for them
+  int heads_per = 1;
+  while (heads_per < 8 && a.tokens * per_head * ((a.heads + 2 * heads_per - 1) / (2 * heads_per)) >=
+                              static_cast<int64_t>(num_sms) * 2048)
+    heads_per *= 2;
+  const int groups = (a.heads + heads_per - 1) / heads_per;
+  const int64_t n = a.tokens * groups * per_head;
+  const int64_t want = (n + 255) / 256, most = static_cast<int64_t>(num_sms) * 64;
+  const int grid = static_cast<int>(want < most ? want : most);
+  if (interleaved)
+    rope_kernel<T, V, true><<<grid, 256, 0, st>>>(a, per_head, groups, heads_per);
+  else
+    rope_kernel<T, V, false><<<grid, 256, 0, st>>>(a, per_head, groups, heads_per);
+  return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t launch_rope_v(const RopeArgs& a, int interleaved, int num_sms, cudaStream_t st) {
+  // widest vector (16 bytes at most) that divides the turned half, the tail
+  // and every stride, and to which the buffers are aligned
+  auto fits = [&](int v) {
+    const size_t b = sizeof(T) * v;
+    return a.half % v == 0 && a.tail % v == 0 && a.xt % v == 0 && a.xh % v == 0 && a.yt % v == 0 && a.yh % v == 0 &&
+           op_aligned(a.x, b) && op_aligned(a.y, b) && op_aligned(a.cos_t, v > 4 ? 16 : 4 * v) &&
+           op_aligned(a.sin_t, v > 4 ? 16 : 4 * v);
+  };
+  if constexpr (sizeof(T) == 2) {
+    if (fits(8)) return launch_rope<T, 8>(a, interleaved, num_sms, st);
+  }
+  if (fits(4)) return launch_rope<T, 4>(a, interleaved, num_sms, st);
+  if (fits(2)) return launch_rope<T, 2>(a, interleaved, num_sms, st);
+  return launch_rope<T, 1>(a, interleaved, num_sms, st);
+}
+
+}  // namespace
+}  // namespace ec
+
+using namespace ec;
+
+extern "C" int ec_rope_table(float* cos_t, float* sin_t, int64_t positions, int rot_dim, double theta, int scaling,
+                             double factor, double p0, double p1, double original, double amplitude, void* stream) {
+  clear_error();
+  if (positions < 0 || positions >= (int64_t(1) << 31)) return set_error(EC_EINVAL, "bad number of positions");
+  if (rot_dim < 2 || rot_dim % 2 || rot_dim > 1024) return set_error(EC_EINVAL, "rot_dim %d: even, 2 .. 1024", rot_dim);
+  if (!(theta > 1.0) || !std::isfinite(theta)) return set_error(EC_EINVAL, "theta must be a finite number above 1");
+  if (scaling < EC_ROPE_NONE || scaling > EC_ROPE_YARN) return set_error(EC_EINVAL, "unknown rope scaling %d", scaling);
+  if (scaling != EC_ROPE_NONE && (!(factor >= 1.0) || !std::isfinite(factor)))
+    return set_error(EC_EINVAL, "rope scaling factor must be a finite number of 1 or more");
+  if (scaling == EC_ROPE_LLAMA3 && !(p0 > 0.0 && p1 > p0 && std::isfinite(p1) && original > 0.0 && std::isfinite(original)))
+    return set_error(EC_EINVAL, "llama3 scaling needs 0 < low factor < high factor and an original length");
+  if (scaling == EC_ROPE_YARN && !(p1 > 0.0 && p0 >= p1 && std::isfinite(p0) && original > 0.0 && std::isfinite(original)))
+    return set_error(EC_EINVAL, "yarn scaling needs beta_fast >= beta_slow > 0 and an original length");
+  if (!std::isfinite(amplitude) || amplitude < 0.0) return set_error(EC_EINVAL, "amplitude must be finite and >= 0");
+  if (positions == 0) return EC_OK;
+  if (!cos_t || !sin_t) return set_error(EC_EINVAL, "cos or sin table is NULL");
+  if (!op_aligned(cos_t, 4) || !op_aligned(sin_t, 4)) return set_error(EC_EINVAL, "tables must be 4-byte aligned");
+  OpDevice dev;
+  if (int rc = dev.enter({cos_t, sin_t})) return rc;
+  if (amplitude == 0.0) amplitude = scaling == EC_ROPE_YARN ? 0.1 * std::log(factor) + 1.0 : 1.0;
+  const TableArgs a{cos_t, sin_t, positions, rot_dim / 2, theta, scaling, factor, p0, p1, original, amplitude};
+  const int64_t want = (positions * a.half + 255) / 256, most = static_cast<int64_t>(dev.num_sms()) * 32;
+  rope_table_kernel<<<static_cast<int>(want < most ? want : most), 256, 0, static_cast<cudaStream_t>(stream)>>>(a);
+  return check_cuda(cudaGetLastError(), "rope table");
+}
+
+extern "C" int ec_rope(const void* x, int64_t x_token, int64_t x_head, void* y, int64_t y_token, int64_t y_head,
+                       int dtype, int64_t tokens, int heads, int head_dim, int rot_dim, int interleaved, int inverse,
+                       const int32_t* pos, const float* cos_t, const float* sin_t, int64_t positions, void* stream) {
+  clear_error();
+  const int es = op_elem_size(dtype);
+  if (!es) return set_error(EC_EINVAL, "unsupported dtype %d", dtype);
+  if (tokens < 0 || heads < 1 || heads > 65536 || head_dim < 2 || head_dim > 4096)
+    return set_error(EC_EINVAL, "bad rope shape: %lld tokens, %d heads of %d", static_cast<long long>(tokens), heads, head_dim);
+  if (rot_dim < 2 || rot_dim % 2 || rot_dim > head_dim)
+    return set_error(EC_EINVAL, "rot_dim %d: even, 2 .. head_dim %d", rot_dim, head_dim);
+  if (positions < 1 || positions >= (int64_t(1) << 31)) return set_error(EC_EINVAL, "bad number of positions");
+  if (tokens >= (int64_t(1) << 38)) return set_error(EC_EINVAL, "too many tokens");
+  if (tokens == 0) return EC_OK;
+  if (!x || !y || !pos || !cos_t || !sin_t) return set_error(EC_EINVAL, "a rope buffer is NULL");
+  if (!op_aligned(x, es) || !op_aligned(y, es) || !op_aligned(pos, 4) || !op_aligned(cos_t, 4) || !op_aligned(sin_t, 4))
+    return set_error(EC_EINVAL, "a rope buffer is not aligned to its element");
+  if ((heads > 1 && (x_head < head_dim || y_head < head_dim)) ||
+      (tokens > 1 && (x_token < head_dim || y_token < head_dim)) || x_head < 0 || y_head < 0 || x_token < 0 || y_token < 0)
+    return set_error(EC_EINVAL, "rope strides overlap heads of %d", head_dim);
+  const bool in_place = x == y;
+  if (in_place && (x_token != y_token || x_head != y_head))
+    return set_error(EC_EINVAL, "in place the strides of x and y must be equal");
+  OpDevice dev;
+  if (int rc = dev.enter({x, y, pos, cos_t, sin_t})) return rc;
+  RopeArgs a{x, y, x_token, x_head, y_token, y_head, tokens, positions, heads, rot_dim / 2,
+             in_place ? 0 : head_dim - rot_dim, inverse ? 1 : 0, pos, cos_t, sin_t};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int il = interleaved ? 1 : 0;
+  const cudaError_t e = dtype == EC_F32    ? launch_rope_v<float>(a, il, dev.num_sms(), st)
+                        : dtype == EC_BF16 ? launch_rope_v<__nv_bfloat16>(a, il, dev.num_sms(), st)
+                                           : launch_rope_v<__half>(a, il, dev.num_sms(), st);
+  return check_cuda(e, "rope");
+}

@@ -63,6 +63,27 @@ _SIGS = {
     "ec_ivf_search": (C.c_int, [FP, C.c_int, C.c_int, C.c_int, I64P, FP]),
     "ec_flat_search": (C.c_int, [FP, C.c_int, C.c_int, I64P, FP]),
     "ec_flat_search_noalloc": (C.c_int, [P, C.c_int64, C.c_int, P, C.c_int, C.c_int, P, P, P]),
+    "ec_op_status": (C.c_int, []),
+    "ec_rope_table": (C.c_int, [P, P, C.c_int64, C.c_int, C.c_double, C.c_int, C.c_double, C.c_double,
+                                C.c_double, C.c_double, C.c_double, P]),
+    "ec_rope": (C.c_int, [P, C.c_int64, C.c_int64, P, C.c_int64, C.c_int64, C.c_int, C.c_int64, C.c_int,
+                          C.c_int, C.c_int, C.c_int, C.c_int, P, P, P, C.c_int64, P]),
+    "ec_attn_prompt": (C.c_int, [P, C.c_int64, C.c_int64, P, C.c_int64, C.c_int64, P, C.c_int64,
+                                 C.c_int64, P, C.c_int64, C.c_int64, P, C.c_int, C.c_int64, C.c_int,
+                                 C.c_int, C.c_int, P, C.c_int, C.c_float, P]),
+    "ec_kv_work_size": (C.c_int64, [C.c_int, C.c_int]),
+    "ec_kv_open": (C.c_int, [P, P, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, P, C.c_int,
+                             C.c_int, P, P, P, C.c_int64, C.POINTER(C.c_int)]),
+    "ec_kv_close": (C.c_int, [C.c_int]),
+    "ec_kv_reserve": (C.c_int, [C.c_int, P, P, C.c_int, P, P]),
+    "ec_kv_fork": (C.c_int, [C.c_int, P, P, C.c_int, P, P]),
+    "ec_kv_free": (C.c_int, [C.c_int, P, C.c_int, P, P]),
+    "ec_kv_compact": (C.c_int, [C.c_int, P, P]),
+    "ec_kv_write": (C.c_int, [C.c_int, C.c_int, P, C.c_int64, C.c_int64, P, C.c_int64, C.c_int64,
+                              C.c_int64, P, P, C.c_int, P]),
+    "ec_attn_cached_work_size": (C.c_int64, [C.c_int, C.c_int64, C.c_int, C.c_int, C.c_int]),
+    "ec_attn_cached": (C.c_int, [C.c_int, C.c_int, P, C.c_int64, C.c_int64, P, C.c_int64, C.c_int64, P,
+                                 C.c_int64, C.c_int, P, P, C.c_int, C.c_int, C.c_float, P, C.c_int64, P]),
     "ec_ann_save": (C.c_int, [C.c_char_p, FP, C.c_int, C.c_int, C.c_int64, U32P, U32P]),
     "ec_ann_read": (C.c_int, [C.c_char_p, C.POINTER(C.c_int), C.POINTER(C.c_int), I64P, FP, U32P,
                               U32P]),

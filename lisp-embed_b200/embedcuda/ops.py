@@ -1,0 +1,227 @@
+"""Operators on device tensors: rotary positions, causal attention of packed
+prompts, and a paged key / value cache with the attention that reads it
+(include/embedcuda.h, "operators on device buffers").
+
+Tensors are anything with torch's interface (``data_ptr()``, ``shape``,
+``stride()``, ``dtype``, ``device``); the buffers stay the caller's and nothing
+is copied.  Work is enqueued on ``stream`` (a cudaStream_t as int; None: torch's
+current stream of the tensors' device) and not waited for.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import sys
+
+from . import _lib
+
+_DTYPES = {"torch.float32": _lib.EC_F32, "torch.bfloat16": _lib.EC_BF16, "torch.float16": _lib.EC_F16}
+ROPE_NONE, ROPE_LINEAR, ROPE_LLAMA3, ROPE_YARN = 0, 1, 2, 3
+KV_OK, KV_FULL, KV_BAD = 0, 1, 2
+
+
+def _stream(stream, t):
+    if stream is not None:
+        return stream
+    torch = sys.modules.get("torch")
+    return torch.cuda.current_stream(t.device).cuda_stream if torch else None
+
+
+def _code(t, what):
+    code = _DTYPES.get(str(t.dtype))
+    if code is None:
+        raise ValueError(f"{what}: dtype {t.dtype} (float32, bfloat16 or float16)")
+    return code
+
+
+def _rows(t, what, heads=None, head_dim=None):
+    """(pointer, token stride, head stride) of a [tokens, heads, head_dim] tensor."""
+    if t.dim() != 3 or (t.shape[2] > 1 and t.stride(2) != 1):
+        raise ValueError(f"{what} must be [tokens, heads, head_dim] with adjacent elements")
+    if (heads is not None and t.shape[1] != heads) or (head_dim is not None and t.shape[2] != head_dim):
+        raise ValueError(f"{what} has {t.shape[1]} heads of {t.shape[2]}, expected {heads} of {head_dim}")
+    return t.data_ptr(), t.stride(0), t.stride(1)
+
+
+def _ints(t, what, size=None, least=0):
+    if str(t.dtype) != "torch.int32" or t.dim() != 1 or not t.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous int32 vector")
+    if (size is not None and t.shape[0] != size) or t.shape[0] < least:
+        raise ValueError(f"{what} has {t.shape[0]} elements, expected {size if size is not None else least}")
+    return t.data_ptr()
+
+
+def _lse(t, tokens, heads):
+    if t is None:
+        return None
+    if str(t.dtype) != "torch.float32" or tuple(t.shape) != (tokens, heads) or not t.is_contiguous():
+        raise ValueError(f"lse must be a contiguous float32[{tokens}, {heads}]")
+    return t.data_ptr()
+
+
+def _tables(cos, sin):
+    for t in (cos, sin):
+        if str(t.dtype) != "torch.float32" or t.dim() != 2 or not t.is_contiguous():
+            raise ValueError("cos and sin must be contiguous float32[positions, rot_dim / 2]")
+    if cos.shape != sin.shape:
+        raise ValueError(f"cos {tuple(cos.shape)} and sin {tuple(sin.shape)} differ")
+    return cos.shape
+
+
+def rope_table(cos, sin, theta, scaling=None, stream=None):
+    """Fill cos and sin float32[positions, rot_dim / 2].  ``scaling`` is
+    config.json's rope_scaling (None, or rope_type linear / llama3 / yarn with
+    their keys)."""
+    positions, half = _tables(cos, sin)
+    s = dict(scaling or {})
+    kind = s.get("rope_type", s.get("type", "default" if not s else None))
+    factor, p0, p1, original, amp = 1.0, 0.0, 0.0, 0.0, 0.0
+    if kind == "default":
+        code = ROPE_NONE
+    elif kind == "linear":
+        code, factor = ROPE_LINEAR, s["factor"]
+    elif kind == "llama3":
+        code, factor = ROPE_LLAMA3, s["factor"]
+        p0, p1, original = s["low_freq_factor"], s["high_freq_factor"], s["original_max_position_embeddings"]
+    elif kind == "yarn":
+        code, factor = ROPE_YARN, s["factor"]
+        p0, p1, original = s.get("beta_fast", 32.0), s.get("beta_slow", 1.0), s["original_max_position_embeddings"]
+        amp = s.get("attention_factor") or 0.0
+    else:
+        raise ValueError(f"rope_scaling type {kind!r} (linear, llama3 or yarn)")
+    _lib.check(_lib.lib().ec_rope_table(cos.data_ptr(), sin.data_ptr(), positions, 2 * half, theta, code, factor,
+                                        p0, p1, original, amp, _stream(stream, cos)), "rope_table")
+
+
+def rope(x, pos, cos, sin, out=None, interleaved=False, inverse=False, stream=None):
+    """Turn the first 2 * cos.shape[1] elements of every head of x [tokens,
+    heads, head_dim] by its token's position (int32[tokens]); into ``out``, or
+    in place.  ``inverse`` turns back (the gradient).  Returns the result."""
+    positions, half = _tables(cos, sin)
+    out = x if out is None else out
+    code = _code(x, "x")
+    if _code(out, "out") != code or out.shape != x.shape:
+        raise ValueError(f"out {tuple(out.shape)} {out.dtype} does not match x {tuple(x.shape)} {x.dtype}")
+    xp, xt, xh = _rows(x, "x")
+    yp, yt, yh = _rows(out, "out")
+    tokens, heads, hd = x.shape
+    _lib.check(_lib.lib().ec_rope(xp, xt, xh, yp, yt, yh, code, tokens, heads, hd, 2 * half, int(interleaved),
+                                  int(inverse), _ints(pos, "pos", tokens), cos.data_ptr(), sin.data_ptr(), positions,
+                                  _stream(stream, x)), "rope")
+    return out
+
+
+def attn_prompt(q, k, v, cu, out, lse=None, scale=0.0, stream=None):
+    """Causal attention of packed prompts: q, out [tokens, q_heads, head_dim],
+    k, v [tokens, kv_heads, head_dim], sequence s the tokens cu[s]:cu[s + 1]
+    (int32 on the device); lse float32[tokens, q_heads] or None.  Returns out."""
+    tokens, hq, hd = q.shape
+    hk = k.shape[1]
+    code = _code(q, "q")
+    for t, what in ((k, "k"), (v, "v"), (out, "out")):
+        if _code(t, what) != code:
+            raise ValueError(f"{what} is {t.dtype}, q is {q.dtype}")
+        if t.shape[0] != tokens:
+            raise ValueError(f"{what} has {t.shape[0]} tokens, q has {tokens}")
+    _lib.check(_lib.lib().ec_attn_prompt(*_rows(q, "q"), *_rows(k, "k", hk, hd), *_rows(v, "v", hk, hd),
+                                         *_rows(out, "out", hq, hd), _lse(lse, tokens, hq), code, tokens, hq, hk, hd,
+                                         _ints(cu, "cu", least=1), cu.shape[0] - 1, scale, _stream(stream, q)),
+               "attn_prompt")
+    return out
+
+
+class KvCache:
+    """A paged cache in the caller's tensors: k, v [layers, pages, page_size,
+    heads, head_dim] (bfloat16 or float16), tables int32[slots, width], lens
+    int32[slots], refs int32[pages].  The object keeps the tensors alive; an
+    empty cache has lens and refs 0.  Calls on one cache must be ordered by
+    their streams.  Results of the page operations arrive in ``status``
+    (int32[2] on the device: KV_OK / KV_FULL / KV_BAD and a page count)."""
+
+    def __init__(self, k, v, tables, lens, refs, work=None):
+        if k.dim() != 5 or k.shape != v.shape or k.dtype != v.dtype or not k.is_contiguous() or not v.is_contiguous():
+            raise ValueError("k and v must be contiguous [layers, pages, page_size, heads, head_dim] of one type")
+        layers, pages, page, heads, hd = k.shape
+        if str(tables.dtype) != "torch.int32" or tables.dim() != 2 or not tables.is_contiguous():
+            raise ValueError("tables must be a contiguous int32[slots, width]")
+        slots, width = tables.shape
+        code = _code(k, "k")
+        lens_p, refs_p = _ints(lens, "lens", slots), _ints(refs, "refs", pages)
+        size = _lib.check(_lib.lib().ec_kv_work_size(pages, slots), "kv_work_size")
+        if work is None:
+            work = refs.new_zeros((size + 3) // 4)
+        if not work.is_contiguous():
+            raise ValueError("work must be contiguous")
+        h = C.c_int()
+        _lib.check(_lib.lib().ec_kv_open(k.data_ptr(), v.data_ptr(), code, layers, pages, page, heads, hd,
+                                         tables.data_ptr(), slots, width, lens_p, refs_p, work.data_ptr(),
+                                         work.numel() * work.element_size(), C.byref(h)), "kv_open")
+        self._handle = h.value
+        self._keep = (k, v, tables, lens, refs, work)
+        self.dtype, self.heads, self.head_dim, self.slots = k.dtype, heads, hd, slots
+
+    def close(self):
+        if self._handle:
+            _lib.lib().ec_kv_close(self._handle)
+        self._handle = 0
+        self._keep = ()
+
+    def __del__(self):
+        if getattr(self, "_handle", 0) and _lib is not None and _lib._lib is not None:
+            self.close()
+
+    def reserve(self, slots, add, status, stream=None):
+        n = slots.shape[0]
+        _lib.check(_lib.lib().ec_kv_reserve(self._handle, _ints(slots, "slots"), _ints(add, "add", n), n,
+                                            _ints(status, "status", 2), _stream(stream, status)), "kv_reserve")
+
+    def fork(self, src, dst, status, stream=None):
+        n = src.shape[0]
+        _lib.check(_lib.lib().ec_kv_fork(self._handle, _ints(src, "src"), _ints(dst, "dst", n), n,
+                                         _ints(status, "status", 2), _stream(stream, status)), "kv_fork")
+
+    def free(self, slots, status, stream=None):
+        _lib.check(_lib.lib().ec_kv_free(self._handle, _ints(slots, "slots"), slots.shape[0],
+                                         _ints(status, "status", 2), _stream(stream, status)), "kv_free")
+
+    def compact(self, status, stream=None):
+        _lib.check(_lib.lib().ec_kv_compact(self._handle, _ints(status, "status", 2), _stream(stream, status)),
+                   "kv_compact")
+
+    def _slots(self, slots, cu):
+        if slots is not None:
+            return _ints(slots, "slots", cu.shape[0] - 1)
+        if cu.shape[0] - 1 > self.slots:
+            raise ValueError(f"{cu.shape[0] - 1} sequences, the cache has {self.slots} slots")
+        return None
+
+    def write(self, layer, k, v, cu, slots=None, stream=None):
+        """Rows k, v [tokens, heads, head_dim] into `layer`: sequence s is the
+        last cu[s + 1] - cu[s] tokens of slots[s] (None: slot s)."""
+        for t, what in ((k, "k"), (v, "v")):
+            if t.dtype != self.dtype or t.shape[0] != k.shape[0]:
+                raise ValueError(f"{what} must be {self.dtype}, {k.shape[0]} tokens")
+        _lib.check(_lib.lib().ec_kv_write(self._handle, layer, *_rows(k, "k", self.heads, self.head_dim),
+                                          *_rows(v, "v", self.heads, self.head_dim), k.shape[0],
+                                          _ints(cu, "cu", least=1), self._slots(slots, cu), cu.shape[0] - 1,
+                                          _stream(stream, k)), "kv_write")
+
+    def attention_workspace(self, q, cu, max_new):
+        """Bytes of `attention`'s workspace for these shapes (zero it before its first use)."""
+        return _lib.check(_lib.lib().ec_attn_cached_work_size(self._handle, q.shape[0], q.shape[1], cu.shape[0] - 1,
+                                                              max_new), "attn_cached_work_size")
+
+    def attention(self, layer, q, cu, out, max_new, workspace, slots=None, lse=None, scale=0.0, stream=None):
+        """Attention of the new tokens q [tokens, q_heads, head_dim] over their
+        slots' pages (their own keys and values included).  Returns out."""
+        tokens, hq, hd = q.shape
+        if q.dtype != self.dtype or out.dtype != self.dtype or out.shape[0] != tokens:
+            raise ValueError(f"q and out must be {self.dtype} rows of the same tokens")
+        if not workspace.is_contiguous():
+            raise ValueError("workspace must be contiguous")
+        _lib.check(_lib.lib().ec_attn_cached(self._handle, layer, *_rows(q, "q", None, self.head_dim),
+                                             *_rows(out, "out", hq, self.head_dim), _lse(lse, tokens, hq), tokens, hq,
+                                             _ints(cu, "cu", least=1), self._slots(slots, cu), cu.shape[0] - 1,
+                                             max_new, scale, workspace.data_ptr(),
+                                             workspace.numel() * workspace.element_size(), _stream(stream, q)),
+                   "attn_cached")
+        return out
