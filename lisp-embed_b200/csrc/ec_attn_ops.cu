@@ -1,129 +1,155 @@
 // ec_attn_ops.cu -- causal grouped-head attention over packed queries, with
 // the keys in packed rows (ec_attn_prompt) or in the pages of a cache
 // (ec_attn_cached).
-#include <cuda_fp16.h>
+#include <cudaTypedefs.h>
 
 #include <algorithm>
 #include <cmath>
+#include <mutex>
 
-#include "ec_ops.h"
+#include "ec_attn_ops.cuh"
 
 namespace ec {
+
+PFN_cuTensorMapEncodeTiled_v12000 gemm_encode_fn();  // ec_gemm.cu
+
 namespace {
 
-struct AttnOpArgs {
-  const void *q, *k, *v;
-  void* out;
-  float* lse;
-  int64_t qt, qh, kt, kh, vt, vh, ot, oh;
-  int64_t tokens;
-  int q_heads, group, head_dim, nseq;
-  const int32_t *cu, *slots;
-  float scale;
-  KvCache c;  // c.k nullptr: packed keys
-  int layer;
-};
-
-template <typename T>
-__device__ __forceinline__ float ld(const T* p);
-template <>
-__device__ __forceinline__ float ld(const __nv_bfloat16* p) { return __bfloat162float(*p); }
-template <>
-__device__ __forceinline__ float ld(const __half* p) { return __half2float(*p); }
-__device__ __forceinline__ void st(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
-__device__ __forceinline__ void st(__half* p, float v) { *p = __float2half_rn(v); }
-
-// One warp per (token, query head): the keys one after the other, running
-// maximum and sum, four elements of the head per lane.
-template <typename T>
-__global__ void attn_rows_kernel(const AttnOpArgs a) {
-  const int64_t w = (blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x) >> 5;
-  const int lane = threadIdx.x & 31;
-  if (w >= a.tokens * a.q_heads) return;
-  const int64_t t = w / a.q_heads;
-  const int h = static_cast<int>(w % a.q_heads), kvh = h / a.group;
-  int lo = 0, hi = a.nseq - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (a.cu[mid] <= t) lo = mid;
-    else hi = mid - 1;
-  }
-  const int64_t begin = max(a.cu[lo], 0), end = a.cu[lo + 1];
-  if (t < begin || t >= end) return;  // behind the last sequence
-  int64_t last;                       // keys [0, last) are seen
-  const int32_t* table = nullptr;
-  if (a.c.k) {
-    const int s = a.slots ? a.slots[lo] : lo;
-    if (s < 0 || s >= a.c.slots) last = 0;
-    else {
-      const int64_t len = min(max(int64_t(a.c.lens[s]), int64_t(0)), int64_t(a.c.width) * a.c.page_size);
-      last = len - (end - t) + 1;
-      table = a.c.tables + static_cast<int64_t>(s) * a.c.width;
-    }
-  } else {
-    last = t - begin + 1;
-  }
-  const T* q = static_cast<const T*>(a.q) + t * a.qt + h * a.qh;
-  float qv[4], o[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) qv[i] = lane + 32 * i < a.head_dim ? ld(q + lane + 32 * i) : 0.f;
-  for (int64_t j = 0; j < last; ++j) {
-    const T *k, *v;
-    if (table) {
-      const int page = table[j / a.c.page_size];
-      const int64_t row = a.c.heads * static_cast<int64_t>(a.head_dim);
-      const bool there = page >= 0 && page < a.c.pages;
-      const int64_t at = ((static_cast<int64_t>(a.layer) * a.c.pages + page) * a.c.page_size + j % a.c.page_size) * row +
-                         kvh * a.head_dim;
-      k = there ? static_cast<const T*>(a.c.k) + at : nullptr;
-      v = there ? static_cast<const T*>(a.c.v) + at : nullptr;
-    } else {
-      k = static_cast<const T*>(a.k) + (begin + j) * a.kt + kvh * a.kh;
-      v = static_cast<const T*>(a.v) + (begin + j) * a.vt + kvh * a.vh;
-    }
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (k && lane + 32 * i < a.head_dim) s += qv[i] * ld(k + lane + 32 * i);
-#pragma unroll
-    for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-    s *= a.scale;
-    const float mn = fmaxf(m, s);
-    const float c = m == -INFINITY ? 0.f : expf(m - mn), p = s == -INFINITY ? 0.f : expf(s - mn);
-    l = l * c + p;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float x = v && lane + 32 * i < a.head_dim ? ld(v + lane + 32 * i) : 0.f;
-      o[i] = o[i] * c + p * x;
-    }
-    m = mn;
-  }
-  T* out = static_cast<T*>(a.out) + t * a.ot + h * a.oh;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (lane + 32 * i < a.head_dim) st(out + lane + 32 * i, l > 0.f ? o[i] / l : l == 0.f ? 0.f : NAN);
-  if (a.lse && lane == 0) a.lse[t * a.q_heads + h] = l == 0.f ? -INFINITY : m + logf(l);
+// tensor map of 16-bit rows: dims and strides (bytes) outermost last, box of
+// 64 columns by `box` of the outer dimensions
+bool encode(CUtensorMap* tm, int dtype, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
+            const cuuint32_t* box) {
+  auto enc = gemm_init_driver() ? gemm_encode_fn() : nullptr;  // no ec_init needed
+  const cuuint32_t es[4] = {1, 1, 1, 1};
+  return enc && enc(tm, dtype == EC_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank,
+                    const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
+
+bool encode_rows(CUtensorMap* tm, int dtype, const OpRows& r, int head_dim, int heads, int64_t tokens, int box_heads,
+                 int box_tokens) {
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(head_dim), static_cast<cuuint64_t>(heads),
+                              static_cast<cuuint64_t>(tokens)};
+  // the stride of a single head or token is never used, but has to be valid
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(heads > 1 ? r.head : head_dim) * 2,
+                                 static_cast<cuuint64_t>(tokens > 1 ? r.token : head_dim) * 2};
+  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_heads), static_cast<cuuint32_t>(box_tokens)};
+  return encode(tm, dtype, r.p, 3, dims, strides, box);
+}
+
+template <int HD, int NT, typename T>
+int launch_flash(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const FlashArgs& a, int grid,
+                 cudaStream_t st) {
+  using Cfg = FlashCfg<HD, NT>;
+  static std::mutex mu;
+  static bool set[64] = {};
+  int dev = 0;
+  if (int rc = check_cuda(cudaGetDevice(&dev), "cudaGetDevice")) return rc;
+  {
+    std::lock_guard<std::mutex> lk(mu);
+    if (!set[dev]) {
+      if (int rc = check_cuda(cudaFuncSetAttribute(flash_kernel<HD, NT, T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   static_cast<int>(Cfg::SMEM)),
+                              "attention shared memory"))
+        return rc;
+      set[dev] = true;
+    }
+  }
+  flash_kernel<HD, NT, T><<<grid, Cfg::THREADS, Cfg::SMEM, st>>>(q, k, v, a);
+  return check_cuda(cudaGetLastError(), "attention");
+}
+
+template <int HD, typename T>
+int launch_flash_t(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const FlashArgs& a, int nt,
+                   int grid, cudaStream_t st) {
+  if (nt == 2) return launch_flash<HD, 2, T>(q, k, v, a, grid, st);
+  if (int rc = launch_flash<HD, 1, T>(q, k, v, a, grid, st)) return rc;
+  if (!a.even) return EC_OK;
+  const int64_t warps = static_cast<int64_t>(a.tokens) * a.q_heads;
+  flash_join_kernel<HD, T><<<static_cast<unsigned>((warps + 3) / 4), 128, 0, st>>>(a);
+  return check_cuda(cudaGetLastError(), "attention join");
+}
+
+// How a call is cut up, from what the host knows
+struct FlashPlan {
+  int nt, even, rows_tok;
+};
+FlashPlan flash_plan(const KvCache* c, int64_t tokens, int q_heads, int kv_heads, int nseq, int max_new, int num_sms) {
+  FlashPlan p;
+  p.rows_tok = 128 / (q_heads / kv_heads);
+  const int64_t tiles = (tokens / p.rows_tok + nseq) * kv_heads;
+  const int64_t pairs = (tokens / (2 * p.rows_tok) + nseq) * kv_heads;
+  p.even = 0;
+  if (c && nseq <= FlashCfg<128, 1>::MAX_SEQS && (max_new <= p.rows_tok || tiles < 2 * num_sms)) {
+    // block counts are 32-bit
+    const int64_t most = (static_cast<int64_t>(c->width) * c->page_size + 127) / 128;
+    p.even = tiles * most < (int64_t(1) << 30);
+  }
+  p.nt = !p.even && tokens > static_cast<int64_t>(nseq) * p.rows_tok && pairs >= num_sms ? 2 : 1;
+  return p;
+}
+
+size_t part_bytes(int hd) { return static_cast<size_t>(2) * kMaxCtas * 128 * hd * 4; }
 
 }  // namespace
 
-size_t attention_work_bytes(const KvCache&, int64_t, int, int, int) { return 256; }
+size_t attention_work_bytes(const KvCache& c, int64_t tokens, int q_heads, int nseq, int max_new) {
+  if (!flash_plan(&c, tokens, q_heads, c.heads, nseq, max_new, kMaxCtas).even) return 256;
+  return part_bytes(c.head_dim <= 64 ? 64 : 128) + 2 * kMaxCtas * 128 * 4 +
+         (static_cast<size_t>(FlashCfg<128, 1>::MAX_SEQS) + 2) * 4;
+}
 
-int run_attention(const AttnOp& op, int, cudaStream_t st) {
-  AttnOpArgs a{};
-  a.q = op.q.p, a.qt = op.q.token, a.qh = op.q.head;
-  a.k = op.k.p, a.kt = op.k.token, a.kh = op.k.head;
-  a.v = op.v.p, a.vt = op.v.token, a.vh = op.v.head;
+int run_attention(const AttnOp& op, int num_sms, cudaStream_t st) {
+  const KvCache* c = op.cache;
+  num_sms = std::min(num_sms, kMaxCtas);
+  const FlashPlan p = flash_plan(c, op.tokens, op.q_heads, op.kv_heads, op.nseq, op.max_new, num_sms);
+  const int group = op.q_heads / op.kv_heads, hd = op.head_dim <= 64 ? 64 : 128;
+  CUtensorMap tq, tk, tv;
+  bool ok = encode_rows(&tq, op.dtype, op.q, op.head_dim, op.q_heads, op.tokens, group, p.rows_tok);
+  if (c) {
+    const cuuint64_t row = static_cast<cuuint64_t>(c->heads) * c->head_dim * 2;
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(c->head_dim), static_cast<cuuint64_t>(c->heads),
+                                static_cast<cuuint64_t>(c->page_size),
+                                static_cast<cuuint64_t>(c->layers) * static_cast<cuuint64_t>(c->pages)};
+    const cuuint64_t strides[3] = {static_cast<cuuint64_t>(c->head_dim) * 2, row, row * c->page_size};
+    const cuuint32_t box[4] = {64, 1, static_cast<cuuint32_t>(c->page_size), 1};
+    ok = ok && encode(&tk, c->dtype, c->k, 4, dims, strides, box) && encode(&tv, c->dtype, c->v, 4, dims, strides, box);
+  } else {
+    ok = ok && encode_rows(&tk, op.dtype, op.k, op.head_dim, op.kv_heads, op.tokens, 1, 128) &&
+         encode_rows(&tv, op.dtype, op.v, op.head_dim, op.kv_heads, op.tokens, 1, 128);
+  }
+  if (!ok) return set_error(EC_EINVAL, "the attention's strides cannot be described to the TMA");
+  FlashArgs a{};
   a.out = const_cast<void*>(op.out.p), a.ot = op.out.token, a.oh = op.out.head;
   a.lse = op.lse;
-  a.tokens = op.tokens, a.q_heads = op.q_heads, a.group = op.q_heads / op.kv_heads, a.head_dim = op.head_dim;
-  a.nseq = op.nseq, a.cu = op.cu, a.slots = op.slots, a.scale = op.scale, a.layer = op.layer;
-  if (op.cache) a.c = *op.cache;
-  const int64_t warps = op.tokens * op.q_heads;
-  const unsigned grid = static_cast<unsigned>((warps + 7) / 8);
-  if (op.dtype == EC_BF16) attn_rows_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(a);
-  else attn_rows_kernel<__half><<<grid, 256, 0, st>>>(a);
-  return check_cuda(cudaGetLastError(), "attention");
+  a.cu = op.cu, a.slots = op.slots;
+  a.tokens = static_cast<int>(op.tokens), a.nseq = op.nseq;
+  a.group = group, a.rows_tok = p.rows_tok, a.q_heads = op.q_heads, a.kv_heads = op.kv_heads;
+  a.head_dim = op.head_dim;
+  a.scale_log2 = op.scale * 1.4426950408889634f;
+  if (c) {
+    a.paged = 1;
+    a.lens = c->lens, a.tables = c->tables, a.width = c->width, a.nslots = c->slots;
+    a.pages = c->pages, a.page_size = c->page_size;
+    a.page0 = op.layer * c->pages, a.page_end = c->layers * c->pages;
+  }
+  int64_t grid = (op.tokens / (p.nt * p.rows_tok) + op.nseq) * op.kv_heads;
+  if (p.even) {
+    char* w = static_cast<char*>(op.work);
+    a.even = 1;
+    a.min_chunk = 4;
+    a.part_o = reinterpret_cast<float*>(w);
+    a.part_l = reinterpret_cast<float*>(w + part_bytes(hd));
+    a.plan = reinterpret_cast<int*>(w + part_bytes(hd) + 2 * kMaxCtas * 128 * 4);
+    grid = num_sms;
+  }
+  const int ctas = static_cast<int>(std::min<int64_t>(grid, num_sms));
+  if (op.dtype == EC_BF16)
+    return hd == 64 ? launch_flash_t<64, __nv_bfloat16>(tq, tk, tv, a, p.nt, ctas, st)
+                    : launch_flash_t<128, __nv_bfloat16>(tq, tk, tv, a, p.nt, ctas, st);
+  return hd == 64 ? launch_flash_t<64, __half>(tq, tk, tv, a, p.nt, ctas, st)
+                  : launch_flash_t<128, __half>(tq, tk, tv, a, p.nt, ctas, st);
 }
 
 namespace {
@@ -131,7 +157,8 @@ namespace {
 int check_attention(const AttnOp& op, int64_t tokens, int nseq, float scale) {
   if (op.dtype != EC_BF16 && op.dtype != EC_F16)
     return set_error(EC_EINVAL, "attention takes bf16 or f16, not dtype %d", op.dtype);
-  if (tokens < 0 || tokens > INT32_MAX || nseq < 0) return set_error(EC_EINVAL, "bad token or sequence count");
+  if (tokens < 0 || tokens > (1 << 30) || nseq < 0 || nseq > (1 << 24))
+    return set_error(EC_EINVAL, "bad token or sequence count");
   if (op.head_dim < 8 || op.head_dim > 128 || op.head_dim % 8)
     return set_error(EC_EINVAL, "head_dim %d (supported: multiples of 8 up to 128)", op.head_dim);
   if (op.q_heads < 1 || op.kv_heads < 1 || op.q_heads > 1024 || op.q_heads % op.kv_heads || op.q_heads / op.kv_heads > 128)
@@ -153,7 +180,12 @@ using namespace ec;
 extern "C" int ec_op_status(void) {
   clear_error();
   if (int rc = check_cuda(cudaDeviceSynchronize(), "operators")) return rc;
-  return EC_OK;
+  unsigned v = 0;
+  if (int rc = check_cuda(cudaMemcpyFromSymbol(&v, g_op_status, sizeof v), "operator status")) return rc;
+  if (v == 0) return EC_OK;
+  const unsigned zero = 0;
+  if (int rc = check_cuda(cudaMemcpyToSymbol(g_op_status, &zero, sizeof zero), "operator status")) return rc;
+  return set_error(v == kDevBadArg ? EC_ECUDA : EC_ETIMEOUT, "a wait inside an attention kernel gave up (code %u)", v);
 }
 
 extern "C" int ec_attn_prompt(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token,
@@ -180,7 +212,7 @@ extern "C" int64_t ec_attn_cached_work_size(int handle, int64_t tokens, int q_he
   clear_error();
   auto c = kv_find(handle);
   if (!c) return EC_EINVAL;
-  if (tokens < 0 || tokens > INT32_MAX || nseq < 0 || max_new < 0 || q_heads < 1 || q_heads % c->heads)
+  if (tokens < 0 || tokens > (1 << 30) || nseq < 0 || nseq > (1 << 24) || max_new < 0 || q_heads < 1 || q_heads % c->heads)
     return set_error(EC_EINVAL, "bad attention shape");
   return static_cast<int64_t>(attention_work_bytes(*c, tokens, q_heads, nseq, max_new));
 }

@@ -1,0 +1,784 @@
+// ec_attn_ops.cuh -- causal grouped-head attention on the 5th-generation
+// tensor cores, keys in packed rows or in the pages of a cache.
+//
+//   o_r = sum_j softmax_j(scale * q_r . k_j) v_j over the keys that row r sees
+//
+// A tile is 128 query rows of one key head: R = 128 / G tokens with their G
+// query heads (row = token * G + head), so that the heads of a group share
+// every key and value that is read.  A CTA takes NT tiles of consecutive
+// tokens through the 128-key blocks that they see:
+//
+//   S = Q K^T      tcgen05.mma, Q and K from shared memory  -> TMEM
+//   P = exp2(..)   one thread per row: 128 scores to registers, running
+//                  maximum and sum without any exchange; P (16 bits) goes
+//                  back to TMEM over S's first 64 columns
+//   O += P V       tcgen05.mma, P from TMEM, V from shared memory -> TMEM
+//
+// NT = 2: while one tile's rows go through the exponential, the tensor core
+// works on the other tile's P V and next S.  NT = 1 (few queries): S is
+// double-buffered instead, so the next block's scores are there when the
+// current block's exponentials are done.
+//
+// O is rescaled only when a row's maximum grows by more than 2^8 (P stays
+// below 2^8 in its 16 bits; sums are fp32).
+//
+// Warps: 4 per tile softmax, then one each for the loads, the MMAs and the
+// work list.  All waits are bounded.
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include "ec_fa.cuh"
+#include "ec_ops.h"
+#include "ec_ptx.cuh"
+
+namespace ec {
+
+// CTAs that an even split can have: one per SM (148 on a B200)
+constexpr int kMaxCtas = 160;
+
+struct FlashArgs {
+  void* out;
+  float* lse;
+  int64_t ot, oh;          // out strides in elements
+  const int32_t *cu, *slots, *lens, *tables;
+  int width, nslots;       // of the cache's tables
+  int pages, page_size, page0, page_end;  // page0: first page of the layer, page_end: pages of all layers
+  int tokens, nseq;
+  int group, rows_tok;     // G, R
+  int q_heads, kv_heads, head_dim;
+  float scale_log2;
+  int paged;
+  int even;                // 1: the blocks are split evenly over the CTAs
+  int min_chunk;           // blocks a CTA takes at least
+  float* part_o;           // [2 * CTAs][128][HD] partial results of cut tiles
+  float* part_l;           // [2 * CTAs][128] their log2-sum-exp2
+  int* plan;               // chunk, prefix sums for the join
+};
+
+// a tile set that one CTA works on
+struct FlashItem {
+  int valid;
+  int tok0, qv;   // first token, tokens
+  int kvh;
+  int pos0;       // position of tok0 in its sequence
+  int kv_len;
+  int kbase;      // packed keys: first token of the sequence; cache: its slot
+  int kb0;        // first key block
+  int nb[2];      // end block of each tile
+  int part;       // partial result, -1: the whole of the tile's keys
+};
+
+template <int HD, int NT>
+struct FlashCfg {
+  static constexpr int AT = HD / 64;                 // 64-column atoms
+  static constexpr uint32_t ATOM = 16384;            // 128 rows x 128 B
+  static constexpr uint32_t TILE = AT * ATOM;
+  static constexpr int STAGES = HD == 128 ? 5 : 8;   // K and V tiles in flight
+  static constexpr int MAX_SEQS = 2048;              // prefix sums of an even split
+  static constexpr int WARPS = 4 * NT + 3;
+  static constexpr int THREADS = 32 * WARPS;
+  static constexpr uint32_t TAIL = 1024 + (NT == 1 ? 4 * (MAX_SEQS + 1) : 0);
+  static constexpr size_t SMEM = NT * TILE + STAGES * TILE + TAIL;
+  static constexpr uint32_t O_COL = 256;
+  static_assert(SMEM <= 232448, "shared memory");
+};
+
+// first wait that gave up on this device since ec_op_status last asked
+static __device__ unsigned g_op_status;
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) { return pack_bf16(a, b); }
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// key blocks that the first n tokens of a sequence's queries see
+__device__ __forceinline__ int blocks_seen(int pos0, int n, int kv_len) {
+  const int seen = min(kv_len, pos0 + n);
+  return seen > 0 ? (seen + 127) >> 7 : 0;
+}
+
+// sequence s: its queries [begin, end) within the rows of the call, and keys
+struct FlashSeq {
+  int begin, end, kv_len, kbase;
+};
+__device__ __forceinline__ FlashSeq flash_seq(const FlashArgs& a, int s) {
+  FlashSeq q;
+  q.begin = min(max(a.cu[s], 0), a.tokens);
+  q.end = min(max(a.cu[s + 1], q.begin), a.tokens);
+  if (a.paged) {
+    const int slot = a.slots ? a.slots[s] : s;
+    const bool ok = slot >= 0 && slot < a.nslots;
+    const int most = a.width * a.page_size;  // fits 31 bits (checked when the cache is opened)
+    q.kv_len = ok ? min(max(a.lens[slot], 0), most) : 0;
+    q.kbase = ok ? slot : 0;
+  } else {
+    q.kv_len = q.end - q.begin;
+    q.kbase = q.begin;
+  }
+  return q;
+}
+
+// ------------------------------------------------------------- work lists --
+// Without a split: slot u of the list is the tile set f(s) + i of sequence s,
+// f(s) = cu[s] / BT + s for BT tokens per set.  f leaves at least
+// ceil(len / BT) slots to every sequence and needs no prefix sum; a sequence
+// is found by a 32-way search.
+__device__ __forceinline__ int flash_find(const FlashArgs& a, int bt, int u, int lane) {
+  int lo = 0, hi = a.nseq;  // f(lo) <= u, f(hi) > u (or hi = nseq)
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 31) / 32;
+    const int s = lo + lane * step;
+    const bool le = s < hi && min(max(a.cu[s], 0), a.tokens) / bt + s <= u;
+    const unsigned m = __ballot_sync(0xffffffffu, le);
+    const int k = m ? 31 - __clz(m) : 0;
+    hi = min(hi, lo + (k + 1) * step);
+    lo = lo + k * step;
+  }
+  return lo;
+}
+
+template <int HD, int NT, typename T>
+__global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
+    flash_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                 const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ FlashArgs a) {
+  using Cfg = FlashCfg<HD, NT>;
+  constexpr int AT = Cfg::AT, ST = Cfg::STAGES;
+  constexpr int FMT = sizeof(T) == 2 && std::is_same<T, __half>::value ? 0 : 1;
+  constexpr uint32_t IDESC_S = make_idesc(FMT, 128, 128);
+  constexpr uint32_t IDESC_PV = make_idesc(FMT, 128, HD) | (1u << 16);  // B MN-major
+  constexpr int W_LOAD = 4 * NT, W_MMA = 4 * NT + 1, W_LIST = 4 * NT + 2;
+  constexpr int READERS = 4 * NT + 2;  // warps that read a list entry
+
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if (smem_u32(smem) & 1023u) {  // swizzled tiles need 1024-byte alignment
+    if (threadIdx.x == 0) report(&g_op_status, kDevBadArg);
+    return;
+  }
+  uint8_t* sQ = smem;
+  uint8_t* sKV = sQ + NT * Cfg::TILE;
+  uint8_t* tail = sKV + ST * Cfg::TILE;
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(tail);
+  uint64_t* q_empty = q_full + 1;
+  uint64_t* kv_full = q_empty + 1;
+  uint64_t* kv_empty = kv_full + ST;
+  uint64_t* s_full = kv_empty + ST;   // [2] tile (NT 2) or buffer (NT 1)
+  uint64_t* p_full = s_full + 2;      // [2]
+  uint64_t* o_full = p_full + 2;      // [2]
+  uint64_t* i_full = o_full + 2;      // [2]
+  uint64_t* i_empty = i_full + 2;     // [2]
+  FlashItem* items = reinterpret_cast<FlashItem*>(i_empty + 2);  // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(items + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* prefix = reinterpret_cast<int*>(tail + 1024);  // [nseq + 1] of an even split
+  static_assert(8 * (2 + 2 * ST + 10) + 2 * sizeof(FlashItem) + 8 <= 1024, "tail");
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    for (int i = 0; i < ST; ++i) {
+      mbar_init(&kv_full[i], 1);
+      mbar_init(&kv_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&o_full[i], 1);
+      mbar_init(&i_full[i], 1);
+      mbar_init(&i_empty[i], READERS);
+    }
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == W_LOAD && lane == 0) {
+    tma_prefetch_desc(&tm_q);
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+  }
+  if (warp == W_MMA) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int R = a.rows_tok, G = a.group, BT = NT * R;
+  bool ok = true;
+  unsigned code = kDevTimeoutOther;
+
+  // the next entry of the list for the reading warps
+  int it_n = 0;
+  auto next_item = [&](FlashItem& it) -> bool {
+    const int b = it_n & 1;
+    if (!mbar_wait_warp(&i_full[b], (it_n >> 1) & 1, abort_flag)) return false;
+    it = items[b];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&i_empty[b]);
+    ++it_n;
+    return true;
+  };
+
+  if (warp == W_LIST) {
+    // ------------------------------------------------------------ work list
+    int n = 0;
+    auto publish = [&](const FlashItem& it) -> bool {
+      const int b = n & 1;
+      if (!mbar_wait_warp(&i_empty[b], ((n >> 1) & 1) ^ 1, abort_flag)) return false;
+      if (lane == 0) {
+        items[b] = it;
+        mbar_arrive(&i_full[b]);
+      }
+      __syncwarp();
+      ++n;
+      return true;
+    };
+    FlashItem it{};
+    if (NT == 1 && a.even) {
+      // every CTA takes the same number of key blocks: blocks in the order
+      // (sequence, tile, key head, block), prefix sums over the sequences
+      int total = 0;
+      for (int s0 = 0; s0 < a.nseq; s0 += 32) {
+        int v = 0;
+        if (s0 + lane < a.nseq) {
+          const FlashSeq q = flash_seq(a, s0 + lane);
+          const int len = q.end - q.begin;
+          for (int i = 0; i < len; i += R) v += blocks_seen(q.kv_len - len + i, min(R, len - i), q.kv_len);
+          v *= a.kv_heads;
+        }
+        int x = v;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+          const int y = __shfl_up_sync(0xffffffffu, x, d);
+          if (lane >= d) x += y;
+        }
+        if (s0 + lane < a.nseq) prefix[s0 + lane] = total + x - v;
+        total += __shfl_sync(0xffffffffu, x, 31);
+      }
+      if (lane == 0) prefix[a.nseq] = total;
+      __syncwarp();
+      const int chunk = max(a.min_chunk, (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x));
+      if (blockIdx.x == 0) {
+        for (int s = lane; s <= a.nseq; s += 32) a.plan[1 + s] = prefix[s];
+        if (lane == 0) a.plan[0] = chunk;
+      }
+      int64_t w64 = static_cast<int64_t>(blockIdx.x) * chunk;
+      const int end = static_cast<int>(min(w64 + chunk, static_cast<int64_t>(total)));
+      int w = static_cast<int>(min(w64, static_cast<int64_t>(total)));
+      const int begin = w;
+      // last sequence with prefix <= w (those without blocks are skipped)
+      int lo = 0, hi = a.nseq;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (prefix[mid] <= w) lo = mid;
+        else hi = mid;
+      }
+      for (int s = lo; ok && w < end; ++s) {
+        const FlashSeq q = flash_seq(a, s);
+        const int len = q.end - q.begin;
+        int at = prefix[s];
+        for (int i = 0; ok && i < len && w < end; i += R) {
+          const int nb = blocks_seen(q.kv_len - len + i, min(R, len - i), q.kv_len);
+          if (at + nb * a.kv_heads <= w) {
+            at += nb * a.kv_heads;
+            continue;
+          }
+          for (int h = 0; ok && h < a.kv_heads && w < end; ++h, at += nb) {
+            if (at + nb <= w) continue;
+            it.valid = 1;
+            it.tok0 = q.begin + i;
+            it.qv = min(R, len - i);
+            it.kvh = h;
+            it.pos0 = q.kv_len - len + i;
+            it.kv_len = q.kv_len;
+            it.kbase = q.kbase;
+            it.kb0 = w - at;
+            it.nb[0] = min(nb, end - at);
+            it.nb[1] = 0;
+            it.part = it.kb0 == 0 && it.nb[0] == nb ? -1 : 2 * static_cast<int>(blockIdx.x) + (w == begin ? 0 : 1);
+            ok = publish(it);
+            w = at + it.nb[0];
+          }
+        }
+      }
+      // tiles that see no key are nobody's blocks: their rows are cleared by
+      // the join
+    } else {
+      const int64_t slots = a.tokens / BT + a.nseq;
+      const int64_t all = slots * a.kv_heads;
+      int64_t round = 0;
+      for (int64_t t0 = 0; ok && t0 < all; t0 += gridDim.x, ++round) {
+        // late (long) tile sets first; the order turns round every pass, so
+        // that no CTA gets the longest of each
+        const int64_t t = t0 + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+        if (t >= all) continue;
+        const int u = static_cast<int>(slots - 1 - t / a.kv_heads);
+        const int s = flash_find(a, BT, u, lane);
+        const FlashSeq q = flash_seq(a, s);
+        const int len = q.end - q.begin;
+        const int64_t q0 = static_cast<int64_t>(u - (q.begin / BT + s)) * BT;
+        if (q0 < 0 || q0 >= len) continue;
+        it.valid = 1;
+        it.tok0 = q.begin + static_cast<int>(q0);
+        it.qv = min(BT, len - static_cast<int>(q0));
+        it.kvh = static_cast<int>(t % a.kv_heads);
+        it.pos0 = q.kv_len - len + static_cast<int>(q0);
+        it.kv_len = q.kv_len;
+        it.kbase = q.kbase;
+        it.kb0 = 0;
+        it.nb[0] = blocks_seen(it.pos0, min(R, it.qv), q.kv_len);
+        it.nb[1] = NT == 2 && it.qv > R ? blocks_seen(it.pos0, it.qv, q.kv_len) : 0;
+        it.part = -1;
+        ok = publish(it);
+      }
+    }
+    it.valid = 0;
+    if (ok) ok = publish(it);
+  } else if (warp == W_LOAD) {
+    // ---------------------------------------------------------------- loads
+    code = kDevTimeoutProducer;
+    FlashItem it;
+    int st = 0;
+    uint32_t ph = 0, q_ph = 0;
+    const int ppb = a.paged ? 128 / a.page_size : 1;
+    while (true) {
+      if (!(ok = next_item(it)) || !it.valid) break;
+      const int nb = max(it.nb[0], NT == 2 ? it.nb[1] : 0);
+      if (nb <= it.kb0) continue;
+      if (!(ok = mbar_wait_warp(q_empty, q_ph ^ 1, abort_flag))) break;
+      q_ph ^= 1;
+      if (lane == 0) {
+        // rows past the tokens of the call are filled with zeros
+        mbar_arrive_expect_tx(q_full, NT * AT * static_cast<uint32_t>(G * R) * 128u);
+        for (int t = 0; t < NT; ++t)
+          for (int c = 0; c < AT; ++c)
+            asm volatile(
+                "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], "
+                "[%2];" ::"r"(smem_u32(sQ + t * Cfg::TILE + c * Cfg::ATOM)),
+                "l"(reinterpret_cast<uint64_t>(&tm_q)), "r"(smem_u32(q_full)), "r"(c * 64), "r"(it.kvh * G),
+                "r"(it.tok0 + t * R)
+                : "memory");
+      }
+      __syncwarp();
+      const int32_t* table = a.tables + static_cast<int64_t>(it.kbase) * a.width;
+      const int in_use = a.paged ? (it.kv_len + a.page_size - 1) / a.page_size : 0;
+      // pages of the next 32 table entries, one per lane; an entry that is
+      // none reads past the pages, which fills the tile with zeros
+      int first = it.kb0 * ppb, page = 0, ahead = 0;
+      auto fetch = [&](int e) -> int {
+        int p = -1;
+        if (a.paged && e < in_use) p = table[e];
+        return p >= 0 && p < a.pages ? a.page0 + p : a.page_end;
+      };
+      page = fetch(first + lane);
+      ahead = fetch(first + 32 + lane);
+      for (int j = it.kb0; ok && j < nb; ++j) {
+        if (a.paged && j * ppb - first == 32) {
+          first += 32;
+          page = ahead;
+          ahead = fetch(first + 32 + lane);
+        }
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          if (!(ok = mbar_wait_warp(&kv_empty[st], ph ^ 1, abort_flag))) break;
+          uint8_t* dst = sKV + st * Cfg::TILE;
+          if (lane == 0) mbar_arrive_expect_tx(&kv_full[st], Cfg::TILE);
+          __syncwarp();
+          const uint64_t map = reinterpret_cast<uint64_t>(kv ? &tm_v : &tm_k);
+          if (a.paged) {
+            const int p = __shfl_sync(0xffffffffu, page, (j * ppb - first + lane / AT) & 31);
+            if (lane < ppb * AT)
+              asm volatile(
+                  "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], "
+                  "[%1, {%3, %4, %5, %6}], [%2];" ::"r"(
+                      smem_u32(dst + (lane % AT) * Cfg::ATOM + (lane / AT) * a.page_size * 128)),
+                  "l"(map), "r"(smem_u32(&kv_full[st])), "r"((lane % AT) * 64), "r"(it.kvh), "r"(0), "r"(p)
+                  : "memory");
+          } else if (lane < AT) {
+            asm volatile(
+                "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], "
+                "[%2];" ::"r"(smem_u32(dst + lane * Cfg::ATOM)),
+                "l"(map), "r"(smem_u32(&kv_full[st])), "r"(lane * 64), "r"(it.kvh), "r"(it.kbase + j * 128)
+                : "memory");
+          }
+          __syncwarp();
+          if (++st == ST) {
+            st = 0;
+            ph ^= 1;
+          }
+        }
+      }
+      if (!ok) break;
+    }
+  } else if (warp == W_MMA) {
+    // ----------------------------------------------------------------- MMAs
+    code = kDevTimeoutMma;
+    FlashItem it;
+    int e = 0;  // entries of the K / V ring used: K of block j is entry base + 2 j
+    uint32_t q_ph = 0;
+    int pf[2] = {0, 0};  // P's waited for, per tile / buffer
+    int g = 0;           // blocks (NT 1)
+    const uint32_t q_addr = smem_u32(sQ), kv_addr = smem_u32(sKV);
+    auto wait_kv = [&](int entry) -> bool {
+      return mbar_wait_warp(&kv_full[entry % ST], (entry / ST) & 1, abort_flag);
+    };
+    auto mma_s = [&](int t, int entry, uint32_t d) {
+      const uint32_t qa = q_addr + t * Cfg::TILE, ka = kv_addr + (entry % ST) * Cfg::TILE;
+#pragma unroll
+      for (int kk = 0; kk < HD / 16; ++kk) {
+        const uint32_t off = (kk >> 2) * Cfg::ATOM + (kk & 3) * 32;
+        umma_f16(d, desc_sw128_kmajor(qa + off), desc_sw128_kmajor(ka + off), IDESC_S, kk > 0);
+      }
+    };
+    auto mma_pv = [&](uint32_t d, uint32_t p, int entry, bool first) {
+      const uint32_t va = kv_addr + (entry % ST) * Cfg::TILE;
+#pragma unroll
+      for (int kk = 0; kk < 8; ++kk)
+        umma_f16_ts(d, p + kk * 8, desc_mnmajor<false>(va + kk * 2048, Cfg::ATOM), IDESC_PV, !first || kk > 0);
+    };
+    // V rows behind the sequence's keys: another sequence's rows, or what a
+    // page held before.  Their probabilities are 0, and 0 * NaN would not be.
+    auto clear_v = [&](int entry, int j, int kv_len) {
+      const int from = kv_len - j * 128;
+      if (from >= 128) return;
+      uint8_t* v = sKV + (entry % ST) * Cfg::TILE;
+      for (int i = from * 8 + lane; i < 1024; i += 32) {
+#pragma unroll
+        for (int c = 0; c < AT; ++c) *reinterpret_cast<uint4*>(v + c * Cfg::ATOM + i * 16) = make_uint4(0, 0, 0, 0);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+    };
+    while (true) {
+      if (!(ok = next_item(it)) || !it.valid) break;
+      const int kb0 = it.kb0;
+      const int n0 = it.nb[0] - kb0, n1 = NT == 2 ? it.nb[1] - kb0 : 0, n = max(n0, n1);
+      if (n <= 0) continue;
+      if (!(ok = mbar_wait_warp(q_full, q_ph, abort_flag)) || !(ok = wait_kv(e))) break;
+      q_ph ^= 1;
+      tc_fence_after();
+      if (NT == 2) {
+        if (lane == 0) {
+          if (n0 > 0) {
+            mma_s(0, e, tmem);
+            umma_commit(&s_full[0]);
+          }
+          if (n1 > 0) {
+            mma_s(1, e, tmem + 128);
+            umma_commit(&s_full[1]);
+          }
+          umma_commit(&kv_empty[e % ST]);
+          if (n == 1) umma_commit(q_empty);
+        }
+        __syncwarp();
+        for (int j = 0; ok && j < n; ++j) {
+          const int ev = e + 2 * j + 1, ek = ev + 1;
+          bool have_v = false, have_k = false;
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const int nt = t ? n1 : n0;
+            if (!ok || j >= nt) continue;
+            if (!have_v) {
+              if (!(ok = wait_kv(ev))) break;
+              clear_v(ev, kb0 + j, it.kv_len);
+              have_v = true;
+            }
+            if (!(ok = mbar_wait_warp(&p_full[t], pf[t] & 1, abort_flag))) break;
+            ++pf[t];
+            tc_fence_after();
+            if (lane == 0) mma_pv(tmem + Cfg::O_COL + t * HD, tmem + t * 128, ev, j == 0);
+            if (j + 1 < nt) {
+              if (!have_k && !(ok = wait_kv(ek))) break;
+              have_k = true;
+              tc_fence_after();
+              if (lane == 0) {
+                mma_s(t, ek, tmem + t * 128);
+                umma_commit(&s_full[t]);
+              }
+            } else if (lane == 0) {
+              umma_commit(&o_full[t]);
+            }
+            __syncwarp();
+          }
+          if (!ok) break;
+          if (lane == 0) {
+            umma_commit(&kv_empty[ev % ST]);
+            if (j + 1 < n) umma_commit(&kv_empty[ek % ST]);
+            if (j + 2 == n) umma_commit(q_empty);
+          }
+          __syncwarp();
+        }
+      } else {
+        if (lane == 0) {
+          mma_s(0, e, tmem + (g & 1) * 128);
+          umma_commit(&s_full[g & 1]);
+          umma_commit(&kv_empty[e % ST]);
+          if (n == 1) umma_commit(q_empty);
+        }
+        __syncwarp();
+        for (int j = 0; j < n; ++j, ++g) {
+          const int ev = e + 2 * j + 1, ek = ev + 1;
+          if (j + 1 < n) {
+            if (!(ok = wait_kv(ek))) break;
+            tc_fence_after();
+            if (lane == 0) {
+              mma_s(0, ek, tmem + ((g + 1) & 1) * 128);
+              umma_commit(&s_full[(g + 1) & 1]);
+              umma_commit(&kv_empty[ek % ST]);
+              if (j + 2 == n) umma_commit(q_empty);
+            }
+            __syncwarp();
+          }
+          if (!(ok = wait_kv(ev))) break;
+          clear_v(ev, kb0 + j, it.kv_len);
+          if (!(ok = mbar_wait_warp(&p_full[g & 1], (g >> 1) & 1, abort_flag))) break;
+          tc_fence_after();
+          if (lane == 0) {
+            mma_pv(tmem + Cfg::O_COL, tmem + (g & 1) * 128, ev, j == 0);
+            umma_commit(&o_full[0]);
+            umma_commit(&kv_empty[ev % ST]);
+          }
+          __syncwarp();
+        }
+      }
+      if (!ok) break;
+      e += 2 * n;
+    }
+  } else {
+    // -------------------------------------------------------------- softmax
+    code = kDevTimeoutEpilogue;
+    FlashItem it;
+    const int t = warp >> 2;               // tile (0 for NT 1)
+    const int r = (warp & 3) * 32 + lane;  // row of the tile = TMEM lane
+    const int tok = r / G, head = r - tok * G;
+    const uint32_t t_lane = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const uint32_t o_addr = t_lane + Cfg::O_COL + t * HD;
+    const float sc = a.scale_log2;
+    int g = 0;       // blocks so far (of this tile)
+    int done = 0;    // tiles whose result was read (NT 2)
+    while (true) {
+      if (!(ok = next_item(it)) || !it.valid) break;
+      const int qt = t * R + tok;          // token within the tile set
+      const bool live = tok < R && qt < it.qv;
+      const bool warp_live = __any_sync(0xffffffffu, live);
+      // keys [0, vis) are seen by this row
+      const int vis = live ? min(it.kv_len, it.pos0 + qt + 1) : 0;
+      const int n = (t ? it.nb[1] : it.nb[0]) - it.kb0;
+      float m = -INFINITY, l = 0.f;  // maximum (raw score) that O and l are relative to
+      for (int j = 0; j < n; ++j, ++g) {
+        const int buf = NT == 2 ? t : g & 1;
+        const uint32_t s_addr = t_lane + buf * 128;
+        if (!(ok = mbar_wait_warp(&s_full[buf], NT == 2 ? g & 1 : (g >> 1) & 1, abort_flag))) break;
+        tc_fence_after();
+        if (warp_live) {
+          uint32_t s[4][32];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(s_addr + c * 32, s[c]);
+          tmem_wait_ld();
+          const int left = vis - (it.kb0 + j) * 128;
+          if (__any_sync(0xffffffffu, live && left < 128)) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (c * 32 + i >= left) s[c][i] = 0xff800000u;  // -infinity
+          }
+          float mx[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            mx[c] = __uint_as_float(s[c][0]);
+#pragma unroll
+            for (int i = 1; i < 32; ++i) mx[c] = fmaxf(mx[c], __uint_as_float(s[c][i]));
+          }
+          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          // keep the older maximum unless the new one is 2^8 above it
+          const bool grow = live && ((top - m) * sc > 8.f || (m == -INFINITY && top > m));
+          if (__any_sync(0xffffffffu, grow)) {
+            const float mn = grow ? top : m;
+            const float corr = mn == -INFINITY ? 1.f : fa_exp2((m - mn) * sc);
+            if (j > 0) {
+              // O holds the blocks before: their last P V has to be done (with
+              // NT 2 this block's S came after it)
+              if (NT == 1 && !(ok = mbar_wait_warp(&o_full[0], (g - 1) & 1, abort_flag))) break;
+              tc_fence_after();
+#pragma unroll
+              for (int c = 0; c < HD / 32; ++c) {
+                uint32_t v[32];
+                tmem_ld_32x32b_x32(o_addr + c * 32, v);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * corr);
+                tmem_st_32x32b_x32(o_addr + c * 32, v);
+              }
+              tmem_wait_st();
+            }
+            l *= corr;
+            m = mn;
+          }
+          const float nm = m == -INFINITY ? 0.f : -m * sc;
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < 4; c += 2) {
+            uint32_t p[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const uint32_t* x = s[c + (i >> 4)] + 2 * (i & 15);
+              const float u = fa_exp2(fmaf(__uint_as_float(x[0]), sc, nm));
+              const float w = fa_exp2(fmaf(__uint_as_float(x[1]), sc, nm));
+              sum[i & 3] += u + w;
+              p[i] = pack2<T>(u, w);
+            }
+            tmem_st_32x32b_x32(s_addr + c * 16, p);
+          }
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          tmem_wait_st();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[buf]);
+      }
+      if (!ok) break;
+      if (n > 0) {
+        // the last P V of this tile; a parity wait must not be two phases
+        // behind, so the one before it first (NT 1: one phase per block)
+        if (NT == 1 && n > 1 && !(ok = mbar_wait_warp(&o_full[0], (g - 2) & 1, abort_flag))) break;
+        if (!(ok = mbar_wait_warp(&o_full[t], NT == 2 ? done & 1 : (g - 1) & 1, abort_flag))) break;
+        ++done;
+        tc_fence_after();
+      }
+      if (warp_live) {
+        const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // NaN stays NaN
+        const float l2 = l == 0.f ? -INFINITY : m * sc + log2f(l);
+        const int64_t row = it.tok0 + qt;
+        if (it.part >= 0) {
+          float* po = a.part_o + (static_cast<int64_t>(it.part) * 128 + r) * HD;
+#pragma unroll
+          for (int c = 0; c < HD / 32; ++c) {
+            uint32_t v[32];
+            tmem_ld_32x32b_x32(o_addr + c * 32, v);
+            tmem_wait_ld();
+            if (live) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                *reinterpret_cast<float4*>(po + c * 32 + 4 * i) =
+                    l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
+                             : make_float4(__uint_as_float(v[4 * i]) * inv, __uint_as_float(v[4 * i + 1]) * inv,
+                                           __uint_as_float(v[4 * i + 2]) * inv, __uint_as_float(v[4 * i + 3]) * inv);
+            }
+          }
+          if (live) a.part_l[it.part * 128 + r] = l2;
+        } else {
+          const int h = it.kvh * G + head;
+          T* o = static_cast<T*>(a.out) + row * a.ot + h * a.oh;
+#pragma unroll
+          for (int c = 0; c < HD / 32; ++c) {
+            uint32_t v[32];
+            if (n > 0) {
+              tmem_ld_32x32b_x32(o_addr + c * 32, v);
+              tmem_wait_ld();
+            }
+            if (live) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                if (c * 32 + 8 * i >= a.head_dim) break;
+                uint4 w = make_uint4(0, 0, 0, 0);  // a row that sees nothing
+                if (l != 0.f) {
+                  w.x = pack2<T>(__uint_as_float(v[8 * i]) * inv, __uint_as_float(v[8 * i + 1]) * inv);
+                  w.y = pack2<T>(__uint_as_float(v[8 * i + 2]) * inv, __uint_as_float(v[8 * i + 3]) * inv);
+                  w.z = pack2<T>(__uint_as_float(v[8 * i + 4]) * inv, __uint_as_float(v[8 * i + 5]) * inv);
+                  w.w = pack2<T>(__uint_as_float(v[8 * i + 6]) * inv, __uint_as_float(v[8 * i + 7]) * inv);
+                }
+                *reinterpret_cast<uint4*>(o + c * 32 + 8 * i) = w;
+              }
+            }
+          }
+          if (live && a.lse) a.lse[row * a.q_heads + h] = l2 * 0.693147180559945309f;
+        }
+      }
+      tc_fence_before();
+    }
+  }
+  if (!ok) {
+    if (lane == 0) report(&g_op_status, code);
+    *abort_flag = 1;
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) {
+    // let copies and MMAs in flight land before the memory goes away
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 2000000ull) {
+    }
+  }
+  if (warp == W_MMA) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// Joins the partial results of the tiles that the even split cut, and clears
+// the rows that see no key.  One warp per (token, query head).
+template <int HD, typename T>
+__global__ void flash_join_kernel(const __grid_constant__ FlashArgs a) {
+  const int64_t w = (blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x) >> 5;
+  const int lane = threadIdx.x & 31;
+  if (w >= static_cast<int64_t>(a.tokens) * a.q_heads) return;
+  const int t = static_cast<int>(w / a.q_heads), h = static_cast<int>(w % a.q_heads);
+  // last sequence that begins at or before t
+  int lo = 0, hi = a.nseq;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (a.cu[mid] <= t) lo = mid;
+    else hi = mid;
+  }
+  const FlashSeq q = flash_seq(a, lo);
+  if (t < q.begin || t >= q.end) return;
+  const int len = q.end - q.begin, R = a.rows_tok;
+  const int tile = (t - q.begin) / R, kvh = h / a.group, row = (t - q.begin - tile * R) * a.group + h % a.group;
+  int at = a.plan[1 + lo], nb = 0;
+  for (int i = 0; i <= tile; ++i) {
+    at += nb * a.kv_heads;
+    nb = blocks_seen(q.kv_len - len + i * R, min(R, len - i * R), q.kv_len);
+  }
+  at += nb * kvh;
+  T* out = static_cast<T*>(a.out) + t * a.ot + h * a.oh;
+  if (nb == 0) {
+    for (int i = lane; i < a.head_dim; i += 32) out[i] = T(0.f);
+    if (lane == 0 && a.lse) a.lse[w] = -INFINITY;
+    return;
+  }
+  const int chunk = max(a.plan[0], 1);
+  const int c0 = at / chunk, c1 = min((at + nb - 1) / chunk, kMaxCtas - 1);
+  if (c0 == c1) return;  // one CTA had all of it
+  const int p0 = 2 * c0 + (at == c0 * chunk ? 0 : 1);  // later parts are their CTA's first
+  float m = -INFINITY;
+  for (int c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, a.part_l[(c == c0 ? p0 : 2 * c) * 128 + row]);
+#pragma unroll
+  for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+  float sum = 0.f, o[HD / 32] = {};
+  for (int c = c0; c <= c1; ++c) {
+    const int p = c == c0 ? p0 : 2 * c;
+    const float l2 = a.part_l[p * 128 + row];
+    const float x = l2 == -INFINITY ? 0.f : fa_exp2(l2 - m);
+    sum += x;
+    const float* po = a.part_o + (static_cast<int64_t>(p) * 128 + row) * HD;
+#pragma unroll
+    for (int i = 0; i < HD / 32; ++i) o[i] += x * po[lane + 32 * i];
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+  for (int i = 0; i < HD / 32; ++i)
+    if (lane + 32 * i < a.head_dim) {
+      const uint32_t v = pack2<T>(o[i] * inv, 0.f);
+      reinterpret_cast<uint16_t*>(out)[lane + 32 * i] = static_cast<uint16_t>(v);
+    }
+  if (lane == 0 && a.lse) a.lse[w] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * 0.693147180559945309f;
+}
+
+}  // namespace ec

@@ -449,8 +449,10 @@ extern "C" int ec_kv_open(void* k, void* v, int dtype, int layers, int pages, in
     return set_error(EC_EINVAL, "page_size %d (supported: 16, 32, 64, 128)", page_size);
   if (head_dim < 8 || head_dim > 128 || head_dim % 8)
     return set_error(EC_EINVAL, "head_dim %d (supported: multiples of 8 up to 128)", head_dim);
-  if (static_cast<int64_t>(table_width) * page_size > INT32_MAX)
-    return set_error(EC_EINVAL, "a table row of %d pages passes 2^31 tokens", table_width);
+  if (static_cast<int64_t>(table_width) * page_size > (1 << 30))
+    return set_error(EC_EINVAL, "a table row of %d pages passes 2^30 tokens", table_width);
+  if (static_cast<int64_t>(layers) * pages > (1 << 30))
+    return set_error(EC_EINVAL, "%d layers of %d pages pass 2^30 pages", layers, pages);
   if (!op_aligned(k, 16) || !op_aligned(v, 16) || !op_aligned(work, 16))
     return set_error(EC_EINVAL, "pages and work must be 16-byte aligned");
   if (!op_aligned(tables, 4) || !op_aligned(lens, 4) || !op_aligned(refs, 4))

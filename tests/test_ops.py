@@ -106,7 +106,8 @@ def test_cache_refusals():
     refused(open_(pages=(1 << 20) + 1)[0], "cache shape")
     refused(open_(page=48)[0], "page_size")
     refused(open_(hd=132)[0], "head_dim")
-    refused(open_(width=1 << 24, page=128)[0], "2^31")
+    refused(open_(width=1 << 24, page=128)[0], "2^30")
+    refused(open_(layers=65536, pages=1 << 20)[0], "2^30")
     refused(open_(k=FAKE + 8)[0], "16-byte")
     refused(open_(size=16)[0], "work holds")
     refused(L().ec_kv_close(0), "unknown cache handle")
