@@ -122,6 +122,7 @@ int run_attention(const AttnOp& op, int num_sms, cudaStream_t st) {
   if (!ok) return set_error(EC_EINVAL, "the attention's strides cannot be described to the TMA");
   FlashArgs a{};
   a.out = const_cast<void*>(op.out.p), a.ot = op.out.token, a.oh = op.out.head;
+  a.wide = op_aligned(a.out, 32) && a.ot % 16 == 0 && a.oh % 16 == 0 && op.head_dim % 16 == 0;
   a.lse = op.lse;
   a.cu = op.cu, a.slots = op.slots;
   a.tokens = static_cast<int>(op.tokens), a.nseq = op.nseq;

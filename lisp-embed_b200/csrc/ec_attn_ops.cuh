@@ -49,6 +49,7 @@ struct FlashArgs {
   int q_heads, kv_heads, head_dim;
   float scale_log2;
   int paged;
+  int wide;                // out rows in 32-byte pieces
   int even;                // 1: the blocks are split evenly over the CTAs
   int min_chunk;           // blocks a CTA takes at least
   float* part_o;           // [2 * CTAs][128][HD] partial results of cut tiles
@@ -68,6 +69,10 @@ struct FlashItem {
   int nb[2];      // end block of each tile
   int part;       // partial result, -1: the whole of the tile's keys
 };
+
+// one of this many pairs of exponentials goes to the FMA units instead of the
+// special-function unit
+constexpr int kFmaEvery = 4;
 
 template <int HD, int NT>
 struct FlashCfg {
@@ -95,6 +100,34 @@ template <>
 __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
   const __half2 v = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// 2^x for two values on the FMA units: x = n + f with n the nearest integer,
+// 2^f by a minimax polynomial of degree 5 on [-1/2, 1/2] (Remez; 7.5e-8 from
+// the truth, 2.4e-7 with the roundings of its evaluation), 2^n put together as
+// an exponent.  x <= -127 gives 0; NaN stays NaN.  For x < 128.
+__device__ __forceinline__ float2 exp2_fma(float2 x) {
+  const float2 magic = make_float2(12582912.f + 127.f, 12582912.f + 127.f);  // 1.5 * 2^23: n + 127 in the low bits
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.x));  // -127
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.y));
+  const float2 t = __fadd2_rn(x, magic);
+  const float2 n = __fadd2_rn(t, make_float2(-magic.x, -magic.y));
+  const float2 f = __ffma2_rn(n, make_float2(-1.f, -1.f), x);
+  auto c = [](float v) { return make_float2(v, v); };
+  float2 p = __ffma2_rn(f, c(0.0013276472454890609f), c(0.009675540961325169f));
+  p = __ffma2_rn(f, p, c(0.05550713092088699f));
+  p = __ffma2_rn(f, p, c(0.24022120237350464f));
+  p = __ffma2_rn(f, p, c(0.6931469440460205f));
+  p = __ffma2_rn(f, p, c(1.0000001192092896f));
+  return __fmul2_rn(p, make_float2(__uint_as_float(__float_as_uint(t.x) << 23),
+                                   __uint_as_float(__float_as_uint(t.y) << 23)));
+}
+
+// 32 bytes to a 32-byte aligned address
+__device__ __forceinline__ void store32(void* p, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
 }
 
 // key blocks that the first n tokens of a sequence's queries see
@@ -127,21 +160,8 @@ __device__ __forceinline__ FlashSeq flash_seq(const FlashArgs& a, int s) {
 // ------------------------------------------------------------- work lists --
 // Without a split: slot u of the list is the tile set f(s) + i of sequence s,
 // f(s) = cu[s] / BT + s for BT tokens per set.  f leaves at least
-// ceil(len / BT) slots to every sequence and needs no prefix sum; a sequence
-// is found by a 32-way search.
-__device__ __forceinline__ int flash_find(const FlashArgs& a, int bt, int u, int lane) {
-  int lo = 0, hi = a.nseq;  // f(lo) <= u, f(hi) > u (or hi = nseq)
-  while (hi - lo > 1) {
-    const int step = (hi - lo + 31) / 32;
-    const int s = lo + lane * step;
-    const bool le = s < hi && min(max(a.cu[s], 0), a.tokens) / bt + s <= u;
-    const unsigned m = __ballot_sync(0xffffffffu, le);
-    const int k = m ? 31 - __clz(m) : 0;
-    hi = min(hi, lo + (k + 1) * step);
-    lo = lo + k * step;
-  }
-  return lo;
-}
+// ceil(len / BT) slots to every sequence and needs no prefix sum; a slot's
+// sequence is found by bisection.
 
 template <int HD, int NT, typename T>
 __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
@@ -169,14 +189,15 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
   uint64_t* kv_empty = kv_full + ST;
   uint64_t* s_full = kv_empty + ST;   // [2] tile (NT 2) or buffer (NT 1)
   uint64_t* p_full = s_full + 2;      // [2]
-  uint64_t* o_full = p_full + 2;      // [2]
+  uint64_t* p_half = p_full + 2;      // [2] the first 64 keys' P
+  uint64_t* o_full = p_half + 2;      // [2]
   uint64_t* i_full = o_full + 2;      // [2]
   uint64_t* i_empty = i_full + 2;     // [2]
   FlashItem* items = reinterpret_cast<FlashItem*>(i_empty + 2);  // [2]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(items + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* prefix = reinterpret_cast<int*>(tail + 1024);  // [nseq + 1] of an even split
-  static_assert(8 * (2 + 2 * ST + 10) + 2 * sizeof(FlashItem) + 8 <= 1024, "tail");
+  static_assert(8 * (2 + 2 * ST + 12) + 2 * sizeof(FlashItem) + 8 <= 1024, "tail");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -189,6 +210,7 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
+      mbar_init(&p_half[i], 4);
       mbar_init(&o_full[i], 1);
       mbar_init(&i_full[i], 1);
       mbar_init(&i_empty[i], READERS);
@@ -228,10 +250,10 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
   if (warp == W_LIST) {
     // ------------------------------------------------------------ work list
     int n = 0;
-    auto publish = [&](const FlashItem& it) -> bool {
+    auto publish = [&](const FlashItem& it, int from) -> bool {  // lane `from`'s entry
       const int b = n & 1;
       if (!mbar_wait_warp(&i_empty[b], ((n >> 1) & 1) ^ 1, abort_flag)) return false;
-      if (lane == 0) {
+      if (lane == from) {
         items[b] = it;
         mbar_arrive(&i_full[b]);
       }
@@ -302,7 +324,7 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
             it.nb[0] = min(nb, end - at);
             it.nb[1] = 0;
             it.part = it.kb0 == 0 && it.nb[0] == nb ? -1 : 2 * static_cast<int>(blockIdx.x) + (w == begin ? 0 : 1);
-            ok = publish(it);
+            ok = publish(it, 0);
             w = at + it.nb[0];
           }
         }
@@ -310,36 +332,45 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
       // tiles that see no key are nobody's blocks: their rows are cleared by
       // the join
     } else {
+      // every lane looks up one of the next 32 candidates
       const int64_t slots = a.tokens / BT + a.nseq;
       const int64_t all = slots * a.kv_heads;
-      int64_t round = 0;
-      for (int64_t t0 = 0; ok && t0 < all; t0 += gridDim.x, ++round) {
+      for (int64_t t0 = 0; ok && t0 < all; t0 += 32 * static_cast<int64_t>(gridDim.x)) {
         // late (long) tile sets first; the order turns round every pass, so
         // that no CTA gets the longest of each
-        const int64_t t = t0 + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-        if (t >= all) continue;
-        const int u = static_cast<int>(slots - 1 - t / a.kv_heads);
-        const int s = flash_find(a, BT, u, lane);
-        const FlashSeq q = flash_seq(a, s);
-        const int len = q.end - q.begin;
-        const int64_t q0 = static_cast<int64_t>(u - (q.begin / BT + s)) * BT;
-        if (q0 < 0 || q0 >= len) continue;
-        it.valid = 1;
-        it.tok0 = q.begin + static_cast<int>(q0);
-        it.qv = min(BT, len - static_cast<int>(q0));
-        it.kvh = static_cast<int>(t % a.kv_heads);
-        it.pos0 = q.kv_len - len + static_cast<int>(q0);
-        it.kv_len = q.kv_len;
-        it.kbase = q.kbase;
-        it.kb0 = 0;
-        it.nb[0] = blocks_seen(it.pos0, min(R, it.qv), q.kv_len);
-        it.nb[1] = NT == 2 && it.qv > R ? blocks_seen(it.pos0, it.qv, q.kv_len) : 0;
-        it.part = -1;
-        ok = publish(it);
+        const int64_t t = t0 + lane * static_cast<int64_t>(gridDim.x) +
+                          ((lane & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+        it.valid = 0;
+        if (t < all) {
+          const int u = static_cast<int>(slots - 1 - t / a.kv_heads);
+          int lo = 0, hi = a.nseq;  // last sequence with f <= u
+          while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (min(max(a.cu[mid], 0), a.tokens) / BT + mid <= u) lo = mid;
+            else hi = mid;
+          }
+          const FlashSeq q = flash_seq(a, lo);
+          const int len = q.end - q.begin;
+          const int64_t q0 = static_cast<int64_t>(u - (q.begin / BT + lo)) * BT;
+          if (q0 >= 0 && q0 < len) {
+            it.valid = 1;
+            it.tok0 = q.begin + static_cast<int>(q0);
+            it.qv = min(BT, len - static_cast<int>(q0));
+            it.kvh = static_cast<int>(t % a.kv_heads);
+            it.pos0 = q.kv_len - len + static_cast<int>(q0);
+            it.kv_len = q.kv_len;
+            it.kbase = q.kbase;
+            it.kb0 = 0;
+            it.nb[0] = blocks_seen(it.pos0, min(R, it.qv), q.kv_len);
+            it.nb[1] = NT == 2 && it.qv > R ? blocks_seen(it.pos0, it.qv, q.kv_len) : 0;
+            it.part = -1;
+          }
+        }
+        for (unsigned m = __ballot_sync(0xffffffffu, it.valid); ok && m; m &= m - 1) ok = publish(it, __ffs(m) - 1);
       }
     }
     it.valid = 0;
-    if (ok) ok = publish(it);
+    if (ok) ok = publish(it, 0);
   } else if (warp == W_LOAD) {
     // ---------------------------------------------------------------- loads
     code = kDevTimeoutProducer;
@@ -436,10 +467,10 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
         umma_f16(d, desc_sw128_kmajor(qa + off), desc_sw128_kmajor(ka + off), IDESC_S, kk > 0);
       }
     };
-    auto mma_pv = [&](uint32_t d, uint32_t p, int entry, bool first) {
+    auto mma_pv = [&](uint32_t d, uint32_t p, int entry, bool first, int half) {
       const uint32_t va = kv_addr + (entry % ST) * Cfg::TILE;
 #pragma unroll
-      for (int kk = 0; kk < 8; ++kk)
+      for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
         umma_f16_ts(d, p + kk * 8, desc_mnmajor<false>(va + kk * 2048, Cfg::ATOM), IDESC_PV, !first || kk > 0);
     };
     // V rows behind the sequence's keys: another sequence's rows, or what a
@@ -489,10 +520,14 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
               clear_v(ev, kb0 + j, it.kv_len);
               have_v = true;
             }
+            if (!(ok = mbar_wait_warp(&p_half[t], pf[t] & 1, abort_flag))) break;
+            tc_fence_after();
+            if (lane == 0) mma_pv(tmem + Cfg::O_COL + t * HD, tmem + t * 128, ev, j == 0, 0);
+            __syncwarp();
             if (!(ok = mbar_wait_warp(&p_full[t], pf[t] & 1, abort_flag))) break;
             ++pf[t];
             tc_fence_after();
-            if (lane == 0) mma_pv(tmem + Cfg::O_COL + t * HD, tmem + t * 128, ev, j == 0);
+            if (lane == 0) mma_pv(tmem + Cfg::O_COL + t * HD, tmem + t * 128, ev, false, 1);
             if (j + 1 < nt) {
               if (!have_k && !(ok = wait_kv(ek))) break;
               have_k = true;
@@ -537,10 +572,14 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
           }
           if (!(ok = wait_kv(ev))) break;
           clear_v(ev, kb0 + j, it.kv_len);
+          if (!(ok = mbar_wait_warp(&p_half[g & 1], (g >> 1) & 1, abort_flag))) break;
+          tc_fence_after();
+          if (lane == 0) mma_pv(tmem + Cfg::O_COL, tmem + (g & 1) * 128, ev, j == 0, 0);
+          __syncwarp();
           if (!(ok = mbar_wait_warp(&p_full[g & 1], (g >> 1) & 1, abort_flag))) break;
           tc_fence_after();
           if (lane == 0) {
-            mma_pv(tmem + Cfg::O_COL, tmem + (g & 1) * 128, ev, j == 0);
+            mma_pv(tmem + Cfg::O_COL, tmem + (g & 1) * 128, ev, false, 1);
             umma_commit(&o_full[0]);
             umma_commit(&kv_empty[ev % ST]);
           }
@@ -582,13 +621,16 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
           for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(s_addr + c * 32, s[c]);
           tmem_wait_ld();
           const int left = vis - (it.kb0 + j) * 128;
-          if (__any_sync(0xffffffffu, live && left < 128)) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
+          const bool cut = __any_sync(0xffffffffu, live && left < 128);
+          auto mask = [&](int c) {
+            if (cut) {
 #pragma unroll
               for (int i = 0; i < 32; ++i)
                 if (c * 32 + i >= left) s[c][i] = 0xff800000u;  // -infinity
-          }
+            }
+          };
+#pragma unroll
+          for (int c = 0; c < 4; ++c) mask(c);
           float mx[4];
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
@@ -622,22 +664,40 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
             m = mn;
           }
           const float nm = m == -INFINITY ? 0.f : -m * sc;
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+          float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+          const float2 sc2 = make_float2(sc, sc), nm2 = make_float2(nm, nm);
 #pragma unroll
           for (int c = 0; c < 4; c += 2) {
             uint32_t p[32];
+            if (c == 2) {
+              // the second half's scores are read again: holding all of them
+              // next to the first half's P takes more registers than there are
+              tmem_ld_32x32b_x32(s_addr + 64, s[2]);
+              tmem_ld_32x32b_x32(s_addr + 96, s[3]);
+              tmem_wait_ld();
+              mask(2);
+              mask(3);
+            }
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
               const uint32_t* x = s[c + (i >> 4)] + 2 * (i & 15);
-              const float u = fa_exp2(fmaf(__uint_as_float(x[0]), sc, nm));
-              const float w = fa_exp2(fmaf(__uint_as_float(x[1]), sc, nm));
-              sum[i & 3] += u + w;
-              p[i] = pack2<T>(u, w);
+              const float2 y = __ffma2_rn(make_float2(__uint_as_float(x[0]), __uint_as_float(x[1])), sc2, nm2);
+              const float2 w = (i % kFmaEvery) == kFmaEvery - 1 ? exp2_fma(y) : make_float2(fa_exp2(y.x), fa_exp2(y.y));
+              sum[i & 1] = __fadd2_rn(sum[i & 1], w);
+              p[i] = pack2<T>(w.x, w.y);
             }
             tmem_st_32x32b_x32(s_addr + c * 16, p);
+            if (c == 0) {
+              tmem_wait_st();
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&p_half[buf]);
+            }
           }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
           tmem_wait_st();
+        } else if (lane == 0) {
+          mbar_arrive(&p_half[buf]);
         }
         tc_fence_before();
         __syncwarp();
@@ -684,17 +744,18 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
               tmem_wait_ld();
             }
             if (live) {
+              uint32_t w[16];
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                if (c * 32 + 8 * i >= a.head_dim) break;
-                uint4 w = make_uint4(0, 0, 0, 0);  // a row that sees nothing
-                if (l != 0.f) {
-                  w.x = pack2<T>(__uint_as_float(v[8 * i]) * inv, __uint_as_float(v[8 * i + 1]) * inv);
-                  w.y = pack2<T>(__uint_as_float(v[8 * i + 2]) * inv, __uint_as_float(v[8 * i + 3]) * inv);
-                  w.z = pack2<T>(__uint_as_float(v[8 * i + 4]) * inv, __uint_as_float(v[8 * i + 5]) * inv);
-                  w.w = pack2<T>(__uint_as_float(v[8 * i + 6]) * inv, __uint_as_float(v[8 * i + 7]) * inv);
-                }
-                *reinterpret_cast<uint4*>(o + c * 32 + 8 * i) = w;
+              for (int i = 0; i < 16; ++i)  // 0: a row that sees nothing
+                w[i] = l == 0.f ? 0u : pack2<T>(__uint_as_float(v[2 * i]) * inv, __uint_as_float(v[2 * i + 1]) * inv);
+              if (a.wide) {
+                if (c * 32 < a.head_dim) store32(o + c * 32, w);
+                if (c * 32 + 16 < a.head_dim) store32(o + c * 32 + 16, w + 8);
+              } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  if (c * 32 + 8 * i < a.head_dim)
+                    *reinterpret_cast<uint4*>(o + c * 32 + 8 * i) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
               }
             }
           }
