@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
   uint64_t* s_full = kv_empty + ST;   // [2] tile (NT 2) or buffer (NT 1)
   uint64_t* p_full = s_full + 2;      // [2]
   uint64_t* p_half = p_full + 2;      // [2] the first 64 keys' P
-  uint64_t* o_full = p_half + 2;      // [2]
+  uint64_t* o_full = p_half + 2;      // [2] tile (NT 2), or even / odd blocks (NT 1)
   uint64_t* i_full = o_full + 2;      // [2]
   uint64_t* i_empty = i_full + 2;     // [2]
   FlashItem* items = reinterpret_cast<FlashItem*>(i_empty + 2);  // [2]
@@ -382,33 +382,17 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
       if (!(ok = next_item(it)) || !it.valid) break;
       const int nb = max(it.nb[0], NT == 2 ? it.nb[1] : 0);
       if (nb <= it.kb0) continue;
-      if (!(ok = mbar_wait_warp(q_empty, q_ph ^ 1, abort_flag))) break;
-      q_ph ^= 1;
-      if (lane == 0) {
-        // rows past the tokens of the call are filled with zeros
-        mbar_arrive_expect_tx(q_full, NT * AT * static_cast<uint32_t>(G * R) * 128u);
-        for (int t = 0; t < NT; ++t)
-          for (int c = 0; c < AT; ++c)
-            asm volatile(
-                "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], "
-                "[%2];" ::"r"(smem_u32(sQ + t * Cfg::TILE + c * Cfg::ATOM)),
-                "l"(reinterpret_cast<uint64_t>(&tm_q)), "r"(smem_u32(q_full)), "r"(c * 64), "r"(it.kvh * G),
-                "r"(it.tok0 + t * R)
-                : "memory");
-      }
-      __syncwarp();
       const int32_t* table = a.tables + static_cast<int64_t>(it.kbase) * a.width;
       const int in_use = a.paged ? (it.kv_len + a.page_size - 1) / a.page_size : 0;
       // pages of the next 32 table entries, one per lane; an entry that is
       // none reads past the pages, which fills the tile with zeros
-      int first = it.kb0 * ppb, page = 0, ahead = 0;
+      int first = it.kb0 * ppb;
       auto fetch = [&](int e) -> int {
         int p = -1;
         if (a.paged && e < in_use) p = table[e];
         return p >= 0 && p < a.pages ? a.page0 + p : a.page_end;
       };
-      page = fetch(first + lane);
-      ahead = fetch(first + 32 + lane);
+      int page = fetch(first + lane), ahead = fetch(first + 32 + lane);
       for (int j = it.kb0; ok && j < nb; ++j) {
         if (a.paged && j * ppb - first == 32) {
           first += 32;
@@ -418,30 +402,59 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
           if (!(ok = mbar_wait_warp(&kv_empty[st], ph ^ 1, abort_flag))) break;
-          uint8_t* dst = sKV + st * Cfg::TILE;
-          if (lane == 0) mbar_arrive_expect_tx(&kv_full[st], Cfg::TILE);
-          __syncwarp();
+          const uint32_t dst = smem_u32(sKV + st * Cfg::TILE), bar = smem_u32(&kv_full[st]);
           const uint64_t map = reinterpret_cast<uint64_t>(kv ? &tm_v : &tm_k);
-          if (a.paged) {
-            const int p = __shfl_sync(0xffffffffu, page, (j * ppb - first + lane / AT) & 31);
-            if (lane < ppb * AT)
-              asm volatile(
-                  "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], "
-                  "[%1, {%3, %4, %5, %6}], [%2];" ::"r"(
-                      smem_u32(dst + (lane % AT) * Cfg::ATOM + (lane / AT) * a.page_size * 128)),
-                  "l"(map), "r"(smem_u32(&kv_full[st])), "r"((lane % AT) * 64), "r"(it.kvh), "r"(0), "r"(p)
-                  : "memory");
-          } else if (lane < AT) {
-            asm volatile(
-                "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], "
-                "[%2];" ::"r"(smem_u32(dst + lane * Cfg::ATOM)),
-                "l"(map), "r"(smem_u32(&kv_full[st])), "r"(lane * 64), "r"(it.kvh), "r"(it.kbase + j * 128)
-                : "memory");
-          }
+          if (elect_one()) mbar_arrive_expect_tx(&kv_full[st], Cfg::TILE);
           __syncwarp();
+          if (a.paged) {
+            for (int i = 0; i < ppb; ++i) {
+              const int p = __shfl_sync(0xffffffffu, page, j * ppb - first + i);
+              if (elect_one()) {
+#pragma unroll
+                for (int c = 0; c < AT; ++c)
+                  asm volatile(
+                      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], "
+                      "[%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst + c * Cfg::ATOM + i * a.page_size * 128),
+                      "l"(map), "r"(bar), "r"(c * 64), "r"(it.kvh), "r"(0), "r"(p)
+                      : "memory");
+              }
+              __syncwarp();
+            }
+          } else {
+            if (elect_one()) {
+#pragma unroll
+              for (int c = 0; c < AT; ++c)
+                asm volatile(
+                    "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], "
+                    "[%1, {%3, %4, %5}], [%2];" ::"r"(dst + c * Cfg::ATOM),
+                    "l"(map), "r"(bar), "r"(c * 64), "r"(it.kvh), "r"(it.kbase + j * 128)
+                    : "memory");
+            }
+            __syncwarp();
+          }
           if (++st == ST) {
             st = 0;
             ph ^= 1;
+          }
+          if (j == it.kb0 && kv == 0) {
+            // the queries, once the tiles before have no more use for theirs;
+            // rows past the tokens of the call are filled with zeros
+            if (!(ok = mbar_wait_warp(q_empty, q_ph ^ 1, abort_flag))) break;
+            q_ph ^= 1;
+            if (elect_one()) {
+              mbar_arrive_expect_tx(q_full, NT * AT * static_cast<uint32_t>(G * R) * 128u);
+#pragma unroll
+              for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int c = 0; c < AT; ++c)
+                  asm volatile(
+                      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], "
+                      "[%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(sQ + t * Cfg::TILE + c * Cfg::ATOM)),
+                      "l"(reinterpret_cast<uint64_t>(&tm_q)), "r"(smem_u32(q_full)), "r"(c * 64), "r"(it.kvh * G),
+                      "r"(it.tok0 + t * R)
+                      : "memory");
+            }
+            __syncwarp();
           }
         }
       }
@@ -449,146 +462,134 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
     }
   } else if (warp == W_MMA) {
     // ----------------------------------------------------------------- MMAs
+    // one thread: operands of tcgen05 instructions are warp-uniform, which the
+    // compiler knows of the elected thread only
     code = kDevTimeoutMma;
-    FlashItem it;
-    int e = 0;  // entries of the K / V ring used: K of block j is entry base + 2 j
-    uint32_t q_ph = 0;
-    int pf[2] = {0, 0};  // P's waited for, per tile / buffer
-    int g = 0;           // blocks (NT 1)
-    const uint32_t q_addr = smem_u32(sQ), kv_addr = smem_u32(sKV);
-    auto wait_kv = [&](int entry) -> bool {
-      return mbar_wait_warp(&kv_full[entry % ST], (entry / ST) & 1, abort_flag);
-    };
-    auto mma_s = [&](int t, int entry, uint32_t d) {
-      const uint32_t qa = q_addr + t * Cfg::TILE, ka = kv_addr + (entry % ST) * Cfg::TILE;
+    if (elect_one()) {
+      int st = 0;            // stage of the next K / V tile
+      uint32_t ph = 0;       // its phase
+      uint32_t q_ph = 0;
+      uint32_t pf[2] = {0, 0};  // P's waited for, per tile
+      uint32_t g = 0;           // blocks (NT 1)
+      const uint64_t dq = desc_sw128_kmajor(smem_u32(sQ));
+      const uint64_t dk = desc_sw128_kmajor(smem_u32(sKV));
+      const uint64_t dv = desc_mnmajor<false>(smem_u32(sKV), Cfg::ATOM);
+      auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+        const bool fine = mbar_wait(bar, parity, abort_flag);
+        tc_fence_after();
+        return fine;
+      };
+      auto advance = [&] {
+        if (++st == ST) {
+          st = 0;
+          ph ^= 1;
+        }
+      };
+      auto mma_s = [&](int t, int stage, uint32_t d) {
+        const uint64_t q = dq + t * (Cfg::TILE >> 4), k = dk + stage * (Cfg::TILE >> 4);
 #pragma unroll
-      for (int kk = 0; kk < HD / 16; ++kk) {
-        const uint32_t off = (kk >> 2) * Cfg::ATOM + (kk & 3) * 32;
-        umma_f16(d, desc_sw128_kmajor(qa + off), desc_sw128_kmajor(ka + off), IDESC_S, kk > 0);
-      }
-    };
-    auto mma_pv = [&](uint32_t d, uint32_t p, int entry, bool first, int half) {
-      const uint32_t va = kv_addr + (entry % ST) * Cfg::TILE;
+        for (int kk = 0; kk < HD / 16; ++kk) {
+          const uint32_t off = ((kk >> 2) * Cfg::ATOM + (kk & 3) * 32) >> 4;
+          umma_f16(d, q + off, k + off, IDESC_S, kk > 0);
+        }
+      };
+      auto mma_pv = [&](uint32_t d, uint32_t p, int stage, bool first, int half) {
+        const uint64_t v = dv + stage * (Cfg::TILE >> 4);
 #pragma unroll
-      for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
-        umma_f16_ts(d, p + kk * 8, desc_mnmajor<false>(va + kk * 2048, Cfg::ATOM), IDESC_PV, !first || kk > 0);
-    };
-    // V rows behind the sequence's keys: another sequence's rows, or what a
-    // page held before.  Their probabilities are 0, and 0 * NaN would not be.
-    auto clear_v = [&](int entry, int j, int kv_len) {
-      const int from = kv_len - j * 128;
-      if (from >= 128) return;
-      uint8_t* v = sKV + (entry % ST) * Cfg::TILE;
-      for (int i = from * 8 + lane; i < 1024; i += 32) {
-#pragma unroll
-        for (int c = 0; c < AT; ++c) *reinterpret_cast<uint4*>(v + c * Cfg::ATOM + i * 16) = make_uint4(0, 0, 0, 0);
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-    };
-    while (true) {
-      if (!(ok = next_item(it)) || !it.valid) break;
-      const int kb0 = it.kb0;
-      const int n0 = it.nb[0] - kb0, n1 = NT == 2 ? it.nb[1] - kb0 : 0, n = max(n0, n1);
-      if (n <= 0) continue;
-      if (!(ok = mbar_wait_warp(q_full, q_ph, abort_flag)) || !(ok = wait_kv(e))) break;
-      q_ph ^= 1;
-      tc_fence_after();
-      if (NT == 2) {
-        if (lane == 0) {
+        for (int kk = 0; kk < 4; ++kk)
+          umma_f16_ts(d, p + (4 * half + kk) * 8, v + (4 * half + kk) * (2048 >> 4), IDESC_PV,
+                      kk > 0 || half > 0 || !first);
+      };
+      while (true) {
+        const int b = it_n & 1;
+        if (!(ok = mbar_wait(&i_full[b], (it_n >> 1) & 1, abort_flag))) break;
+        const int valid = items[b].valid, kb0 = items[b].kb0;
+        const int n0 = items[b].nb[0] - kb0, n1 = NT == 2 ? items[b].nb[1] - kb0 : 0, n = max(n0, n1);
+        mbar_arrive(&i_empty[b]);
+        ++it_n;
+        if (!valid) break;
+        if (n <= 0) continue;
+        if (!(ok = wait(q_full, q_ph)) || !(ok = wait(&kv_full[st], ph))) break;
+        q_ph ^= 1;
+        if constexpr (NT == 2) {
           if (n0 > 0) {
-            mma_s(0, e, tmem);
+            mma_s(0, st, tmem);
             umma_commit(&s_full[0]);
           }
           if (n1 > 0) {
-            mma_s(1, e, tmem + 128);
+            mma_s(1, st, tmem + 128);
             umma_commit(&s_full[1]);
           }
-          umma_commit(&kv_empty[e % ST]);
+          umma_commit(&kv_empty[st]);
           if (n == 1) umma_commit(q_empty);
-        }
-        __syncwarp();
-        for (int j = 0; ok && j < n; ++j) {
-          const int ev = e + 2 * j + 1, ek = ev + 1;
-          bool have_v = false, have_k = false;
+          advance();
+          for (int j = 0; ok && j < n; ++j) {
+            const int sv = st;
+            const uint32_t phv = ph;
+            advance();
+            bool have_v = false, have_k = false;
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            const int nt = t ? n1 : n0;
-            if (!ok || j >= nt) continue;
-            if (!have_v) {
-              if (!(ok = wait_kv(ev))) break;
-              clear_v(ev, kb0 + j, it.kv_len);
+            for (int t = 0; t < 2; ++t) {
+              const int nt = t ? n1 : n0;
+              if (!ok || j >= nt) continue;
+              if (!have_v && !(ok = wait(&kv_full[sv], phv))) break;
               have_v = true;
-            }
-            if (!(ok = mbar_wait_warp(&p_half[t], pf[t] & 1, abort_flag))) break;
-            tc_fence_after();
-            if (lane == 0) mma_pv(tmem + Cfg::O_COL + t * HD, tmem + t * 128, ev, j == 0, 0);
-            __syncwarp();
-            if (!(ok = mbar_wait_warp(&p_full[t], pf[t] & 1, abort_flag))) break;
-            ++pf[t];
-            tc_fence_after();
-            if (lane == 0) mma_pv(tmem + Cfg::O_COL + t * HD, tmem + t * 128, ev, false, 1);
-            if (j + 1 < nt) {
-              if (!have_k && !(ok = wait_kv(ek))) break;
-              have_k = true;
-              tc_fence_after();
-              if (lane == 0) {
-                mma_s(t, ek, tmem + t * 128);
+              if (!(ok = wait(&p_half[t], pf[t] & 1))) break;
+              mma_pv(tmem + Cfg::O_COL + t * HD, tmem + t * 128, sv, j == 0, 0);
+              if (!(ok = wait(&p_full[t], pf[t] & 1))) break;
+              ++pf[t];
+              mma_pv(tmem + Cfg::O_COL + t * HD, tmem + t * 128, sv, false, 1);
+              if (j + 1 < nt) {
+                if (!have_k && !(ok = wait(&kv_full[st], ph))) break;
+                have_k = true;
+                mma_s(t, st, tmem + t * 128);
                 umma_commit(&s_full[t]);
+              } else {
+                umma_commit(&o_full[t]);
               }
-            } else if (lane == 0) {
-              umma_commit(&o_full[t]);
             }
-            __syncwarp();
-          }
-          if (!ok) break;
-          if (lane == 0) {
-            umma_commit(&kv_empty[ev % ST]);
-            if (j + 1 < n) umma_commit(&kv_empty[ek % ST]);
-            if (j + 2 == n) umma_commit(q_empty);
-          }
-          __syncwarp();
-        }
-      } else {
-        if (lane == 0) {
-          mma_s(0, e, tmem + (g & 1) * 128);
-          umma_commit(&s_full[g & 1]);
-          umma_commit(&kv_empty[e % ST]);
-          if (n == 1) umma_commit(q_empty);
-        }
-        __syncwarp();
-        for (int j = 0; j < n; ++j, ++g) {
-          const int ev = e + 2 * j + 1, ek = ev + 1;
-          if (j + 1 < n) {
-            if (!(ok = wait_kv(ek))) break;
-            tc_fence_after();
-            if (lane == 0) {
-              mma_s(0, ek, tmem + ((g + 1) & 1) * 128);
-              umma_commit(&s_full[(g + 1) & 1]);
-              umma_commit(&kv_empty[ek % ST]);
+            if (!ok) break;
+            umma_commit(&kv_empty[sv]);
+            if (j + 1 < n) {
+              umma_commit(&kv_empty[st]);
               if (j + 2 == n) umma_commit(q_empty);
+              advance();
             }
-            __syncwarp();
           }
-          if (!(ok = wait_kv(ev))) break;
-          clear_v(ev, kb0 + j, it.kv_len);
-          if (!(ok = mbar_wait_warp(&p_half[g & 1], (g >> 1) & 1, abort_flag))) break;
-          tc_fence_after();
-          if (lane == 0) mma_pv(tmem + Cfg::O_COL, tmem + (g & 1) * 128, ev, j == 0, 0);
-          __syncwarp();
-          if (!(ok = mbar_wait_warp(&p_full[g & 1], (g >> 1) & 1, abort_flag))) break;
-          tc_fence_after();
-          if (lane == 0) {
-            mma_pv(tmem + Cfg::O_COL, tmem + (g & 1) * 128, ev, false, 1);
-            umma_commit(&o_full[0]);
-            umma_commit(&kv_empty[ev % ST]);
+        } else {
+          mma_s(0, st, tmem + (g & 1) * 128);
+          umma_commit(&s_full[g & 1]);
+          umma_commit(&kv_empty[st]);
+          if (n == 1) umma_commit(q_empty);
+          advance();
+          for (int j = 0; j < n; ++j, ++g) {
+            const int sv = st;
+            const uint32_t phv = ph;
+            advance();
+            if (j + 1 < n) {
+              if (!(ok = wait(&kv_full[st], ph))) break;
+              mma_s(0, st, tmem + ((g + 1) & 1) * 128);
+              umma_commit(&s_full[(g + 1) & 1]);
+              umma_commit(&kv_empty[st]);
+              if (j + 2 == n) umma_commit(q_empty);
+              advance();
+            }
+            if (!(ok = wait(&kv_full[sv], phv)) || !(ok = wait(&p_half[g & 1], (g >> 1) & 1))) break;
+            mma_pv(tmem + Cfg::O_COL, tmem + (g & 1) * 128, sv, j == 0, 0);
+            if (!(ok = wait(&p_full[g & 1], (g >> 1) & 1))) break;
+            mma_pv(tmem + Cfg::O_COL, tmem + (g & 1) * 128, sv, false, 1);
+            umma_commit(&o_full[g & 1]);
+            umma_commit(&kv_empty[sv]);
           }
-          __syncwarp();
         }
+        if (!ok) break;
       }
-      if (!ok) break;
-      e += 2 * n;
+      if (!ok) {
+        report(&g_op_status, code);
+        *abort_flag = 1;
+      }
     }
+    __syncwarp();
   } else {
     // -------------------------------------------------------------- softmax
     code = kDevTimeoutEpilogue;
@@ -600,7 +601,20 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
     const uint32_t o_addr = t_lane + Cfg::O_COL + t * HD;
     const float sc = a.scale_log2;
     int g = 0;       // blocks so far (of this tile)
+    int e = 0;       // K / V tiles before this item's
     int done = 0;    // tiles whose result was read (NT 2)
+    auto clear_v = [&](int entry, int from) {
+      // the tile has landed: these writes come after the copy's
+      ok = mbar_wait_warp(&kv_full[entry % ST], (entry / ST) & 1, abort_flag) && ok;
+      if (ok && r >= from) {
+        uint8_t* v = sKV + (entry % ST) * Cfg::TILE + r * 128;
+#pragma unroll
+        for (int c = 0; c < AT; ++c)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(v + c * Cfg::ATOM + i * 16) = make_uint4(0, 0, 0, 0);
+      }
+      fence_proxy_async_smem();
+    };
     while (true) {
       if (!(ok = next_item(it)) || !it.valid) break;
       const int qt = t * R + tok;          // token within the tile set
@@ -621,6 +635,11 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
           for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(s_addr + c * 32, s[c]);
           tmem_wait_ld();
           const int left = vis - (it.kb0 + j) * 128;
+          // V rows behind the sequence's keys are another sequence's, or what
+          // a page held before: their probabilities are 0, and 0 * NaN would
+          // not be.  Cleared by the tile's own warps before its P V.
+          const int rows = it.kv_len - (it.kb0 + j) * 128;
+          if (rows < 128) clear_v(e + 2 * j + 1, rows);
           const bool cut = __any_sync(0xffffffffu, live && left < 128);
           auto mask = [&](int c) {
             if (cut) {
@@ -647,7 +666,7 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
             if (j > 0) {
               // O holds the blocks before: their last P V has to be done (with
               // NT 2 this block's S came after it)
-              if (NT == 1 && !(ok = mbar_wait_warp(&o_full[0], (g - 1) & 1, abort_flag))) break;
+              if (NT == 1 && !(ok = mbar_wait_warp(&o_full[(g - 1) & 1], ((g - 1) >> 1) & 1, abort_flag))) break;
               tc_fence_after();
 #pragma unroll
               for (int c = 0; c < HD / 32; ++c) {
@@ -696,19 +715,24 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
           }
           l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
           tmem_wait_st();
-        } else if (lane == 0) {
-          mbar_arrive(&p_half[buf]);
+        } else {
+          const int rows = it.kv_len - (it.kb0 + j) * 128;
+          if (rows < 128) clear_v(e + 2 * j + 1, rows);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_half[buf]);
         }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[buf]);
       }
       if (!ok) break;
+      e += 2 * max(0, max(it.nb[0], NT == 2 ? it.nb[1] : 0) - it.kb0);
       if (n > 0) {
-        // the last P V of this tile; a parity wait must not be two phases
-        // behind, so the one before it first (NT 1: one phase per block)
-        if (NT == 1 && n > 1 && !(ok = mbar_wait_warp(&o_full[0], (g - 2) & 1, abort_flag))) break;
-        if (!(ok = mbar_wait_warp(&o_full[t], NT == 2 ? done & 1 : (g - 1) & 1, abort_flag))) break;
+        // the last P V of this tile.  NT 1 alternates between two barriers:
+        // the scores of block g came after P V of g - 2, so a wait for g - 1
+        // is never two phases from its barrier's
+        if (!(ok = mbar_wait_warp(&o_full[NT == 2 ? t : (g - 1) & 1], NT == 2 ? done & 1 : ((g - 1) >> 1) & 1, abort_flag)))
+          break;
         ++done;
         tc_fence_after();
       }
@@ -766,7 +790,7 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
     }
   }
   if (!ok) {
-    if (lane == 0) report(&g_op_status, code);
+    report(&g_op_status, code);
     *abort_flag = 1;
   }
   tc_fence_before();
