@@ -306,7 +306,7 @@ int ec_kv_write(int handle, int layer, const void *k, int64_t k_token, int64_t k
                 const int32_t *cu, const int32_t *slots, int nseq, void *stream);
 
 /* Bytes of the scratch (`work`) of ec_attn_cached for up to `tokens` new
- * tokens of `nseq` sequences.  It must be zero before its first use, belongs
+ * tokens of `nseq` sequences.  It must be 32-byte aligned and zero before its first use, belongs
  * to one call at a time (calls in order on one stream may share it, two that
  * may run at once may not) and is left ready for the next call. */
 int64_t ec_attn_cached_work_size(int handle, int64_t tokens, int q_heads, int nseq, int max_new);

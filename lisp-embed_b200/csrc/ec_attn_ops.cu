@@ -86,6 +86,8 @@ FlashPlan flash_plan(const KvCache* c, int64_t tokens, int q_heads, int kv_heads
     const int64_t most = (static_cast<int64_t>(c->width) * c->page_size + 127) / 128;
     p.even = tiles * most < (int64_t(1) << 30);
   }
+  // single tokens: tiles of 64 rows, so that queries can be double-buffered
+  if (p.even && max_new * (q_heads / kv_heads) <= 64) p.rows_tok = std::max(1, 64 / (q_heads / kv_heads));
   p.nt = !p.even && tokens > static_cast<int64_t>(nseq) * p.rows_tok && pairs >= num_sms ? 2 : 1;
   return p;
 }
@@ -119,6 +121,9 @@ int run_attention(const AttnOp& op, int num_sms, cudaStream_t st) {
     ok = ok && encode_rows(&tk, op.dtype, op.k, op.head_dim, op.kv_heads, op.tokens, 1, 128) &&
          encode_rows(&tv, op.dtype, op.v, op.head_dim, op.kv_heads, op.tokens, 1, 128);
   }
+  if ((op.tokens / (p.nt * p.rows_tok) + op.nseq) * op.kv_heads >= INT32_MAX / 2)
+    return set_error(EC_EINVAL, "%lld tokens of %d sequences and %d key heads: too many for one call",
+                     static_cast<long long>(op.tokens), op.nseq, op.kv_heads);
   if (!ok) return set_error(EC_EINVAL, "the attention's strides cannot be described to the TMA");
   FlashArgs a{};
   a.out = const_cast<void*>(op.out.p), a.ot = op.out.token, a.oh = op.out.head;
@@ -135,6 +140,7 @@ int run_attention(const AttnOp& op, int num_sms, cudaStream_t st) {
     a.pages = c->pages, a.page_size = c->page_size;
     a.page0 = op.layer * c->pages, a.page_end = c->layers * c->pages;
   }
+  a.q_bufs = p.nt == 1 && group * p.rows_tok <= 64 ? 2 : 1;
   int64_t grid = (op.tokens / (p.nt * p.rows_tok) + op.nseq) * op.kv_heads;
   if (p.even) {
     char* w = static_cast<char*>(op.work);
@@ -234,8 +240,8 @@ extern "C" int ec_attn_cached(int handle, int layer, const void* q, int64_t q_to
   if (int rc = check_attention(op, tokens, nseq, scale)) return rc;
   if (max_new < 0) return set_error(EC_EINVAL, "max_new is negative");
   const int64_t need = static_cast<int64_t>(attention_work_bytes(*c, tokens, q_heads, nseq, max_new));
-  if (!work || !op_aligned(work, 16) || work_bytes < need)
-    return set_error(EC_EINVAL, "work must be 16-byte aligned and hold %lld bytes", static_cast<long long>(need));
+  if (!work || !op_aligned(work, 32) || work_bytes < need)
+    return set_error(EC_EINVAL, "work must be 32-byte aligned and hold %lld bytes", static_cast<long long>(need));
   if (!slots && nseq > c->slots) return set_error(EC_EINVAL, "%d sequences, the cache has %d slots", nseq, c->slots);
   if (tokens == 0 || nseq == 0) return EC_OK;
   op.work = work, op.work_bytes = static_cast<size_t>(work_bytes);

@@ -50,6 +50,7 @@ struct FlashArgs {
   float scale_log2;
   int paged;
   int wide;                // out rows in 32-byte pieces
+  int q_bufs;              // 2: queries are double-buffered (NT 1, at most 64 rows)
   int even;                // 1: the blocks are split evenly over the CTAs
   int min_chunk;           // blocks a CTA takes at least
   float* part_o;           // [2 * CTAs][128][HD] partial results of cut tiles
@@ -58,7 +59,7 @@ struct FlashArgs {
 };
 
 // a tile set that one CTA works on
-struct FlashItem {
+struct FlashEntry {
   int valid;
   int tok0, qv;   // first token, tokens
   int kvh;
@@ -69,10 +70,20 @@ struct FlashItem {
   int nb[2];      // end block of each tile
   int part;       // partial result, -1: the whole of the tile's keys
 };
+struct FlashItem : FlashEntry {
+  int pages[32];  // cache: the first 32 pages from block kb0 on
+};
 
 // one of this many pairs of exponentials goes to the FMA units instead of the
 // special-function unit
 constexpr int kFmaEvery = 4;
+
+// work-list entries in flight
+constexpr int kFlashRing = 4;
+// Second query buffer of NT 1: 64 rows of 128 bytes after the first.  A tile's
+// operand is 128 rows all the same; what the rest reads (the other buffer, or
+// keys) only reaches rows of S and O that belong to no query.
+constexpr uint32_t kQBuf = 64 * 128;
 
 template <int HD, int NT>
 struct FlashCfg {
@@ -83,7 +94,7 @@ struct FlashCfg {
   static constexpr int MAX_SEQS = 2048;              // prefix sums of an even split
   static constexpr int WARPS = 4 * NT + 3;
   static constexpr int THREADS = 32 * WARPS;
-  static constexpr uint32_t TAIL = 1024 + (NT == 1 ? 4 * (MAX_SEQS + 1) : 0);
+  static constexpr uint32_t TAIL = 1280 + (NT == 1 ? 4 * (MAX_SEQS + 1) : 0);
   static constexpr size_t SMEM = NT * TILE + STAGES * TILE + TAIL;
   static constexpr uint32_t O_COL = 256;
   static_assert(SMEM <= 232448, "shared memory");
@@ -183,35 +194,37 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
   uint8_t* sQ = smem;
   uint8_t* sKV = sQ + NT * Cfg::TILE;
   uint8_t* tail = sKV + ST * Cfg::TILE;
-  uint64_t* q_full = reinterpret_cast<uint64_t*>(tail);
-  uint64_t* q_empty = q_full + 1;
-  uint64_t* kv_full = q_empty + 1;
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(tail);  // [2]
+  uint64_t* q_empty = q_full + 2;     // [2]
+  uint64_t* kv_full = q_empty + 2;
   uint64_t* kv_empty = kv_full + ST;
   uint64_t* s_full = kv_empty + ST;   // [2] tile (NT 2) or buffer (NT 1)
   uint64_t* p_full = s_full + 2;      // [2]
   uint64_t* p_half = p_full + 2;      // [2] the first 64 keys' P
   uint64_t* o_full = p_half + 2;      // [2] tile (NT 2), or even / odd blocks (NT 1)
-  uint64_t* i_full = o_full + 2;      // [2]
-  uint64_t* i_empty = i_full + 2;     // [2]
-  FlashItem* items = reinterpret_cast<FlashItem*>(i_empty + 2);  // [2]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(items + 2);
+  uint64_t* i_full = o_full + 2;      // [kFlashRing]
+  uint64_t* i_empty = i_full + kFlashRing;
+  FlashItem* items = reinterpret_cast<FlashItem*>(i_empty + kFlashRing);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(items + kFlashRing);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  int* prefix = reinterpret_cast<int*>(tail + 1024);  // [nseq + 1] of an even split
-  static_assert(8 * (2 + 2 * ST + 12) + 2 * sizeof(FlashItem) + 8 <= 1024, "tail");
+  int* prefix = reinterpret_cast<int*>(tail + 1280);  // [nseq + 1] of an even split
+  static_assert(8 * (4 + 2 * ST + 8 + 2 * kFlashRing) + kFlashRing * sizeof(FlashItem) + 8 <= 1280, "tail");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    mbar_init(q_full, 1);
-    mbar_init(q_empty, 1);
     for (int i = 0; i < ST; ++i) {
       mbar_init(&kv_full[i], 1);
       mbar_init(&kv_empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], 1);
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
       mbar_init(&p_half[i], 4);
       mbar_init(&o_full[i], 1);
+    }
+    for (int i = 0; i < kFlashRing; ++i) {
       mbar_init(&i_full[i], 1);
       mbar_init(&i_empty[i], READERS);
     }
@@ -235,33 +248,48 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
   bool ok = true;
   unsigned code = kDevTimeoutOther;
 
-  // the next entry of the list for the reading warps
+  // the next entry of the list for the reading warps; it stays readable until
+  // done_item
   int it_n = 0;
-  auto next_item = [&](FlashItem& it) -> bool {
-    const int b = it_n & 1;
-    if (!mbar_wait_warp(&i_full[b], (it_n >> 1) & 1, abort_flag)) return false;
-    it = items[b];
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&i_empty[b]);
-    ++it_n;
-    return true;
+  auto next_item = [&]() -> const FlashItem* {
+    const int b = it_n % kFlashRing;
+    if (!mbar_wait_warp(&i_full[b], (it_n / kFlashRing) & 1, abort_flag)) return nullptr;
+    return &items[b];
   };
+  auto done_item = [&] {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&i_empty[it_n % kFlashRing]);
+    ++it_n;
+  };
+  const int ppb = a.paged ? 128 / a.page_size : 1;  // pages per key block
+  // page of table entry e of a slot with `in_use` pages; one that is none
+  // reads past the pages, which fills the tile with zeros
+  auto fetch = [&](int slot, int e, int in_use) -> int {
+    int p = -1;
+    if (e < in_use) p = a.tables[static_cast<int64_t>(slot) * a.width + e];
+    return p >= 0 && p < a.pages ? a.page0 + p : a.page_end;
+  };
+  auto pages_in_use = [&](int kv_len) { return (kv_len + a.page_size - 1) / a.page_size; };
 
   if (warp == W_LIST) {
+    using Entry = FlashEntry;
     // ------------------------------------------------------------ work list
     int n = 0;
-    auto publish = [&](const FlashItem& it, int from) -> bool {  // lane `from`'s entry
-      const int b = n & 1;
-      if (!mbar_wait_warp(&i_empty[b], ((n >> 1) & 1) ^ 1, abort_flag)) return false;
-      if (lane == from) {
-        items[b] = it;
-        mbar_arrive(&i_full[b]);
+    auto publish = [&](const Entry& it, int from) -> bool {  // lane `from`'s entry
+      const int b = n % kFlashRing;
+      if (!mbar_wait_warp(&i_empty[b], ((n / kFlashRing) & 1) ^ 1, abort_flag)) return false;
+      if (a.paged && __shfl_sync(0xffffffffu, it.valid, from)) {
+        // looked up here, ahead of the loads: the table is far away
+        const int slot = __shfl_sync(0xffffffffu, it.kbase, from), kv_len = __shfl_sync(0xffffffffu, it.kv_len, from);
+        items[b].pages[lane] = fetch(slot, __shfl_sync(0xffffffffu, it.kb0, from) * ppb + lane, pages_in_use(kv_len));
       }
+      if (lane == from) *static_cast<Entry*>(&items[b]) = it;
       __syncwarp();
+      if (lane == 0) mbar_arrive(&i_full[b]);
       ++n;
       return true;
     };
-    FlashItem it{};
+    Entry it{};
     if (NT == 1 && a.even) {
       // every CTA takes the same number of key blocks: blocks in the order
       // (sequence, tile, key head, block), prefix sums over the sequences
@@ -333,13 +361,12 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
       // the join
     } else {
       // every lane looks up one of the next 32 candidates
-      const int64_t slots = a.tokens / BT + a.nseq;
-      const int64_t all = slots * a.kv_heads;
-      for (int64_t t0 = 0; ok && t0 < all; t0 += 32 * static_cast<int64_t>(gridDim.x)) {
+      // (their number fits 31 bits, checked on the host)
+      const uint32_t slots = a.tokens / BT + a.nseq, all = slots * a.kv_heads, step = gridDim.x;
+      for (uint32_t t0 = 0; ok && t0 < all; t0 += 32 * step) {
         // late (long) tile sets first; the order turns round every pass, so
         // that no CTA gets the longest of each
-        const int64_t t = t0 + lane * static_cast<int64_t>(gridDim.x) +
-                          ((lane & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+        const uint32_t t = t0 + lane * step + ((lane & 1) ? step - 1 - blockIdx.x : blockIdx.x);
         it.valid = 0;
         if (t < all) {
           const int u = static_cast<int>(slots - 1 - t / a.kv_heads);
@@ -351,13 +378,14 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
           }
           const FlashSeq q = flash_seq(a, lo);
           const int len = q.end - q.begin;
-          const int64_t q0 = static_cast<int64_t>(u - (q.begin / BT + lo)) * BT;
-          if (q0 >= 0 && q0 < len) {
+          const int i = u - (q.begin / BT + lo);  // tile set of the sequence
+          if (i >= 0 && i < (len + BT - 1) / BT) {
+            const int q0 = i * BT;
             it.valid = 1;
-            it.tok0 = q.begin + static_cast<int>(q0);
-            it.qv = min(BT, len - static_cast<int>(q0));
+            it.tok0 = q.begin + q0;
+            it.qv = min(BT, len - q0);
             it.kvh = static_cast<int>(t % a.kv_heads);
-            it.pos0 = q.kv_len - len + static_cast<int>(q0);
+            it.pos0 = q.kv_len - len + q0;
             it.kv_len = q.kv_len;
             it.kbase = q.kbase;
             it.kb0 = 0;
@@ -374,32 +402,25 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
   } else if (warp == W_LOAD) {
     // ---------------------------------------------------------------- loads
     code = kDevTimeoutProducer;
-    FlashItem it;
-    int st = 0;
-    uint32_t ph = 0, q_ph = 0;
-    const int ppb = a.paged ? 128 / a.page_size : 1;
+    int st = 0, qi = 0;
+    uint32_t ph = 0;
     while (true) {
-      if (!(ok = next_item(it)) || !it.valid) break;
-      const int nb = max(it.nb[0], NT == 2 ? it.nb[1] : 0);
-      if (nb <= it.kb0) continue;
-      const int32_t* table = a.tables + static_cast<int64_t>(it.kbase) * a.width;
-      const int in_use = a.paged ? (it.kv_len + a.page_size - 1) / a.page_size : 0;
-      // pages of the next 32 table entries, one per lane; an entry that is
-      // none reads past the pages, which fills the tile with zeros
-      int first = it.kb0 * ppb;
-      auto fetch = [&](int e) -> int {
-        int p = -1;
-        if (a.paged && e < in_use) p = table[e];
-        return p >= 0 && p < a.pages ? a.page0 + p : a.page_end;
-      };
-      int page = fetch(first + lane), ahead = fetch(first + 32 + lane);
-      for (int j = it.kb0; ok && j < nb; ++j) {
+      const FlashItem* it = next_item();
+      if (!(ok = it != nullptr) || !it->valid) break;
+      const int kb0 = it->kb0, nb = max(it->nb[0], NT == 2 ? it->nb[1] : 0);
+      const int kvh = it->kvh, kbase = it->kbase, tok0 = it->tok0, in_use = a.paged ? pages_in_use(it->kv_len) : 0;
+      int page = a.paged ? it->pages[lane] : 0, ahead = 0;
+      done_item();
+      if (nb <= kb0) continue;
+      int first = kb0 * ppb;  // table entry of lane 0's page
+      if (a.paged && nb * ppb > first + 32) ahead = fetch(kbase, first + 32 + lane, in_use);
+      for (int j = kb0; ok && j < nb; ++j) {
         if (a.paged && j * ppb - first == 32) {
           first += 32;
           page = ahead;
-          ahead = fetch(first + 32 + lane);
+          ahead = fetch(kbase, first + 32 + lane, in_use);
         }
-#pragma unroll
+#pragma unroll 1
         for (int kv = 0; kv < 2; ++kv) {
           if (!(ok = mbar_wait_warp(&kv_empty[st], ph ^ 1, abort_flag))) break;
           const uint32_t dst = smem_u32(sKV + st * Cfg::TILE), bar = smem_u32(&kv_full[st]);
@@ -407,51 +428,53 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
           if (elect_one()) mbar_arrive_expect_tx(&kv_full[st], Cfg::TILE);
           __syncwarp();
           if (a.paged) {
-            for (int i = 0; i < ppb; ++i) {
-              const int p = __shfl_sync(0xffffffffu, page, j * ppb - first + i);
-              if (elect_one()) {
+            int p[8];
 #pragma unroll
-                for (int c = 0; c < AT; ++c)
-                  asm volatile(
-                      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], "
-                      "[%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst + c * Cfg::ATOM + i * a.page_size * 128),
-                      "l"(map), "r"(bar), "r"(c * 64), "r"(it.kvh), "r"(0), "r"(p)
-                      : "memory");
-              }
-              __syncwarp();
-            }
-          } else {
+            for (int i = 0; i < 8; ++i) p[i] = __shfl_sync(0xffffffffu, page, (j * ppb - first + i) & 31);
             if (elect_one()) {
 #pragma unroll
-              for (int c = 0; c < AT; ++c)
-                asm volatile(
-                    "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], "
-                    "[%1, {%3, %4, %5}], [%2];" ::"r"(dst + c * Cfg::ATOM),
-                    "l"(map), "r"(bar), "r"(c * 64), "r"(it.kvh), "r"(it.kbase + j * 128)
-                    : "memory");
+              for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int c = 0; c < AT; ++c)
+                  if (i < ppb)
+                    asm volatile(
+                        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], "
+                        "[%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst + c * Cfg::ATOM + i * a.page_size * 128),
+                        "l"(map), "r"(bar), "r"(c * 64), "r"(kvh), "r"(0), "r"(p[i])
+                        : "memory");
             }
-            __syncwarp();
+          } else if (elect_one()) {
+#pragma unroll
+            for (int c = 0; c < AT; ++c)
+              asm volatile(
+                  "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], "
+                  "[%1, {%3, %4, %5}], [%2];" ::"r"(dst + c * Cfg::ATOM),
+                  "l"(map), "r"(bar), "r"(c * 64), "r"(kvh), "r"(kbase + j * 128)
+                  : "memory");
           }
+          __syncwarp();
           if (++st == ST) {
             st = 0;
             ph ^= 1;
           }
-          if (j == it.kb0 && kv == 0) {
+          if (j == kb0 && kv == 0) {
             // the queries, once the tiles before have no more use for theirs;
             // rows past the tokens of the call are filled with zeros
-            if (!(ok = mbar_wait_warp(q_empty, q_ph ^ 1, abort_flag))) break;
-            q_ph ^= 1;
+            const int qb = a.q_bufs == 2 ? qi & 1 : 0;
+            const uint32_t qp = (a.q_bufs == 2 ? qi >> 1 : qi) & 1;
+            ++qi;
+            if (!(ok = mbar_wait_warp(&q_empty[qb], qp ^ 1, abort_flag))) break;
             if (elect_one()) {
-              mbar_arrive_expect_tx(q_full, NT * AT * static_cast<uint32_t>(G * R) * 128u);
+              mbar_arrive_expect_tx(&q_full[qb], NT * AT * static_cast<uint32_t>(G * R) * 128u);
 #pragma unroll
               for (int t = 0; t < NT; ++t)
 #pragma unroll
                 for (int c = 0; c < AT; ++c)
                   asm volatile(
                       "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], "
-                      "[%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(sQ + t * Cfg::TILE + c * Cfg::ATOM)),
-                      "l"(reinterpret_cast<uint64_t>(&tm_q)), "r"(smem_u32(q_full)), "r"(c * 64), "r"(it.kvh * G),
-                      "r"(it.tok0 + t * R)
+                      "[%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(sQ + qb * kQBuf + t * Cfg::TILE + c * Cfg::ATOM)),
+                      "l"(reinterpret_cast<uint64_t>(&tm_q)), "r"(smem_u32(&q_full[qb])), "r"(c * 64), "r"(kvh * G),
+                      "r"(tok0 + t * R)
                       : "memory");
             }
             __syncwarp();
@@ -468,7 +491,7 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
     if (elect_one()) {
       int st = 0;            // stage of the next K / V tile
       uint32_t ph = 0;       // its phase
-      uint32_t q_ph = 0;
+      int qi = 0;            // items so far
       uint32_t pf[2] = {0, 0};  // P's waited for, per tile
       uint32_t g = 0;           // blocks (NT 1)
       const uint64_t dq = desc_sw128_kmajor(smem_u32(sQ));
@@ -485,8 +508,8 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
           ph ^= 1;
         }
       };
-      auto mma_s = [&](int t, int stage, uint32_t d) {
-        const uint64_t q = dq + t * (Cfg::TILE >> 4), k = dk + stage * (Cfg::TILE >> 4);
+      auto mma_s = [&](int qb, int t, int stage, uint32_t d) {
+        const uint64_t q = dq + qb * (kQBuf >> 4) + t * (Cfg::TILE >> 4), k = dk + stage * (Cfg::TILE >> 4);
 #pragma unroll
         for (int kk = 0; kk < HD / 16; ++kk) {
           const uint32_t off = ((kk >> 2) * Cfg::ATOM + (kk & 3) * 32) >> 4;
@@ -501,27 +524,28 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
                       kk > 0 || half > 0 || !first);
       };
       while (true) {
-        const int b = it_n & 1;
-        if (!(ok = mbar_wait(&i_full[b], (it_n >> 1) & 1, abort_flag))) break;
+        const int b = it_n % kFlashRing;
+        if (!(ok = mbar_wait(&i_full[b], (it_n / kFlashRing) & 1, abort_flag))) break;
         const int valid = items[b].valid, kb0 = items[b].kb0;
         const int n0 = items[b].nb[0] - kb0, n1 = NT == 2 ? items[b].nb[1] - kb0 : 0, n = max(n0, n1);
         mbar_arrive(&i_empty[b]);
         ++it_n;
         if (!valid) break;
         if (n <= 0) continue;
-        if (!(ok = wait(q_full, q_ph)) || !(ok = wait(&kv_full[st], ph))) break;
-        q_ph ^= 1;
+        const int qb = a.q_bufs == 2 ? qi & 1 : 0;
+        if (!(ok = wait(&q_full[qb], (a.q_bufs == 2 ? qi >> 1 : qi) & 1)) || !(ok = wait(&kv_full[st], ph))) break;
+        ++qi;
         if constexpr (NT == 2) {
           if (n0 > 0) {
-            mma_s(0, st, tmem);
+            mma_s(qb, 0, st, tmem);
             umma_commit(&s_full[0]);
           }
           if (n1 > 0) {
-            mma_s(1, st, tmem + 128);
+            mma_s(qb, 1, st, tmem + 128);
             umma_commit(&s_full[1]);
           }
           umma_commit(&kv_empty[st]);
-          if (n == 1) umma_commit(q_empty);
+          if (n == 1) umma_commit(&q_empty[qb]);
           advance();
           for (int j = 0; ok && j < n; ++j) {
             const int sv = st;
@@ -542,7 +566,7 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
               if (j + 1 < nt) {
                 if (!have_k && !(ok = wait(&kv_full[st], ph))) break;
                 have_k = true;
-                mma_s(t, st, tmem + t * 128);
+                mma_s(qb, t, st, tmem + t * 128);
                 umma_commit(&s_full[t]);
               } else {
                 umma_commit(&o_full[t]);
@@ -552,15 +576,15 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
             umma_commit(&kv_empty[sv]);
             if (j + 1 < n) {
               umma_commit(&kv_empty[st]);
-              if (j + 2 == n) umma_commit(q_empty);
+              if (j + 2 == n) umma_commit(&q_empty[qb]);
               advance();
             }
           }
         } else {
-          mma_s(0, st, tmem + (g & 1) * 128);
+          mma_s(qb, 0, st, tmem + (g & 1) * 128);
           umma_commit(&s_full[g & 1]);
           umma_commit(&kv_empty[st]);
-          if (n == 1) umma_commit(q_empty);
+          if (n == 1) umma_commit(&q_empty[qb]);
           advance();
           for (int j = 0; j < n; ++j, ++g) {
             const int sv = st;
@@ -568,10 +592,10 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
             advance();
             if (j + 1 < n) {
               if (!(ok = wait(&kv_full[st], ph))) break;
-              mma_s(0, st, tmem + ((g + 1) & 1) * 128);
+              mma_s(qb, 0, st, tmem + ((g + 1) & 1) * 128);
               umma_commit(&s_full[(g + 1) & 1]);
               umma_commit(&kv_empty[st]);
-              if (j + 2 == n) umma_commit(q_empty);
+              if (j + 2 == n) umma_commit(&q_empty[qb]);
               advance();
             }
             if (!(ok = wait(&kv_full[sv], phv)) || !(ok = wait(&p_half[g & 1], (g >> 1) & 1))) break;
@@ -593,7 +617,6 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
   } else {
     // -------------------------------------------------------------- softmax
     code = kDevTimeoutEpilogue;
-    FlashItem it;
     const int t = warp >> 2;               // tile (0 for NT 1)
     const int r = (warp & 3) * 32 + lane;  // row of the tile = TMEM lane
     const int tok = r / G, head = r - tok * G;
@@ -603,20 +626,11 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
     int g = 0;       // blocks so far (of this tile)
     int e = 0;       // K / V tiles before this item's
     int done = 0;    // tiles whose result was read (NT 2)
-    auto clear_v = [&](int entry, int from) {
-      // the tile has landed: these writes come after the copy's
-      ok = mbar_wait_warp(&kv_full[entry % ST], (entry / ST) & 1, abort_flag) && ok;
-      if (ok && r >= from) {
-        uint8_t* v = sKV + (entry % ST) * Cfg::TILE + r * 128;
-#pragma unroll
-        for (int c = 0; c < AT; ++c)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(v + c * Cfg::ATOM + i * 16) = make_uint4(0, 0, 0, 0);
-      }
-      fence_proxy_async_smem();
-    };
     while (true) {
-      if (!(ok = next_item(it)) || !it.valid) break;
+      const FlashItem* ip = next_item();
+      if (!(ok = ip != nullptr) || !ip->valid) break;
+      const FlashEntry it = *ip;
+      done_item();
       const int qt = t * R + tok;          // token within the tile set
       const bool live = tok < R && qt < it.qv;
       const bool warp_live = __any_sync(0xffffffffu, live);
@@ -629,35 +643,53 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
         const uint32_t s_addr = t_lane + buf * 128;
         if (!(ok = mbar_wait_warp(&s_full[buf], NT == 2 ? g & 1 : (g >> 1) & 1, abort_flag))) break;
         tc_fence_after();
-        if (warp_live) {
-          uint32_t s[4][32];
+        // V rows behind the sequence's keys are another sequence's, or what a
+        // page held before: their probabilities are 0, and 0 * NaN would not
+        // be.  Cleared by the tile's own warps before its P V.
+        const int rows = it.kv_len - (it.kb0 + j) * 128;
+        if (rows < 128) {
+          // the tile has landed: these writes come after the copy's
+          const int entry = e + 2 * j + 1;
+          if (!(ok = mbar_wait_warp(&kv_full[entry % ST], (entry / ST) & 1, abort_flag))) break;
+          if (r >= rows) {
+            uint8_t* v = sKV + (entry % ST) * Cfg::TILE + r * 128;
+#pragma unroll 1
+            for (int i = 0; i < 8; ++i)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(s_addr + c * 32, s[c]);
-          tmem_wait_ld();
+              for (int c = 0; c < AT; ++c) *reinterpret_cast<uint4*>(v + c * Cfg::ATOM + i * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+        if (warp_live) {
+          // The scores are read twice, 64 at a time (first their maximum, then
+          // P): half the code and a third of the registers of holding all 128
           const int left = vis - (it.kb0 + j) * 128;
-          // V rows behind the sequence's keys are another sequence's, or what
-          // a page held before: their probabilities are 0, and 0 * NaN would
-          // not be.  Cleared by the tile's own warps before its P V.
-          const int rows = it.kv_len - (it.kb0 + j) * 128;
-          if (rows < 128) clear_v(e + 2 * j + 1, rows);
           const bool cut = __any_sync(0xffffffffu, live && left < 128);
-          auto mask = [&](int c) {
+          uint32_t s[2][32];
+          auto scores = [&](int h) {
+            tmem_ld_32x32b_x32(s_addr + h * 64, s[0]);
+            tmem_ld_32x32b_x32(s_addr + h * 64 + 32, s[1]);
+            tmem_wait_ld();
             if (cut) {
 #pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (c * 32 + i >= left) s[c][i] = 0xff800000u;  // -infinity
+              for (int i = 0; i < 64; ++i)
+                if (h * 64 + i >= left) s[i >> 5][i & 31] = 0xff800000u;  // -infinity
             }
           };
+          float top = -INFINITY;
+#pragma unroll 1
+          for (int h = 0; h < 2; ++h) {
+            scores(h);
+            float mx[4];
 #pragma unroll
-          for (int c = 0; c < 4; ++c) mask(c);
-          float mx[4];
+            for (int c = 0; c < 4; ++c) {
+              mx[c] = __uint_as_float(s[c >> 1][(c & 1) * 16]);
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            mx[c] = __uint_as_float(s[c][0]);
-#pragma unroll
-            for (int i = 1; i < 32; ++i) mx[c] = fmaxf(mx[c], __uint_as_float(s[c][i]));
+              for (int i = 1; i < 16; ++i) mx[c] = fmaxf(mx[c], __uint_as_float(s[c >> 1][(c & 1) * 16 + i]));
+            }
+            top = fmaxf(top, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
           }
-          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
           // keep the older maximum unless the new one is 2^8 above it
           const bool grow = live && ((top - m) * sc > 8.f || (m == -INFINITY && top > m));
           if (__any_sync(0xffffffffu, grow)) {
@@ -668,7 +700,7 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
               // NT 2 this block's S came after it)
               if (NT == 1 && !(ok = mbar_wait_warp(&o_full[(g - 1) & 1], ((g - 1) >> 1) & 1, abort_flag))) break;
               tc_fence_after();
-#pragma unroll
+#pragma unroll 1
               for (int c = 0; c < HD / 32; ++c) {
                 uint32_t v[32];
                 tmem_ld_32x32b_x32(o_addr + c * 32, v);
@@ -685,45 +717,32 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
           const float nm = m == -INFINITY ? 0.f : -m * sc;
           float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
           const float2 sc2 = make_float2(sc, sc), nm2 = make_float2(nm, nm);
-#pragma unroll
-          for (int c = 0; c < 4; c += 2) {
+#pragma unroll 1
+          for (int h = 0; h < 2; ++h) {
+            scores(h);
             uint32_t p[32];
-            if (c == 2) {
-              // the second half's scores are read again: holding all of them
-              // next to the first half's P takes more registers than there are
-              tmem_ld_32x32b_x32(s_addr + 64, s[2]);
-              tmem_ld_32x32b_x32(s_addr + 96, s[3]);
-              tmem_wait_ld();
-              mask(2);
-              mask(3);
-            }
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
-              const uint32_t* x = s[c + (i >> 4)] + 2 * (i & 15);
+              const uint32_t* x = s[i >> 4] + 2 * (i & 15);
               const float2 y = __ffma2_rn(make_float2(__uint_as_float(x[0]), __uint_as_float(x[1])), sc2, nm2);
               const float2 w = (i % kFmaEvery) == kFmaEvery - 1 ? exp2_fma(y) : make_float2(fa_exp2(y.x), fa_exp2(y.y));
               sum[i & 1] = __fadd2_rn(sum[i & 1], w);
               p[i] = pack2<T>(w.x, w.y);
             }
-            tmem_st_32x32b_x32(s_addr + c * 16, p);
-            if (c == 0) {
-              tmem_wait_st();
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&p_half[buf]);
-            }
+            tmem_st_32x32b_x32(s_addr + h * 32, p);
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(h ? &p_full[buf] : &p_half[buf]);
           }
           l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-          tmem_wait_st();
         } else {
-          const int rows = it.kv_len - (it.kb0 + j) * 128;
-          if (rows < 128) clear_v(e + 2 * j + 1, rows);
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&p_half[buf]);
+          tc_fence_before();
+          if (lane == 0) {
+            mbar_arrive(&p_half[buf]);
+            mbar_arrive(&p_full[buf]);
+          }
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[buf]);
       }
       if (!ok) break;
       e += 2 * max(0, max(it.nb[0], NT == 2 ? it.nb[1] : 0) - it.kb0);
@@ -740,50 +759,40 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
         const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // NaN stays NaN
         const float l2 = l == 0.f ? -INFINITY : m * sc + log2f(l);
         const int64_t row = it.tok0 + qt;
-        if (it.part >= 0) {
-          float* po = a.part_o + (static_cast<int64_t>(it.part) * 128 + r) * HD;
-#pragma unroll
-          for (int c = 0; c < HD / 32; ++c) {
-            uint32_t v[32];
+        const int h = it.kvh * G + head;
+        T* o = static_cast<T*>(a.out) + row * a.ot + h * a.oh;
+        float* po = a.part_o + (static_cast<int64_t>(max(it.part, 0)) * 128 + r) * HD;
+#pragma unroll 1
+        for (int c = 0; c < HD / 32; ++c) {
+          uint32_t v[32];
+          if (n > 0) {
             tmem_ld_32x32b_x32(o_addr + c * 32, v);
             tmem_wait_ld();
-            if (live) {
+          }
+          if (!live) continue;
 #pragma unroll
-              for (int i = 0; i < 8; ++i)
-                *reinterpret_cast<float4*>(po + c * 32 + 4 * i) =
-                    l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
-                             : make_float4(__uint_as_float(v[4 * i]) * inv, __uint_as_float(v[4 * i + 1]) * inv,
-                                           __uint_as_float(v[4 * i + 2]) * inv, __uint_as_float(v[4 * i + 3]) * inv);
+          for (int i = 0; i < 32; ++i)  // 0: a row that sees nothing
+            v[i] = l == 0.f ? 0u : __float_as_uint(__uint_as_float(v[i]) * inv);
+          if (it.part >= 0) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) store32(po + c * 32 + 8 * i, v + 8 * i);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] = pack2<T>(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+            if (a.wide) {
+              if (c * 32 < a.head_dim) store32(o + c * 32, v);
+              if (c * 32 + 16 < a.head_dim) store32(o + c * 32 + 16, v + 8);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (c * 32 + 8 * i < a.head_dim)
+                  *reinterpret_cast<uint4*>(o + c * 32 + 8 * i) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
             }
           }
-          if (live) a.part_l[it.part * 128 + r] = l2;
-        } else {
-          const int h = it.kvh * G + head;
-          T* o = static_cast<T*>(a.out) + row * a.ot + h * a.oh;
-#pragma unroll
-          for (int c = 0; c < HD / 32; ++c) {
-            uint32_t v[32];
-            if (n > 0) {
-              tmem_ld_32x32b_x32(o_addr + c * 32, v);
-              tmem_wait_ld();
-            }
-            if (live) {
-              uint32_t w[16];
-#pragma unroll
-              for (int i = 0; i < 16; ++i)  // 0: a row that sees nothing
-                w[i] = l == 0.f ? 0u : pack2<T>(__uint_as_float(v[2 * i]) * inv, __uint_as_float(v[2 * i + 1]) * inv);
-              if (a.wide) {
-                if (c * 32 < a.head_dim) store32(o + c * 32, w);
-                if (c * 32 + 16 < a.head_dim) store32(o + c * 32 + 16, w + 8);
-              } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                  if (c * 32 + 8 * i < a.head_dim)
-                    *reinterpret_cast<uint4*>(o + c * 32 + 8 * i) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-              }
-            }
-          }
-          if (live && a.lse) a.lse[row * a.q_heads + h] = l2 * 0.693147180559945309f;
+        }
+        if (live) {
+          if (it.part >= 0) a.part_l[it.part * 128 + r] = l2;
+          else if (a.lse) a.lse[row * a.q_heads + h] = l2 * 0.693147180559945309f;
         }
       }
       tc_fence_before();
