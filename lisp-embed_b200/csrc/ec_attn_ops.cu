@@ -38,34 +38,53 @@ bool encode_rows(CUtensorMap* tm, int dtype, const OpRows& r, int head_dim, int 
   return encode(tm, dtype, r.p, 3, dims, strides, box);
 }
 
-template <int HD, int NT, typename T>
-int launch_flash(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const FlashArgs& a, int grid,
-                 cudaStream_t st) {
-  using Cfg = FlashCfg<HD, NT>;
+using FlashFn = void (*)(CUtensorMap, CUtensorMap, CUtensorMap, FlashArgs);
+
+// kernel `id` (its shared memory is set once per device)
+int launch_one(int id, FlashFn fn, int threads, size_t smem, const CUtensorMap& q, const CUtensorMap& k,
+               const CUtensorMap& v, const FlashArgs& a, int grid, cudaStream_t st) {
   static std::mutex mu;
-  static bool set[64] = {};
+  static uint32_t set[64] = {};
   int dev = 0;
   if (int rc = check_cuda(cudaGetDevice(&dev), "cudaGetDevice")) return rc;
   {
     std::lock_guard<std::mutex> lk(mu);
-    if (!set[dev]) {
-      if (int rc = check_cuda(cudaFuncSetAttribute(flash_kernel<HD, NT, T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                   static_cast<int>(Cfg::SMEM)),
+    if (!(set[dev] >> id & 1)) {
+      if (int rc = check_cuda(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   static_cast<int>(smem)),
                               "attention shared memory"))
         return rc;
-      set[dev] = true;
+      set[dev] |= 1u << id;
     }
   }
-  flash_kernel<HD, NT, T><<<grid, Cfg::THREADS, Cfg::SMEM, st>>>(q, k, v, a);
+  fn<<<grid, threads, smem, st>>>(q, k, v, a);
   return check_cuda(cudaGetLastError(), "attention");
 }
 
+// tile sets of 256 rows, tiles of 128 rows, tiles of at most 32 / 16 rows
+enum FlashKind { kPairs, kTiles, kFew32, kFew16 };
+
 template <int HD, typename T>
-int launch_flash_t(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const FlashArgs& a, int nt,
-                   int grid, cudaStream_t st) {
-  if (nt == 2) return launch_flash<HD, 2, T>(q, k, v, a, grid, st);
-  if (int rc = launch_flash<HD, 1, T>(q, k, v, a, grid, st)) return rc;
-  if (!a.even) return EC_OK;
+int launch_flash(FlashKind kind, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const FlashArgs& a,
+                 int grid, cudaStream_t st) {
+  const int id = (HD == 64 ? 0 : 8) + (std::is_same<T, __half>::value ? 4 : 0) + kind;
+  int rc;
+  switch (kind) {
+    case kPairs:
+      rc = launch_one(id, flash_kernel<HD, 2, T>, FlashCfg<HD, 2>::THREADS, FlashCfg<HD, 2>::SMEM, q, k, v, a, grid, st);
+      break;
+    case kTiles:
+      rc = launch_one(id, flash_kernel<HD, 1, T>, FlashCfg<HD, 1>::THREADS, FlashCfg<HD, 1>::SMEM, q, k, v, a, grid, st);
+      break;
+    case kFew32:
+      rc = launch_one(id, flash_token_kernel<HD, 32, T>, TokenCfg<HD, 32>::THREADS, TokenCfg<HD, 32>::SMEM, q, k, v, a,
+                      grid, st);
+      break;
+    default:
+      rc = launch_one(id, flash_token_kernel<HD, 16, T>, TokenCfg<HD, 16>::THREADS, TokenCfg<HD, 16>::SMEM, q, k, v, a,
+                      grid, st);
+  }
+  if (rc || !a.even) return rc;
   const int64_t warps = static_cast<int64_t>(a.tokens) * a.q_heads;
   flash_join_kernel<HD, T><<<static_cast<unsigned>((warps + 3) / 4), 128, 0, st>>>(a);
   return check_cuda(cudaGetLastError(), "attention join");
@@ -73,33 +92,43 @@ int launch_flash_t(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap
 
 // How a call is cut up, from what the host knows
 struct FlashPlan {
-  int nt, even, rows_tok;
+  FlashKind kind;
+  int even, rows_tok;  // tokens of a tile
+  int part_rows;
 };
 FlashPlan flash_plan(const KvCache* c, int64_t tokens, int q_heads, int kv_heads, int nseq, int max_new, int num_sms) {
-  FlashPlan p;
-  p.rows_tok = 128 / (q_heads / kv_heads);
-  const int64_t tiles = (tokens / p.rows_tok + nseq) * kv_heads;
-  const int64_t pairs = (tokens / (2 * p.rows_tok) + nseq) * kv_heads;
-  p.even = 0;
-  if (c && nseq <= FlashCfg<128, 1>::MAX_SEQS && (max_new <= p.rows_tok || tiles < 2 * num_sms)) {
-    // block counts are 32-bit
-    const int64_t most = (static_cast<int64_t>(c->width) * c->page_size + 127) / 128;
-    p.even = tiles * most < (int64_t(1) << 30);
+  const int group = q_heads / kv_heads;
+  FlashPlan p{kTiles, 0, 128 / group, 128};
+  if (c && nseq <= FlashCfg<128, 1>::MAX_SEQS) {
+    const int64_t tiles = (tokens / p.rows_tok + nseq) * kv_heads;
+    const int64_t few = static_cast<int64_t>(std::max(1, max_new)) * group;  // rows of a sequence's new tokens
+    // unit counts of the split are 32-bit
+    const int64_t most = (static_cast<int64_t>(c->width) * c->page_size + 127) / 128 + 8;
+    const bool fits = (tokens + nseq) * kv_heads * most < (int64_t(1) << 30);
+    if (fits && few <= 32) {
+      p.kind = few <= 16 ? kFew16 : kFew32;
+      p.part_rows = few <= 16 ? 16 : 32;
+      p.rows_tok = p.part_rows / group;
+      p.even = 1;
+    } else if (fits && tiles < 2 * num_sms) {
+      p.even = 1;
+    }
   }
-  // single tokens: tiles of 64 rows, so that queries can be double-buffered
-  if (p.even && max_new * (q_heads / kv_heads) <= 64) p.rows_tok = std::max(1, 64 / (q_heads / kv_heads));
-  p.nt = !p.even && tokens > static_cast<int64_t>(nseq) * p.rows_tok && pairs >= num_sms ? 2 : 1;
+  if (!p.even && tokens > static_cast<int64_t>(nseq) * p.rows_tok &&
+      (tokens / (2 * p.rows_tok) + nseq) * kv_heads >= num_sms)
+    p.kind = kPairs;
   return p;
 }
 
-size_t part_bytes(int hd) { return static_cast<size_t>(2) * kMaxCtas * 128 * hd * 4; }
+size_t part_bytes(int rows, int hd) { return static_cast<size_t>(2) * kMaxCtas * rows * hd * 4; }
 
 }  // namespace
 
 size_t attention_work_bytes(const KvCache& c, int64_t tokens, int q_heads, int nseq, int max_new) {
-  if (!flash_plan(&c, tokens, q_heads, c.heads, nseq, max_new, kMaxCtas).even) return 256;
-  return part_bytes(c.head_dim <= 64 ? 64 : 128) + 2 * kMaxCtas * 128 * 4 +
-         (static_cast<size_t>(FlashCfg<128, 1>::MAX_SEQS) + 2) * 4;
+  const FlashPlan p = flash_plan(&c, tokens, q_heads, c.heads, nseq, max_new, kMaxCtas);
+  if (!p.even) return 256;
+  return part_bytes(p.part_rows, c.head_dim <= 64 ? 64 : 128) + part_bytes(p.part_rows, 1) +
+         (static_cast<size_t>(nseq) + 2) * 4;
 }
 
 int run_attention(const AttnOp& op, int num_sms, cudaStream_t st) {
@@ -121,9 +150,6 @@ int run_attention(const AttnOp& op, int num_sms, cudaStream_t st) {
     ok = ok && encode_rows(&tk, op.dtype, op.k, op.head_dim, op.kv_heads, op.tokens, 1, 128) &&
          encode_rows(&tv, op.dtype, op.v, op.head_dim, op.kv_heads, op.tokens, 1, 128);
   }
-  if ((op.tokens / (p.nt * p.rows_tok) + op.nseq) * op.kv_heads >= INT32_MAX / 2)
-    return set_error(EC_EINVAL, "%lld tokens of %d sequences and %d key heads: too many for one call",
-                     static_cast<long long>(op.tokens), op.nseq, op.kv_heads);
   if (!ok) return set_error(EC_EINVAL, "the attention's strides cannot be described to the TMA");
   FlashArgs a{};
   a.out = const_cast<void*>(op.out.p), a.ot = op.out.token, a.oh = op.out.head;
@@ -140,23 +166,29 @@ int run_attention(const AttnOp& op, int num_sms, cudaStream_t st) {
     a.pages = c->pages, a.page_size = c->page_size;
     a.page0 = op.layer * c->pages, a.page_end = c->layers * c->pages;
   }
-  a.q_bufs = p.nt == 1 && group * p.rows_tok <= 64 ? 2 : 1;
-  int64_t grid = (op.tokens / (p.nt * p.rows_tok) + op.nseq) * op.kv_heads;
+  a.q_bufs = p.kind == kTiles && group * p.rows_tok <= 64 ? 2 : 1;
+  const int sets = p.rows_tok * (p.kind == kPairs ? 2 : 1);
+  int64_t grid = (op.tokens / sets + op.nseq) * op.kv_heads;
+  if (grid >= INT32_MAX / 2)
+    return set_error(EC_EINVAL, "%lld tokens of %d sequences and %d key heads: too many for one call",
+                     static_cast<long long>(op.tokens), op.nseq, op.kv_heads);
   if (p.even) {
     char* w = static_cast<char*>(op.work);
     a.even = 1;
     a.min_chunk = 4;
+    a.over = 2;
+    a.part_rows = p.part_rows;
     a.part_o = reinterpret_cast<float*>(w);
-    a.part_l = reinterpret_cast<float*>(w + part_bytes(hd));
-    a.plan = reinterpret_cast<int*>(w + part_bytes(hd) + 2 * kMaxCtas * 128 * 4);
+    a.part_l = reinterpret_cast<float*>(w + part_bytes(p.part_rows, hd));
+    a.plan = reinterpret_cast<int*>(w + part_bytes(p.part_rows, hd) + part_bytes(p.part_rows, 1));
     grid = num_sms;
   }
   const int ctas = static_cast<int>(std::min<int64_t>(grid, num_sms));
   if (op.dtype == EC_BF16)
-    return hd == 64 ? launch_flash_t<64, __nv_bfloat16>(tq, tk, tv, a, p.nt, ctas, st)
-                    : launch_flash_t<128, __nv_bfloat16>(tq, tk, tv, a, p.nt, ctas, st);
-  return hd == 64 ? launch_flash_t<64, __half>(tq, tk, tv, a, p.nt, ctas, st)
-                  : launch_flash_t<128, __half>(tq, tk, tv, a, p.nt, ctas, st);
+    return hd == 64 ? launch_flash<64, __nv_bfloat16>(p.kind, tq, tk, tv, a, ctas, st)
+                    : launch_flash<128, __nv_bfloat16>(p.kind, tq, tk, tv, a, ctas, st);
+  return hd == 64 ? launch_flash<64, __half>(p.kind, tq, tk, tv, a, ctas, st)
+                  : launch_flash<128, __half>(p.kind, tq, tk, tv, a, ctas, st);
 }
 
 namespace {

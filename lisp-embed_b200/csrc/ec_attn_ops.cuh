@@ -52,9 +52,11 @@ struct FlashArgs {
   int wide;                // out rows in 32-byte pieces
   int q_bufs;              // 2: queries are double-buffered (NT 1, at most 64 rows)
   int even;                // 1: the blocks are split evenly over the CTAs
-  int min_chunk;           // blocks a CTA takes at least
-  float* part_o;           // [2 * CTAs][128][HD] partial results of cut tiles
-  float* part_l;           // [2 * CTAs][128] their log2-sum-exp2
+  int min_chunk;           // units a CTA takes at least
+  int over;                // units of a tile besides its blocks
+  int part_rows;
+  float* part_o;           // [2 * CTAs][part_rows][HD] partial results of cut tiles
+  float* part_l;           // [2 * CTAs][part_rows] their log2-sum-exp2
   int* plan;               // chunk, prefix sums for the join
 };
 
@@ -172,7 +174,139 @@ __device__ __forceinline__ FlashSeq flash_seq(const FlashArgs& a, int s) {
 // Without a split: slot u of the list is the tile set f(s) + i of sequence s,
 // f(s) = cu[s] / BT + s for BT tokens per set.  f leaves at least
 // ceil(len / BT) slots to every sequence and needs no prefix sum; a slot's
-// sequence is found by bisection.
+// sequence is found by bisection, 32 slots at a time.  Their number (times the
+// key heads) fits 31 bits, checked on the host.
+template <int NT, typename Publish>
+__device__ __noinline__ bool flash_slots(const FlashArgs& a, int lane, Publish publish) {
+  const int R = a.rows_tok, BT = NT * R;
+  const uint32_t slots = a.tokens / BT + a.nseq, all = slots * a.kv_heads, step = gridDim.x;
+  bool ok = true;
+#pragma unroll 1
+  for (uint32_t t0 = 0; ok && t0 < all; t0 += 32 * step) {
+    // late (long) tile sets first; the order turns round every pass, so that
+    // no CTA gets the longest of each
+    const uint32_t t = t0 + lane * step + ((lane & 1) ? step - 1 - blockIdx.x : blockIdx.x);
+    FlashEntry it{};
+    if (t < all) {
+      const int u = static_cast<int>(slots - 1 - t / a.kv_heads);
+      int lo = 0, hi = a.nseq;  // last sequence with f <= u
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (min(max(a.cu[mid], 0), a.tokens) / BT + mid <= u) lo = mid;
+        else hi = mid;
+      }
+      const FlashSeq q = flash_seq(a, lo);
+      const int len = q.end - q.begin;
+      const int i = u - (q.begin / BT + lo);  // tile set of the sequence
+      if (i >= 0 && i < (len + BT - 1) / BT) {
+        const int q0 = i * BT;
+        it.valid = 1;
+        it.tok0 = q.begin + q0;
+        it.qv = min(BT, len - q0);
+        it.kvh = static_cast<int>(t % a.kv_heads);
+        it.pos0 = q.kv_len - len + q0;
+        it.kv_len = q.kv_len;
+        it.kbase = q.kbase;
+        it.nb[0] = blocks_seen(it.pos0, min(R, it.qv), q.kv_len);
+        it.nb[1] = NT == 2 && it.qv > R ? blocks_seen(it.pos0, it.qv, q.kv_len) : 0;
+        it.part = -1;
+      }
+    }
+    __syncwarp();
+    for (unsigned m = __ballot_sync(0xffffffffu, it.valid); ok && m; m &= m - 1) ok = publish(it, __ffs(m) - 1);
+  }
+  return ok;
+}
+
+// Even split: every CTA takes the same share of the key blocks, in the order
+// (sequence, tile, key head, block).  A tile costs its blocks and `over` units
+// more, for its start and end, which come first.  prefix: [nseq + 1] in shared
+// memory, units before each sequence; CTA 0 leaves it in the plan for the join.
+// (Kept out of line, as the next one: inlined into the kernels, the optimiser
+// dropped an iteration of the sequence loop.)
+template <typename Publish>
+__device__ __noinline__ bool flash_even(const FlashArgs& a, int lane, int* prefix, Publish publish) {
+  const int R = a.rows_tok;
+  int total = 0;
+#pragma unroll 1
+  for (int s0 = 0; s0 < a.nseq; s0 += 32) {
+    int v = 0;
+    if (s0 + lane < a.nseq) {
+      const FlashSeq q = flash_seq(a, s0 + lane);
+      const int len = q.end - q.begin;
+#pragma unroll 1
+      for (int i = 0; i < len; i += R) {
+        const int nb = blocks_seen(q.kv_len - len + i, min(R, len - i), q.kv_len);
+        v += nb ? nb + a.over : 0;
+      }
+      v *= a.kv_heads;
+    }
+    int x = v;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, d);
+      if (lane >= d) x += y;
+    }
+    if (s0 + lane < a.nseq) prefix[s0 + lane] = total + x - v;
+    total += __shfl_sync(0xffffffffu, x, 31);
+  }
+  if (lane == 0) prefix[a.nseq] = total;
+  __syncwarp();
+  const int chunk = max(a.min_chunk, (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x));
+  if (blockIdx.x == 0) {
+    for (int s = lane; s <= a.nseq; s += 32) a.plan[1 + s] = prefix[s];
+    if (lane == 0) a.plan[0] = chunk;
+  }
+  const int64_t w64 = static_cast<int64_t>(blockIdx.x) * chunk;
+  const int begin = static_cast<int>(min(w64, static_cast<int64_t>(total)));
+  const int end = static_cast<int>(min(w64 + chunk, static_cast<int64_t>(total)));
+  // last sequence with prefix <= begin (those without blocks are skipped)
+  int lo = 0, hi = a.nseq;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (prefix[mid] <= begin) lo = mid;
+    else hi = mid;
+  }
+  FlashEntry it{};
+  it.valid = 1;
+  bool ok = true;
+#pragma unroll 1
+  for (int s = lo; ok && s < a.nseq; ++s) {
+    int at = prefix[s];
+    if (at >= end) break;
+    const FlashSeq q = flash_seq(a, s);
+    const int len = q.end - q.begin;
+    it.kv_len = q.kv_len;
+    it.kbase = q.kbase;
+#pragma unroll 1
+    for (int i = 0; ok && i < len; i += R) {
+      it.tok0 = q.begin + i;
+      it.qv = min(R, len - i);
+      it.pos0 = q.kv_len - len + i;
+      const int nb = blocks_seen(it.pos0, it.qv, q.kv_len);
+      const int cost = nb ? nb + a.over : 0;
+      // key heads that end before this CTA's share are skipped
+      int h = nb && at < begin ? min(a.kv_heads, (begin - at) / cost) : 0;
+#pragma unroll 1
+      for (; ok && h < a.kv_heads; ++h) {
+        const int block0 = at + h * cost + a.over;  // unit of the tile's first block
+        const int from = max(0, begin - block0), to = min(nb, end - block0);
+        if (from < to) {
+          it.kvh = h;
+          it.kb0 = from;
+          it.nb[0] = to;
+          // a CTA has at most one part that goes on from another CTA and one
+          // that another CTA goes on with
+          it.part = from == 0 && to == nb ? -1 : 2 * static_cast<int>(blockIdx.x) + (from == 0);
+          ok = publish(it);
+        }
+      }
+      at += a.kv_heads * cost;
+    }
+  }
+  // tiles that see no key are nobody's blocks: the join clears their rows
+  return ok;
+}
 
 template <int HD, int NT, typename T>
 __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
@@ -244,7 +378,7 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const int R = a.rows_tok, G = a.group, BT = NT * R;
+  const int R = a.rows_tok, G = a.group;
   bool ok = true;
   unsigned code = kDevTimeoutOther;
 
@@ -289,116 +423,13 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
       ++n;
       return true;
     };
-    Entry it{};
     if (NT == 1 && a.even) {
-      // every CTA takes the same number of key blocks: blocks in the order
-      // (sequence, tile, key head, block), prefix sums over the sequences
-      int total = 0;
-      for (int s0 = 0; s0 < a.nseq; s0 += 32) {
-        int v = 0;
-        if (s0 + lane < a.nseq) {
-          const FlashSeq q = flash_seq(a, s0 + lane);
-          const int len = q.end - q.begin;
-          for (int i = 0; i < len; i += R) v += blocks_seen(q.kv_len - len + i, min(R, len - i), q.kv_len);
-          v *= a.kv_heads;
-        }
-        int x = v;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-          const int y = __shfl_up_sync(0xffffffffu, x, d);
-          if (lane >= d) x += y;
-        }
-        if (s0 + lane < a.nseq) prefix[s0 + lane] = total + x - v;
-        total += __shfl_sync(0xffffffffu, x, 31);
-      }
-      if (lane == 0) prefix[a.nseq] = total;
-      __syncwarp();
-      const int chunk = max(a.min_chunk, (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x));
-      if (blockIdx.x == 0) {
-        for (int s = lane; s <= a.nseq; s += 32) a.plan[1 + s] = prefix[s];
-        if (lane == 0) a.plan[0] = chunk;
-      }
-      int64_t w64 = static_cast<int64_t>(blockIdx.x) * chunk;
-      const int end = static_cast<int>(min(w64 + chunk, static_cast<int64_t>(total)));
-      int w = static_cast<int>(min(w64, static_cast<int64_t>(total)));
-      const int begin = w;
-      // last sequence with prefix <= w (those without blocks are skipped)
-      int lo = 0, hi = a.nseq;
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (prefix[mid] <= w) lo = mid;
-        else hi = mid;
-      }
-      for (int s = lo; ok && w < end; ++s) {
-        const FlashSeq q = flash_seq(a, s);
-        const int len = q.end - q.begin;
-        int at = prefix[s];
-        for (int i = 0; ok && i < len && w < end; i += R) {
-          const int nb = blocks_seen(q.kv_len - len + i, min(R, len - i), q.kv_len);
-          if (at + nb * a.kv_heads <= w) {
-            at += nb * a.kv_heads;
-            continue;
-          }
-          for (int h = 0; ok && h < a.kv_heads && w < end; ++h, at += nb) {
-            if (at + nb <= w) continue;
-            it.valid = 1;
-            it.tok0 = q.begin + i;
-            it.qv = min(R, len - i);
-            it.kvh = h;
-            it.pos0 = q.kv_len - len + i;
-            it.kv_len = q.kv_len;
-            it.kbase = q.kbase;
-            it.kb0 = w - at;
-            it.nb[0] = min(nb, end - at);
-            it.nb[1] = 0;
-            it.part = it.kb0 == 0 && it.nb[0] == nb ? -1 : 2 * static_cast<int>(blockIdx.x) + (w == begin ? 0 : 1);
-            ok = publish(it, 0);
-            w = at + it.nb[0];
-          }
-        }
-      }
-      // tiles that see no key are nobody's blocks: their rows are cleared by
-      // the join
+      ok = flash_even(a, lane, prefix, [&](const Entry& e) { return publish(e, 0); });
     } else {
-      // every lane looks up one of the next 32 candidates
-      // (their number fits 31 bits, checked on the host)
-      const uint32_t slots = a.tokens / BT + a.nseq, all = slots * a.kv_heads, step = gridDim.x;
-      for (uint32_t t0 = 0; ok && t0 < all; t0 += 32 * step) {
-        // late (long) tile sets first; the order turns round every pass, so
-        // that no CTA gets the longest of each
-        const uint32_t t = t0 + lane * step + ((lane & 1) ? step - 1 - blockIdx.x : blockIdx.x);
-        it.valid = 0;
-        if (t < all) {
-          const int u = static_cast<int>(slots - 1 - t / a.kv_heads);
-          int lo = 0, hi = a.nseq;  // last sequence with f <= u
-          while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (min(max(a.cu[mid], 0), a.tokens) / BT + mid <= u) lo = mid;
-            else hi = mid;
-          }
-          const FlashSeq q = flash_seq(a, lo);
-          const int len = q.end - q.begin;
-          const int i = u - (q.begin / BT + lo);  // tile set of the sequence
-          if (i >= 0 && i < (len + BT - 1) / BT) {
-            const int q0 = i * BT;
-            it.valid = 1;
-            it.tok0 = q.begin + q0;
-            it.qv = min(BT, len - q0);
-            it.kvh = static_cast<int>(t % a.kv_heads);
-            it.pos0 = q.kv_len - len + q0;
-            it.kv_len = q.kv_len;
-            it.kbase = q.kbase;
-            it.kb0 = 0;
-            it.nb[0] = blocks_seen(it.pos0, min(R, it.qv), q.kv_len);
-            it.nb[1] = NT == 2 && it.qv > R ? blocks_seen(it.pos0, it.qv, q.kv_len) : 0;
-            it.part = -1;
-          }
-        }
-        for (unsigned m = __ballot_sync(0xffffffffu, it.valid); ok && m; m &= m - 1) ok = publish(it, __ffs(m) - 1);
-      }
+      ok = flash_slots<NT>(a, lane, publish);
     }
-    it.valid = 0;
-    if (ok) ok = publish(it, 0);
+    Entry end{};
+    if (ok) ok = publish(end, 0);
   } else if (warp == W_LOAD) {
     // ---------------------------------------------------------------- loads
     code = kDevTimeoutProducer;
@@ -761,7 +792,7 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
         const int64_t row = it.tok0 + qt;
         const int h = it.kvh * G + head;
         T* o = static_cast<T*>(a.out) + row * a.ot + h * a.oh;
-        float* po = a.part_o + (static_cast<int64_t>(max(it.part, 0)) * 128 + r) * HD;
+        float* po = a.part_o + (static_cast<int64_t>(max(it.part, 0)) * a.part_rows + r) * HD;
 #pragma unroll 1
         for (int c = 0; c < HD / 32; ++c) {
           uint32_t v[32];
@@ -769,31 +800,34 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
             tmem_ld_32x32b_x32(o_addr + c * 32, v);
             tmem_wait_ld();
           }
-          if (!live) continue;
+          if (live) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i)  // 0: a row that sees nothing
-            v[i] = l == 0.f ? 0u : __float_as_uint(__uint_as_float(v[i]) * inv);
-          if (it.part >= 0) {
+            for (int i = 0; i < 32; ++i)  // 0: a row that sees nothing
+              v[i] = l == 0.f ? 0u : __float_as_uint(__uint_as_float(v[i]) * inv);
+            if (it.part >= 0) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) store32(po + c * 32 + 8 * i, v + 8 * i);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] = pack2<T>(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
-            if (a.wide) {
-              if (c * 32 < a.head_dim) store32(o + c * 32, v);
-              if (c * 32 + 16 < a.head_dim) store32(o + c * 32 + 16, v + 8);
+              for (int i = 0; i < 4; ++i) store32(po + c * 32 + 8 * i, v + 8 * i);
             } else {
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
-                if (c * 32 + 8 * i < a.head_dim)
-                  *reinterpret_cast<uint4*>(o + c * 32 + 8 * i) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+              for (int i = 0; i < 16; ++i) v[i] = pack2<T>(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+              if (a.wide) {
+                if (c * 32 < a.head_dim) store32(o + c * 32, v);
+                if (c * 32 + 16 < a.head_dim) store32(o + c * 32 + 16, v + 8);
+              } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  if (c * 32 + 8 * i < a.head_dim)
+                    *reinterpret_cast<uint4*>(o + c * 32 + 8 * i) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+              }
             }
           }
+          __syncwarp();  // the loads from TMEM are the whole warp's
         }
         if (live) {
-          if (it.part >= 0) a.part_l[it.part * 128 + r] = l2;
+          if (it.part >= 0) a.part_l[it.part * a.part_rows + r] = l2;
           else if (a.lse) a.lse[row * a.q_heads + h] = l2 * 0.693147180559945309f;
         }
+        __syncwarp();
       }
       tc_fence_before();
     }
@@ -813,6 +847,458 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
   if (warp == W_MMA) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
+  }
+}
+
+// --------------------------------------------------------------- few rows --
+// The same for tiles of at most NR rows (single tokens and their query heads),
+// with the operands the other way round: S^T = K Q^T has a key per TMEM lane
+// and a row per column, so that the four softmax warps share a block's keys
+// and every lane has work, and O^T += V^T P^T has an element of the head per
+// lane.  What bounds it then is reading K and V.  The warps agree on a block's
+// row maxima through shared memory.
+template <int HD, int NR>
+struct TokenCfg {
+  static constexpr int AT = HD / 64;
+  static constexpr uint32_t ATOM = 16384;
+  static constexpr uint32_t TILE = AT * ATOM;          // 128 keys
+  static constexpr int STAGES = (NR == 16 ? 6 : 5) * (HD == 128 ? 1 : 2);
+  static constexpr uint32_t QATOM = NR * 128;          // 64 columns of the queries
+  static constexpr uint32_t QBUF = AT * QATOM;
+  static constexpr uint32_t PBUF = 2 * NR * 128;       // P^T: NR rows x 128 keys
+  static constexpr int MAX_SEQS = FlashCfg<HD, 1>::MAX_SEQS;
+  static constexpr int THREADS = 7 * 32;
+  static constexpr uint32_t XCH = 2 * 4 * NR * 4;      // row maxima of the warps
+  static constexpr uint32_t TAIL = 1280 + XCH + 4 * (MAX_SEQS + 1);
+  static constexpr size_t SMEM = STAGES * TILE + 2 * QBUF + 2 * PBUF + TAIL;
+  static constexpr uint32_t COLS = NR == 16 ? 64 : 128;  // two S^T, one O^T
+  static_assert(SMEM <= 232448, "shared memory");
+};
+
+__device__ __forceinline__ float warp_max(float v) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+template <int NR>
+__device__ __forceinline__ void tmem_ld_rows(uint32_t addr, uint32_t (&r)[NR]) {
+  if constexpr (NR == 16) tmem_ld_32x32b_x16(addr, r);
+  else tmem_ld_32x32b_x32(addr, r);
+}
+template <int NR>
+__device__ __forceinline__ void tmem_st_rows(uint32_t addr, const uint32_t (&r)[NR]) {
+  if constexpr (NR == 16) tmem_st_32x32b_x16(addr, r);
+  else tmem_st_32x32b_x32(addr, r);
+}
+
+template <int HD, int NR, typename T>
+__global__ void __launch_bounds__(TokenCfg<HD, NR>::THREADS, 1)
+    flash_token_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                       const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ FlashArgs a) {
+  using Cfg = TokenCfg<HD, NR>;
+  constexpr int AT = Cfg::AT, ST = Cfg::STAGES;
+  constexpr int FMT = std::is_same<T, __half>::value ? 0 : 1;
+  constexpr uint32_t IDESC_S = make_idesc(FMT, 128, NR);
+  constexpr uint32_t IDESC_PV = make_idesc(FMT, 128, NR) | (1u << 15);  // A (V^T) MN-major
+  constexpr int W_LOAD = 4, W_MMA = 5, W_LIST = 6, READERS = 6;
+
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if (smem_u32(smem) & 1023u) {
+    if (threadIdx.x == 0) report(&g_op_status, kDevBadArg);
+    return;
+  }
+  uint8_t* sKV = smem;
+  uint8_t* sQ = sKV + ST * Cfg::TILE;
+  uint8_t* sP = sQ + 2 * Cfg::QBUF;
+  uint8_t* tail = sP + 2 * Cfg::PBUF;
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(tail);  // [2]
+  uint64_t* q_empty = q_full + 2;
+  uint64_t* kv_full = q_empty + 2;
+  uint64_t* kv_empty = kv_full + ST;
+  uint64_t* s_full = kv_empty + ST;  // [2] even / odd blocks, as the next two
+  uint64_t* p_full = s_full + 2;
+  uint64_t* o_full = p_full + 2;
+  uint64_t* x_bar = o_full + 2;      // [2] the four softmax warps
+  uint64_t* i_full = x_bar + 2;
+  uint64_t* i_empty = i_full + kFlashRing;
+  FlashItem* items = reinterpret_cast<FlashItem*>(i_empty + kFlashRing);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(items + kFlashRing);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  static_assert(8 * (4 + 2 * ST + 8 + 2 * kFlashRing) + kFlashRing * sizeof(FlashItem) + 8 <= 1280, "tail");
+  float* xch = reinterpret_cast<float*>(tail + 1280);  // [2][4][NR]
+  int* prefix = reinterpret_cast<int*>(tail + 1280 + Cfg::XCH);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < ST; ++i) {
+      mbar_init(&kv_full[i], 1);
+      mbar_init(&kv_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], 1);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&o_full[i], 1);
+      mbar_init(&x_bar[i], 4);
+    }
+    for (int i = 0; i < kFlashRing; ++i) {
+      mbar_init(&i_full[i], 1);
+      mbar_init(&i_empty[i], READERS);
+    }
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == W_LOAD && lane == 0) {
+    tma_prefetch_desc(&tm_q);
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+  }
+  if (warp == W_MMA) {
+    tmem_alloc(tmem_slot, Cfg::COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int R = a.rows_tok, G = a.group;
+  bool ok = true;
+  unsigned code = kDevTimeoutOther;
+  int it_n = 0;
+  auto next_item = [&]() -> const FlashItem* {
+    const int b = it_n % kFlashRing;
+    if (!mbar_wait_warp(&i_full[b], (it_n / kFlashRing) & 1, abort_flag)) return nullptr;
+    return &items[b];
+  };
+  auto done_item = [&] {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&i_empty[it_n % kFlashRing]);
+    ++it_n;
+  };
+  const int ppb = 128 / a.page_size;
+  auto fetch = [&](int slot, int e, int in_use) -> int {
+    int p = -1;
+    if (e < in_use) p = a.tables[static_cast<int64_t>(slot) * a.width + e];
+    return p >= 0 && p < a.pages ? a.page0 + p : a.page_end;
+  };
+
+  if (warp == W_LIST) {
+    int n = 0;
+    auto publish = [&](const FlashEntry& it) -> bool {
+      const int b = n % kFlashRing;
+      if (!mbar_wait_warp(&i_empty[b], ((n / kFlashRing) & 1) ^ 1, abort_flag)) return false;
+      if (it.valid)
+        items[b].pages[lane] = fetch(it.kbase, it.kb0 * ppb + lane, (it.kv_len + a.page_size - 1) / a.page_size);
+      if (lane == 0) *static_cast<FlashEntry*>(&items[b]) = it;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&i_full[b]);
+      ++n;
+      return true;
+    };
+    ok = flash_even(a, lane, prefix, publish);
+    FlashEntry end{};
+    if (ok) ok = publish(end);
+  } else if (warp == W_LOAD) {
+    code = kDevTimeoutProducer;
+    int st = 0, qi = 0;
+    uint32_t ph = 0;
+    while (true) {
+      const FlashItem* it = next_item();
+      if (!(ok = it != nullptr) || !it->valid) break;
+      const int kb0 = it->kb0, nb = it->nb[0], kvh = it->kvh, kbase = it->kbase, tok0 = it->tok0;
+      const int in_use = (it->kv_len + a.page_size - 1) / a.page_size;
+      int page = it->pages[lane], ahead = 0;
+      done_item();
+      int first = kb0 * ppb;
+      if (nb * ppb > first + 32) ahead = fetch(kbase, first + 32 + lane, in_use);
+      for (int j = kb0; ok && j < nb; ++j) {
+        if (j * ppb - first == 32) {
+          first += 32;
+          page = ahead;
+          ahead = fetch(kbase, first + 32 + lane, in_use);
+        }
+        int p[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p[i] = __shfl_sync(0xffffffffu, page, (j * ppb - first + i) & 31);
+#pragma unroll 1
+        for (int kv = 0; kv < 2; ++kv) {
+          if (!(ok = mbar_wait_warp(&kv_empty[st], ph ^ 1, abort_flag))) break;
+          const uint32_t dst = smem_u32(sKV + st * Cfg::TILE), bar = smem_u32(&kv_full[st]);
+          const uint64_t map = reinterpret_cast<uint64_t>(kv ? &tm_v : &tm_k);
+          if (elect_one()) {
+            mbar_arrive_expect_tx(&kv_full[st], Cfg::TILE);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+              for (int c = 0; c < AT; ++c)
+                if (i < ppb)
+                  asm volatile(
+                      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], "
+                      "[%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst + c * Cfg::ATOM + i * a.page_size * 128),
+                      "l"(map), "r"(bar), "r"(c * 64), "r"(kvh), "r"(0), "r"(p[i])
+                      : "memory");
+          }
+          __syncwarp();
+          if (++st == ST) {
+            st = 0;
+            ph ^= 1;
+          }
+          if (j == kb0 && kv == 0) {
+            const int qb = qi & 1;
+            const uint32_t qp = (qi >> 1) & 1;
+            ++qi;
+            if (!(ok = mbar_wait_warp(&q_empty[qb], qp ^ 1, abort_flag))) break;
+            if (elect_one()) {
+              mbar_arrive_expect_tx(&q_full[qb], AT * static_cast<uint32_t>(G * R) * 128u);
+#pragma unroll
+              for (int c = 0; c < AT; ++c)
+                asm volatile(
+                    "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], "
+                    "[%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(sQ + qb * Cfg::QBUF + c * Cfg::QATOM)),
+                    "l"(reinterpret_cast<uint64_t>(&tm_q)), "r"(smem_u32(&q_full[qb])), "r"(c * 64), "r"(kvh * G),
+                    "r"(tok0)
+                    : "memory");
+            }
+            __syncwarp();
+          }
+        }
+      }
+      if (!ok) break;
+    }
+  } else if (warp == W_MMA) {
+    code = kDevTimeoutMma;
+    if (elect_one()) {
+      int st = 0, qi = 0;
+      uint32_t ph = 0, g = 0;
+      const uint64_t dq = desc_sw128_kmajor(smem_u32(sQ));
+      const uint64_t dk = desc_sw128_kmajor(smem_u32(sKV));
+      const uint64_t dp = desc_sw128_kmajor(smem_u32(sP));
+      // a 64-wide head has one atom: rows 64 .. 127 of O^T repeat the first
+      const uint64_t dv = desc_mnmajor<false>(smem_u32(sKV), AT == 2 ? Cfg::ATOM : 0);
+      auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+        const bool fine = mbar_wait(bar, parity, abort_flag);
+        tc_fence_after();
+        return fine;
+      };
+      auto advance = [&] {
+        if (++st == ST) {
+          st = 0;
+          ph ^= 1;
+        }
+      };
+      auto mma_s = [&](int qb, int stage, uint32_t d) {
+        const uint64_t q = dq + qb * (Cfg::QBUF >> 4), k = dk + stage * (Cfg::TILE >> 4);
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; ++kk)
+          umma_f16(d, k + (((kk >> 2) * Cfg::ATOM + (kk & 3) * 32) >> 4),
+                   q + (((kk >> 2) * Cfg::QATOM + (kk & 3) * 32) >> 4), IDESC_S, kk > 0);
+      };
+      while (true) {
+        const int b = it_n % kFlashRing;
+        if (!(ok = mbar_wait(&i_full[b], (it_n / kFlashRing) & 1, abort_flag))) break;
+        const int valid = items[b].valid, n = items[b].nb[0] - items[b].kb0;
+        mbar_arrive(&i_empty[b]);
+        ++it_n;
+        if (!valid) break;
+        const int qb = qi & 1;
+        if (!(ok = wait(&q_full[qb], (qi >> 1) & 1)) || !(ok = wait(&kv_full[st], ph))) break;
+        ++qi;
+        mma_s(qb, st, tmem + (g & 1) * NR);
+        umma_commit(&s_full[g & 1]);
+        umma_commit(&kv_empty[st]);
+        if (n == 1) umma_commit(&q_empty[qb]);
+        advance();
+        for (int j = 0; j < n; ++j, ++g) {
+          const int sv = st;
+          const uint32_t phv = ph;
+          advance();
+          if (j + 1 < n) {
+            if (!(ok = wait(&kv_full[st], ph))) break;
+            mma_s(qb, st, tmem + ((g + 1) & 1) * NR);
+            umma_commit(&s_full[(g + 1) & 1]);
+            umma_commit(&kv_empty[st]);
+            if (j + 2 == n) umma_commit(&q_empty[qb]);
+            advance();
+          }
+          if (!(ok = wait(&kv_full[sv], phv)) || !(ok = wait(&p_full[g & 1], (g >> 1) & 1))) break;
+          const uint64_t v = dv + sv * (Cfg::TILE >> 4), p = dp + (g & 1) * (Cfg::PBUF >> 4);
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk)
+            umma_f16(tmem + 2 * NR, v + kk * (2048 >> 4), p + (((kk >> 2) * (NR * 128) + (kk & 3) * 32) >> 4), IDESC_PV,
+                     j > 0 || kk > 0);
+          umma_commit(&o_full[g & 1]);
+          umma_commit(&kv_empty[sv]);
+        }
+        if (!ok) break;
+      }
+      if (!ok) {
+        report(&g_op_status, code);
+        *abort_flag = 1;
+      }
+    }
+    __syncwarp();
+  } else {
+    // -------------------------------------------------------------- softmax
+    code = kDevTimeoutEpilogue;
+    const int key = warp * 32 + lane;  // TMEM lane: key of the block / element of the head
+    const uint32_t t_lane = tmem + (static_cast<uint32_t>(warp * 32) << 16);
+    const uint32_t o_addr = t_lane + 2 * NR;
+    const float sc = a.scale_log2;
+    const int nr = G * R;  // rows in use
+    int g = 0, e = 0, x = 0;
+    // every warp's values of the rows, from all four warps
+    auto exchange = [&](float mine) -> const float* {
+      float* slot = xch + (x & 1) * 4 * NR;
+      if (lane < NR) slot[warp * NR + lane] = mine;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&x_bar[x & 1]);
+      ok = mbar_wait_warp(&x_bar[x & 1], (x >> 1) & 1, abort_flag);
+      ++x;
+      return slot;
+    };
+    while (true) {
+      const FlashItem* ip = next_item();
+      if (!(ok = ip != nullptr) || !ip->valid) break;
+      const FlashEntry it = *ip;
+      done_item();
+      const int n = it.nb[0] - it.kb0, rows = min(nr, it.qv * G);
+      float m[NR], l[NR];
+#pragma unroll
+      for (int i = 0; i < NR; ++i) m[i] = -INFINITY, l[i] = 0.f;
+      for (int j = 0; j < n; ++j, ++g) {
+        const int buf = g & 1;
+        if (!(ok = mbar_wait_warp(&s_full[buf], (g >> 1) & 1, abort_flag))) break;
+        tc_fence_after();
+        const int at = (it.kb0 + j) * 128 + key;  // this lane's key
+        if (it.kv_len - (it.kb0 + j) * 128 < 128) {
+          // what a page holds behind the sequence: 0 * NaN would not be 0
+          const int entry = e + 2 * j + 1;
+          if (!(ok = mbar_wait_warp(&kv_full[entry % ST], (entry / ST) & 1, abort_flag))) break;
+          if (at >= it.kv_len) {
+            uint8_t* v = sKV + (entry % ST) * Cfg::TILE + key * 128;
+#pragma unroll 1
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+              for (int c = 0; c < AT; ++c) *reinterpret_cast<uint4*>(v + c * Cfg::ATOM + i * 16) = make_uint4(0, 0, 0, 0);
+          }
+          __syncwarp();
+        }
+        uint32_t s[NR];
+        tmem_ld_rows<NR>(t_lane + buf * NR, s);
+        tmem_wait_ld();
+        float mine = -INFINITY;
+        int own = it.pos0, head = 0;  // position of row i's token: the last key that it sees
+        // (all NR rows: what lies in those without a query reaches nothing)
+#pragma unroll
+        for (int i = 0; i < NR; ++i) {
+          if (at >= it.kv_len || at > own) s[i] = 0xff800000u;
+          if (++head == G) head = 0, ++own;
+          const float v = warp_max(__uint_as_float(s[i]));
+          mine = lane == i ? v : mine;
+        }
+        const float* top4 = exchange(mine);
+        if (!ok) break;
+        float corr[NR];
+        bool grown = false;
+#pragma unroll
+        for (int i = 0; i < NR; ++i) {
+          const float top = fmaxf(fmaxf(top4[i], top4[NR + i]), fmaxf(top4[2 * NR + i], top4[3 * NR + i]));
+          // keep the older maximum unless the new one is 2^8 above it
+          const bool grow = i < rows && ((top - m[i]) * sc > 8.f || (m[i] == -INFINITY && top > m[i]));
+          corr[i] = grow ? fa_exp2((m[i] - top) * sc) : 1.f;
+          l[i] *= corr[i];
+          m[i] = grow ? top : m[i];
+          grown |= grow;
+        }
+        if (grown && j > 0) {  // the same in every thread
+          if (!(ok = mbar_wait_warp(&o_full[(g - 1) & 1], ((g - 1) >> 1) & 1, abort_flag))) break;
+          tc_fence_after();
+          uint32_t o[NR];
+          tmem_ld_rows<NR>(o_addr, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < NR; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr[i]);
+          tmem_st_rows<NR>(o_addr, o);
+          tmem_wait_st();
+        }
+        uint8_t* prow = sP + buf * Cfg::PBUF + (key >> 6) * (NR * 128) + (key & 7) * 2;
+#pragma unroll
+        for (int i = 0; i < NR; ++i) {
+          const float nm = m[i] == -INFINITY ? 0.f : -m[i] * sc;
+          const float p = fa_exp2(fmaf(__uint_as_float(s[i]), sc, nm));
+          l[i] += p;
+          *reinterpret_cast<uint16_t*>(prow + i * 128 + ((((key & 63) >> 3) ^ (i & 7)) << 4)) =
+              static_cast<uint16_t>(pack2<T>(p, 0.f));
+        }
+        fence_proxy_async_smem();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[buf]);
+      }
+      if (!ok) break;
+      e += 2 * n;
+      // the rows' sums over the lanes, then over the warps
+      float mine = 0.f;
+#pragma unroll
+      for (int i = 0; i < NR; ++i) {
+        float v = l[i];
+#pragma unroll
+        for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+        mine = lane == i ? v : mine;
+      }
+      const float* l4 = exchange(mine);
+      if (!ok) break;
+      if (!(ok = mbar_wait_warp(&o_full[(g - 1) & 1], ((g - 1) >> 1) & 1, abort_flag))) break;
+      tc_fence_after();
+      uint32_t o[NR];
+      tmem_ld_rows<NR>(o_addr, o);
+      tmem_wait_ld();
+      tc_fence_before();
+      // the row of this lane's statistics, and its element of every row
+      const float mine_l = lane < NR ? (l4[lane] + l4[NR + lane]) + (l4[2 * NR + lane] + l4[3 * NR + lane]) : 0.f;
+      float mine_m = 0.f;
+#pragma unroll
+      for (int i = 0; i < NR; ++i) mine_m = lane == i ? m[i] : mine_m;
+      if (warp == 0 && lane < rows) {
+        const float l2 = mine_l == 0.f ? -INFINITY : mine_m * sc + log2f(mine_l);
+        if (it.part >= 0) a.part_l[it.part * a.part_rows + lane] = l2;
+        else if (a.lse)
+          a.lse[static_cast<int64_t>(it.tok0 + lane / G) * a.q_heads + it.kvh * G + lane % G] = l2 * 0.693147180559945309f;
+      }
+      const float mine_inv = mine_l > 0.f ? 1.f / mine_l : mine_l;  // 0 stays 0, NaN NaN
+      int64_t to = it.tok0 * a.ot + static_cast<int64_t>(it.kvh) * G * a.oh + key;
+      int head = 0;
+#pragma unroll
+      for (int i = 0; i < NR; ++i) {
+        const float inv = __shfl_sync(0xffffffffu, mine_inv, i);
+        const float v = inv == 0.f ? 0.f : __uint_as_float(o[i]) * inv;
+        if (it.part >= 0) {
+          if (key < HD && i < rows) a.part_o[(static_cast<int64_t>(it.part) * a.part_rows + i) * HD + key] = v;
+        } else if (key < a.head_dim && i < rows) {
+          reinterpret_cast<uint16_t*>(a.out)[to] = static_cast<uint16_t>(pack2<T>(v, 0.f));
+        }
+        to += a.oh;
+        if (++head == G) head = 0, to += a.ot - G * a.oh;
+      }
+      __syncwarp();
+    }
+  }
+  if (!ok) {
+    report(&g_op_status, code);
+    *abort_flag = 1;
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) {
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 2000000ull) {
+    }
+  }
+  if (warp == W_MMA) {
+    tc_fence_after();
+    tmem_dealloc(tmem, Cfg::COLS);
   }
 }
 
@@ -836,11 +1322,12 @@ __global__ void flash_join_kernel(const __grid_constant__ FlashArgs a) {
   const int len = q.end - q.begin, R = a.rows_tok;
   const int tile = (t - q.begin) / R, kvh = h / a.group, row = (t - q.begin - tile * R) * a.group + h % a.group;
   int at = a.plan[1 + lo], nb = 0;
+#pragma unroll 1
   for (int i = 0; i <= tile; ++i) {
-    at += nb * a.kv_heads;
+    at += nb ? (nb + a.over) * a.kv_heads : 0;
     nb = blocks_seen(q.kv_len - len + i * R, min(R, len - i * R), q.kv_len);
   }
-  at += nb * kvh;
+  at += (nb + a.over) * kvh + a.over;  // unit of its first block
   T* out = static_cast<T*>(a.out) + t * a.ot + h * a.oh;
   if (nb == 0) {
     for (int i = lane; i < a.head_dim; i += 32) out[i] = T(0.f);
@@ -850,18 +1337,18 @@ __global__ void flash_join_kernel(const __grid_constant__ FlashArgs a) {
   const int chunk = max(a.plan[0], 1);
   const int c0 = at / chunk, c1 = min((at + nb - 1) / chunk, kMaxCtas - 1);
   if (c0 == c1) return;  // one CTA had all of it
-  const int p0 = 2 * c0 + (at == c0 * chunk ? 0 : 1);  // later parts are their CTA's first
+  auto part = [&](int c) { return 2 * c + (c == c0); };
   float m = -INFINITY;
-  for (int c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, a.part_l[(c == c0 ? p0 : 2 * c) * 128 + row]);
+  for (int c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, a.part_l[part(c) * a.part_rows + row]);
 #pragma unroll
   for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
   float sum = 0.f, o[HD / 32] = {};
+#pragma unroll 2
   for (int c = c0; c <= c1; ++c) {
-    const int p = c == c0 ? p0 : 2 * c;
-    const float l2 = a.part_l[p * 128 + row];
+    const float l2 = a.part_l[part(c) * a.part_rows + row];
     const float x = l2 == -INFINITY ? 0.f : fa_exp2(l2 - m);
     sum += x;
-    const float* po = a.part_o + (static_cast<int64_t>(p) * 128 + row) * HD;
+    const float* po = a.part_o + (static_cast<int64_t>(part(c)) * a.part_rows + row) * HD;
 #pragma unroll
     for (int i = 0; i < HD / 32; ++i) o[i] += x * po[lane + 32 * i];
   }
