@@ -61,13 +61,20 @@ int launch_one(int id, FlashFn fn, int threads, size_t smem, const CUtensorMap& 
   return check_cuda(cudaGetLastError(), "attention");
 }
 
-// tile sets of 256 rows, tiles of 128 rows, tiles of at most 32 / 16 rows
-enum FlashKind { kPairs, kTiles, kFew32, kFew16 };
+// tile sets of 256 rows, tiles of 128 rows, tiles of at most 32 .. 4 rows
+enum FlashKind { kPairs, kTiles, kFew32, kFew16, kFew8, kFew4 };
+
+template <int HD, int NP, typename T>
+int launch_token(int id, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const FlashArgs& a, int grid,
+                 cudaStream_t st) {
+  using Cfg = TokenCfg<HD, NP>;
+  return launch_one(id, flash_token_kernel<HD, NP, T>, Cfg::THREADS, Cfg::SMEM, q, k, v, a, grid, st);
+}
 
 template <int HD, typename T>
 int launch_flash(FlashKind kind, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const FlashArgs& a,
                  int grid, cudaStream_t st) {
-  const int id = (HD == 64 ? 0 : 8) + (std::is_same<T, __half>::value ? 4 : 0) + kind;
+  const int id = (HD == 64 ? 0 : 16) + (std::is_same<T, __half>::value ? 8 : 0) + kind;
   int rc;
   switch (kind) {
     case kPairs:
@@ -76,13 +83,10 @@ int launch_flash(FlashKind kind, const CUtensorMap& q, const CUtensorMap& k, con
     case kTiles:
       rc = launch_one(id, flash_kernel<HD, 1, T>, FlashCfg<HD, 1>::THREADS, FlashCfg<HD, 1>::SMEM, q, k, v, a, grid, st);
       break;
-    case kFew32:
-      rc = launch_one(id, flash_token_kernel<HD, 32, T>, TokenCfg<HD, 32>::THREADS, TokenCfg<HD, 32>::SMEM, q, k, v, a,
-                      grid, st);
-      break;
-    default:
-      rc = launch_one(id, flash_token_kernel<HD, 16, T>, TokenCfg<HD, 16>::THREADS, TokenCfg<HD, 16>::SMEM, q, k, v, a,
-                      grid, st);
+    case kFew32: rc = launch_token<HD, 32, T>(id, q, k, v, a, grid, st); break;
+    case kFew16: rc = launch_token<HD, 16, T>(id, q, k, v, a, grid, st); break;
+    case kFew8: rc = launch_token<HD, 8, T>(id, q, k, v, a, grid, st); break;
+    default: rc = launch_token<HD, 4, T>(id, q, k, v, a, grid, st);
   }
   if (rc || !a.even) return rc;
   const int64_t warps = static_cast<int64_t>(a.tokens) * a.q_heads;
@@ -106,8 +110,8 @@ FlashPlan flash_plan(const KvCache* c, int64_t tokens, int q_heads, int kv_heads
     const int64_t most = (static_cast<int64_t>(c->width) * c->page_size + 127) / 128 + 8;
     const bool fits = (tokens + nseq) * kv_heads * most < (int64_t(1) << 30);
     if (fits && few <= 32) {
-      p.kind = few <= 16 ? kFew16 : kFew32;
-      p.part_rows = few <= 16 ? 16 : 32;
+      p.kind = few <= 4 ? kFew4 : few <= 8 ? kFew8 : few <= 16 ? kFew16 : kFew32;
+      p.part_rows = few <= 4 ? 4 : few <= 8 ? 8 : few <= 16 ? 16 : 32;
       p.rows_tok = p.part_rows / group;
       p.even = 1;
     } else if (fits && tiles < 2 * num_sms) {

@@ -445,6 +445,7 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
       if (nb <= kb0) continue;
       int first = kb0 * ppb;  // table entry of lane 0's page
       if (a.paged && nb * ppb > first + 32) ahead = fetch(kbase, first + 32 + lane, in_use);
+#pragma unroll 1
       for (int j = kb0; ok && j < nb; ++j) {
         if (a.paged && j * ppb - first == 32) {
           first += 32;
@@ -578,6 +579,7 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
           umma_commit(&kv_empty[st]);
           if (n == 1) umma_commit(&q_empty[qb]);
           advance();
+#pragma unroll 1
           for (int j = 0; ok && j < n; ++j) {
             const int sv = st;
             const uint32_t phv = ph;
@@ -617,6 +619,7 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
           umma_commit(&kv_empty[st]);
           if (n == 1) umma_commit(&q_empty[qb]);
           advance();
+#pragma unroll 1
           for (int j = 0; j < n; ++j, ++g) {
             const int sv = st;
             const uint32_t phv = ph;
@@ -669,6 +672,7 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
       const int vis = live ? min(it.kv_len, it.pos0 + qt + 1) : 0;
       const int n = (t ? it.nb[1] : it.nb[0]) - it.kb0;
       float m = -INFINITY, l = 0.f;  // maximum (raw score) that O and l are relative to
+#pragma unroll 1
       for (int j = 0; j < n; ++j, ++g) {
         const int buf = NT == 2 ? t : g & 1;
         const uint32_t s_addr = t_lane + buf * 128;
@@ -851,14 +855,18 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
 }
 
 // --------------------------------------------------------------- few rows --
-// The same for tiles of at most NR rows (single tokens and their query heads),
+// The same for tiles of at most NP rows (single tokens and their query heads),
 // with the operands the other way round: S^T = K Q^T has a key per TMEM lane
 // and a row per column, so that the four softmax warps share a block's keys
 // and every lane has work, and O^T += V^T P^T has an element of the head per
 // lane.  What bounds it then is reading K and V.  The warps agree on a block's
-// row maxima through shared memory.
-template <int HD, int NR>
+// row maxima through shared memory.  One warp runs per scheduler, so a block
+// takes as long as its instructions do, one after the other: NP = 4, 8, 16 and
+// 32 rows each have their own kernel (the MMA's N is 16 at least; what the
+// columns behind NP hold reaches nothing).
+template <int HD, int NP>
 struct TokenCfg {
+  static constexpr int NR = NP < 16 ? 16 : NP;         // columns of the MMAs
   static constexpr int AT = HD / 64;
   static constexpr uint32_t ATOM = 16384;
   static constexpr uint32_t TILE = AT * ATOM;          // 128 keys
@@ -868,7 +876,7 @@ struct TokenCfg {
   static constexpr uint32_t PBUF = 2 * NR * 128;       // P^T: NR rows x 128 keys
   static constexpr int MAX_SEQS = FlashCfg<HD, 1>::MAX_SEQS;
   static constexpr int THREADS = 7 * 32;
-  static constexpr uint32_t XCH = 2 * 4 * NR * 4;      // row maxima of the warps
+  static constexpr uint32_t XCH = 2 * 4 * NP * 4;      // row maxima of the warps
   static constexpr uint32_t TAIL = 1280 + XCH + 4 * (MAX_SEQS + 1);
   static constexpr size_t SMEM = STAGES * TILE + 2 * QBUF + 2 * PBUF + TAIL;
   static constexpr uint32_t COLS = NR == 16 ? 64 : 128;  // two S^T, one O^T
@@ -881,23 +889,48 @@ __device__ __forceinline__ float warp_max(float v) {
   return r;
 }
 
-template <int NR>
-__device__ __forceinline__ void tmem_ld_rows(uint32_t addr, uint32_t (&r)[NR]) {
-  if constexpr (NR == 16) tmem_ld_32x32b_x16(addr, r);
-  else tmem_ld_32x32b_x32(addr, r);
+// NP 32-bit columns of this thread's TMEM lane
+template <int NP>
+__device__ __forceinline__ void tmem_ld_rows(uint32_t addr, uint32_t (&r)[NP]) {
+  if constexpr (NP == 4) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+  } else if constexpr (NP == 8) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(addr)
+                 : "memory");
+  } else if constexpr (NP == 16) {
+    tmem_ld_32x32b_x16(addr, r);
+  } else {
+    tmem_ld_32x32b_x32(addr, r);
+  }
 }
-template <int NR>
-__device__ __forceinline__ void tmem_st_rows(uint32_t addr, const uint32_t (&r)[NR]) {
-  if constexpr (NR == 16) tmem_st_32x32b_x16(addr, r);
-  else tmem_st_32x32b_x32(addr, r);
+template <int NP>
+__device__ __forceinline__ void tmem_st_rows(uint32_t addr, const uint32_t (&r)[NP]) {
+  if constexpr (NP == 4) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(r[0]), "r"(r[1]),
+                 "r"(r[2]), "r"(r[3])
+                 : "memory");
+  } else if constexpr (NP == 8) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr), "r"(r[0]),
+                 "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+  } else if constexpr (NP == 16) {
+    tmem_st_32x32b_x16(addr, r);
+  } else {
+    tmem_st_32x32b_x32(addr, r);
+  }
 }
 
-template <int HD, int NR, typename T>
-__global__ void __launch_bounds__(TokenCfg<HD, NR>::THREADS, 1)
+template <int HD, int NP, typename T>
+__global__ void __launch_bounds__(TokenCfg<HD, NP>::THREADS, 1)
     flash_token_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                        const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ FlashArgs a) {
-  using Cfg = TokenCfg<HD, NR>;
-  constexpr int AT = Cfg::AT, ST = Cfg::STAGES;
+  using Cfg = TokenCfg<HD, NP>;
+  constexpr int AT = Cfg::AT, ST = Cfg::STAGES, NR = Cfg::NR;
   constexpr int FMT = std::is_same<T, __half>::value ? 0 : 1;
   constexpr uint32_t IDESC_S = make_idesc(FMT, 128, NR);
   constexpr uint32_t IDESC_PV = make_idesc(FMT, 128, NR) | (1u << 15);  // A (V^T) MN-major
@@ -926,7 +959,7 @@ __global__ void __launch_bounds__(TokenCfg<HD, NR>::THREADS, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(items + kFlashRing);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   static_assert(8 * (4 + 2 * ST + 8 + 2 * kFlashRing) + kFlashRing * sizeof(FlashItem) + 8 <= 1280, "tail");
-  float* xch = reinterpret_cast<float*>(tail + 1280);  // [2][4][NR]
+  float* xch = reinterpret_cast<float*>(tail + 1280);  // [2][4][NP]
   int* prefix = reinterpret_cast<int*>(tail + 1280 + Cfg::XCH);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -1013,6 +1046,7 @@ __global__ void __launch_bounds__(TokenCfg<HD, NR>::THREADS, 1)
       done_item();
       int first = kb0 * ppb;
       if (nb * ppb > first + 32) ahead = fetch(kbase, first + 32 + lane, in_use);
+#pragma unroll 1
       for (int j = kb0; ok && j < nb; ++j) {
         if (j * ppb - first == 32) {
           first += 32;
@@ -1110,6 +1144,7 @@ __global__ void __launch_bounds__(TokenCfg<HD, NR>::THREADS, 1)
         umma_commit(&kv_empty[st]);
         if (n == 1) umma_commit(&q_empty[qb]);
         advance();
+#pragma unroll 1
         for (int j = 0; j < n; ++j, ++g) {
           const int sv = st;
           const uint32_t phv = ph;
@@ -1148,15 +1183,21 @@ __global__ void __launch_bounds__(TokenCfg<HD, NR>::THREADS, 1)
     const float sc = a.scale_log2;
     const int nr = G * R;  // rows in use
     int g = 0, e = 0, x = 0;
-    // every warp's values of the rows, from all four warps
-    auto exchange = [&](float mine) -> const float* {
-      float* slot = xch + (x & 1) * 4 * NR;
-      if (lane < NR) slot[warp * NR + lane] = mine;
+    // every warp's values of the rows (lane i: row i), from all four warps
+    auto exchange = [&](float mine, float (&all)[4][NP]) {
+      float* slot = xch + (x & 1) * 4 * NP;
+      if (lane < NP) slot[warp * NP + lane] = mine;
       __syncwarp();
       if (lane == 0) mbar_arrive(&x_bar[x & 1]);
       ok = mbar_wait_warp(&x_bar[x & 1], (x >> 1) & 1, abort_flag);
       ++x;
-      return slot;
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int i = 0; i < NP; i += 4) {
+          const float4 v = *reinterpret_cast<const float4*>(slot + c * NP + i);
+          all[c][i] = v.x, all[c][i + 1] = v.y, all[c][i + 2] = v.z, all[c][i + 3] = v.w;
+        }
     };
     while (true) {
       const FlashItem* ip = next_item();
@@ -1164,9 +1205,10 @@ __global__ void __launch_bounds__(TokenCfg<HD, NR>::THREADS, 1)
       const FlashEntry it = *ip;
       done_item();
       const int n = it.nb[0] - it.kb0, rows = min(nr, it.qv * G);
-      float m[NR], l[NR];
+      float m[NP], l[NP];
 #pragma unroll
-      for (int i = 0; i < NR; ++i) m[i] = -INFINITY, l[i] = 0.f;
+      for (int i = 0; i < NP; ++i) m[i] = -INFINITY, l[i] = 0.f;
+#pragma unroll 1
       for (int j = 0; j < n; ++j, ++g) {
         const int buf = g & 1;
         if (!(ok = mbar_wait_warp(&s_full[buf], (g >> 1) & 1, abort_flag))) break;
@@ -1185,26 +1227,27 @@ __global__ void __launch_bounds__(TokenCfg<HD, NR>::THREADS, 1)
           }
           __syncwarp();
         }
-        uint32_t s[NR];
-        tmem_ld_rows<NR>(t_lane + buf * NR, s);
+        uint32_t s[NP];
+        tmem_ld_rows<NP>(t_lane + buf * NR, s);
         tmem_wait_ld();
         float mine = -INFINITY;
         int own = it.pos0, head = 0;  // position of row i's token: the last key that it sees
-        // (all NR rows: what lies in those without a query reaches nothing)
+        // (all NP rows: what lies in those without a query reaches nothing)
 #pragma unroll
-        for (int i = 0; i < NR; ++i) {
+        for (int i = 0; i < NP; ++i) {
           if (at >= it.kv_len || at > own) s[i] = 0xff800000u;
           if (++head == G) head = 0, ++own;
           const float v = warp_max(__uint_as_float(s[i]));
           mine = lane == i ? v : mine;
         }
-        const float* top4 = exchange(mine);
+        float all[4][NP];
+        exchange(mine, all);
         if (!ok) break;
-        float corr[NR];
+        float corr[NP];
         bool grown = false;
 #pragma unroll
-        for (int i = 0; i < NR; ++i) {
-          const float top = fmaxf(fmaxf(top4[i], top4[NR + i]), fmaxf(top4[2 * NR + i], top4[3 * NR + i]));
+        for (int i = 0; i < NP; ++i) {
+          const float top = fmaxf(fmaxf(all[0][i], all[1][i]), fmaxf(all[2][i], all[3][i]));
           // keep the older maximum unless the new one is 2^8 above it
           const bool grow = i < rows && ((top - m[i]) * sc > 8.f || (m[i] == -INFINITY && top > m[i]));
           corr[i] = grow ? fa_exp2((m[i] - top) * sc) : 1.f;
@@ -1215,17 +1258,17 @@ __global__ void __launch_bounds__(TokenCfg<HD, NR>::THREADS, 1)
         if (grown && j > 0) {  // the same in every thread
           if (!(ok = mbar_wait_warp(&o_full[(g - 1) & 1], ((g - 1) >> 1) & 1, abort_flag))) break;
           tc_fence_after();
-          uint32_t o[NR];
-          tmem_ld_rows<NR>(o_addr, o);
+          uint32_t o[NP];
+          tmem_ld_rows<NP>(o_addr, o);
           tmem_wait_ld();
 #pragma unroll
-          for (int i = 0; i < NR; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr[i]);
-          tmem_st_rows<NR>(o_addr, o);
+          for (int i = 0; i < NP; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr[i]);
+          tmem_st_rows<NP>(o_addr, o);
           tmem_wait_st();
         }
         uint8_t* prow = sP + buf * Cfg::PBUF + (key >> 6) * (NR * 128) + (key & 7) * 2;
 #pragma unroll
-        for (int i = 0; i < NR; ++i) {
+        for (int i = 0; i < NP; ++i) {
           const float nm = m[i] == -INFINITY ? 0.f : -m[i] * sc;
           const float p = fa_exp2(fmaf(__uint_as_float(s[i]), sc, nm));
           l[i] += p;
@@ -1242,25 +1285,28 @@ __global__ void __launch_bounds__(TokenCfg<HD, NR>::THREADS, 1)
       // the rows' sums over the lanes, then over the warps
       float mine = 0.f;
 #pragma unroll
-      for (int i = 0; i < NR; ++i) {
+      for (int i = 0; i < NP; ++i) {
         float v = l[i];
 #pragma unroll
         for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
         mine = lane == i ? v : mine;
       }
-      const float* l4 = exchange(mine);
+      float all[4][NP];
+      exchange(mine, all);
       if (!ok) break;
       if (!(ok = mbar_wait_warp(&o_full[(g - 1) & 1], ((g - 1) >> 1) & 1, abort_flag))) break;
       tc_fence_after();
-      uint32_t o[NR];
-      tmem_ld_rows<NR>(o_addr, o);
+      uint32_t o[NP];
+      tmem_ld_rows<NP>(o_addr, o);
       tmem_wait_ld();
       tc_fence_before();
       // the row of this lane's statistics, and its element of every row
-      const float mine_l = lane < NR ? (l4[lane] + l4[NR + lane]) + (l4[2 * NR + lane] + l4[3 * NR + lane]) : 0.f;
-      float mine_m = 0.f;
+      float mine_l = 0.f, mine_m = 0.f;
 #pragma unroll
-      for (int i = 0; i < NR; ++i) mine_m = lane == i ? m[i] : mine_m;
+      for (int i = 0; i < NP; ++i) {
+        mine_l = lane == i ? (all[0][i] + all[1][i]) + (all[2][i] + all[3][i]) : mine_l;
+        mine_m = lane == i ? m[i] : mine_m;
+      }
       if (warp == 0 && lane < rows) {
         const float l2 = mine_l == 0.f ? -INFINITY : mine_m * sc + log2f(mine_l);
         if (it.part >= 0) a.part_l[it.part * a.part_rows + lane] = l2;
@@ -1271,7 +1317,7 @@ __global__ void __launch_bounds__(TokenCfg<HD, NR>::THREADS, 1)
       int64_t to = it.tok0 * a.ot + static_cast<int64_t>(it.kvh) * G * a.oh + key;
       int head = 0;
 #pragma unroll
-      for (int i = 0; i < NR; ++i) {
+      for (int i = 0; i < NP; ++i) {
         const float inv = __shfl_sync(0xffffffffu, mine_inv, i);
         const float v = inv == 0.f ? 0.f : __uint_as_float(o[i]) * inv;
         if (it.part >= 0) {
