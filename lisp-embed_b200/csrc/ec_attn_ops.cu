@@ -88,10 +88,7 @@ int launch_flash(FlashKind kind, const CUtensorMap& q, const CUtensorMap& k, con
     case kFew8: rc = launch_token<HD, 8, T>(id, q, k, v, a, grid, st); break;
     default: rc = launch_token<HD, 4, T>(id, q, k, v, a, grid, st);
   }
-  if (rc || !a.even) return rc;
-  const int64_t warps = static_cast<int64_t>(a.tokens) * a.q_heads;
-  flash_join_kernel<HD, T><<<static_cast<unsigned>((warps + 3) / 4), 128, 0, st>>>(a);
-  return check_cuda(cudaGetLastError(), "attention join");
+  return rc;
 }
 
 // How a call is cut up, from what the host knows
@@ -131,8 +128,7 @@ size_t part_bytes(int rows, int hd) { return static_cast<size_t>(2) * kMaxCtas *
 size_t attention_work_bytes(const KvCache& c, int64_t tokens, int q_heads, int nseq, int max_new) {
   const FlashPlan p = flash_plan(&c, tokens, q_heads, c.heads, nseq, max_new, kMaxCtas);
   if (!p.even) return 256;
-  return part_bytes(p.part_rows, c.head_dim <= 64 ? 64 : 128) + part_bytes(p.part_rows, 1) +
-         (static_cast<size_t>(nseq) + 2) * 4;
+  return part_bytes(p.part_rows, c.head_dim <= 64 ? 64 : 128) + part_bytes(p.part_rows, 1) + kMaxCtas * 4;
 }
 
 int run_attention(const AttnOp& op, int num_sms, cudaStream_t st) {
@@ -180,11 +176,11 @@ int run_attention(const AttnOp& op, int num_sms, cudaStream_t st) {
     char* w = static_cast<char*>(op.work);
     a.even = 1;
     a.min_chunk = 4;
-    a.over = 2;
+    a.over = 1;
     a.part_rows = p.part_rows;
     a.part_o = reinterpret_cast<float*>(w);
     a.part_l = reinterpret_cast<float*>(w + part_bytes(p.part_rows, hd));
-    a.plan = reinterpret_cast<int*>(w + part_bytes(p.part_rows, hd) + part_bytes(p.part_rows, 1));
+    a.arrived = reinterpret_cast<int*>(w + part_bytes(p.part_rows, hd) + part_bytes(p.part_rows, 1));
     grid = num_sms;
   }
   const int ctas = static_cast<int>(std::min<int64_t>(grid, num_sms));

@@ -57,7 +57,7 @@ struct FlashArgs {
   int part_rows;
   float* part_o;           // [2 * CTAs][part_rows][HD] partial results of cut tiles
   float* part_l;           // [2 * CTAs][part_rows] their log2-sum-exp2
-  int* plan;               // chunk, prefix sums for the join
+  int* arrived;            // [CTAs] parts done of the tile whose first part is the CTA's; 0 between calls
 };
 
 // a tile set that one CTA works on
@@ -71,6 +71,7 @@ struct FlashEntry {
   int kb0;        // first key block
   int nb[2];      // end block of each tile
   int part;       // partial result, -1: the whole of the tile's keys
+  int c0, parts;  // CTA of the tile's first part, their number
 };
 struct FlashItem : FlashEntry {
   int pages[32];  // cache: the first 32 pages from block kb0 on
@@ -96,7 +97,7 @@ struct FlashCfg {
   static constexpr int MAX_SEQS = 2048;              // prefix sums of an even split
   static constexpr int WARPS = 4 * NT + 3;
   static constexpr int THREADS = 32 * WARPS;
-  static constexpr uint32_t TAIL = 1280 + (NT == 1 ? 4 * (MAX_SEQS + 1) : 0);
+  static constexpr uint32_t TAIL = 1536 + (NT == 1 ? 8 * MAX_SEQS : 0);
   static constexpr size_t SMEM = NT * TILE + STAGES * TILE + TAIL;
   static constexpr uint32_t O_COL = 256;
   static_assert(SMEM <= 232448, "shared memory");
@@ -220,27 +221,46 @@ __device__ __noinline__ bool flash_slots(const FlashArgs& a, int lane, Publish p
 
 // Even split: every CTA takes the same share of the key blocks, in the order
 // (sequence, tile, key head, block).  A tile costs its blocks and `over` units
-// more, for its start and end, which come first.  prefix: [nseq + 1] in shared
-// memory, units before each sequence; CTA 0 leaves it in the plan for the join.
-// (Kept out of line, as the next one: inlined into the kernels, the optimiser
-// dropped an iteration of the sequence loop.)
+// more, for its start and end, which come first.  Where there are fewer tiles
+// than CTAs and all are short, every tile has a CTA of its own instead.
+//
+// Each thread of the CTA first looks at some sequences (the loads are far
+// away, and the CTA has nothing else to do yet): units[s], and tiles | longest
+// tile << 16, with the sign bit where a tile sees no key.
+constexpr int kTileAlone = 8;  // units of a tile that is not worth cutting
+__device__ __forceinline__ void flash_measure(const FlashArgs& a, int* units, int* about) {
+  for (int s = threadIdx.x; s < a.nseq; s += blockDim.x) {
+    const FlashSeq q = flash_seq(a, s);
+    const int len = q.end - q.begin, R = a.rows_tok;
+    int v = 0, n = 0, most = 0, none = 0;
+#pragma unroll 1
+    for (int i = 0; i < len; i += R) {
+      const int nb = blocks_seen(q.kv_len - len + i, min(R, len - i), q.kv_len);
+      if (nb) v += nb + a.over, ++n, most = nb + a.over;
+      else none = 1;
+    }
+    units[s] = v * a.kv_heads;
+    about[s] = min(n * a.kv_heads, 0xffff) | min(most, 0x7fff) << 16 | none << 31;
+  }
+}
+// (Kept out of line, as the list above: inlined into the kernels, the
+// optimiser dropped an iteration of the sequence loop.)
 template <typename Publish>
-__device__ __noinline__ bool flash_even(const FlashArgs& a, int lane, int* prefix, Publish publish) {
-  const int R = a.rows_tok;
+__device__ __noinline__ bool flash_even(const FlashArgs& a, int lane, int* prefix, const int* about, Publish publish) {
+  const int R = a.rows_tok, ctas = gridDim.x, me = blockIdx.x;
+  int tiles = 0, most = 0;
+  for (int s = lane; s < a.nseq; s += 32) {
+    tiles += about[s] & 0xffff;
+    most = max(most, about[s] >> 16 & 0x7fff);
+  }
+  tiles = __reduce_add_sync(0xffffffffu, min(tiles, 1 << 20));
+  most = __reduce_max_sync(0xffffffffu, most);
+  const bool alone = tiles <= ctas && most <= kTileAlone;  // every tile padded to the longest
   int total = 0;
 #pragma unroll 1
   for (int s0 = 0; s0 < a.nseq; s0 += 32) {
     int v = 0;
-    if (s0 + lane < a.nseq) {
-      const FlashSeq q = flash_seq(a, s0 + lane);
-      const int len = q.end - q.begin;
-#pragma unroll 1
-      for (int i = 0; i < len; i += R) {
-        const int nb = blocks_seen(q.kv_len - len + i, min(R, len - i), q.kv_len);
-        v += nb ? nb + a.over : 0;
-      }
-      v *= a.kv_heads;
-    }
+    if (s0 + lane < a.nseq) v = alone ? (about[s0 + lane] & 0xffff) * most : prefix[s0 + lane];
     int x = v;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -250,14 +270,9 @@ __device__ __noinline__ bool flash_even(const FlashArgs& a, int lane, int* prefi
     if (s0 + lane < a.nseq) prefix[s0 + lane] = total + x - v;
     total += __shfl_sync(0xffffffffu, x, 31);
   }
-  if (lane == 0) prefix[a.nseq] = total;
   __syncwarp();
-  const int chunk = max(a.min_chunk, (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x));
-  if (blockIdx.x == 0) {
-    for (int s = lane; s <= a.nseq; s += 32) a.plan[1 + s] = prefix[s];
-    if (lane == 0) a.plan[0] = chunk;
-  }
-  const int64_t w64 = static_cast<int64_t>(blockIdx.x) * chunk;
+  const int chunk = alone ? max(most, 1) : max(a.min_chunk, (total + ctas - 1) / ctas);
+  const int64_t w64 = static_cast<int64_t>(me) * chunk;
   const int begin = static_cast<int>(min(w64, static_cast<int64_t>(total)));
   const int end = static_cast<int>(min(w64 + chunk, static_cast<int64_t>(total)));
   // last sequence with prefix <= begin (those without blocks are skipped)
@@ -284,7 +299,7 @@ __device__ __noinline__ bool flash_even(const FlashArgs& a, int lane, int* prefi
       it.qv = min(R, len - i);
       it.pos0 = q.kv_len - len + i;
       const int nb = blocks_seen(it.pos0, it.qv, q.kv_len);
-      const int cost = nb ? nb + a.over : 0;
+      const int cost = nb == 0 ? 0 : alone ? most : nb + a.over;
       // key heads that end before this CTA's share are skipped
       int h = nb && at < begin ? min(a.kv_heads, (begin - at) / cost) : 0;
 #pragma unroll 1
@@ -297,15 +312,83 @@ __device__ __noinline__ bool flash_even(const FlashArgs& a, int lane, int* prefi
           it.nb[0] = to;
           // a CTA has at most one part that goes on from another CTA and one
           // that another CTA goes on with
-          it.part = from == 0 && to == nb ? -1 : 2 * static_cast<int>(blockIdx.x) + (from == 0);
+          it.part = from == 0 && to == nb ? -1 : 2 * me + (from == 0);
+          it.c0 = block0 / chunk;
+          it.parts = (block0 + nb - 1) / chunk - it.c0 + 1;
           ok = publish(it);
         }
       }
       at += a.kv_heads * cost;
     }
   }
-  // tiles that see no key are nobody's blocks: the join clears their rows
+  // tiles that see no key: entries without blocks, whose rows are cleared
+#pragma unroll 1
+  for (int s = me; ok && s < a.nseq; s += ctas) {
+    if (about[s] >= 0) continue;
+    const FlashSeq q = flash_seq(a, s);
+    const int len = q.end - q.begin;
+    it.kv_len = q.kv_len;
+    it.kbase = q.kbase;
+    it.kb0 = it.nb[0] = 0;
+    it.part = -1;
+#pragma unroll 1
+    for (int i = 0; ok && i < len; i += R) {
+      it.tok0 = q.begin + i;
+      it.qv = min(R, len - i);
+      it.pos0 = q.kv_len - len + i;
+      if (blocks_seen(it.pos0, it.qv, q.kv_len)) break;
+#pragma unroll 1
+      for (int h = 0; ok && h < a.kv_heads; ++h) {
+        it.kvh = h;
+        ok = publish(it);
+      }
+    }
+  }
   return ok;
+}
+
+// The CTA that finishes a cut tile's last part joins the parts: one warp per
+// row, in the order of the keys.
+template <int HD, typename T>
+__device__ __noinline__ void flash_join(const FlashArgs& a, int tok0, int qv, int kvh, int c0, int parts, int warp,
+                                        int lane) {
+  const int rows = qv * a.group;
+  auto part = [&](int i) { return static_cast<int64_t>(2 * (c0 + i) + (i == 0)) * a.part_rows; };
+#pragma unroll 1
+  for (int row = warp; row < rows; row += 4) {
+    float m = -INFINITY;
+    for (int i = lane; i < parts; i += 32) m = fmaxf(m, __ldcg(&a.part_l[part(i) + row]));
+#pragma unroll
+    for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+    float sum = 0.f, o[HD / 32] = {};
+#pragma unroll 4
+    for (int i = 0; i < parts; ++i) {
+      const float l2 = __ldcg(&a.part_l[part(i) + row]);
+      const float x = l2 == -INFINITY ? 0.f : fa_exp2(l2 - m);
+      sum += x;
+#pragma unroll
+      for (int e = 0; e < HD / 32; ++e) o[e] += x * __ldcg(&a.part_o[(part(i) + row) * HD + lane + 32 * e]);
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const int64_t tok = tok0 + row / a.group;
+    const int h = kvh * a.group + row % a.group;
+    uint16_t* out = static_cast<uint16_t*>(a.out) + tok * a.ot + h * a.oh;
+#pragma unroll
+    for (int e = 0; e < HD / 32; ++e)
+      if (lane + 32 * e < a.head_dim) out[lane + 32 * e] = static_cast<uint16_t>(pack2<T>(o[e] * inv, 0.f));
+    if (lane == 0 && a.lse)
+      a.lse[tok * a.q_heads + h] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * 0.693147180559945309f;
+  }
+}
+
+// Counts a finished part; true in the CTA that finished the last one, which
+// leaves the count at 0 for the next call.  By one thread, after all threads
+// have written the part and fenced.
+__device__ __forceinline__ bool flash_arrive(const FlashArgs& a, const FlashEntry& it) {
+  const bool last = atomicAdd(&a.arrived[it.c0], 1) == it.parts - 1;
+  if (last) a.arrived[it.c0] = 0;
+  __threadfence();
+  return last;
 }
 
 template <int HD, int NT, typename T>
@@ -336,13 +419,15 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
   uint64_t* p_full = s_full + 2;      // [2]
   uint64_t* p_half = p_full + 2;      // [2] the first 64 keys' P
   uint64_t* o_full = p_half + 2;      // [2] tile (NT 2), or even / odd blocks (NT 1)
-  uint64_t* i_full = o_full + 2;      // [kFlashRing]
+  uint64_t* x_bar = o_full + 2;       // [2] the softmax warps of NT 1
+  uint64_t* i_full = x_bar + 2;       // [kFlashRing]
   uint64_t* i_empty = i_full + kFlashRing;
   FlashItem* items = reinterpret_cast<FlashItem*>(i_empty + kFlashRing);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(items + kFlashRing);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  int* prefix = reinterpret_cast<int*>(tail + 1280);  // [nseq + 1] of an even split
-  static_assert(8 * (4 + 2 * ST + 8 + 2 * kFlashRing) + kFlashRing * sizeof(FlashItem) + 8 <= 1280, "tail");
+  volatile int* last_part = abort_flag + 1;
+  int* prefix = reinterpret_cast<int*>(tail + 1536);  // [MAX_SEQS] of an even split
+  static_assert(8 * (4 + 2 * ST + 10 + 2 * kFlashRing) + kFlashRing * sizeof(FlashItem) + 12 <= 1536, "tail");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -357,6 +442,7 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
       mbar_init(&p_full[i], 4);
       mbar_init(&p_half[i], 4);
       mbar_init(&o_full[i], 1);
+      mbar_init(&x_bar[i], 4);
     }
     for (int i = 0; i < kFlashRing; ++i) {
       mbar_init(&i_full[i], 1);
@@ -374,6 +460,7 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
+  if (NT == 1 && a.even) flash_measure(a, prefix, prefix + Cfg::MAX_SEQS);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -424,7 +511,7 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
       return true;
     };
     if (NT == 1 && a.even) {
-      ok = flash_even(a, lane, prefix, [&](const Entry& e) { return publish(e, 0); });
+      ok = flash_even(a, lane, prefix, prefix + Cfg::MAX_SEQS, [&](const Entry& e) { return publish(e, 0); });
     } else {
       ok = flash_slots<NT>(a, lane, publish);
     }
@@ -660,6 +747,7 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
     int g = 0;       // blocks so far (of this tile)
     int e = 0;       // K / V tiles before this item's
     int done = 0;    // tiles whose result was read (NT 2)
+    int x = 0;       // meetings of the four warps (NT 1)
     while (true) {
       const FlashItem* ip = next_item();
       if (!(ok = ip != nullptr) || !ip->valid) break;
@@ -833,6 +921,21 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
         }
         __syncwarp();
       }
+      if (NT == 1 && it.part >= 0) {
+        __threadfence();
+        auto meet = [&]() -> bool {  // the four warps
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&x_bar[x & 1]);
+          const bool fine = mbar_wait_warp(&x_bar[x & 1], (x >> 1) & 1, abort_flag);
+          ++x;
+          return fine;
+        };
+        if (!(ok = meet())) break;  // every warp has written its rows
+        if (warp == 0 && lane == 0) *last_part = flash_arrive(a, it);
+        if (!(ok = meet())) break;
+        if (*last_part) flash_join<HD, T>(a, it.tok0, it.qv, it.kvh, it.c0, it.parts, warp, lane);
+        __syncwarp();
+      }
       tc_fence_before();
     }
   }
@@ -877,7 +980,7 @@ struct TokenCfg {
   static constexpr int MAX_SEQS = FlashCfg<HD, 1>::MAX_SEQS;
   static constexpr int THREADS = 7 * 32;
   static constexpr uint32_t XCH = 2 * 4 * NP * 4;      // row maxima of the warps
-  static constexpr uint32_t TAIL = 1280 + XCH + 4 * (MAX_SEQS + 1);
+  static constexpr uint32_t TAIL = 1536 + XCH + 8 * MAX_SEQS;
   static constexpr size_t SMEM = STAGES * TILE + 2 * QBUF + 2 * PBUF + TAIL;
   static constexpr uint32_t COLS = NR == 16 ? 64 : 128;  // two S^T, one O^T
   static_assert(SMEM <= 232448, "shared memory");
@@ -958,9 +1061,9 @@ __global__ void __launch_bounds__(TokenCfg<HD, NP>::THREADS, 1)
   FlashItem* items = reinterpret_cast<FlashItem*>(i_empty + kFlashRing);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(items + kFlashRing);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  static_assert(8 * (4 + 2 * ST + 8 + 2 * kFlashRing) + kFlashRing * sizeof(FlashItem) + 8 <= 1280, "tail");
-  float* xch = reinterpret_cast<float*>(tail + 1280);  // [2][4][NP]
-  int* prefix = reinterpret_cast<int*>(tail + 1280 + Cfg::XCH);
+  static_assert(8 * (4 + 2 * ST + 8 + 2 * kFlashRing) + kFlashRing * sizeof(FlashItem) + 8 <= 1536, "tail");
+  float* xch = reinterpret_cast<float*>(tail + 1536);  // [2][4][NP]
+  int* prefix = reinterpret_cast<int*>(tail + 1536 + Cfg::XCH);  // [MAX_SEQS]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -992,6 +1095,7 @@ __global__ void __launch_bounds__(TokenCfg<HD, NP>::THREADS, 1)
     tmem_alloc(tmem_slot, Cfg::COLS);
     tmem_relinquish();
   }
+  flash_measure(a, prefix, prefix + Cfg::MAX_SEQS);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -1030,7 +1134,7 @@ __global__ void __launch_bounds__(TokenCfg<HD, NP>::THREADS, 1)
       ++n;
       return true;
     };
-    ok = flash_even(a, lane, prefix, publish);
+    ok = flash_even(a, lane, prefix, prefix + Cfg::MAX_SEQS, publish);
     FlashEntry end{};
     if (ok) ok = publish(end);
   } else if (warp == W_LOAD) {
@@ -1044,6 +1148,7 @@ __global__ void __launch_bounds__(TokenCfg<HD, NP>::THREADS, 1)
       const int in_use = (it->kv_len + a.page_size - 1) / a.page_size;
       int page = it->pages[lane], ahead = 0;
       done_item();
+      if (nb <= kb0) continue;
       int first = kb0 * ppb;
       if (nb * ppb > first + 32) ahead = fetch(kbase, first + 32 + lane, in_use);
 #pragma unroll 1
@@ -1136,6 +1241,7 @@ __global__ void __launch_bounds__(TokenCfg<HD, NP>::THREADS, 1)
         mbar_arrive(&i_empty[b]);
         ++it_n;
         if (!valid) break;
+        if (n <= 0) continue;
         const int qb = qi & 1;
         if (!(ok = wait(&q_full[qb], (qi >> 1) & 1)) || !(ok = wait(&kv_full[st], ph))) break;
         ++qi;
@@ -1294,12 +1400,14 @@ __global__ void __launch_bounds__(TokenCfg<HD, NP>::THREADS, 1)
       float all[4][NP];
       exchange(mine, all);
       if (!ok) break;
-      if (!(ok = mbar_wait_warp(&o_full[(g - 1) & 1], ((g - 1) >> 1) & 1, abort_flag))) break;
-      tc_fence_after();
       uint32_t o[NP];
-      tmem_ld_rows<NP>(o_addr, o);
-      tmem_wait_ld();
-      tc_fence_before();
+      if (n > 0) {
+        if (!(ok = mbar_wait_warp(&o_full[(g - 1) & 1], ((g - 1) >> 1) & 1, abort_flag))) break;
+        tc_fence_after();
+        tmem_ld_rows<NP>(o_addr, o);
+        tmem_wait_ld();
+        tc_fence_before();
+      }
       // the row of this lane's statistics, and its element of every row
       float mine_l = 0.f, mine_m = 0.f;
 #pragma unroll
@@ -1329,6 +1437,15 @@ __global__ void __launch_bounds__(TokenCfg<HD, NP>::THREADS, 1)
         if (++head == G) head = 0, to += a.ot - G * a.oh;
       }
       __syncwarp();
+      if (it.part >= 0) {
+        __threadfence();
+        exchange(0.f, all);  // every warp has written its share
+        if (!ok) break;
+        exchange(warp == 0 && lane == 0 && flash_arrive(a, it) ? 1.f : 0.f, all);
+        if (!ok) break;
+        if (all[0][0] != 0.f) flash_join<HD, T>(a, it.tok0, it.qv, it.kvh, it.c0, it.parts, warp, lane);
+        __syncwarp();
+      }
     }
   }
   if (!ok) {
@@ -1346,66 +1463,6 @@ __global__ void __launch_bounds__(TokenCfg<HD, NP>::THREADS, 1)
     tc_fence_after();
     tmem_dealloc(tmem, Cfg::COLS);
   }
-}
-
-// Joins the partial results of the tiles that the even split cut, and clears
-// the rows that see no key.  One warp per (token, query head).
-template <int HD, typename T>
-__global__ void flash_join_kernel(const __grid_constant__ FlashArgs a) {
-  const int64_t w = (blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x) >> 5;
-  const int lane = threadIdx.x & 31;
-  if (w >= static_cast<int64_t>(a.tokens) * a.q_heads) return;
-  const int t = static_cast<int>(w / a.q_heads), h = static_cast<int>(w % a.q_heads);
-  // last sequence that begins at or before t
-  int lo = 0, hi = a.nseq;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (a.cu[mid] <= t) lo = mid;
-    else hi = mid;
-  }
-  const FlashSeq q = flash_seq(a, lo);
-  if (t < q.begin || t >= q.end) return;
-  const int len = q.end - q.begin, R = a.rows_tok;
-  const int tile = (t - q.begin) / R, kvh = h / a.group, row = (t - q.begin - tile * R) * a.group + h % a.group;
-  int at = a.plan[1 + lo], nb = 0;
-#pragma unroll 1
-  for (int i = 0; i <= tile; ++i) {
-    at += nb ? (nb + a.over) * a.kv_heads : 0;
-    nb = blocks_seen(q.kv_len - len + i * R, min(R, len - i * R), q.kv_len);
-  }
-  at += (nb + a.over) * kvh + a.over;  // unit of its first block
-  T* out = static_cast<T*>(a.out) + t * a.ot + h * a.oh;
-  if (nb == 0) {
-    for (int i = lane; i < a.head_dim; i += 32) out[i] = T(0.f);
-    if (lane == 0 && a.lse) a.lse[w] = -INFINITY;
-    return;
-  }
-  const int chunk = max(a.plan[0], 1);
-  const int c0 = at / chunk, c1 = min((at + nb - 1) / chunk, kMaxCtas - 1);
-  if (c0 == c1) return;  // one CTA had all of it
-  auto part = [&](int c) { return 2 * c + (c == c0); };
-  float m = -INFINITY;
-  for (int c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, a.part_l[part(c) * a.part_rows + row]);
-#pragma unroll
-  for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-  float sum = 0.f, o[HD / 32] = {};
-#pragma unroll 2
-  for (int c = c0; c <= c1; ++c) {
-    const float l2 = a.part_l[part(c) * a.part_rows + row];
-    const float x = l2 == -INFINITY ? 0.f : fa_exp2(l2 - m);
-    sum += x;
-    const float* po = a.part_o + (static_cast<int64_t>(part(c)) * a.part_rows + row) * HD;
-#pragma unroll
-    for (int i = 0; i < HD / 32; ++i) o[i] += x * po[lane + 32 * i];
-  }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll
-  for (int i = 0; i < HD / 32; ++i)
-    if (lane + 32 * i < a.head_dim) {
-      const uint32_t v = pack2<T>(o[i] * inv, 0.f);
-      reinterpret_cast<uint16_t*>(out)[lane + 32 * i] = static_cast<uint16_t>(v);
-    }
-  if (lane == 0 && a.lse) a.lse[w] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * 0.693147180559945309f;
 }
 
 }  // namespace ec
