@@ -82,7 +82,7 @@ struct FlashItem : FlashEntry {
 constexpr int kFmaEvery = 4;
 
 // work-list entries in flight
-constexpr int kFlashRing = 4;
+constexpr int kFlashRing = 3;
 // Second query buffer of NT 1: 64 rows of 128 bytes after the first.  A tile's
 // operand is 128 rows all the same; what the rest reads (the other buffer, or
 // keys) only reaches rows of S and O that belong to no query.

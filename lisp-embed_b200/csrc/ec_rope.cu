@@ -45,14 +45,29 @@ __device__ double rope_freq(const TableArgs& a, int i) {
   return f;
 }
 
-__global__ void rope_table_kernel(const TableArgs a) {
-  const int64_t n = a.positions * a.half;
+// Thread (i, r): pair i of `run` consecutive positions.  The first angle and the
+// step of one position are turned into cos and sin once; the rest follows by
+// rotating in double, which drifts by a few 2^-53 a step (run <= 64: far below
+// the fp32 result).  Computing every angle's cos and sin took 150 us for
+// 262144 x 32; this is bounded by the stores.
+__global__ void rope_table_kernel(const TableArgs a, int run) {
+  const int64_t runs = (a.positions + run - 1) / run, n = runs * a.half;
   for (int64_t e = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; e < n;
        e += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-    double s, c;
-    sincos(static_cast<double>(e / a.half) * rope_freq(a, static_cast<int>(e % a.half)), &s, &c);
-    a.cos_t[e] = static_cast<float>(c * a.amplitude);
-    a.sin_t[e] = static_cast<float>(s * a.amplitude);
+    const int i = static_cast<int>(e % a.half);
+    const int64_t p0 = e / a.half * run;
+    const double f = rope_freq(a, i);
+    double s, c, s1, c1;
+    sincos(static_cast<double>(p0) * f, &s, &c);
+    sincos(f, &s1, &c1);
+    const int64_t end = min(p0 + run, a.positions);
+    for (int64_t p = p0; p < end; ++p) {
+      a.cos_t[p * a.half + i] = static_cast<float>(c * a.amplitude);
+      a.sin_t[p * a.half + i] = static_cast<float>(s * a.amplitude);
+      const double t = c * c1 - s * s1;
+      s = s * c1 + c * s1;
+      c = t;
+    }
   }
 }
 
@@ -85,17 +100,19 @@ struct alignas(sizeof(T) * V) Vec {
   T e[V];
 };
 
-// One thread: V pairs (or V elements of the tail) of one token's head.  The
-// angle's cos and sin are read once for `V` pairs and kept for the heads.
-template <typename T, int V, bool INTER>
+// One thread: V pairs (or V elements of the tail) of a token's heads h0 ..
+// h0 + heads_per - 1.  The angle's cos and sin are read once for them, and the
+// elements of up to four heads are under way together.  I: index type that
+// holds the number of threads.
+template <typename T, int V, bool INTER, typename I>
 __global__ void rope_kernel(const RopeArgs a, int per_head, int groups, int heads_per) {
   using VT = Vec<T, V>;
   using VF = Vec<float, V>;
-  const int64_t n = a.tokens * groups * per_head;
-  for (int64_t e = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; e < n;
-       e += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+  constexpr int B = 4;
+  const I n = static_cast<I>(a.tokens) * groups * per_head;
+  for (I e = static_cast<I>(blockIdx.x) * blockDim.x + threadIdx.x; e < n; e += static_cast<I>(gridDim.x) * blockDim.x) {
     const int c = static_cast<int>(e % per_head);
-    const int64_t tg = e / per_head;
+    const I tg = e / per_head;
     const int g = static_cast<int>(tg % groups);
     const int64_t t = tg / groups;
     const int32_t p = a.pos[t];
@@ -104,7 +121,7 @@ __global__ void rope_kernel(const RopeArgs a, int per_head, int groups, int head
     const T* x = static_cast<const T*>(a.x) + t * a.xt;
     T* y = static_cast<T*>(a.y) + t * a.yt;
     if (c * V >= a.half) {
-      const int i = 2 * a.half + c * V - a.half;
+      const int i = a.half + c * V;
       for (int h = h0; h < h1; ++h)
         *reinterpret_cast<VT*>(y + h * a.yh + i) = *reinterpret_cast<const VT*>(x + h * a.xh + i);
       continue;
@@ -121,31 +138,38 @@ __global__ void rope_kernel(const RopeArgs a, int per_head, int groups, int head
 #pragma unroll
       for (int i = 0; i < V; ++i) si.e[i] = -si.e[i];
     }
-    for (int h = h0; h < h1; ++h) {
-      const T* xp = x + h * a.xh + (INTER ? 2 * c * V : c * V);
-      T* yp = y + h * a.yh + (INTER ? 2 * c * V : c * V);
-      const int second = INTER ? V : a.half;
-      VT u = *reinterpret_cast<const VT*>(xp), w = *reinterpret_cast<const VT*>(xp + second), ru, rw;
+    const int first = INTER ? 2 * c * V : c * V, second = first + (INTER ? V : a.half);
+    for (int hb = h0; hb < h1; hb += B) {
+      VT u[B], w[B];
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        if (INTER) {
-          // V consecutive pairs: elements 2i, 2i + 1 of the two vectors
-          if constexpr (V > 1) {
-            const VT& s = 2 * i < V ? u : w;
-            VT& r = 2 * i < V ? ru : rw;
-            const int k = (2 * i) % V;
-            const float x0 = to_f(s.e[k]), x1 = to_f(s.e[k + 1]);
-            r.e[k] = from_f<T>(x0 * co.e[i] - x1 * si.e[i]);
-            r.e[k + 1] = from_f<T>(x1 * co.e[i] + x0 * si.e[i]);
-            continue;
-          }
+      for (int b = 0; b < B; ++b)
+        if (hb + b < h1) {
+          u[b] = *reinterpret_cast<const VT*>(x + (hb + b) * a.xh + first);
+          w[b] = *reinterpret_cast<const VT*>(x + (hb + b) * a.xh + second);
         }
-        const float x0 = to_f(u.e[i]), x1 = to_f(w.e[i]);
-        ru.e[i] = from_f<T>(x0 * co.e[i] - x1 * si.e[i]);
-        rw.e[i] = from_f<T>(x1 * co.e[i] + x0 * si.e[i]);
-      }
-      *reinterpret_cast<VT*>(yp) = ru;
-      *reinterpret_cast<VT*>(yp + second) = rw;
+#pragma unroll
+      for (int b = 0; b < B; ++b)
+        if (hb + b < h1) {
+          VT ru, rw;
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            if constexpr (INTER && V > 1) {
+              // V consecutive pairs: elements 2i, 2i + 1 of the two vectors
+              const VT& s = 2 * i < V ? u[b] : w[b];
+              VT& r = 2 * i < V ? ru : rw;
+              const int k = (2 * i) % V;
+              const float x0 = to_f(s.e[k]), x1 = to_f(s.e[k + 1]);
+              r.e[k] = from_f<T>(x0 * co.e[i] - x1 * si.e[i]);
+              r.e[k + 1] = from_f<T>(x1 * co.e[i] + x0 * si.e[i]);
+            } else {
+              const float x0 = to_f(u[b].e[i]), x1 = to_f(w[b].e[i]);
+              ru.e[i] = from_f<T>(x0 * co.e[i] - x1 * si.e[i]);
+              rw.e[i] = from_f<T>(x1 * co.e[i] + x0 * si.e[i]);
+            }
+          }
+          *reinterpret_cast<VT*>(y + (hb + b) * a.yh + first) = ru;
+          *reinterpret_cast<VT*>(y + (hb + b) * a.yh + second) = rw;
+        }
     }
   }
 }
@@ -163,10 +187,13 @@ cudaError_t launch_rope(const RopeArgs& a, int interleaved, int num_sms, cudaStr
   const int64_t n = a.tokens * groups * per_head;
   const int64_t want = (n + 255) / 256, most = static_cast<int64_t>(num_sms) * 64;
   const int grid = static_cast<int>(want < most ? want : most);
-  if (interleaved)
-    rope_kernel<T, V, true><<<grid, 256, 0, st>>>(a, per_head, groups, heads_per);
-  else
-    rope_kernel<T, V, false><<<grid, 256, 0, st>>>(a, per_head, groups, heads_per);
+  auto run = [&](auto index) {
+    using I = decltype(index);
+    if (interleaved) rope_kernel<T, V, true, I><<<grid, 256, 0, st>>>(a, per_head, groups, heads_per);
+    else rope_kernel<T, V, false, I><<<grid, 256, 0, st>>>(a, per_head, groups, heads_per);
+  };
+  if (n < (int64_t(1) << 31)) run(uint32_t{});
+  else run(int64_t{});
   return cudaGetLastError();
 }
 
@@ -214,8 +241,11 @@ extern "C" int ec_rope_table(float* cos_t, float* sin_t, int64_t positions, int 
   if (int rc = dev.enter({cos_t, sin_t})) return rc;
   if (amplitude == 0.0) amplitude = scaling == EC_ROPE_YARN ? 0.1 * std::log(factor) + 1.0 : 1.0;
   const TableArgs a{cos_t, sin_t, positions, rot_dim / 2, theta, scaling, factor, p0, p1, original, amplitude};
-  const int64_t want = (positions * a.half + 255) / 256, most = static_cast<int64_t>(dev.num_sms()) * 32;
-  rope_table_kernel<<<static_cast<int>(want < most ? want : most), 256, 0, static_cast<cudaStream_t>(stream)>>>(a);
+  // long runs while that leaves a few warps to every scheduler
+  int run = 64;
+  while (run > 4 && positions * a.half / run < static_cast<int64_t>(dev.num_sms()) * 512) run /= 2;
+  const int64_t want = ((positions + run - 1) / run * a.half + 127) / 128, most = int64_t(1) << 20;
+  rope_table_kernel<<<static_cast<int>(want < most ? want : most), 128, 0, static_cast<cudaStream_t>(stream)>>>(a, run);
   return check_cuda(cudaGetLastError(), "rope table");
 }
 
