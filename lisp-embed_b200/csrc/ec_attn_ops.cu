@@ -57,8 +57,7 @@ int launch_one(int id, FlashFn fn, int threads, size_t smem, const CUtensorMap& 
       set[dev] |= 1u << id;
     }
   }
-  fn<<<grid, threads, smem, st>>>(q, k, v, a);
-  return check_cuda(cudaGetLastError(), "attention");
+  return check_cuda(launch_pdl(fn, dim3(grid), dim3(threads), smem, st, q, k, v, a), "attention");
 }
 
 // tile sets of 256 rows, tiles of 128 rows, tiles of at most 32 .. 4 rows

@@ -460,6 +460,8 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
+  pdl_wait();  // what comes before may still be running up to here
+  pdl_trigger();
   if (NT == 1 && a.even) flash_measure(a, prefix, prefix + Cfg::MAX_SEQS);
   tc_fence_before();
   __syncthreads();
@@ -1095,6 +1097,8 @@ __global__ void __launch_bounds__(TokenCfg<HD, NP>::THREADS, 1)
     tmem_alloc(tmem_slot, Cfg::COLS);
     tmem_relinquish();
   }
+  pdl_wait();
+  pdl_trigger();
   flash_measure(a, prefix, prefix + Cfg::MAX_SEQS);
   tc_fence_before();
   __syncthreads();

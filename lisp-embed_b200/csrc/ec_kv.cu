@@ -52,50 +52,71 @@ constexpr int kPlanScalars = 16;
 
 __device__ __forceinline__ int pages_of(int len, int page) { return (len + page - 1) / page; }
 
-// exclusive prefix sum of v over the CTA (kPlanThreads threads), total in sum
-__device__ __forceinline__ int block_scan(int v, int& sum) {
-  __shared__ int part[32];
+// exclusive prefix sums of x and y over the CTA (kPlanThreads threads), totals
+// in sum
+__device__ __forceinline__ int2 block_scan2(int x, int y, int2& sum) {
+  __shared__ int2 part[32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int x = v;
+  int2 v = make_int2(x, y);
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, x, d);
-    if (lane >= d) x += y;
+    const int px = __shfl_up_sync(0xffffffffu, v.x, d), py = __shfl_up_sync(0xffffffffu, v.y, d);
+    if (lane >= d) v.x += px, v.y += py;
   }
-  if (lane == 31) part[warp] = x;
+  if (lane == 31) part[warp] = v;
   __syncthreads();
   if (warp == 0) {
-    int p = part[lane];
+    int2 p = part[lane];
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, p, d);
-      if (lane >= d) p += y;
+      const int px = __shfl_up_sync(0xffffffffu, p.x, d), py = __shfl_up_sync(0xffffffffu, p.y, d);
+      if (lane >= d) p.x += px, p.y += py;
     }
     part[lane] = p;
   }
   __syncthreads();
   sum = part[31];
-  const int before = (warp ? part[warp - 1] : 0) + x - v;
+  const int2 before = warp ? part[warp - 1] : make_int2(0, 0);
   __syncthreads();
+  return make_int2(before.x + v.x - x, before.y + v.y - y);
+}
+__device__ __forceinline__ int block_scan(int v, int& sum) {
+  int2 s2;
+  const int before = block_scan2(v, 0, s2).x;
+  sum = s2.x;
   return before;
 }
 
+// The first pages' counts, read at the start of a plan so that they are there
+// when it gets to the free pages: bit i, page 4 * thread + i is free
+__device__ __forceinline__ int free_ahead(const KvCache& c) {
+  int f = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int p = threadIdx.x * 4 + i;
+    f |= (p < c.pages && c.refs[p] == 0) << i;
+  }
+  return f;
+}
+
 // The `need` lowest free pages into list; false if there are fewer.
-__device__ bool find_free(const KvCache& c, int32_t* list, int64_t need) {
+__device__ bool find_free(const KvCache& c, int32_t* list, int64_t need, int ahead) {
   int64_t got = 0;
   for (int p0 = 0; p0 < c.pages && got < need; p0 += kPlanThreads * 4) {
-    int free_[4], n = 0;
+    int f = ahead;
+    if (p0) {
+      f = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int p = p0 + threadIdx.x * 4 + i;
-      free_[i] = p < c.pages && c.refs[p] == 0;
-      n += free_[i];
+      for (int i = 0; i < 4; ++i) {
+        const int p = p0 + threadIdx.x * 4 + i;
+        f |= (p < c.pages && c.refs[p] == 0) << i;
+      }
     }
     int sum;
-    int64_t r = got + block_scan(n, sum);
+    int64_t r = got + block_scan(__popc(f), sum);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (free_[i]) {
+      if (f >> i & 1) {
         if (r < need) list[r] = p0 + threadIdx.x * 4 + i;
         ++r;
       }
@@ -129,14 +150,17 @@ __device__ __forceinline__ bool bad_len(const KvCache& c, int len) {
 // ---------------------------------------------------------------- reserve --
 __global__ void __launch_bounds__(kPlanThreads) kv_reserve_kernel(const KvCache c, const int32_t* slots,
                                                                   const int32_t* add, int n, int32_t* status) {
+  __shared__ int4 request[kPlanThreads];  // slot, pages it has, pages more, their place in the list
+  pdl_wait();
+  pdl_trigger();
   const Plan plan(c);
-  bool ok = claim_slots(c, plan.claim, slots, n);
+  const int ahead = free_ahead(c);
+  const bool ok = claim_slots(c, plan.claim, slots, n);
   bool bad = false;
   if (ok)
     for (int i = threadIdx.x; i < n; i += kPlanThreads) {
-      const int len = c.lens[slots[i]];
-      bad |= bad_len(c, len) || add[i] < 0 ||
-             static_cast<int64_t>(len) + add[i] > static_cast<int64_t>(c.width) * c.page_size;
+      const int len = c.lens[slots[i]], more = add[i];
+      bad |= bad_len(c, len) || more < 0 || static_cast<int64_t>(len) + more > static_cast<int64_t>(c.width) * c.page_size;
     }
   if (__syncthreads_or(bad || !ok)) {
     if (threadIdx.x == 0) status[0] = EC_KV_BAD, status[1] = 0;
@@ -155,28 +179,36 @@ __global__ void __launch_bounds__(kPlanThreads) kv_reserve_kernel(const KvCache 
     block_scan(v, sum);
     need += sum;
   }
-  if (need > c.pages || !find_free(c, plan.list, need)) {
+  if (need > c.pages || !find_free(c, plan.list, need, ahead)) {
     if (threadIdx.x == 0) status[0] = EC_KV_FULL, status[1] = static_cast<int32_t>(min(need, int64_t(INT32_MAX)));
     return;
   }
+  const int lane = threadIdx.x & 31;
   int at = 0;
   for (int i0 = 0; i0 < n; i0 += kPlanThreads) {
     const int i = i0 + threadIdx.x;
-    int have = 0, v = 0, s = 0, len = 0;
+    int have = 0, v = 0, s = 0;
     if (i < n) {
       s = slots[i];
-      len = c.lens[s];
+      const int len = c.lens[s], more = add[i];
       have = pages_of(len, c.page_size);
-      v = pages_of(len + add[i], c.page_size) - have;
+      v = pages_of(len + more, c.page_size) - have;
+      c.lens[s] = len + more;
     }
     int sum;
     const int off = at + block_scan(v, sum);
-    for (int j = 0; j < v; ++j) {
-      const int p = plan.list[off + j];
-      c.tables[static_cast<int64_t>(s) * c.width + have + j] = p;
-      c.refs[p] = 1;
+    request[threadIdx.x] = make_int4(s, have, v, off);
+    __syncthreads();
+    // a warp per request
+    for (int k = threadIdx.x >> 5; k < min(n - i0, kPlanThreads); k += kPlanThreads / 32) {
+      const int4 q = request[k];
+      for (int j = lane; j < q.z; j += 32) {
+        const int p = plan.list[q.w + j];
+        c.tables[static_cast<int64_t>(q.x) * c.width + q.y + j] = p;
+        c.refs[p] = 1;
+      }
     }
-    if (i < n) c.lens[s] = len + add[i];
+    __syncthreads();
     at += sum;
   }
   if (threadIdx.x == 0) status[0] = EC_KV_OK, status[1] = static_cast<int32_t>(need);
@@ -186,7 +218,10 @@ __global__ void __launch_bounds__(kPlanThreads) kv_reserve_kernel(const KvCache 
 // the copy of every source's partly filled page goes to list[rank]
 __global__ void __launch_bounds__(kPlanThreads) kv_fork_plan_kernel(const KvCache c, const int32_t* src,
                                                                     const int32_t* dst, int n, int32_t* status) {
+  pdl_wait();
+  pdl_trigger();
   const Plan plan(c);
+  const int ahead = free_ahead(c);
   const bool ok = claim_slots(c, plan.claim, dst, n);
   bool bad = false;
   if (ok)
@@ -212,7 +247,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_fork_plan_kernel(const KvCach
     block_scan(i < n && c.lens[src[i]] % c.page_size ? 1 : 0, sum);
     need += sum;
   }
-  if (need > c.pages || !find_free(c, plan.list, need)) {
+  if (need > c.pages || !find_free(c, plan.list, need, ahead)) {
     if (threadIdx.x == 0) status[0] = EC_KV_FULL, status[1] = need, plan.scalars[0] = 0;
     return;
   }
@@ -241,12 +276,23 @@ __device__ __forceinline__ void copy_rows(const KvCache& c, int l, int kv, int f
   uint4* base = static_cast<uint4*>(kv ? c.v : c.k) + static_cast<int64_t>(l) * c.pages * c.page_size * row;
   const uint4* s = base + static_cast<int64_t>(from) * c.page_size * row;
   uint4* d = base + static_cast<int64_t>(to) * c.page_size * row;
-  const int64_t n = rows * row;
-  for (int64_t i = threadIdx.x; i < n; i += blockDim.x) d[i] = s[i];
+  const int n = static_cast<int>(rows * row);  // at most 128 x 1024 x 16
+  constexpr int B = 8;  // pieces under way per thread
+  for (int i0 = threadIdx.x; i0 < n; i0 += B * blockDim.x) {
+    uint4 v[B];
+#pragma unroll
+    for (int b = 0; b < B; ++b)
+      if (i0 + b * blockDim.x < n) v[b] = s[i0 + b * blockDim.x];
+#pragma unroll
+    for (int b = 0; b < B; ++b)
+      if (i0 + b * blockDim.x < n) d[i0 + b * blockDim.x] = v[b];
+  }
 }
 
 // block (i, piece): piece 0 also shares the whole pages of request i
 __global__ void kv_fork_copy_kernel(const KvCache c, const int32_t* src, const int32_t* dst) {
+  pdl_wait();
+  pdl_trigger();
   const Plan plan(c);
   if (plan.scalars[0] == 0) return;
   const int i = blockIdx.x, s = src[i], d = dst[i];
@@ -267,19 +313,47 @@ __global__ void kv_fork_copy_kernel(const KvCache c, const int32_t* src, const i
 }
 
 // ------------------------------------------------------------------- free --
+// lets entry j of a slot's row with np pages go; 1 if its page is free now
+__device__ __forceinline__ int let_go(const KvCache& c, int32_t* row, int j, int np) {
+  const int p = row[j];
+  row[j] = -1;
+  return j < np && p >= 0 && p < c.pages && atomicSub(&c.refs[p], 1) == 1;
+}
+
+// kFreeAlone table entries or fewer: this CTA does it all; else it plans for
+// kv_free_kernel
+constexpr int kFreeAlone = 16384;
 __global__ void __launch_bounds__(kPlanThreads) kv_free_plan_kernel(const KvCache c, const int32_t* slots, int n,
-                                                                    int32_t* status) {
+                                                                    int32_t* status, int alone) {
+  pdl_wait();
+  pdl_trigger();
   const Plan plan(c);
   const bool ok = claim_slots(c, plan.claim, slots, n);
   bool bad = false;
   if (ok)
     for (int i = threadIdx.x; i < n; i += kPlanThreads) bad |= bad_len(c, c.lens[slots[i]]);
   bad = __syncthreads_or(bad || !ok);
-  if (threadIdx.x == 0) status[0] = bad ? EC_KV_BAD : EC_KV_OK, status[1] = 0, plan.scalars[0] = !bad;
+  int gone = 0;
+  if (alone && !bad) {
+    const int lane = threadIdx.x & 31;
+    for (int i = threadIdx.x >> 5; i < n; i += kPlanThreads / 32) {  // a warp per slot
+      const int s = slots[i], np = pages_of(c.lens[s], c.page_size);
+      int32_t* row = c.tables + static_cast<int64_t>(s) * c.width;
+      for (int j = lane; j < c.width; j += 32) gone += let_go(c, row, j, np);
+      __syncwarp();
+      if (lane == 0) c.lens[s] = 0;
+    }
+    int sum;
+    block_scan(gone, sum);
+    gone = sum;
+  }
+  if (threadIdx.x == 0) status[0] = bad ? EC_KV_BAD : EC_KV_OK, status[1] = gone, plan.scalars[0] = !bad;
 }
 
 // block per slot: its pages let go, its row of the table cleared
 __global__ void kv_free_kernel(const KvCache c, const int32_t* slots, int32_t* status) {
+  pdl_wait();
+  pdl_trigger();
   const Plan plan(c);
   if (plan.scalars[0] == 0) return;
   const int s = slots[blockIdx.x];
@@ -287,11 +361,7 @@ __global__ void kv_free_kernel(const KvCache c, const int32_t* slots, int32_t* s
   __syncthreads();
   int32_t* row = c.tables + static_cast<int64_t>(s) * c.width;
   int gone = 0;
-  for (int j = threadIdx.x; j < c.width; j += blockDim.x) {
-    const int p = row[j];
-    if (j < np && p >= 0 && p < c.pages) gone += atomicSub(&c.refs[p], 1) == 1;
-    row[j] = -1;
-  }
+  for (int j = threadIdx.x; j < c.width; j += blockDim.x) gone += let_go(c, row, j, np);
   gone = __reduce_add_sync(0xffffffffu, gone);
   if ((threadIdx.x & 31) == 0 && gone) atomicAdd(&status[1], gone);
   if (threadIdx.x == 0) c.lens[s] = 0;
@@ -301,6 +371,8 @@ __global__ void kv_free_kernel(const KvCache c, const int32_t* slots, int32_t* s
 // list[r]: the r-th hole below the number of live pages; map[p]: the hole
 // that live page p above it moves to; scalars: {live, moves}
 __global__ void __launch_bounds__(kPlanThreads) kv_compact_plan_kernel(const KvCache c, int32_t* status) {
+  pdl_wait();
+  pdl_trigger();
   const Plan plan(c);
   int live = 0;
   for (int p0 = 0; p0 < c.pages; p0 += kPlanThreads * 4) {
@@ -348,6 +420,8 @@ __global__ void __launch_bounds__(kPlanThreads) kv_compact_plan_kernel(const KvC
 }
 
 __global__ void kv_compact_copy_kernel(const KvCache c) {
+  pdl_wait();
+  pdl_trigger();
   const Plan plan(c);
   const int live = plan.scalars[0], moves = plan.scalars[1];
   if (moves == 0) return;
@@ -375,26 +449,32 @@ struct WriteArgs {
   int nseq, layer;
 };
 
-// A block takes kWriteTokens tokens: their sequence and place in the cache,
-// then 16-byte pieces of their rows.
+// A block takes kWriteTokens tokens: a warp finds each one's sequence (32 ways
+// at a time) and place in the cache, then all copy 16-byte pieces, four of the
+// keys and four of the values under way per thread.
 constexpr int kWriteTokens = 8;
-__global__ void kv_write_kernel(const KvCache c, const WriteArgs a) {
+__global__ void __launch_bounds__(kWriteTokens * 32) kv_write_kernel(const KvCache c, const WriteArgs a) {
   __shared__ int64_t at[kWriteTokens];  // row in the pool, -1: none
+  pdl_wait();
+  pdl_trigger();
   const int64_t t0 = static_cast<int64_t>(blockIdx.x) * kWriteTokens;
-  if (threadIdx.x < kWriteTokens) {
-    const int64_t t = t0 + threadIdx.x;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  {
+    const int64_t t = t0 + warp;
     int64_t row = -1;
     if (t < a.tokens) {
       // last sequence that starts at or before t
-      int lo = 0, hi = a.nseq - 1;
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (a.cu[mid] <= t) lo = mid;
-        else hi = mid - 1;
+      int lo = 0, hi = a.nseq;
+      while (hi - lo > 1) {
+        const int step = (hi - lo + 31) / 32, s = lo + lane * step;
+        const unsigned m = __ballot_sync(0xffffffffu, s < hi && a.cu[s] <= t);
+        const int k = m ? 31 - __clz(m) : 0;
+        hi = min(hi, lo + (k + 1) * step);
+        lo = lo + k * step;
       }
-      const int64_t end = a.cu[lo + 1];
+      const int64_t begin = a.cu[lo], end = a.cu[lo + 1];
       const int s = a.slots ? a.slots[lo] : lo;
-      if (a.cu[lo] <= t && t < end && s >= 0 && s < c.slots) {
+      if (begin <= t && t < end && s >= 0 && s < c.slots) {
         const int64_t p = c.lens[s] - (end - t);
         if (p >= 0 && p < static_cast<int64_t>(c.width) * c.page_size) {
           const int page = c.tables[static_cast<int64_t>(s) * c.width + p / c.page_size];
@@ -402,17 +482,33 @@ __global__ void kv_write_kernel(const KvCache c, const WriteArgs a) {
         }
       }
     }
-    at[threadIdx.x] = row;
+    if (lane == 0) at[warp] = row;
   }
   __syncthreads();
-  const int piece = c.head_dim / 8, row = c.heads * piece;
+  const int piece = c.head_dim / 8, row = c.heads * piece, n = kWriteTokens * row;
   const int64_t pool = static_cast<int64_t>(a.layer) * c.pages * c.page_size * row;
   uint4 *dk = static_cast<uint4*>(c.k) + pool, *dv = static_cast<uint4*>(c.v) + pool;
-  for (int e = threadIdx.x; e < kWriteTokens * row; e += blockDim.x) {
-    const int i = e / row, r = e % row, h = r / piece, x = r % piece;
-    if (at[i] < 0) continue;
-    dk[at[i] * row + r] = a.k[(t0 + i) * a.kt + h * a.kh + x];
-    dv[at[i] * row + r] = a.v[(t0 + i) * a.vt + h * a.vh + x];
+  constexpr int B = 4;
+  for (int e0 = threadIdx.x; e0 < n; e0 += B * blockDim.x) {
+    uint4 k[B], v[B];
+    int64_t to[B];
+#pragma unroll
+    for (int b = 0; b < B; ++b) {
+      const int e = e0 + b * blockDim.x;
+      to[b] = -1;
+      if (e >= n) continue;
+      const int i = e / row, r = e % row, h = r / piece, x = r % piece;
+      if (at[i] < 0) continue;
+      to[b] = at[i] * row + r;
+      k[b] = a.k[(t0 + i) * a.kt + h * a.kh + x];
+      v[b] = a.v[(t0 + i) * a.vt + h * a.vh + x];
+    }
+#pragma unroll
+    for (int b = 0; b < B; ++b)
+      if (to[b] >= 0) {
+        dk[to[b]] = k[b];
+        dv[to[b]] = v[b];
+      }
   }
 }
 
@@ -484,8 +580,9 @@ extern "C" int ec_kv_reserve(int handle, const int32_t* slots, const int32_t* ad
   if (int rc = check_lists(slots, add, n, status)) return rc;
   OpDevice dev;
   if (int rc = dev.enter({c->refs, slots, add, status})) return rc;
-  kv_reserve_kernel<<<1, kPlanThreads, 0, static_cast<cudaStream_t>(stream)>>>(*c, slots, add, n, status);
-  return check_cuda(cudaGetLastError(), "kv reserve");
+  return check_cuda(launch_pdl(kv_reserve_kernel, dim3(1), dim3(kPlanThreads), 0, static_cast<cudaStream_t>(stream), *c,
+                               slots, add, n, status),
+                    "kv reserve");
 }
 
 extern "C" int ec_kv_fork(int handle, const int32_t* src, const int32_t* dst, int n, int32_t* status, void* stream) {
@@ -496,11 +593,13 @@ extern "C" int ec_kv_fork(int handle, const int32_t* src, const int32_t* dst, in
   OpDevice dev;
   if (int rc = dev.enter({c->refs, src, dst, status})) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  kv_fork_plan_kernel<<<1, kPlanThreads, 0, st>>>(*c, src, dst, n, status);
-  if (int rc = check_cuda(cudaGetLastError(), "kv fork")) return rc;
+  if (int rc = check_cuda(launch_pdl(kv_fork_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, *c, src, dst, n, status),
+                          "kv fork"))
+    return rc;
   if (n == 0) return EC_OK;
-  kv_fork_copy_kernel<<<dim3(n, std::min(2 * c->layers, 65535)), 256, 0, st>>>(*c, src, dst);
-  return check_cuda(cudaGetLastError(), "kv fork copy");
+  return check_cuda(launch_pdl(kv_fork_copy_kernel, dim3(n, std::min(2 * c->layers, 65535)), dim3(256), 0, st, *c, src,
+                               dst),
+                    "kv fork copy");
 }
 
 extern "C" int ec_kv_free(int handle, const int32_t* slots, int n, int32_t* status, void* stream) {
@@ -511,11 +610,12 @@ extern "C" int ec_kv_free(int handle, const int32_t* slots, int n, int32_t* stat
   OpDevice dev;
   if (int rc = dev.enter({c->refs, slots, status})) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  kv_free_plan_kernel<<<1, kPlanThreads, 0, st>>>(*c, slots, n, status);
-  if (int rc = check_cuda(cudaGetLastError(), "kv free")) return rc;
-  if (n == 0) return EC_OK;
-  kv_free_kernel<<<n, 128, 0, st>>>(*c, slots, status);
-  return check_cuda(cudaGetLastError(), "kv free");
+  const int alone = static_cast<int64_t>(n) * c->width <= kFreeAlone;
+  if (int rc = check_cuda(launch_pdl(kv_free_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, *c, slots, n, status, alone),
+                          "kv free"))
+    return rc;
+  if (alone) return EC_OK;
+  return check_cuda(launch_pdl(kv_free_kernel, dim3(n), dim3(128), 0, st, *c, slots, status), "kv free");
 }
 
 extern "C" int ec_kv_compact(int handle, int32_t* status, void* stream) {
@@ -526,10 +626,9 @@ extern "C" int ec_kv_compact(int handle, int32_t* status, void* stream) {
   OpDevice dev;
   if (int rc = dev.enter({c->refs, status})) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  kv_compact_plan_kernel<<<1, kPlanThreads, 0, st>>>(*c, status);
-  if (int rc = check_cuda(cudaGetLastError(), "kv compact")) return rc;
-  kv_compact_copy_kernel<<<dev.num_sms() * 8, 256, 0, st>>>(*c);
-  return check_cuda(cudaGetLastError(), "kv compact copy");
+  if (int rc = check_cuda(launch_pdl(kv_compact_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, *c, status), "kv compact"))
+    return rc;
+  return check_cuda(launch_pdl(kv_compact_copy_kernel, dim3(dev.num_sms() * 8), dim3(256), 0, st, *c), "kv compact copy");
 }
 
 extern "C" int ec_kv_write(int handle, int layer, const void* k, int64_t k_token, int64_t k_head, const void* v,
@@ -549,6 +648,7 @@ extern "C" int ec_kv_write(int handle, int layer, const void* k, int64_t k_token
   const WriteArgs a{static_cast<const uint4*>(k), static_cast<const uint4*>(v), k_token / 8, k_head / 8, v_token / 8,
                     v_head / 8, tokens, cu, slots, nseq, layer};
   const int64_t grid = (tokens + kWriteTokens - 1) / kWriteTokens;
-  kv_write_kernel<<<static_cast<unsigned>(grid), 256, 0, static_cast<cudaStream_t>(stream)>>>(*c, a);
-  return check_cuda(cudaGetLastError(), "kv write");
+  return check_cuda(launch_pdl(kv_write_kernel, dim3(static_cast<unsigned>(grid)), dim3(kWriteTokens * 32), 0,
+                               static_cast<cudaStream_t>(stream), *c, a),
+                    "kv write");
 }

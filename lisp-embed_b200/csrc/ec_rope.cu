@@ -51,6 +51,8 @@ __device__ double rope_freq(const TableArgs& a, int i) {
 // the fp32 result).  Computing every angle's cos and sin took 150 us for
 // 262144 x 32; this is bounded by the stores.
 __global__ void rope_table_kernel(const TableArgs a, int run) {
+  pdl_wait();
+  pdl_trigger();
   const int64_t runs = (a.positions + run - 1) / run, n = runs * a.half;
   for (int64_t e = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; e < n;
        e += static_cast<int64_t>(gridDim.x) * blockDim.x) {
@@ -109,6 +111,8 @@ __global__ void rope_kernel(const RopeArgs a, int per_head, int groups, int head
   using VT = Vec<T, V>;
   using VF = Vec<float, V>;
   constexpr int B = 4;
+  pdl_wait();
+  pdl_trigger();
   const I n = static_cast<I>(a.tokens) * groups * per_head;
   for (I e = static_cast<I>(blockIdx.x) * blockDim.x + threadIdx.x; e < n; e += static_cast<I>(gridDim.x) * blockDim.x) {
     const int c = static_cast<int>(e % per_head);
@@ -189,12 +193,10 @@ cudaError_t launch_rope(const RopeArgs& a, int interleaved, int num_sms, cudaStr
   const int grid = static_cast<int>(want < most ? want : most);
   auto run = [&](auto index) {
     using I = decltype(index);
-    if (interleaved) rope_kernel<T, V, true, I><<<grid, 256, 0, st>>>(a, per_head, groups, heads_per);
-    else rope_kernel<T, V, false, I><<<grid, 256, 0, st>>>(a, per_head, groups, heads_per);
+    return launch_pdl(interleaved ? rope_kernel<T, V, true, I> : rope_kernel<T, V, false, I>, dim3(grid), dim3(256), 0, st,
+                      a, per_head, groups, heads_per);
   };
-  if (n < (int64_t(1) << 31)) run(uint32_t{});
-  else run(int64_t{});
-  return cudaGetLastError();
+  return n < (int64_t(1) << 31) ? run(uint32_t{}) : run(int64_t{});
 }
 
 template <typename T>
@@ -245,8 +247,9 @@ extern "C" int ec_rope_table(float* cos_t, float* sin_t, int64_t positions, int 
   int run = 64;
   while (run > 4 && positions * a.half / run < static_cast<int64_t>(dev.num_sms()) * 512) run /= 2;
   const int64_t want = ((positions + run - 1) / run * a.half + 127) / 128, most = int64_t(1) << 20;
-  rope_table_kernel<<<static_cast<int>(want < most ? want : most), 128, 0, static_cast<cudaStream_t>(stream)>>>(a, run);
-  return check_cuda(cudaGetLastError(), "rope table");
+  return check_cuda(launch_pdl(rope_table_kernel, dim3(static_cast<int>(want < most ? want : most)), dim3(128), 0,
+                               static_cast<cudaStream_t>(stream), a, run),
+                    "rope table");
 }
 
 extern "C" int ec_rope(const void* x, int64_t x_token, int64_t x_head, void* y, int64_t y_token, int64_t y_head,
