@@ -40,15 +40,17 @@ namespace {
 
 constexpr int kPlanThreads = 1024;
 
-// scratch: [0, pages) pages handed out or holes, [pages, 2 pages) new page of
-// a moved page, then one claim per slot, then the plan's scalars
-struct Plan {
-  int32_t *list, *map, *claim, *scalars;
-  __host__ __device__ explicit Plan(const KvCache& c)
-      : list(c.work), map(c.work + c.pages), claim(c.work + 2 * static_cast<int64_t>(c.pages)),
-        scalars(c.work + 2 * static_cast<int64_t>(c.pages) + c.slots) {}
-};
+// scratch: the plan's scalars, then per slot a copy (from, to, rows) and a
+// claim, then pages handed out or holes, then the new page of a moved page
 constexpr int kPlanScalars = 16;
+struct Plan {
+  int32_t* scalars;
+  int4* copies;
+  int32_t *claim, *list, *map;
+  __host__ __device__ explicit Plan(const KvCache& c)
+      : scalars(c.work), copies(reinterpret_cast<int4*>(c.work + kPlanScalars)),
+        claim(c.work + kPlanScalars + 4 * static_cast<int64_t>(c.slots)), list(claim + c.slots), map(list + c.pages) {}
+};
 
 __device__ __forceinline__ int pages_of(int len, int page) { return (len + page - 1) / page; }
 
@@ -255,14 +257,19 @@ __global__ void __launch_bounds__(kPlanThreads) kv_fork_plan_kernel(const KvCach
   int at = 0;
   for (int i0 = 0; i0 < n; i0 += kPlanThreads) {
     const int i = i0 + threadIdx.x;
-    const int len = i < n ? c.lens[src[i]] : 0;
+    const int s = i < n ? src[i] : 0, len = i < n ? c.lens[s] : 0;
     const int v = len % c.page_size ? 1 : 0;
     int sum;
     const int off = at + block_scan(v, sum);
-    if (v) {
-      const int p = plan.list[off];
-      c.tables[static_cast<int64_t>(dst[i]) * c.width + len / c.page_size] = p;
-      c.refs[p] = 1;
+    if (i < n) {
+      int4 copy = make_int4(-1, -1, 0, len);
+      if (v) {
+        const int p = plan.list[off], from = c.tables[static_cast<int64_t>(s) * c.width + len / c.page_size];
+        c.tables[static_cast<int64_t>(dst[i]) * c.width + len / c.page_size] = p;
+        c.refs[p] = 1;
+        if (from >= 0 && from < c.pages) copy = make_int4(from, p, len % c.page_size, len);
+      }
+      plan.copies[i] = copy;
     }
     at += sum;
   }
@@ -294,32 +301,24 @@ __global__ void kv_fork_copy_kernel(const KvCache c, const int32_t* src, const i
   pdl_wait();
   pdl_trigger();
   const Plan plan(c);
+  const int i = blockIdx.x;
+  const int4 copy = plan.copies[i];
   if (plan.scalars[0] == 0) return;
-  const int i = blockIdx.x, s = src[i], d = dst[i];
-  const int len = c.lens[s];
-  const int full = len / c.page_size, rest = len % c.page_size;
-  const int32_t* from = c.tables + static_cast<int64_t>(s) * c.width;
-  int32_t* to = c.tables + static_cast<int64_t>(d) * c.width;
   if (blockIdx.y == 0) {
+    const int full = copy.w / c.page_size;
+    const int32_t* from = c.tables + static_cast<int64_t>(src[i]) * c.width;
+    int32_t* to = c.tables + static_cast<int64_t>(dst[i]) * c.width;
     for (int j = threadIdx.x; j < full; j += blockDim.x) {
       const int p = from[j];
       to[j] = p;
       if (p >= 0 && p < c.pages) atomicAdd(&c.refs[p], 1);
     }
-    if (threadIdx.x == 0) c.lens[d] = len;
+    if (threadIdx.x == 0) c.lens[dst[i]] = copy.w;
   }
-  if (rest && from[full] >= 0 && from[full] < c.pages)
-    for (int l = blockIdx.y; l < 2 * c.layers; l += gridDim.y) copy_rows(c, l >> 1, l & 1, from[full], to[full], rest);
+  for (int l = blockIdx.y; copy.z && l < 2 * c.layers; l += gridDim.y) copy_rows(c, l >> 1, l & 1, copy.x, copy.y, copy.z);
 }
 
 // ------------------------------------------------------------------- free --
-// lets entry j of a slot's row with np pages go; 1 if its page is free now
-__device__ __forceinline__ int let_go(const KvCache& c, int32_t* row, int j, int np) {
-  const int p = row[j];
-  row[j] = -1;
-  return j < np && p >= 0 && p < c.pages && atomicSub(&c.refs[p], 1) == 1;
-}
-
 // kFreeAlone table entries or fewer: this CTA does it all; else it plans for
 // kv_free_kernel
 constexpr int kFreeAlone = 16384;
@@ -335,17 +334,29 @@ __global__ void __launch_bounds__(kPlanThreads) kv_free_plan_kernel(const KvCach
   bad = __syncthreads_or(bad || !ok);
   int gone = 0;
   if (alone && !bad) {
-    const int lane = threadIdx.x & 31;
-    for (int i = threadIdx.x >> 5; i < n; i += kPlanThreads / 32) {  // a warp per slot
-      const int s = slots[i], np = pages_of(c.lens[s], c.page_size);
-      int32_t* row = c.tables + static_cast<int64_t>(s) * c.width;
-      for (int j = lane; j < c.width; j += 32) gone += let_go(c, row, j, np);
-      __syncwarp();
-      if (lane == 0) c.lens[s] = 0;
+    // four table entries under way per thread; the lengths go last
+    constexpr int B = 4;
+    const int all = n * c.width;
+    for (int e0 = threadIdx.x; e0 < all; e0 += B * kPlanThreads) {
+      int32_t* at[B];
+      int page[B], held[B];
+#pragma unroll
+      for (int b = 0; b < B; ++b) {
+        const int e = e0 + b * kPlanThreads, s = e < all ? slots[e / c.width] : 0;
+        at[b] = c.tables + static_cast<int64_t>(s) * c.width + e % c.width;
+        page[b] = e < all ? *at[b] : -1;
+        held[b] = e < all && e % c.width < pages_of(c.lens[s], c.page_size);
+      }
+#pragma unroll
+      for (int b = 0; b < B; ++b) {
+        if (e0 + b * kPlanThreads < all) *at[b] = -1;
+        if (held[b] && page[b] >= 0 && page[b] < c.pages) gone += atomicSub(&c.refs[page[b]], 1) == 1;
+      }
     }
     int sum;
-    block_scan(gone, sum);
+    block_scan(gone, sum);  // also: every length has been read
     gone = sum;
+    for (int i = threadIdx.x; i < n; i += kPlanThreads) c.lens[slots[i]] = 0;
   }
   if (threadIdx.x == 0) status[0] = bad ? EC_KV_BAD : EC_KV_OK, status[1] = gone, plan.scalars[0] = !bad;
 }
@@ -361,7 +372,11 @@ __global__ void kv_free_kernel(const KvCache c, const int32_t* slots, int32_t* s
   __syncthreads();
   int32_t* row = c.tables + static_cast<int64_t>(s) * c.width;
   int gone = 0;
-  for (int j = threadIdx.x; j < c.width; j += blockDim.x) gone += let_go(c, row, j, np);
+  for (int j = threadIdx.x; j < c.width; j += blockDim.x) {
+    const int p = row[j];
+    if (j < np && p >= 0 && p < c.pages) gone += atomicSub(&c.refs[p], 1) == 1;
+    row[j] = -1;
+  }
   gone = __reduce_add_sync(0xffffffffu, gone);
   if ((threadIdx.x & 31) == 0 && gone) atomicAdd(&status[1], gone);
   if (threadIdx.x == 0) c.lens[s] = 0;
@@ -528,7 +543,7 @@ using namespace ec;
 extern "C" int64_t ec_kv_work_size(int pages, int slots) {
   clear_error();
   if (pages < 1 || slots < 1) return set_error(EC_EINVAL, "pages and slots must be positive");
-  return 4 * (2 * static_cast<int64_t>(pages) + slots + kPlanScalars);
+  return 4 * (2 * static_cast<int64_t>(pages) + 5 * static_cast<int64_t>(slots) + kPlanScalars);
 }
 
 extern "C" int ec_kv_open(void* k, void* v, int dtype, int layers, int pages, int page_size, int heads, int head_dim,

@@ -14,57 +14,83 @@ import sys
 
 from . import _lib
 
-_DTYPES = {"torch.float32": _lib.EC_F32, "torch.bfloat16": _lib.EC_BF16, "torch.float16": _lib.EC_F16}
+_F32, _BF16, _F16, _I32 = _lib.EC_F32, _lib.EC_BF16, _lib.EC_F16, -1
+_NAMES = {"torch.float32": _F32, "torch.bfloat16": _BF16, "torch.float16": _F16, "torch.int32": _I32}
+_codes = {}  # the same by dtype object (its name is slow to form on every call)
+_fns = {}    # bound C entry points
 ROPE_NONE, ROPE_LINEAR, ROPE_LLAMA3, ROPE_YARN = 0, 1, 2, 3
 KV_OK, KV_FULL, KV_BAD = 0, 1, 2
+
+
+def _call(name, *args):
+    fn = _fns.get(name)
+    if fn is None:
+        fn = _fns[name] = getattr(_lib.lib(), name)
+    rc = fn(*args)
+    if rc < 0:
+        _lib.check(rc, name[3:])
+    return rc
 
 
 def _stream(stream, t):
     if stream is not None:
         return stream
     torch = sys.modules.get("torch")
-    return torch.cuda.current_stream(t.device).cuda_stream if torch else None
+    if torch is None:
+        return None
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # the handle alone, without a Stream object
+    return raw(t.get_device()) if raw and t.is_cuda else torch.cuda.current_stream(t.device).cuda_stream
+
+
+def _kind(t):
+    code = _codes.get(t.dtype)
+    if code is None:
+        code = _codes[t.dtype] = _NAMES.get(str(t.dtype), -2)
+    return code
 
 
 def _code(t, what):
-    code = _DTYPES.get(str(t.dtype))
-    if code is None:
+    code = _kind(t)
+    if code < 0:
         raise ValueError(f"{what}: dtype {t.dtype} (float32, bfloat16 or float16)")
     return code
 
 
 def _rows(t, what, heads=None, head_dim=None):
     """(pointer, token stride, head stride) of a [tokens, heads, head_dim] tensor."""
-    if t.dim() != 3 or (t.shape[2] > 1 and t.stride(2) != 1):
+    shape, stride = t.shape, t.stride()
+    if len(stride) != 3 or (stride[2] != 1 and shape[2] > 1):
         raise ValueError(f"{what} must be [tokens, heads, head_dim] with adjacent elements")
-    if (heads is not None and t.shape[1] != heads) or (head_dim is not None and t.shape[2] != head_dim):
-        raise ValueError(f"{what} has {t.shape[1]} heads of {t.shape[2]}, expected {heads} of {head_dim}")
-    return t.data_ptr(), t.stride(0), t.stride(1)
+    if (heads is not None and shape[1] != heads) or (head_dim is not None and shape[2] != head_dim):
+        raise ValueError(f"{what} has {shape[1]} heads of {shape[2]}, expected {heads} of {head_dim}")
+    return t.data_ptr(), stride[0], stride[1]
 
 
 def _ints(t, what, size=None, least=0):
-    if str(t.dtype) != "torch.int32" or t.dim() != 1 or not t.is_contiguous():
+    shape = t.shape
+    if _kind(t) != _I32 or len(shape) != 1 or not t.is_contiguous():
         raise ValueError(f"{what} must be a contiguous int32 vector")
-    if (size is not None and t.shape[0] != size) or t.shape[0] < least:
-        raise ValueError(f"{what} has {t.shape[0]} elements, expected {size if size is not None else least}")
+    if (size is not None and shape[0] != size) or shape[0] < least:
+        raise ValueError(f"{what} has {shape[0]} elements, expected {size if size is not None else least}")
     return t.data_ptr()
 
 
 def _lse(t, tokens, heads):
     if t is None:
         return None
-    if str(t.dtype) != "torch.float32" or tuple(t.shape) != (tokens, heads) or not t.is_contiguous():
+    if _kind(t) != _F32 or t.shape != (tokens, heads) or not t.is_contiguous():
         raise ValueError(f"lse must be a contiguous float32[{tokens}, {heads}]")
     return t.data_ptr()
 
 
 def _tables(cos, sin):
+    shape = cos.shape
     for t in (cos, sin):
-        if str(t.dtype) != "torch.float32" or t.dim() != 2 or not t.is_contiguous():
+        if _kind(t) != _F32 or len(shape) != 2 or not t.is_contiguous():
             raise ValueError("cos and sin must be contiguous float32[positions, rot_dim / 2]")
-    if cos.shape != sin.shape:
+    if shape != sin.shape:
         raise ValueError(f"cos {tuple(cos.shape)} and sin {tuple(sin.shape)} differ")
-    return cos.shape
+    return shape
 
 
 def rope_table(cos, sin, theta, scaling=None, stream=None):
@@ -88,8 +114,8 @@ def rope_table(cos, sin, theta, scaling=None, stream=None):
         amp = s.get("attention_factor") or 0.0
     else:
         raise ValueError(f"rope_scaling type {kind!r} (linear, llama3 or yarn)")
-    _lib.check(_lib.lib().ec_rope_table(cos.data_ptr(), sin.data_ptr(), positions, 2 * half, theta, code, factor,
-                                        p0, p1, original, amp, _stream(stream, cos)), "rope_table")
+    _call("ec_rope_table", cos.data_ptr(), sin.data_ptr(), positions, 2 * half, theta, code, factor, p0, p1, original,
+          amp, _stream(stream, cos))
 
 
 def rope(x, pos, cos, sin, out=None, interleaved=False, inverse=False, stream=None):
@@ -97,16 +123,18 @@ def rope(x, pos, cos, sin, out=None, interleaved=False, inverse=False, stream=No
     heads, head_dim] by its token's position (int32[tokens]); into ``out``, or
     in place.  ``inverse`` turns back (the gradient).  Returns the result."""
     positions, half = _tables(cos, sin)
-    out = x if out is None else out
     code = _code(x, "x")
-    if _code(out, "out") != code or out.shape != x.shape:
-        raise ValueError(f"out {tuple(out.shape)} {out.dtype} does not match x {tuple(x.shape)} {x.dtype}")
-    xp, xt, xh = _rows(x, "x")
-    yp, yt, yh = _rows(out, "out")
-    tokens, heads, hd = x.shape
-    _lib.check(_lib.lib().ec_rope(xp, xt, xh, yp, yt, yh, code, tokens, heads, hd, 2 * half, int(interleaved),
-                                  int(inverse), _ints(pos, "pos", tokens), cos.data_ptr(), sin.data_ptr(), positions,
-                                  _stream(stream, x)), "rope")
+    shape = x.shape
+    xr = yr = _rows(x, "x")
+    if out is None:
+        out = x
+    else:
+        if _code(out, "out") != code or out.shape != shape:
+            raise ValueError(f"out {tuple(out.shape)} {out.dtype} does not match x {tuple(shape)} {x.dtype}")
+        yr = _rows(out, "out")
+    tokens, heads, hd = shape
+    _call("ec_rope", *xr, *yr, code, tokens, heads, hd, 2 * half, 1 if interleaved else 0, 1 if inverse else 0,
+          _ints(pos, "pos", tokens), cos.data_ptr(), sin.data_ptr(), positions, _stream(stream, x))
     return out
 
 
@@ -118,14 +146,13 @@ def attn_prompt(q, k, v, cu, out, lse=None, scale=0.0, stream=None):
     hk = k.shape[1]
     code = _code(q, "q")
     for t, what in ((k, "k"), (v, "v"), (out, "out")):
-        if _code(t, what) != code:
+        if _kind(t) != code:
             raise ValueError(f"{what} is {t.dtype}, q is {q.dtype}")
         if t.shape[0] != tokens:
             raise ValueError(f"{what} has {t.shape[0]} tokens, q has {tokens}")
-    _lib.check(_lib.lib().ec_attn_prompt(*_rows(q, "q"), *_rows(k, "k", hk, hd), *_rows(v, "v", hk, hd),
-                                         *_rows(out, "out", hq, hd), _lse(lse, tokens, hq), code, tokens, hq, hk, hd,
-                                         _ints(cu, "cu", least=1), cu.shape[0] - 1, scale, _stream(stream, q)),
-               "attn_prompt")
+    _call("ec_attn_prompt", *_rows(q, "q"), *_rows(k, "k", hk, hd), *_rows(v, "v", hk, hd), *_rows(out, "out", hq, hd),
+          _lse(lse, tokens, hq), code, tokens, hq, hk, hd, _ints(cu, "cu", least=1), cu.shape[0] - 1, scale,
+          _stream(stream, q))
     return out
 
 
@@ -141,7 +168,7 @@ class KvCache:
         if k.dim() != 5 or k.shape != v.shape or k.dtype != v.dtype or not k.is_contiguous() or not v.is_contiguous():
             raise ValueError("k and v must be contiguous [layers, pages, page_size, heads, head_dim] of one type")
         layers, pages, page, heads, hd = k.shape
-        if str(tables.dtype) != "torch.int32" or tables.dim() != 2 or not tables.is_contiguous():
+        if _kind(tables) != _I32 or tables.dim() != 2 or not tables.is_contiguous():
             raise ValueError("tables must be a contiguous int32[slots, width]")
         slots, width = tables.shape
         code = _code(k, "k")
@@ -170,58 +197,57 @@ class KvCache:
             self.close()
 
     def reserve(self, slots, add, status, stream=None):
+        """Room for add[i] more tokens in slots[i]."""
         n = slots.shape[0]
-        _lib.check(_lib.lib().ec_kv_reserve(self._handle, _ints(slots, "slots"), _ints(add, "add", n), n,
-                                            _ints(status, "status", 2), _stream(stream, status)), "kv_reserve")
+        _call("ec_kv_reserve", self._handle, _ints(slots, "slots"), _ints(add, "add", n), n, _ints(status, "status", 2),
+              _stream(stream, status))
 
     def fork(self, src, dst, status, stream=None):
+        """Empty slots dst[i] become copies of src[i] (whole pages shared)."""
         n = src.shape[0]
-        _lib.check(_lib.lib().ec_kv_fork(self._handle, _ints(src, "src"), _ints(dst, "dst", n), n,
-                                         _ints(status, "status", 2), _stream(stream, status)), "kv_fork")
+        _call("ec_kv_fork", self._handle, _ints(src, "src"), _ints(dst, "dst", n), n, _ints(status, "status", 2),
+              _stream(stream, status))
 
     def free(self, slots, status, stream=None):
-        _lib.check(_lib.lib().ec_kv_free(self._handle, _ints(slots, "slots"), slots.shape[0],
-                                         _ints(status, "status", 2), _stream(stream, status)), "kv_free")
+        """Empty the slots."""
+        _call("ec_kv_free", self._handle, _ints(slots, "slots"), slots.shape[0], _ints(status, "status", 2),
+              _stream(stream, status))
 
     def compact(self, status, stream=None):
-        _lib.check(_lib.lib().ec_kv_compact(self._handle, _ints(status, "status", 2), _stream(stream, status)),
-                   "kv_compact")
+        """Move the pages in use to the front."""
+        _call("ec_kv_compact", self._handle, _ints(status, "status", 2), _stream(stream, status))
 
-    def _slots(self, slots, cu):
+    def _slots(self, slots, n):
         if slots is not None:
-            return _ints(slots, "slots", cu.shape[0] - 1)
-        if cu.shape[0] - 1 > self.slots:
-            raise ValueError(f"{cu.shape[0] - 1} sequences, the cache has {self.slots} slots")
+            return _ints(slots, "slots", n)
+        if n > self.slots:
+            raise ValueError(f"{n} sequences, the cache has {self.slots} slots")
         return None
 
     def write(self, layer, k, v, cu, slots=None, stream=None):
         """Rows k, v [tokens, heads, head_dim] into `layer`: sequence s is the
         last cu[s + 1] - cu[s] tokens of slots[s] (None: slot s)."""
-        for t, what in ((k, "k"), (v, "v")):
-            if t.dtype != self.dtype or t.shape[0] != k.shape[0]:
-                raise ValueError(f"{what} must be {self.dtype}, {k.shape[0]} tokens")
-        _lib.check(_lib.lib().ec_kv_write(self._handle, layer, *_rows(k, "k", self.heads, self.head_dim),
-                                          *_rows(v, "v", self.heads, self.head_dim), k.shape[0],
-                                          _ints(cu, "cu", least=1), self._slots(slots, cu), cu.shape[0] - 1,
-                                          _stream(stream, k)), "kv_write")
+        tokens, n = k.shape[0], cu.shape[0] - 1
+        if k.dtype != self.dtype or v.dtype != self.dtype or v.shape[0] != tokens:
+            raise ValueError(f"k and v must be {self.dtype} rows of the same tokens")
+        _call("ec_kv_write", self._handle, layer, *_rows(k, "k", self.heads, self.head_dim),
+              *_rows(v, "v", self.heads, self.head_dim), tokens, _ints(cu, "cu", least=1), self._slots(slots, n), n,
+              _stream(stream, k))
 
     def attention_workspace(self, q, cu, max_new):
         """Bytes of `attention`'s workspace for these shapes (zero it before its first use)."""
-        return _lib.check(_lib.lib().ec_attn_cached_work_size(self._handle, q.shape[0], q.shape[1], cu.shape[0] - 1,
-                                                              max_new), "attn_cached_work_size")
+        return _call("ec_attn_cached_work_size", self._handle, q.shape[0], q.shape[1], cu.shape[0] - 1, max_new)
 
     def attention(self, layer, q, cu, out, max_new, workspace, slots=None, lse=None, scale=0.0, stream=None):
         """Attention of the new tokens q [tokens, q_heads, head_dim] over their
         slots' pages (their own keys and values included).  Returns out."""
         tokens, hq, hd = q.shape
+        n = cu.shape[0] - 1
         if q.dtype != self.dtype or out.dtype != self.dtype or out.shape[0] != tokens:
             raise ValueError(f"q and out must be {self.dtype} rows of the same tokens")
         if not workspace.is_contiguous():
             raise ValueError("workspace must be contiguous")
-        _lib.check(_lib.lib().ec_attn_cached(self._handle, layer, *_rows(q, "q", None, self.head_dim),
-                                             *_rows(out, "out", hq, self.head_dim), _lse(lse, tokens, hq), tokens, hq,
-                                             _ints(cu, "cu", least=1), self._slots(slots, cu), cu.shape[0] - 1,
-                                             max_new, scale, workspace.data_ptr(),
-                                             workspace.numel() * workspace.element_size(), _stream(stream, q)),
-                   "attn_cached")
+        _call("ec_attn_cached", self._handle, layer, *_rows(q, "q", None, self.head_dim),
+              *_rows(out, "out", hq, self.head_dim), _lse(lse, tokens, hq), tokens, hq, _ints(cu, "cu", least=1),
+              self._slots(slots, n), n, max_new, scale, workspace.data_ptr(), workspace.nbytes, _stream(stream, q))
         return out
