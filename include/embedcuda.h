@@ -100,6 +100,24 @@ int ec_embed_batch(const int32_t *ids, const int64_t *offsets, int nseq, float *
 int ec_embed_batch_device(const int32_t *d_ids, const int64_t *offsets, int nseq,
                           float *d_out, int out_stride, void *stream);
 
+/* ---- texts behind a shared prefix (llama family) ------------------------------
+ * A prefix (the instruction in front of every query) is computed once: its
+ * keys and values stay in a paged cache on every device, and each text's
+ * forward runs over the text's own tokens.  ids[0..n): 1 <= n < the model's
+ * positions.  At most 8 are open at a time (EC_ENOMEM); a prefix ends with
+ * ec_prefix_close, with the next ec_load_model and with ec_shutdown.
+ * EC_EUNSUPPORTED: a model whose attention is not causal.  Device memory
+ * while any is open: layers x 2304 pages x 32 tokens x kv_heads x head_dim x
+ * 4 bytes (8.5 GB for 28 layers of 8 x 128). */
+int ec_prefix_open(const int32_t *ids, int n, int *prefix);
+int ec_prefix_close(int prefix);
+
+/* ec_embed_batch of the texts prefix + ids[offsets[s]..offsets[s + 1])
+ * (llama:embed, llama.lisp:296-344), each of at least one token of its own
+ * and, with the prefix, at most the model's positions. */
+int ec_embed_batch_prefix(int prefix, const int32_t *ids, const int64_t *offsets, int nseq,
+                          float *out, int out_stride);
+
 /* ---- IVF (ann.lisp, kb.lisp) ------------------------------------------------- */
 
 /* Lloyd k-means over the rows of x (n x d, row-major f32).  The training set

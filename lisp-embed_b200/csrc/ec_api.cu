@@ -373,6 +373,56 @@ static size_t env_size(const char* name, size_t def) {
 
 using namespace ec;
 
+namespace ec {
+
+int embed_batch_split(const int32_t* ids, const int64_t* offsets, int nseq, float* out, int out_stride, int prefix) {
+  if (nseq == 0) return EC_OK;
+  if (nseq < 0 || !offsets || !out || (!ids && offsets[nseq] > 0))
+    return set_error(EC_EINVAL, "bad batch arguments");
+  const ModelW& m = G().devs[0]->model;
+  if (!m.family) return set_error(EC_ESTATE, "no model loaded");
+  if (out_stride < m.out_dim)
+    return set_error(EC_EINVAL, "out_stride %d < dim %d", out_stride, m.out_dim);
+  for (int s = 0; s < nseq; ++s)
+    if (offsets[s + 1] < offsets[s]) return set_error(EC_EINVAL, "offsets not ascending at %d", s);
+  const int nd = static_cast<int>(G().devs.size());
+  // length-sorted greedy split over devices (embed.lisp / shard.lisp ranges
+  // on one box): cost of a sequence ~ L * (1 + L / 4H)
+  std::vector<int> order(nseq);
+  std::iota(order.begin(), order.end(), 0);
+  std::stable_sort(order.begin(), order.end(), [&](int a, int b) {
+    return offsets[a + 1] - offsets[a] > offsets[b + 1] - offsets[b];
+  });
+  std::vector<std::vector<int>> part(nd);
+  std::vector<double> load(nd, 0.0);
+  for (int s : order) {
+    const double L = static_cast<double>(offsets[s + 1] - offsets[s]);
+    int best = 0;
+    for (int k = 1; k < nd; ++k)
+      if (load[k] < load[best]) best = k;
+    part[best].push_back(s);
+    load[best] += L * (1.0 + L / (4.0 * m.H));
+  }
+  for (auto& p : part) std::sort(p.begin(), p.end());
+  if (nd == 1) return embed_on_device(*G().devs[0], ids, nullptr, part[0], offsets, out, out_stride, nullptr, prefix);
+  std::vector<int> rcs(nd, EC_OK);
+  std::vector<std::string> errs(nd);
+  std::vector<std::thread> th;
+  for (int k = 0; k < nd; ++k) {
+    th.emplace_back([&, k] {
+      if (part[k].empty()) return;
+      rcs[k] = embed_on_device(*G().devs[k], ids, nullptr, part[k], offsets, out, out_stride, nullptr, prefix);
+      if (rcs[k]) errs[k] = t_err;
+    });
+  }
+  for (auto& t : th) t.join();
+  for (int k = 0; k < nd; ++k)
+    if (rcs[k]) return set_error(rcs[k], "device %d: %s", G().devs[k]->ordinal, errs[k].c_str());
+  return EC_OK;
+}
+
+}  // namespace ec
+
 extern "C" {
 
 const char* ec_last_error(void) { return t_err.c_str(); }
@@ -524,6 +574,7 @@ int ec_upload_tensor(const char* name, int dtype, const int64_t* shape, int ndim
       dev_free(*d, t.p, dev_bytes);
       return rc;
     }
+    t.model = d->models;
     d->uploads[name] = t;
   }
   return EC_OK;
@@ -570,49 +621,7 @@ int ec_embed_batch(const int32_t* ids, const int64_t* offsets, int nseq, float* 
   std::lock_guard<std::mutex> lk(G().mu);
   clear_error();
   if (!G().inited) return set_error(EC_ESTATE, "ec_init first");
-  if (nseq == 0) return EC_OK;
-  if (nseq < 0 || !offsets || !out || (!ids && offsets[nseq] > 0))
-    return set_error(EC_EINVAL, "bad batch arguments");
-  const ModelW& m = G().devs[0]->model;
-  if (!m.family) return set_error(EC_ESTATE, "no model loaded");
-  if (out_stride < m.out_dim)
-    return set_error(EC_EINVAL, "out_stride %d < dim %d", out_stride, m.out_dim);
-  for (int s = 0; s < nseq; ++s)
-    if (offsets[s + 1] < offsets[s]) return set_error(EC_EINVAL, "offsets not ascending at %d", s);
-  const int nd = static_cast<int>(G().devs.size());
-  // length-sorted greedy split over devices (embed.lisp / shard.lisp ranges
-  // on one box): cost of a sequence ~ L * (1 + L / 4H)
-  std::vector<int> order(nseq);
-  std::iota(order.begin(), order.end(), 0);
-  std::stable_sort(order.begin(), order.end(), [&](int a, int b) {
-    return offsets[a + 1] - offsets[a] > offsets[b + 1] - offsets[b];
-  });
-  std::vector<std::vector<int>> part(nd);
-  std::vector<double> load(nd, 0.0);
-  for (int s : order) {
-    const double L = static_cast<double>(offsets[s + 1] - offsets[s]);
-    int best = 0;
-    for (int k = 1; k < nd; ++k)
-      if (load[k] < load[best]) best = k;
-    part[best].push_back(s);
-    load[best] += L * (1.0 + L / (4.0 * m.H));
-  }
-  for (auto& p : part) std::sort(p.begin(), p.end());
-  if (nd == 1) return embed_on_device(*G().devs[0], ids, nullptr, part[0], offsets, out, out_stride, nullptr);
-  std::vector<int> rcs(nd, EC_OK);
-  std::vector<std::string> errs(nd);
-  std::vector<std::thread> th;
-  for (int k = 0; k < nd; ++k) {
-    th.emplace_back([&, k] {
-      if (part[k].empty()) return;
-      rcs[k] = embed_on_device(*G().devs[k], ids, nullptr, part[k], offsets, out, out_stride, nullptr);
-      if (rcs[k]) errs[k] = t_err;
-    });
-  }
-  for (auto& t : th) t.join();
-  for (int k = 0; k < nd; ++k)
-    if (rcs[k]) return set_error(rcs[k], "device %d: %s", G().devs[k]->ordinal, errs[k].c_str());
-  return EC_OK;
+  return embed_batch_split(ids, offsets, nseq, out, out_stride, -1);
 }
 
 int ec_embed_batch_device(const int32_t* d_ids, const int64_t* offsets, int nseq, float* d_out,

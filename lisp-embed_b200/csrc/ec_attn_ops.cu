@@ -130,6 +130,16 @@ size_t attention_work_bytes(const KvCache& c, int64_t tokens, int q_heads, int n
   return part_bytes(p.part_rows, c.head_dim <= 64 ? 64 : 128) + part_bytes(p.part_rows, 1) + kMaxCtas * 4;
 }
 
+int op_status_fetch(unsigned* host, cudaStream_t st) {
+  void* p = nullptr;
+  if (int rc = check_cuda(cudaGetSymbolAddress(&p, g_op_status), "operator status")) return rc;
+  return check_cuda(cudaMemcpyAsync(host, p, sizeof(unsigned), cudaMemcpyDeviceToHost, st), "operator status");
+}
+
+size_t attention_work_most(int head_dim) {
+  return part_bytes(128, head_dim <= 64 ? 64 : 128) + part_bytes(128, 1) + kMaxCtas * 4;
+}
+
 int run_attention(const AttnOp& op, int num_sms, cudaStream_t st) {
   const KvCache* c = op.cache;
   num_sms = std::min(num_sms, kMaxCtas);

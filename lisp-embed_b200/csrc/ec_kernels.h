@@ -174,7 +174,7 @@ cudaError_t launch_qk_norm_rope(const QkRopeArgs& a, cudaStream_t st);
 cudaError_t launch_pool_l2(const PoolArgs& a, int nseq, cudaStream_t st);
 cudaError_t launch_gather_rows(const void* table, int dtype, const int* ids, float* out, int T,
                                int H, cudaStream_t st);
-cudaError_t launch_positions(const int* cu, int nseq, int* pos, cudaStream_t st);
+cudaError_t launch_positions(const int* cu, int nseq, int first, int* pos, cudaStream_t st);
 cudaError_t launch_convert(int kind, const void* src, void* dst, size_t n, cudaStream_t st);
 
 // ---- GEMM (ec_gemm.cu) -------------------------------------------------------

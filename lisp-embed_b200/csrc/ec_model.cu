@@ -20,6 +20,8 @@
 
 #include "ec_gemm.cuh"
 #include "ec_json.h"
+#include "ec_ops.h"
+#include "ec_prefix.h"
 #include "ec_state.h"
 
 namespace ec {
@@ -129,6 +131,7 @@ void graphs_clear(Device& d) {
 }
 
 void free_model(Device& d) {
+  prefix_drop(d);
   graphs_clear(d);
   for (void* p : d.model.owned) cudaFree(p);
   d.model = ModelW();
@@ -296,9 +299,14 @@ static int load_llama(Device& d, const JVal& cfg) {
   m.family = EC_FAMILY_LLAMA;
   m.pooling = 2;      // llama::*pooling* :last (llama.lisp:19)
   m.max_pos = 1024;   // llama::*max-pos* (llama.lisp:21)
-  if (m.hd != 128) return set_error(EC_EUNSUPPORTED, "llama head_dim %d (supported: 128)", m.hd);
-  if (m.kv_heads <= 0 || m.heads % m.kv_heads)
+  if (m.kv_heads <= 0 || m.heads <= 0 || m.heads % m.kv_heads)
     return set_error(EC_EINVAL, "heads %d not a multiple of kv heads %d", m.heads, m.kv_heads);
+  // head dim 128 has fused q/k norm + RoPE and its own attention; others run
+  // ec_rope and ec_attn_prompt, and the GEMMs want rows in 64-wide tiles
+  if (m.hd != 128 && (m.hd < 8 || m.hd > 128 || m.hd % 8 || m.heads * m.hd % 64 ||
+                      (m.heads + 2 * m.kv_heads) * m.hd % 64 || m.heads / m.kv_heads > 128))
+    return set_error(EC_EUNSUPPORTED, "llama head_dim %d with %d + 2 * %d heads (supported: multiples of 8 "
+                     "up to 128, rows a multiple of 64)", m.hd, m.heads, m.kv_heads);
   if (m.H % 128 || m.H > 2048 || m.F % 128)
     return set_error(EC_EUNSUPPORTED, "hidden %d / ffn %d outside this build", m.H, m.F);
   const int H = m.H, F = m.F, qd = m.heads * m.hd, kvd = m.kv_heads * m.hd;
@@ -351,6 +359,11 @@ static int load_llama(Device& d, const JVal& cfg) {
       return rc;
     const Tensor* qn = find_t(d, pf + "self_attn.q_norm.weight");  // get-tensor-opt
     const Tensor* kn = find_t(d, pf + "self_attn.k_norm.weight");
+    // uploads stay: one of an earlier model is not this layer's
+    if (qn && qn->model < qw->model) qn = nullptr;
+    if (kn && kn->model < kw->model) kn = nullptr;
+    if (m.hd != 128 && (qn || kn))
+      return set_error(EC_EUNSUPPORTED, "q/k norm with head_dim %d (supported: 128)", m.hd);
     if ((rc = as_f32(d, in, &L.in_ln)) || (rc = as_f32(d, post, &L.post_ln)) ||
         (rc = concat_bf16(d, {qw, kw, vw}, H, &L.wqkv)) || (rc = concat_bf16(d, {ow}, qd, &L.wo)) ||
         (rc = concat_bf16(d, {dw}, F, &L.wdown)))
@@ -528,6 +541,7 @@ int load_model_on(Device& d, const JVal& cfg, const JVal* pool) {
   d.ws_bytes = 0;
   d.ws_tokens = 0;
   d.ws_seqs = 0;
+  ++d.models;
   const JVal* tc = cfg.get("text_config");
   std::string mt;
   if (tc && tc->kind == JVal::Obj && tc->get("model_type") && tc->get("model_type")->kind == JVal::Str)
@@ -607,6 +621,7 @@ static int ensure_ws(Device& d, int T, int nseq) {
   const size_t pin = static_cast<size_t>(t2) * 4 + (static_cast<size_t>(s2) + 1) * 4 +
                      (static_cast<size_t>(t2) / 64 + s2 + 1) * 8 +
                      (static_cast<size_t>(t2) / 128 + s2 + 1) * 16 + static_cast<size_t>(s2) * 8 + 768 +
+                     static_cast<size_t>(kPrefixSeqs) * 4 + 256 +
                      static_cast<size_t>(s2) * std::max(d.model.H, d.model.out_dim) * 4 + 1024;
   if (!d.ws || L.total > d.ws_bytes || t2 != d.ws_tokens || s2 != d.ws_seqs || pin > d.pin_bytes)
     graphs_clear(d);  // the layout or the buffers change
@@ -657,7 +672,8 @@ struct AttnTables {
 };
 
 static int forward_packed(Device& d, const WsLayout& L, int T, int nseq, const AttnTables& tb,
-                          double attn_pairs, float* out, int out_stride) {
+                          double attn_pairs, float* out, int out_stride,
+                          const PrefixRun* px = nullptr) {
   const int nblk = tb.nblk, nblk128 = tb.nblk128;
   ModelW& m = d.model;
   char* ws = static_cast<char*>(d.ws);
@@ -685,7 +701,7 @@ static int forward_packed(Device& d, const WsLayout& L, int T, int nseq, const A
   const double TH = static_cast<double>(T) * H;
   {
     const int e0 = prof_begin(d);
-    EC_TRY(rows(launch_positions(cu, nseq, pos, st), "positions", T * 4.0, e0));
+    EC_TRY(rows(launch_positions(cu, nseq, px ? px->first : 0, pos, st), "positions", T * 4.0, e0));
   }
 
   auto gemm = [&](const bf16* A, int lda, const bf16* W, int N, int K, const float* bias,
@@ -788,8 +804,28 @@ static int forward_packed(Device& d, const WsLayout& L, int T, int nseq, const A
   at.rows = T;
   at.status = d.status;
   at.num_sms = d.num_sms;
-  auto attention = [&]() -> int {
+  auto attention = [&](int layer) -> int {
     const int e0 = prof_begin(d);
+    if (px) {
+      // the texts' keys and values go behind the prefix's, into pages of the
+      // pool; the queries read both
+      int rc = ec_kv_write(px->handle, layer, qkv + at.k_off, nqkv, m.hd, qkv + at.v_off, nqkv, m.hd, T, cu, px->slots,
+                           nseq, st);
+      trace_launch(d, "cache write");
+      if (rc == EC_OK)
+        rc = ec_attn_cached(px->handle, layer, qkv, nqkv, m.hd, ctx, nctx, m.hd, nullptr, T, m.heads, cu, px->slots,
+                            nseq, px->longest, 0.f, px->work, static_cast<int64_t>(px->work_bytes), st);
+      prof_end(d, 1, attn_pairs * 4.0 * m.heads * m.hd, 2.0 * T * (nqkv + nctx), e0);
+      trace_launch(d, "cached attention");
+      return rc;
+    }
+    if (m.family == EC_FAMILY_LLAMA && m.hd != 128) {
+      const int rc = ec_attn_prompt(qkv, nqkv, m.hd, qkv + at.k_off, nqkv, m.hd, qkv + at.v_off, nqkv, m.hd, ctx, nctx,
+                                    m.hd, nullptr, EC_BF16, T, m.heads, m.kv_heads, m.hd, cu, nseq, 0.f, st);
+      prof_end(d, 1, attn_pairs * 4.0 * m.heads * m.hd, 2.0 * T * (nqkv + nctx), e0);
+      trace_launch(d, "prompt attention");
+      return rc;
+    }
     const cudaError_t e = launch_attention(at, st);
     prof_end(d, 1, attn_pairs * 4.0 * m.heads * m.hd, 2.0 * T * (nqkv + nctx), e0);
     trace_launch(d, "attention");
@@ -839,7 +875,7 @@ static int forward_packed(Device& d, const WsLayout& L, int T, int nseq, const A
       const BertLayerW& w = m.bl[li];
       if (skinny) {
         EC_TRY(sk(hb, H, w.wqkv, nqkv, H, w.bqkv, kSkBf16, qkv, nqkv));
-        EC_TRY(attention());
+        EC_TRY(attention(li));
         EC_TRY(sk(ctx, nctx, w.wo, H, nctx, w.bo, kSkF32Resid, tmp, H));
         EC_TRY(ln_rows(w.ln1g, w.ln1b));
         EC_TRY(sk(hb, H, w.wff, F, H, w.bff, kSkGelu, ff, F));
@@ -848,7 +884,7 @@ static int forward_packed(Device& d, const WsLayout& L, int T, int nseq, const A
         continue;
       }
       EC_TRY(gemm(hb, H, w.wqkv, nqkv, H, w.bqkv, nullptr, qkv, nqkv, kEpiBf16));
-      EC_TRY(attention());
+      EC_TRY(attention(li));
       if (fuse_ln) {
         EC_TRY(gemm_ln(ctx, nctx, w.wo, w.bo, w.ln1g, w.ln1b, false));
       } else {
@@ -950,7 +986,7 @@ static int forward_packed(Device& d, const WsLayout& L, int T, int nseq, const A
         EC_TRY(row([&] { return launch_head_norm_rope(hr, st); }, "head norm rope",
                    4.0 * T * nqkv));
       }
-      EC_TRY(attention());
+      EC_TRY(attention(li));
       if (fuse_rms) {
         // h = h + RMSNorm(o) * g, hb = RMSNorm(h) * g' in the O GEMM
         EC_TRY(gemm_norm(ctx, nctx, w.wo, 2, h32, w.post_ln, w.pre_ff_ln, h32, hb, 1.f, 0, H));
@@ -1038,7 +1074,7 @@ static int forward_packed(Device& d, const WsLayout& L, int T, int nseq, const A
       // QKV projection with the per-head q/k RMSNorm and RoPE in its epilogue
       const QkRopeEpi qe{w.q_norm, w.k_norm, m.heads, m.kv_heads, m.eps, pos, m.cos_t, m.sin_t};
       EC_TRY(gemm(hb, H, w.wqkv, nqkv, H, nullptr, nullptr, qkv, nqkv, kEpiBf16QkRope, &qe));
-      EC_TRY(attention());
+      EC_TRY(attention(li));
       if (fuse_res_rms) {
         EC_TRY(gemm_norm(ctx, nctx, w.wo, 1, h32, w.post_ln, nullptr, h32, hb, 1.f, 0, H));
       } else {
@@ -1071,10 +1107,15 @@ static int forward_packed(Device& d, const WsLayout& L, int T, int nseq, const A
     q.T = T;
     {
       const int e0 = prof_begin(d);
-      EC_TRY(rows(launch_qk_norm_rope(q, st), "qk norm rope",
-                  4.0 * T * (m.heads + m.kv_heads) * m.hd, e0));
+      cudaError_t e = cudaSuccess;
+      if (m.hd == 128)
+        e = launch_qk_norm_rope(q, st);
+      else  // query and key heads follow each other in a row
+        EC_TRY(ec_rope(qkv, nqkv, m.hd, qkv, nqkv, m.hd, EC_BF16, T, m.heads + m.kv_heads, m.hd, m.hd, 0, 0, pos,
+                       m.cos_t, m.sin_t, m.max_pos, st));
+      EC_TRY(rows(e, "qk norm rope", 4.0 * T * (m.heads + m.kv_heads) * m.hd, e0));
     }
-    EC_TRY(attention());
+    EC_TRY(attention(li));
     EC_TRY(gemm(ctx, nctx, w.wo, H, nctx, nullptr, h32, h32, H, kEpiF32Resid));
     RmsArgs r2{h32, nullptr, w.post_ln, m.eps, hb, nullptr, T, H};
     {
@@ -1161,7 +1202,7 @@ static int copy_tables(Device& d, const WsLayout& L, int nseq, const AttnTables&
 
 int embed_on_device(Device& d, const int32_t* ids_host, const int32_t* ids_dev,
                     const std::vector<int>& seqs, const int64_t* offsets, float* out_host,
-                    int out_stride, float* out_dev) {
+                    int out_stride, float* out_dev, int prefix, bool fill) {
   ModelW& m = d.model;
   if (!m.family) return set_error(EC_ESTATE, "no model loaded");
   EC_TRY(check_cuda(cudaSetDevice(d.ordinal), "set device"));
@@ -1176,15 +1217,18 @@ int embed_on_device(Device& d, const int32_t* ids_host, const int32_t* ids_dev,
     t_last = now;
   };
   // validate lengths and ids (host ids only; device ids are trusted)
-  const int maxlen = m.family == EC_FAMILY_LLAMA ? m.max_pos : m.max_pos - m.pos_offset;
+  PrefixPool* pool = prefix >= 0 ? d.prefixes : nullptr;
+  if (prefix >= 0 && !pool) return set_error(EC_ESTATE, "no prefix on device %d", d.ordinal);
+  const int first = pool && !fill ? pool->len[prefix] : 0;  // position of the sequences' first token
+  const int maxlen = m.family == EC_FAMILY_LLAMA ? m.max_pos - first : m.max_pos - m.pos_offset;
   for (int s : seqs) {
     const int64_t L = offsets[s + 1] - offsets[s];
     if (offsets[s] < 0)  // before the start of the ids (host or device)
       return set_error(EC_EINVAL, "sequence %d starts at offset %lld", s, static_cast<long long>(offsets[s]));
     if (L <= 0) return set_error(EC_EINVAL, "sequence %d is empty", s);
     if (L > maxlen)
-      return set_error(EC_EINVAL, "sequence %d has %lld tokens, above the %d positions of the model",
-                       s, static_cast<long long>(L), maxlen);
+      return set_error(EC_EINVAL, "sequence %d has %lld tokens, above the %d positions of the model%s",
+                       s, static_cast<long long>(L), maxlen, first ? " behind the prefix" : "");
     if (m.family == EC_FAMILY_MPNET && L > 512)
       return set_error(EC_EUNSUPPORTED, "MPNet sequence %d longer than 512 tokens", s);
     if (ids_host) {
@@ -1210,7 +1254,8 @@ int embed_on_device(Device& d, const int32_t* ids_host, const int32_t* ids_dev,
     int64_t T = 0;
     while (j < seqs.size()) {
       const int64_t L = offsets[seqs[j] + 1] - offsets[seqs[j]];
-      if (j > i && T + L > G().max_tokens) break;
+      if (j > i && T + L > (pool ? std::min(G().max_tokens, kPrefixTokens) : G().max_tokens)) break;
+      if (pool && j - i >= static_cast<size_t>(kPrefixSeqs)) break;
       T += L;
       ++j;
     }
@@ -1227,17 +1272,19 @@ int embed_on_device(Device& d, const int32_t* ids_host, const int32_t* ids_dev,
       lens[k] = static_cast<int>(offsets[seqs[i + k] + 1] - offsets[seqs[i + k]]);
     AttnTables tb;
     char* ws = static_cast<char*>(d.ws);
-    // pinned layout: tables at the front, ids at the back, outputs below them
+    // pinned layout: tables at the front, ids (and the lengths behind a
+    // prefix) at the back, outputs below them
+    const size_t ids_room = al256(static_cast<size_t>(T) * 4) + 256 + (pool ? al256(kPrefixSeqs * 4 + 64) : 0);
     int* hid = reinterpret_cast<int*>(static_cast<char*>(d.pin) + d.pin_bytes -
-                                      al256(static_cast<size_t>(T) * 4) - 256);
+                                      ids_room);
     const size_t obytes = static_cast<size_t>(nseq) * m.out_dim * 4;
     float* hout = reinterpret_cast<float*>(static_cast<char*>(d.pin) + d.pin_bytes -
-                                           al256(static_cast<size_t>(T) * 4) - 256 - al256(obytes));
+                                           ids_room - al256(obytes));
     // consecutive sequences: their ids and output rows are contiguous in
     // the caller's arrays, which the copies then use directly
     bool contig = true;
     for (int k = 1; k < nseq && contig; ++k) contig = seqs[i + k] == seqs[i + k - 1] + 1;
-    const bool graph = ids_host && !out_dev && j - i == seqs.size() && T <= kGraphMaxTokens &&
+    const bool graph = ids_host && !out_dev && !fill && j - i == seqs.size() && T <= kGraphMaxTokens &&
                        !G().profile && !G().sync_each && getenv("EC_NO_GRAPH") == nullptr;
     const bool direct = contig && !graph;
     const bool direct_out = direct && !out_dev && out_stride == m.out_dim;
@@ -1254,10 +1301,19 @@ int embed_on_device(Device& d, const int32_t* ids_host, const int32_t* ids_dev,
     const int ostride = out_dev ? out_stride : m.out_dim;
     double pairs = 0.0;  // (query, key) pairs that attention scores
     for (int k = 0; k < nseq; ++k)
-      pairs += m.family == EC_FAMILY_LLAMA ? 0.5 * lens[k] * (lens[k] + 1.0)
+      pairs += m.family == EC_FAMILY_LLAMA ? lens[k] * (0.5 * (lens[k] + 1.0) + first)
                                            : static_cast<double>(lens[k]) * lens[k];
+    // the attention operators' bounded waits have a status word of their own
+    const bool operators = pool || (m.family == EC_FAMILY_LLAMA && m.hd != 128);
+    PrefixRun run{};
+    int* hadd = hid + T + 8;  // lengths of the sequences, behind the ids
+    if (pool) {
+      run = prefix_run(*pool, prefix, fill, *std::max_element(lens.begin(), lens.end()));
+      std::memcpy(hadd, lens.data(), static_cast<size_t>(nseq) * 4);
+    }
     // the stream work of this chunk: tables and ids up, forward, rows down
     auto enqueue = [&]() -> int {
+      if (pool) EC_TRY(prefix_plan(d, *pool, prefix, fill, hadd, nseq));
       EC_TRY(copy_tables(d, L, nseq, tb));
       if (ids_dev) {
         EC_TRY(check_cuda(cudaMemcpyAsync(ws + L.ids, ids_dev + offsets[seqs[i]],
@@ -1269,11 +1325,13 @@ int embed_on_device(Device& d, const int32_t* ids_host, const int32_t* ids_dev,
                                           static_cast<size_t>(T) * 4, cudaMemcpyHostToDevice, d.stream),
                           "ids upload"));
       }
-      EC_TRY(forward_packed(d, L, static_cast<int>(T), nseq, tb, pairs, dout, ostride));
+      EC_TRY(forward_packed(d, L, static_cast<int>(T), nseq, tb, pairs, dout, ostride, pool ? &run : nullptr));
       if (!out_dev)
         EC_TRY(check_cuda(cudaMemcpyAsync(direct_out ? out_host + static_cast<size_t>(seqs[i]) * out_stride : hout,
                                           dout, obytes, cudaMemcpyDeviceToHost, d.stream),
                           "output download"));
+      if (pool) EC_TRY(prefix_fetch(d, *pool));
+      if (operators && d.status_host) EC_TRY(op_status_fetch(d.status_host + 4, d.stream));
       return EC_OK;
     };
     fill_tables(d, lens, &tb);
@@ -1286,7 +1344,7 @@ int embed_on_device(Device& d, const int32_t* ids_host, const int32_t* ids_dev,
     if (graph) {
       for (auto& e : d.graphs)
         if (e.lens == lens && e.ws == d.ws && e.ws_tokens == d.ws_tokens && e.ws_seqs == d.ws_seqs &&
-            e.pin == d.pin && e.pin_bytes == d.pin_bytes) {
+            e.pin == d.pin && e.pin_bytes == d.pin_bytes && e.prefix == prefix) {
           g = &e;
           break;
         }
@@ -1316,7 +1374,7 @@ int embed_on_device(Device& d, const int32_t* ids_host, const int32_t* ids_dev,
           cudaGraphExecDestroy(d.graphs[lru].exec);
           d.graphs.erase(d.graphs.begin() + static_cast<std::ptrdiff_t>(lru));
         }
-        d.graphs.push_back({lens, d.ws, d.ws_tokens, d.ws_seqs, d.pin, d.pin_bytes, ex, 0});
+        d.graphs.push_back({lens, d.ws, d.ws_tokens, d.ws_seqs, d.pin, d.pin_bytes, ex, 0, prefix});
         g = &d.graphs.back();
       }
       g->used = ++d.graph_clock;
@@ -1326,6 +1384,8 @@ int embed_on_device(Device& d, const int32_t* ids_host, const int32_t* ids_dev,
     }
     tmark(g ? "graph launch" : "enqueue");
     EC_TRY(sync_and_check(d, "forward"));
+    if (pool) EC_TRY(prefix_check(*pool));
+    if (operators && (!d.status_host || d.status_host[4])) EC_TRY(ec_op_status());
     tmark("device (wait)");
     prof_collect(d);
     if (!out_dev && !direct_out)

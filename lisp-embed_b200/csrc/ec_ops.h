@@ -81,5 +81,9 @@ struct AttnOp {
 };
 int run_attention(const AttnOp& op, int num_sms, cudaStream_t st);
 size_t attention_work_bytes(const KvCache& c, int64_t tokens, int q_heads, int nseq, int max_new);
+// copies the mark of a wait that gave up (0: none) to `host`, in stream order
+int op_status_fetch(unsigned* host, cudaStream_t st);
+// enough for every call on a cache of this head size
+size_t attention_work_most(int head_dim);
 
 }  // namespace ec

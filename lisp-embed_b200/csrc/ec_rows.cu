@@ -237,14 +237,15 @@ __global__ void gather_rows_kernel(const void* table, int dtype, const int* ids,
   for (int c = lane; c < H / 4; c += 32) dst[c] = ld_row4(table, dtype, src + c);
 }
 
-// position of every packed token within its sequence
-__global__ void positions_kernel(const int* cu, int nseq, int* pos) {
+// position of every packed token within its sequence, whose first token is at
+// position `first`
+__global__ void positions_kernel(const int* cu, int nseq, int first, int* pos) {
   pdl_trigger();
   pdl_wait();
   const int s = blockIdx.x;
   if (s >= nseq) return;
   const int b = cu[s], e = cu[s + 1];
-  for (int t = b + threadIdx.x; t < e; t += blockDim.x) pos[t] = t - b;
+  for (int t = b + threadIdx.x; t < e; t += blockDim.x) pos[t] = t - b + first;
 }
 
 // st::half-to-float (st.lisp:22-30), exponent 31 -> +-most-positive-single.
@@ -342,8 +343,8 @@ cudaError_t launch_gather_rows(const void* table, int dtype, const int* ids, flo
   return cudaGetLastError();
 }
 
-cudaError_t launch_positions(const int* cu, int nseq, int* pos, cudaStream_t st) {
-  return launch_pdl(positions_kernel, dim3(nseq), dim3(128), 0, st, cu, nseq, pos);
+cudaError_t launch_positions(const int* cu, int nseq, int first, int* pos, cudaStream_t st) {
+  return launch_pdl(positions_kernel, dim3(nseq), dim3(128), 0, st, cu, nseq, first, pos);
 }
 
 cudaError_t launch_convert(int kind, const void* src, void* dst, size_t n, cudaStream_t st) {

@@ -25,6 +25,7 @@ struct Tensor {
   int dtype = kDtF32;  // kDtF32 or kDtBf16 on the device (F16 is widened to F32)
   std::vector<int64_t> shape;
   size_t numel = 0;
+  int model = 0;  // models loaded before it was uploaded
 };
 
 struct BertLayerW {
@@ -102,6 +103,8 @@ struct PendingEv {
   int e0, e1;
 };
 
+struct PrefixPool;  // ec_prefix.h
+
 struct Device {
   int ordinal = 0;
   std::vector<cudaEvent_t> evpool;  // profiling events, reused
@@ -109,6 +112,7 @@ struct Device {
   cudaStream_t stream = nullptr;
   int num_sms = 148;
   std::map<std::string, Tensor> uploads;
+  int models = 0;  // ec_load_model calls so far
   ModelW model;
   IndexW index;
   unsigned* status = nullptr;  // device status word of bounded waits
@@ -145,7 +149,9 @@ struct Device {
     size_t pin_bytes;
     cudaGraphExec_t exec;
     uint64_t used;
+    int prefix;  // slot of the prefix the texts follow, -1: none
   };
+  PrefixPool* prefixes = nullptr;  // cached prefixes of the model (ec_prefix_open)
   std::vector<FwdGraph> graphs;
   uint64_t graph_clock = 0;
 };
@@ -196,10 +202,15 @@ struct JVal;
 // build the model of config.json (+ pooling config) from d.uploads
 int load_model_on(Device& d, const JVal& cfg, const JVal* pool);
 
-// forward entry used by ec_embed_batch / ec_embed_batch_device
+// forward entry used by ec_embed_batch / ec_embed_batch_device /
+// ec_embed_batch_prefix: prefix = slot of d.prefixes that every sequence
+// follows (-1: none); with `fill` the one sequence becomes that prefix
 int embed_on_device(Device& d, const int32_t* ids_host, const int32_t* ids_dev,
                     const std::vector<int>& seqs, const int64_t* offsets, float* out_host,
-                    int out_stride, float* out_dev);
+                    int out_stride, float* out_dev, int prefix = -1, bool fill = false);
+// a host batch over all devices (ec_api.cu)
+int embed_batch_split(const int32_t* ids, const int64_t* offsets, int nseq, float* out, int out_stride,
+                      int prefix);
 
 // profiling helpers: bracket one launch with events (no-op unless profiling)
 int prof_begin(Device& d);

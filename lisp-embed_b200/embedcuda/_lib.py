@@ -54,6 +54,9 @@ _SIGS = {
     "ec_dim": (C.c_int, []),
     "ec_embed_batch": (C.c_int, [I32P, I64P, C.c_int, FP, C.c_int]),
     "ec_embed_batch_device": (C.c_int, [P, I64P, C.c_int, P, C.c_int, P]),
+    "ec_prefix_open": (C.c_int, [I32P, C.c_int, C.POINTER(C.c_int)]),
+    "ec_prefix_close": (C.c_int, [C.c_int]),
+    "ec_embed_batch_prefix": (C.c_int, [C.c_int, I32P, I64P, C.c_int, FP, C.c_int]),
     "ec_kmeans": (C.c_int, [FP, C.c_int64, C.c_int, I64P, C.c_int64, C.c_int, C.c_int, FP, FP]),
     "ec_assign_all": (C.c_int, [FP, C.c_int64, C.c_int, FP, C.c_int, U32P, U32P]),
     "ec_ann_build": (C.c_int, [FP, C.c_int64, C.c_int, I64P, C.c_int64, C.c_int, C.c_int, FP, FP,

@@ -54,6 +54,10 @@ def path():
 def embed_batch(ids, offsets, out=None):
     """Embed packed sequences: ids int32[total], offsets int64[nseq + 1].
     Returns float32[nseq, dim], L2-normalised, in input order."""
+    return _embed_batch(ids, offsets, out, None)
+
+
+def _embed_batch(ids, offsets, out, prefix):
     ids = np.ascontiguousarray(ids, np.int32)
     offsets = np.ascontiguousarray(offsets, np.int64)
     # the library reads ids[offsets[0] .. offsets[nseq]) and cannot see the
@@ -71,10 +75,51 @@ def embed_batch(ids, offsets, out=None):
           not out.flags.c_contiguous or not out.flags.writeable or out.shape[0] < nseq or
           out.shape[1] < D):
         raise ValueError(f"out must be a writeable C-contiguous float32[>= {nseq}, >= {D}] array")
-    _lib.check(_lib.lib().ec_embed_batch(_lib.ptr(ids, C.c_int32), _lib.ptr(offsets, C.c_int64),
-                                         nseq, _lib.ptr(out, C.c_float), out.shape[1]),
-               "embed_batch")
+    args = (_lib.ptr(ids, C.c_int32), _lib.ptr(offsets, C.c_int64), nseq, _lib.ptr(out, C.c_float),
+            out.shape[1])
+    if prefix is None:
+        _lib.check(_lib.lib().ec_embed_batch(*args), "embed_batch")
+    else:
+        _lib.check(_lib.lib().ec_embed_batch_prefix(prefix, *args), "embed_batch_prefix")
     return out
+
+
+class Prefix:
+    """Token ids in front of every text of a Llama-family model (the
+    instruction of a query), computed once: ``embed_batch(ids, offsets)`` equals
+    the module's ``embed_batch`` of prefix + text, at the cost of the texts'
+    own tokens.  Usable as a context manager; ends with ``close`` or the next
+    ``load_model``."""
+
+    def __init__(self, ids):
+        ids = np.ascontiguousarray(ids, np.int32)
+        if ids.ndim != 1:
+            raise ValueError("a prefix is int32[n]")
+        self._id = 0
+        out = C.c_int(0)
+        _lib.check(_lib.lib().ec_prefix_open(_lib.ptr(ids, C.c_int32), ids.size, C.byref(out)),
+                   "prefix_open")
+        self._id = out.value
+
+    def embed_batch(self, ids, offsets, out=None):
+        """``embed_batch`` of the texts behind this prefix."""
+        return _embed_batch(ids, offsets, out, self._id)
+
+    def embed(self, ids):
+        """One text behind this prefix -> float32[dim]."""
+        ids = np.ascontiguousarray(ids, np.int32)
+        return self.embed_batch(ids, np.array([0, ids.size], np.int64))[0]
+
+    def close(self):
+        if self._id:
+            prefix, self._id = self._id, 0
+            _lib.check(_lib.lib().ec_prefix_close(prefix), "prefix_close")
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        self.close()
 
 
 def embed(ids):

@@ -25,6 +25,7 @@
 (defpackage :cuda
   (:use :cl)
   (:export #:init #:available-p #:load-model #:dim #:embed-ids #:embed-batch
+           #:prefix-open #:prefix-close
            #:load-tokenizer #:embed-texts
            #:kmeans #:assign-all #:ann-build #:index-load #:index-load-files #:ann-build-file
            #:top-k #:top-k-brute #:top-k-batch #:*nprobe*
@@ -54,6 +55,13 @@
 (sb-alien:define-alien-routine ("ec_embed_batch" %embed-batch) sb-alien:int
   (ids sb-sys:system-area-pointer) (offsets sb-sys:system-area-pointer) (nseq sb-alien:int)
   (out sb-sys:system-area-pointer) (out-stride sb-alien:int))
+(sb-alien:define-alien-routine ("ec_prefix_open" %prefix-open) sb-alien:int
+  (ids sb-sys:system-area-pointer) (n sb-alien:int) (prefix sb-sys:system-area-pointer))
+(sb-alien:define-alien-routine ("ec_prefix_close" %prefix-close) sb-alien:int
+  (prefix sb-alien:int))
+(sb-alien:define-alien-routine ("ec_embed_batch_prefix" %embed-batch-prefix) sb-alien:int
+  (prefix sb-alien:int) (ids sb-sys:system-area-pointer) (offsets sb-sys:system-area-pointer)
+  (nseq sb-alien:int) (out sb-sys:system-area-pointer) (out-stride sb-alien:int))
 (sb-alien:define-alien-routine ("ec_kmeans" %kmeans) sb-alien:int
   (x sb-sys:system-area-pointer) (n (sb-alien:signed 64)) (d sb-alien:int)
   (sample sb-sys:system-area-pointer) (nsample (sb-alien:signed 64)) (k sb-alien:int)
@@ -172,9 +180,22 @@ family keyword as model:load-model does (model.lisp:28-46)."
 
 (defun dim () *dim*)
 
-(defun embed-batch (id-vectors)
+(defun prefix-open (ids)
+  "Token ids in front of every text of a llama model (the instruction of a
+query), computed once -> prefix for EMBED-BATCH; ends with PREFIX-CLOSE."
+  (let ((v (coerce ids '(simple-array (signed-byte 32) (*))))
+        (id (make-array 1 :element-type '(signed-byte 32))))
+    (with-saps ((vp v) (ip id))
+      (check (%prefix-open vp (length v) ip) "ec_prefix_open"))
+    (aref id 0)))
+
+(defun prefix-close (prefix)
+  (check (%prefix-close prefix) "ec_prefix_close"))
+
+(defun embed-batch (id-vectors &key prefix)
   "List of token-id vectors -> list of L2-normalised (simple-array
-single-float (dim)), in input order (model:embed for a whole batch)."
+single-float (dim)), in input order (model:embed for a whole batch).
+PREFIX (PREFIX-OPEN) stands in front of every text."
   (let* ((n (length id-vectors))
          (offsets (make-array (1+ n) :element-type '(signed-byte 64)))
          (total (reduce #'+ id-vectors :key #'length))
@@ -187,7 +208,9 @@ single-float (dim)), in input order (model:embed for a whole batch)."
              (loop for x across v do (setf (aref ids pos) x) (incf pos))
           finally (setf (aref offsets n) pos))
     (with-saps ((ip ids) (op offsets) (outp out))
-      (check (%embed-batch ip op n outp *dim*) "ec_embed_batch"))
+      (if prefix
+          (check (%embed-batch-prefix prefix ip op n outp *dim*) "ec_embed_batch_prefix")
+          (check (%embed-batch ip op n outp *dim*) "ec_embed_batch")))
     (loop for i below n
           collect (subseq out (* i *dim*) (* (1+ i) *dim*)))))
 
