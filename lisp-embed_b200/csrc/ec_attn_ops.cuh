@@ -23,7 +23,20 @@
 // below 2^8 in its 16 bits; sums are fp32).
 //
 // Warps: 4 per tile softmax, then one each for the loads, the MMAs and the
-// work list.  All waits are bounded.
+// work list.  NT = 2 has four more that divide O by the row sums and write it,
+// and the MMA warp issues a tile's first scores of the next tile set as soon as
+// the tile is through: a softmax warp has nothing to wait for between two sets
+// (256 prompts of 320 tokens: 305 -> 276 us; a trace had shown 35% of the
+// softmax warps' time between their last exponentials and the next scores).
+// All waits are bounded.
+//
+// What bounds it: the exponentials.  16384 tokens of 8 heads of 128 take 473
+// us; the MMAs alone 344 (the peak rate 328), the softmax warps alone 426.  A
+// block costs a warp 128 exponentials (three of four on the special-function
+// unit, 16 a cycle and SM, every fourth on the FMA units: all on the former 522
+// us, every third on the FMA units 490), the scale, sum and packing two values
+// an instruction, the maximum three, and two reads of the scores from TMEM,
+// which keep a thread within 168 registers.
 #pragma once
 
 #include <cuda_fp16.h>
@@ -95,9 +108,11 @@ struct FlashCfg {
   static constexpr uint32_t TILE = AT * ATOM;
   static constexpr int STAGES = HD == 128 ? 5 : 8;   // K and V tiles in flight
   static constexpr int MAX_SEQS = 2048;              // prefix sums of an even split
-  static constexpr int WARPS = 4 * NT + 3;
+  // NT 1: four softmax warps, loads, MMAs, list.  NT 2: eight, loads, MMAs,
+  // list, none, and four that write the results.
+  static constexpr int WARPS = NT == 2 ? 16 : 7;
   static constexpr int THREADS = 32 * WARPS;
-  static constexpr uint32_t TAIL = 1536 + (NT == 1 ? 8 * MAX_SEQS : 0);
+  static constexpr uint32_t TAIL = 1536 + (NT == 1 ? 8 * MAX_SEQS : 1024);
   static constexpr size_t SMEM = NT * TILE + STAGES * TILE + TAIL;
   static constexpr uint32_t O_COL = 256;
   static_assert(SMEM <= 232448, "shared memory");
@@ -176,12 +191,33 @@ __device__ __forceinline__ FlashSeq flash_seq(const FlashArgs& a, int s) {
 // f(s) = cu[s] / BT + s for BT tokens per set.  f leaves at least
 // ceil(len / BT) slots to every sequence and needs no prefix sum; a slot's
 // sequence is found by bisection, 32 slots at a time.  Their number (times the
-// key heads) fits 31 bits, checked on the host.
+// key heads) fits 31 bits, checked on the host.  The key heads of a set and the
+// sets of a sequence follow each other, so that the CTAs read the same keys at
+// about the same time: with a run of the list for every CTA, of equal work, 256
+// prompts of 320 tokens took 383 us instead of 272.
+//
+// Up to 32 sequences go by set, the latest sets of all of them first (slot u:
+// set u / nseq of sequence u % nseq), so that a CTA's few turns cost the same:
+// 4 prompts of 2048 tokens 84 us instead of 135.  With more sequences that
+// costs the keys' reuse: 96 texts behind 650 cached tokens 182 us instead of
+// 160 (64 prompts of 300 tokens 139 instead of 153).
 template <int NT, typename Publish>
 __device__ __noinline__ bool flash_slots(const FlashArgs& a, int lane, Publish publish) {
   const int R = a.rows_tok, BT = NT * R;
-  const uint32_t slots = a.tokens / BT + a.nseq, all = slots * a.kv_heads, step = gridDim.x;
+  uint32_t slots = a.tokens / BT + a.nseq;
+  const uint32_t step = gridDim.x;
+  const bool few = a.nseq <= 32;
+  if (few) {
+    const FlashSeq q = flash_seq(a, min(lane, a.nseq - 1));
+    slots = __reduce_max_sync(0xffffffffu, (q.end - q.begin + BT - 1) / BT) * a.nseq;
+  }
+  const uint32_t all = slots * a.kv_heads;
   bool ok = true;
+  // the offsets are far away: their lines all at once, not one after the other
+  // in the bisections
+#pragma unroll 1
+  for (int s = lane * 32; s < min(a.nseq + 1, 8192); s += 1024) asm volatile("" ::"r"(a.cu[s]));
+  __syncwarp();
 #pragma unroll 1
   for (uint32_t t0 = 0; ok && t0 < all; t0 += 32 * step) {
     // late (long) tile sets first; the order turns round every pass, so that
@@ -190,7 +226,7 @@ __device__ __noinline__ bool flash_slots(const FlashArgs& a, int lane, Publish p
     FlashEntry it{};
     if (t < all) {
       const int u = static_cast<int>(slots - 1 - t / a.kv_heads);
-      int lo = 0, hi = a.nseq;  // last sequence with f <= u
+      int lo = few ? u % a.nseq : 0, hi = few ? 0 : a.nseq;  // last sequence with f <= u
       while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
         if (min(max(a.cu[mid], 0), a.tokens) / BT + mid <= u) lo = mid;
@@ -198,7 +234,7 @@ __device__ __noinline__ bool flash_slots(const FlashArgs& a, int lane, Publish p
       }
       const FlashSeq q = flash_seq(a, lo);
       const int len = q.end - q.begin;
-      const int i = u - (q.begin / BT + lo);  // tile set of the sequence
+      const int i = few ? u / a.nseq : u - (q.begin / BT + lo);  // tile set of the sequence
       if (i >= 0 && i < (len + BT - 1) / BT) {
         const int q0 = i * BT;
         it.valid = 1;
@@ -401,7 +437,8 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
   constexpr uint32_t IDESC_S = make_idesc(FMT, 128, 128);
   constexpr uint32_t IDESC_PV = make_idesc(FMT, 128, HD) | (1u << 16);  // B MN-major
   constexpr int W_LOAD = 4 * NT, W_MMA = 4 * NT + 1, W_LIST = 4 * NT + 2;
-  constexpr int READERS = 4 * NT + 2;  // warps that read a list entry
+  constexpr int W_EPI = 12;                         // NT 2: warps 12 .. 15
+  constexpr int READERS = NT == 2 ? 14 : 6;         // warps that read a list entry
 
   extern __shared__ __align__(1024) uint8_t smem[];
   if (smem_u32(smem) & 1023u) {  // swizzled tiles need 1024-byte alignment
@@ -420,14 +457,17 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
   uint64_t* p_half = p_full + 2;      // [2] the first 64 keys' P
   uint64_t* o_full = p_half + 2;      // [2] tile (NT 2), or even / odd blocks (NT 1)
   uint64_t* x_bar = o_full + 2;       // [2] the softmax warps of NT 1
-  uint64_t* i_full = x_bar + 2;       // [kFlashRing]
+  uint64_t* r_full = x_bar + 2;       // [2] a tile's sums (NT 2)
+  uint64_t* o_free = r_full + 2;      // [2] a tile's O has been read (NT 2)
+  uint64_t* i_full = o_free + 2;      // [kFlashRing]
   uint64_t* i_empty = i_full + kFlashRing;
   FlashItem* items = reinterpret_cast<FlashItem*>(i_empty + kFlashRing);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(items + kFlashRing);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* last_part = abort_flag + 1;
   int* prefix = reinterpret_cast<int*>(tail + 1536);  // [MAX_SEQS] of an even split
-  static_assert(8 * (4 + 2 * ST + 10 + 2 * kFlashRing) + kFlashRing * sizeof(FlashItem) + 12 <= 1536, "tail");
+  float* inverse = reinterpret_cast<float*>(tail + 1536);  // [2][128] 1 / l (NT 2)
+  static_assert(8 * (4 + 2 * ST + 14 + 2 * kFlashRing) + kFlashRing * sizeof(FlashItem) + 12 <= 1536, "tail");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -443,6 +483,8 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
       mbar_init(&p_half[i], 4);
       mbar_init(&o_full[i], 1);
       mbar_init(&x_bar[i], 4);
+      mbar_init(&r_full[i], 4);
+      mbar_init(&o_free[i], 4);
     }
     for (int i = 0; i < kFlashRing; ++i) {
       mbar_init(&i_full[i], 1);
@@ -494,6 +536,53 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
   };
   auto pages_in_use = [&](int kv_len) { return (kv_len + a.page_size - 1) / a.page_size; };
 
+  // writes this warp's rows of tile t: O / l, or 0 where inv is 0 (a row that
+  // sees nothing)
+  auto write_rows = [&](const FlashEntry& it, int t, int n, bool live, float inv, uint32_t o_addr) {
+    const int r = (warp & 3) * 32 + lane, tok = r / G;
+    const int64_t row = it.tok0 + t * R + tok;
+    T* o = static_cast<T*>(a.out) + row * a.ot + (it.kvh * G + r - tok * G) * a.oh;
+    float* po = a.part_o + (static_cast<int64_t>(max(it.part, 0)) * a.part_rows + r) * HD;
+#pragma unroll 1
+    for (int c = 0; c < HD / 32; ++c) {
+      uint32_t v[32];
+      if (n > 0) {
+        tmem_ld_32x32b_x32(o_addr + c * 32, v);
+        tmem_wait_ld();
+      }
+      if (NT == 2 && n > 0 && c == HD / 32 - 1) {  // the next P V may overwrite it
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&o_free[t]);
+      }
+      if (live) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = inv == 0.f ? 0u : __float_as_uint(__uint_as_float(v[i]) * inv);
+        if (NT == 1 && it.part >= 0) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) store32(po + c * 32 + 8 * i, v + 8 * i);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) v[i] = pack2<T>(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+          if (a.wide) {
+            if (c * 32 < a.head_dim) store32(o + c * 32, v);
+            if (c * 32 + 16 < a.head_dim) store32(o + c * 32 + 16, v + 8);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (c * 32 + 8 * i < a.head_dim)
+                *reinterpret_cast<uint4*>(o + c * 32 + 8 * i) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+          }
+        }
+      }
+      __syncwarp();  // the loads from TMEM are the whole warp's
+    }
+  };
+
+  if constexpr (NT == 2) {
+    // 512 threads of 128 registers: 168 for the softmax, 88 for the rest
+    if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+  }
   if (warp == W_LIST) {
     using Entry = FlashEntry;
     // ------------------------------------------------------------ work list
@@ -614,6 +703,7 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
       uint32_t ph = 0;       // its phase
       int qi = 0;            // items so far
       uint32_t pf[2] = {0, 0};  // P's waited for, per tile
+      uint32_t of[2] = {0, 0};  // results begun, per tile (NT 2)
       uint32_t g = 0;           // blocks (NT 1)
       const uint64_t dq = desc_sw128_kmajor(smem_u32(sQ));
       const uint64_t dk = desc_sw128_kmajor(smem_u32(sKV));
@@ -644,30 +734,42 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
           umma_f16_ts(d, p + (4 * half + kk) * 8, v + (4 * half + kk) * (2048 >> 4), IDESC_PV,
                       kk > 0 || half > 0 || !first);
       };
-      while (true) {
-        const int b = it_n % kFlashRing;
-        if (!(ok = mbar_wait(&i_full[b], (it_n / kFlashRing) & 1, abort_flag))) break;
-        const int valid = items[b].valid, kb0 = items[b].kb0;
-        const int n0 = items[b].nb[0] - kb0, n1 = NT == 2 ? items[b].nb[1] - kb0 : 0, n = max(n0, n1);
-        mbar_arrive(&i_empty[b]);
-        ++it_n;
-        if (!valid) break;
-        if (n <= 0) continue;
-        const int qb = a.q_bufs == 2 ? qi & 1 : 0;
-        if (!(ok = wait(&q_full[qb], (a.q_bufs == 2 ? qi >> 1 : qi) & 1)) || !(ok = wait(&kv_full[st], ph))) break;
-        ++qi;
-        if constexpr (NT == 2) {
-          if (n0 > 0) {
-            mma_s(qb, 0, st, tmem);
-            umma_commit(&s_full[0]);
+      int n0 = 0, n1 = 0;  // key blocks of the tiles of the item that `take` found
+      bool more = true;    // there was one
+      auto take = [&]() -> bool {
+        while (true) {
+          const int b = it_n % kFlashRing;
+          if (!mbar_wait(&i_full[b], (it_n / kFlashRing) & 1, abort_flag)) return false;
+          const int kb0 = items[b].kb0;
+          more = items[b].valid;
+          n0 = items[b].nb[0] - kb0, n1 = NT == 2 ? items[b].nb[1] - kb0 : 0;
+          mbar_arrive(&i_empty[b]);
+          ++it_n;
+          if (!more || max(n0, n1) > 0) return true;
+        }
+      };
+      if constexpr (NT == 2) {
+        // the first scores of the item taken last, tile t
+        auto begin = [&](int t) -> bool {
+          if (t == 0) {
+            if (!wait(&q_full[0], qi & 1) || !wait(&kv_full[st], ph)) return false;
+            ++qi;
           }
-          if (n1 > 0) {
-            mma_s(qb, 1, st, tmem + 128);
-            umma_commit(&s_full[1]);
+          if ((t ? n1 : n0) > 0) {
+            mma_s(0, t, st, tmem + t * 128);
+            umma_commit(&s_full[t]);
           }
-          umma_commit(&kv_empty[st]);
-          if (n == 1) umma_commit(&q_empty[qb]);
-          advance();
+          if (t == 1) {
+            umma_commit(&kv_empty[st]);
+            if (max(n0, n1) == 1) umma_commit(&q_empty[0]);
+            advance();
+          }
+          return true;
+        };
+        ok = take();
+        if (ok && more) ok = begin(0) && begin(1);
+        while (ok && more) {
+          const int c0 = n0, c1 = n1, n = max(c0, c1);
 #pragma unroll 1
           for (int j = 0; ok && j < n; ++j) {
             const int sv = st;
@@ -676,33 +778,51 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
             bool have_v = false, have_k = false;
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-              const int nt = t ? n1 : n0;
-              if (!ok || j >= nt) continue;
-              if (!have_v && !(ok = wait(&kv_full[sv], phv))) break;
-              have_v = true;
-              if (!(ok = wait(&p_half[t], pf[t] & 1))) break;
-              mma_pv(tmem + Cfg::O_COL + t * HD, tmem + t * 128, sv, j == 0, 0);
-              if (!(ok = wait(&p_full[t], pf[t] & 1))) break;
-              ++pf[t];
-              mma_pv(tmem + Cfg::O_COL + t * HD, tmem + t * 128, sv, false, 1);
+              const int nt = t ? c1 : c0;
+              if (!ok) continue;
+              if (j < nt) {
+                if (!have_v && !(ok = wait(&kv_full[sv], phv))) continue;
+                have_v = true;
+                if (!(ok = wait(&p_half[t], pf[t] & 1))) continue;
+                if (j == 0) {
+                  if (of[t] > 0 && !(ok = wait(&o_free[t], (of[t] - 1) & 1))) continue;
+                  ++of[t];
+                }
+                mma_pv(tmem + Cfg::O_COL + t * HD, tmem + t * 128, sv, j == 0, 0);
+                if (!(ok = wait(&p_full[t], pf[t] & 1))) continue;
+                ++pf[t];
+                mma_pv(tmem + Cfg::O_COL + t * HD, tmem + t * 128, sv, false, 1);
+              }
+              if (j + 1 == nt) umma_commit(&o_full[t]);
+              if (t == 1) umma_commit(&kv_empty[sv]);
               if (j + 1 < nt) {
-                if (!have_k && !(ok = wait(&kv_full[st], ph))) break;
+                if (!have_k && !(ok = wait(&kv_full[st], ph))) continue;
                 have_k = true;
-                mma_s(qb, t, st, tmem + t * 128);
+                mma_s(0, t, st, tmem + t * 128);
                 umma_commit(&s_full[t]);
-              } else {
-                umma_commit(&o_full[t]);
+              }
+              if (j + 1 == n) {
+                // this tile is done: the next item's scores do not wait for
+                // the other tile's last block
+                if (t == 0) ok = take();
+                if (ok && more) ok = begin(t);
               }
             }
             if (!ok) break;
-            umma_commit(&kv_empty[sv]);
             if (j + 1 < n) {
               umma_commit(&kv_empty[st]);
-              if (j + 2 == n) umma_commit(&q_empty[qb]);
+              if (j + 2 == n) umma_commit(&q_empty[0]);
               advance();
             }
           }
-        } else {
+        }
+      }
+      while (NT == 1) {
+        if (!(ok = take()) || !more) break;
+        const int n = n0, qb = a.q_bufs == 2 ? qi & 1 : 0;
+        if (!(ok = wait(&q_full[qb], (a.q_bufs == 2 ? qi >> 1 : qi) & 1)) || !(ok = wait(&kv_full[st], ph))) break;
+        ++qi;
+        {
           mma_s(qb, 0, st, tmem + (g & 1) * 128);
           umma_commit(&s_full[g & 1]);
           umma_commit(&kv_empty[st]);
@@ -737,8 +857,37 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
       }
     }
     __syncwarp();
+  } else if (NT == 2 && warp >= 8) {
+    // -------------------------------------------------------------- results
+    code = kDevTimeoutEpilogue;
+    uint32_t done[2] = {0, 0};
+    while (warp >= W_EPI) {
+      const FlashItem* ip = next_item();
+      if (!(ok = ip != nullptr) || !ip->valid) break;
+      const FlashEntry it = *ip;
+      done_item();
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int r = (warp & 3) * 32 + lane, tok = r / G;
+        const bool live = tok < R && t * R + tok < it.qv;
+        const int n = it.nb[t] - it.kb0;
+        float inv = 0.f;
+        if (n > 0) {
+          if (!(ok = mbar_wait_warp(&r_full[t], done[t] & 1, abort_flag)) ||
+              !(ok = mbar_wait_warp(&o_full[t], done[t] & 1, abort_flag)))
+            break;
+          ++done[t];
+          tc_fence_after();
+          inv = inverse[t * 128 + r];
+        }
+        if (n > 0 || __any_sync(0xffffffffu, live))
+          write_rows(it, t, n, live, inv, tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + Cfg::O_COL + t * HD);
+      }
+      if (!ok) break;
+    }
   } else {
     // -------------------------------------------------------------- softmax
+    if constexpr (NT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
     code = kDevTimeoutEpilogue;
     const int t = warp >> 2;               // tile (0 for NT 1)
     const int r = (warp & 3) * 32 + lane;  // row of the tile = TMEM lane
@@ -748,7 +897,7 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
     const float sc = a.scale_log2;
     int g = 0;       // blocks so far (of this tile)
     int e = 0;       // K / V tiles before this item's
-    int done = 0;    // tiles whose result was read (NT 2)
+    int done = 0;    // results handed on (NT 2)
     int x = 0;       // meetings of the four warps (NT 1)
     while (true) {
       const FlashItem* ip = next_item();
@@ -791,27 +940,38 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
           // P): half the code and a third of the registers of holding all 128
           const int left = vis - (it.kb0 + j) * 128;
           const bool cut = __any_sync(0xffffffffu, live && left < 128);
+          // the second 64 keys may be behind every row of the warp (NT 1: 512
+          // prompts of 64 tokens 146 -> 133 us; with NT 2 the loop over fewer
+          // halves slows the others down, 16384 tokens 473 -> 492 us)
+          const int halves = NT == 1 && !__any_sync(0xffffffffu, live && left > 64) ? 1 : 2;
           uint32_t s[2][32];
           auto scores = [&](int h) {
             tmem_ld_32x32b_x32(s_addr + h * 64, s[0]);
             tmem_ld_32x32b_x32(s_addr + h * 64 + 32, s[1]);
             tmem_wait_ld();
             if (cut) {
+              const int see = left - h * 64;
+              const uint32_t w0 = see >= 32 ? 0xffffffffu : see <= 0 ? 0u : (1u << see) - 1u;
+              const uint32_t w1 = see >= 64 ? 0xffffffffu : see <= 32 ? 0u : (1u << (see - 32)) - 1u;
 #pragma unroll
-              for (int i = 0; i < 64; ++i)
-                if (h * 64 + i >= left) s[i >> 5][i & 31] = 0xff800000u;  // -infinity
+              for (int i = 0; i < 32; ++i) {
+                if (!(w0 & (1u << i))) s[0][i] = 0xff800000u;  // -infinity
+                if (!(w1 & (1u << i))) s[1][i] = 0xff800000u;
+              }
             }
           };
           float top = -INFINITY;
 #pragma unroll 1
-          for (int h = 0; h < 2; ++h) {
+          for (int h = 0; h < halves; ++h) {
             scores(h);
             float mx[4];
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
               mx[c] = __uint_as_float(s[c >> 1][(c & 1) * 16]);
 #pragma unroll
-              for (int i = 1; i < 16; ++i) mx[c] = fmaxf(mx[c], __uint_as_float(s[c >> 1][(c & 1) * 16 + i]));
+              for (int i = 1; i < 15; i += 2)
+                asm("max.f32 %0, %0, %1, %2;" : "+f"(mx[c]) : "f"(__uint_as_float(s[c >> 1][(c & 1) * 16 + i])), "f"(__uint_as_float(s[c >> 1][(c & 1) * 16 + i + 1])));
+              mx[c] = fmaxf(mx[c], __uint_as_float(s[c >> 1][(c & 1) * 16 + 15]));
             }
             top = fmaxf(top, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
           }
@@ -843,7 +1003,7 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
           float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
           const float2 sc2 = make_float2(sc, sc), nm2 = make_float2(nm, nm);
 #pragma unroll 1
-          for (int h = 0; h < 2; ++h) {
+          for (int h = 0; h < halves; ++h) {
             scores(h);
             uint32_t p[32];
 #pragma unroll
@@ -861,6 +1021,16 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
             if (lane == 0) mbar_arrive(h ? &p_full[buf] : &p_half[buf]);
           }
           l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+          if (halves == 1) {
+            uint32_t z[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) z[i] = 0u;
+            tmem_st_32x32b_x32(s_addr + 32, z);
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[buf]);
+          }
         } else {
           tc_fence_before();
           if (lane == 0) {
@@ -871,55 +1041,33 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
       }
       if (!ok) break;
       e += 2 * max(0, max(it.nb[0], NT == 2 ? it.nb[1] : 0) - it.kb0);
-      if (n > 0) {
-        // the last P V of this tile.  NT 1 alternates between two barriers:
-        // the scores of block g came after P V of g - 2, so a wait for g - 1
-        // is never two phases from its barrier's
-        if (!(ok = mbar_wait_warp(&o_full[NT == 2 ? t : (g - 1) & 1], NT == 2 ? done & 1 : ((g - 1) >> 1) & 1, abort_flag)))
-          break;
-        ++done;
-        tc_fence_after();
-      }
-      if (warp_live) {
-        const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // NaN stays NaN
-        const float l2 = l == 0.f ? -INFINITY : m * sc + log2f(l);
-        const int64_t row = it.tok0 + qt;
-        const int h = it.kvh * G + head;
-        T* o = static_cast<T*>(a.out) + row * a.ot + h * a.oh;
-        float* po = a.part_o + (static_cast<int64_t>(max(it.part, 0)) * a.part_rows + r) * HD;
-#pragma unroll 1
-        for (int c = 0; c < HD / 32; ++c) {
-          uint32_t v[32];
-          if (n > 0) {
-            tmem_ld_32x32b_x32(o_addr + c * 32, v);
-            tmem_wait_ld();
-          }
-          if (live) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i)  // 0: a row that sees nothing
-              v[i] = l == 0.f ? 0u : __float_as_uint(__uint_as_float(v[i]) * inv);
-            if (it.part >= 0) {
-#pragma unroll
-              for (int i = 0; i < 4; ++i) store32(po + c * 32 + 8 * i, v + 8 * i);
-            } else {
-#pragma unroll
-              for (int i = 0; i < 16; ++i) v[i] = pack2<T>(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
-              if (a.wide) {
-                if (c * 32 < a.head_dim) store32(o + c * 32, v);
-                if (c * 32 + 16 < a.head_dim) store32(o + c * 32 + 16, v + 8);
-              } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                  if (c * 32 + 8 * i < a.head_dim)
-                    *reinterpret_cast<uint4*>(o + c * 32 + 8 * i) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-              }
-            }
-          }
-          __syncwarp();  // the loads from TMEM are the whole warp's
+      const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // NaN stays NaN
+      const float l2 = l == 0.f ? -INFINITY : m * sc + log2f(l);
+      if (live && it.part < 0 && a.lse)
+        a.lse[static_cast<int64_t>(it.tok0 + qt) * a.q_heads + it.kvh * G + head] = l2 * 0.693147180559945309f;
+      if constexpr (NT == 2) {
+        if (n > 0) {
+          // the warps that write the results take it from here, once they
+          // are done with the tile's last ones
+          if (done > 0 && !(ok = mbar_wait_warp(&o_free[t], (done - 1) & 1, abort_flag))) break;
+          ++done;
+          inverse[t * 128 + r] = inv;
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&r_full[t]);
         }
-        if (live) {
-          if (it.part >= 0) a.part_l[it.part * a.part_rows + r] = l2;
-          else if (a.lse) a.lse[row * a.q_heads + h] = l2 * 0.693147180559945309f;
+        continue;
+      } else {
+        if (n > 0) {
+          // the last P V.  Two barriers alternate: the scores of block g came
+          // after P V of g - 2, so a wait for g - 1 is never two phases from
+          // its barrier's
+          if (!(ok = mbar_wait_warp(&o_full[(g - 1) & 1], ((g - 1) >> 1) & 1, abort_flag))) break;
+          tc_fence_after();
+        }
+        if (warp_live) {
+          write_rows(it, t, n, live, inv, o_addr);
+          if (live && it.part >= 0) a.part_l[it.part * a.part_rows + r] = l2;
         }
         __syncwarp();
       }
