@@ -60,8 +60,8 @@ int launch_one(int id, FlashFn fn, int threads, size_t smem, const CUtensorMap& 
   return check_cuda(launch_pdl(fn, dim3(grid), dim3(threads), smem, st, q, k, v, a), "attention");
 }
 
-// tile sets of 256 rows, tiles of 128 rows, tiles of at most 32 .. 4 rows
-enum FlashKind { kPairs, kTiles, kFew32, kFew16, kFew8, kFew4 };
+// tile sets of 256 rows (kHalves: of short sequences), tiles of 128 rows, tiles of at most 32 .. 4 rows
+enum FlashKind { kPairs, kHalves, kTiles, kFew32, kFew16, kFew8, kFew4 };
 
 template <int HD, int NP, typename T>
 int launch_token(int id, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const FlashArgs& a, int grid,
@@ -77,10 +77,13 @@ int launch_flash(FlashKind kind, const CUtensorMap& q, const CUtensorMap& k, con
   int rc;
   switch (kind) {
     case kPairs:
-      rc = launch_one(id, flash_kernel<HD, 2, T>, FlashCfg<HD, 2>::THREADS, FlashCfg<HD, 2>::SMEM, q, k, v, a, grid, st);
+      rc = launch_one(id, flash_kernel<HD, 2, false, T>, FlashCfg<HD, 2>::THREADS, FlashCfg<HD, 2>::SMEM, q, k, v, a, grid, st);
+      break;
+    case kHalves:
+      rc = launch_one(id, flash_kernel<HD, 2, true, T>, FlashCfg<HD, 2>::THREADS, FlashCfg<HD, 2>::SMEM, q, k, v, a, grid, st);
       break;
     case kTiles:
-      rc = launch_one(id, flash_kernel<HD, 1, T>, FlashCfg<HD, 1>::THREADS, FlashCfg<HD, 1>::SMEM, q, k, v, a, grid, st);
+      rc = launch_one(id, flash_kernel<HD, 1, true, T>, FlashCfg<HD, 1>::THREADS, FlashCfg<HD, 1>::SMEM, q, k, v, a, grid, st);
       break;
     case kFew32: rc = launch_token<HD, 32, T>(id, q, k, v, a, grid, st); break;
     case kFew16: rc = launch_token<HD, 16, T>(id, q, k, v, a, grid, st); break;
@@ -91,6 +94,9 @@ int launch_flash(FlashKind kind, const CUtensorMap& q, const CUtensorMap& k, con
 }
 
 // How a call is cut up, from what the host knows
+// packed prompts below this many tokens on average run the kernel that leaves
+// out halves of blocks (measured beside it)
+constexpr int kHalvesBelow = 1024;
 struct FlashPlan {
   FlashKind kind;
   int even, rows_tok;  // tokens of a tile
@@ -116,7 +122,7 @@ FlashPlan flash_plan(const KvCache* c, int64_t tokens, int q_heads, int kv_heads
   }
   if (!p.even && tokens > static_cast<int64_t>(nseq) * p.rows_tok &&
       (tokens / (2 * p.rows_tok) + nseq) * kv_heads >= num_sms)
-    p.kind = kPairs;
+    p.kind = !c && tokens < static_cast<int64_t>(nseq) * kHalvesBelow ? kHalves : kPairs;
   return p;
 }
 
@@ -176,7 +182,7 @@ int run_attention(const AttnOp& op, int num_sms, cudaStream_t st) {
     a.page0 = op.layer * c->pages, a.page_end = c->layers * c->pages;
   }
   a.q_bufs = p.kind == kTiles && group * p.rows_tok <= 64 ? 2 : 1;
-  const int sets = p.rows_tok * (p.kind == kPairs ? 2 : 1);
+  const int sets = p.rows_tok * (p.kind == kPairs || p.kind == kHalves ? 2 : 1);
   int64_t grid = (op.tokens / sets + op.nseq) * op.kv_heads;
   if (grid >= INT32_MAX / 2)
     return set_error(EC_EINVAL, "%lld tokens of %d sequences and %d key heads: too many for one call",

@@ -427,14 +427,14 @@ __device__ __forceinline__ bool flash_arrive(const FlashArgs& a, const FlashEntr
   return last;
 }
 
-template <int HD, int NT, typename T>
+template <int HD, int NT, bool HALF, typename T>
 __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
     flash_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                  const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ FlashArgs a) {
   using Cfg = FlashCfg<HD, NT>;
   constexpr int AT = Cfg::AT, ST = Cfg::STAGES;
   constexpr int FMT = sizeof(T) == 2 && std::is_same<T, __half>::value ? 0 : 1;
-  constexpr uint32_t IDESC_S = make_idesc(FMT, 128, 128);
+  constexpr uint32_t IDESC_S = make_idesc(FMT, 128, 128), IDESC_S64 = make_idesc(FMT, 128, 64);
   constexpr uint32_t IDESC_PV = make_idesc(FMT, 128, HD) | (1u << 16);  // B MN-major
   constexpr int W_LOAD = 4 * NT, W_MMA = 4 * NT + 1, W_LIST = 4 * NT + 2;
   constexpr int W_EPI = 12;                         // NT 2: warps 12 .. 15
@@ -526,6 +526,16 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
     if (lane == 0) mbar_arrive(&i_empty[it_n % kFlashRing]);
     ++it_n;
   };
+  // Keys that the last query of tile t sees, from the block `at` on.  HALF: in
+  // a block where that is 64 or less, the other half takes no part in anything.
+  // It pays with short sequences, whose last blocks are many (1024 prompts of
+  // 130 tokens 590 -> 545 us, 256 of 320 279 -> 273); elsewhere the loops of one
+  // or two halves slow the others down (one of 16384 481 -> 496, of 4096 82 ->
+  // 86, 32 of 1024 190 -> 188).
+  auto tile_sees = [&](const FlashEntry& it, int t, int at) {
+    return HALF ? min(it.kv_len, it.pos0 + min((t + 1) * R, it.qv)) - at * 128 : 128;
+  };
+  auto one_half = [&](int sees, int j) { return HALF && sees - j * 128 <= 64; };
   const int ppb = a.paged ? 128 / a.page_size : 1;  // pages per key block
   // page of table entry e of a slot with `in_use` pages; one that is none
   // reads past the pages, which fills the tile with zeros
@@ -719,12 +729,12 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
           ph ^= 1;
         }
       };
-      auto mma_s = [&](int qb, int t, int stage, uint32_t d) {
+      auto mma_s = [&](int qb, int t, int stage, uint32_t d, bool half) {
         const uint64_t q = dq + qb * (kQBuf >> 4) + t * (Cfg::TILE >> 4), k = dk + stage * (Cfg::TILE >> 4);
 #pragma unroll
         for (int kk = 0; kk < HD / 16; ++kk) {
           const uint32_t off = ((kk >> 2) * Cfg::ATOM + (kk & 3) * 32) >> 4;
-          umma_f16(d, q + off, k + off, IDESC_S, kk > 0);
+          umma_f16(d, q + off, k + off, half ? IDESC_S64 : IDESC_S, kk > 0);
         }
       };
       auto mma_pv = [&](uint32_t d, uint32_t p, int stage, bool first, int half) {
@@ -735,6 +745,7 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
                       kk > 0 || half > 0 || !first);
       };
       int n0 = 0, n1 = 0;  // key blocks of the tiles of the item that `take` found
+      int k0 = 0, k1 = 0;  // and keys that they see of them
       bool more = true;    // there was one
       auto take = [&]() -> bool {
         while (true) {
@@ -743,6 +754,7 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
           const int kb0 = items[b].kb0;
           more = items[b].valid;
           n0 = items[b].nb[0] - kb0, n1 = NT == 2 ? items[b].nb[1] - kb0 : 0;
+          k0 = tile_sees(items[b], 0, kb0), k1 = NT == 2 ? tile_sees(items[b], 1, kb0) : 0;
           mbar_arrive(&i_empty[b]);
           ++it_n;
           if (!more || max(n0, n1) > 0) return true;
@@ -756,7 +768,7 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
             ++qi;
           }
           if ((t ? n1 : n0) > 0) {
-            mma_s(0, t, st, tmem + t * 128);
+            mma_s(0, t, st, tmem + t * 128, one_half(t ? k1 : k0, 0));
             umma_commit(&s_full[t]);
           }
           if (t == 1) {
@@ -769,7 +781,7 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
         ok = take();
         if (ok && more) ok = begin(0) && begin(1);
         while (ok && more) {
-          const int c0 = n0, c1 = n1, n = max(c0, c1);
+          const int c0 = n0, c1 = n1, n = max(c0, c1), e0 = k0, e1 = k1;
 #pragma unroll 1
           for (int j = 0; ok && j < n; ++j) {
             const int sv = st;
@@ -791,14 +803,14 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
                 mma_pv(tmem + Cfg::O_COL + t * HD, tmem + t * 128, sv, j == 0, 0);
                 if (!(ok = wait(&p_full[t], pf[t] & 1))) continue;
                 ++pf[t];
-                mma_pv(tmem + Cfg::O_COL + t * HD, tmem + t * 128, sv, false, 1);
+                if (!one_half(t ? e1 : e0, j)) mma_pv(tmem + Cfg::O_COL + t * HD, tmem + t * 128, sv, false, 1);
               }
               if (j + 1 == nt) umma_commit(&o_full[t]);
               if (t == 1) umma_commit(&kv_empty[sv]);
               if (j + 1 < nt) {
                 if (!have_k && !(ok = wait(&kv_full[st], ph))) continue;
                 have_k = true;
-                mma_s(0, t, st, tmem + t * 128);
+                mma_s(0, t, st, tmem + t * 128, one_half(t ? e1 : e0, j + 1));
                 umma_commit(&s_full[t]);
               }
               if (j + 1 == n) {
@@ -823,7 +835,7 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
         if (!(ok = wait(&q_full[qb], (a.q_bufs == 2 ? qi >> 1 : qi) & 1)) || !(ok = wait(&kv_full[st], ph))) break;
         ++qi;
         {
-          mma_s(qb, 0, st, tmem + (g & 1) * 128);
+          mma_s(qb, 0, st, tmem + (g & 1) * 128, one_half(k0, 0));
           umma_commit(&s_full[g & 1]);
           umma_commit(&kv_empty[st]);
           if (n == 1) umma_commit(&q_empty[qb]);
@@ -835,7 +847,7 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
             advance();
             if (j + 1 < n) {
               if (!(ok = wait(&kv_full[st], ph))) break;
-              mma_s(qb, 0, st, tmem + ((g + 1) & 1) * 128);
+              mma_s(qb, 0, st, tmem + ((g + 1) & 1) * 128, one_half(k0, j + 1));
               umma_commit(&s_full[(g + 1) & 1]);
               umma_commit(&kv_empty[st]);
               if (j + 2 == n) umma_commit(&q_empty[qb]);
@@ -844,7 +856,7 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
             if (!(ok = wait(&kv_full[sv], phv)) || !(ok = wait(&p_half[g & 1], (g >> 1) & 1))) break;
             mma_pv(tmem + Cfg::O_COL, tmem + (g & 1) * 128, sv, j == 0, 0);
             if (!(ok = wait(&p_full[g & 1], (g >> 1) & 1))) break;
-            mma_pv(tmem + Cfg::O_COL, tmem + (g & 1) * 128, sv, false, 1);
+            if (!one_half(k0, j)) mma_pv(tmem + Cfg::O_COL, tmem + (g & 1) * 128, sv, false, 1);
             umma_commit(&o_full[g & 1]);
             umma_commit(&kv_empty[sv]);
           }
@@ -940,10 +952,7 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
           // P): half the code and a third of the registers of holding all 128
           const int left = vis - (it.kb0 + j) * 128;
           const bool cut = __any_sync(0xffffffffu, live && left < 128);
-          // the second 64 keys may be behind every row of the warp (NT 1: 512
-          // prompts of 64 tokens 146 -> 133 us; with NT 2 the loop over fewer
-          // halves slows the others down, 16384 tokens 473 -> 492 us)
-          const int halves = NT == 1 && !__any_sync(0xffffffffu, live && left > 64) ? 1 : 2;
+          const int halves = HALF && tile_sees(it, t, it.kb0 + j) <= 64 ? 1 : 2;
           uint32_t s[2][32];
           auto scores = [&](int h) {
             tmem_ld_32x32b_x32(s_addr + h * 64, s[0]);
@@ -1021,16 +1030,7 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
             if (lane == 0) mbar_arrive(h ? &p_full[buf] : &p_half[buf]);
           }
           l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-          if (halves == 1) {
-            uint32_t z[32];
-#pragma unroll
-            for (int i = 0; i < 32; ++i) z[i] = 0u;
-            tmem_st_32x32b_x32(s_addr + 32, z);
-            tmem_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[buf]);
-          }
+          if (halves == 1 && lane == 0) mbar_arrive(&p_full[buf]);
         } else {
           tc_fence_before();
           if (lane == 0) {
