@@ -220,14 +220,15 @@ int ec_flat_search_noalloc(const float *d_x, int64_t n, int d, const float *d_q,
  * kernels, which read and write nothing out of range.
  *
  * Packed rows: element i of head h of token t lies at p[t * token_stride +
- * h * head_stride + i] (strides in elements).  Sequence s is the tokens
+ * h * head_stride + i] (strides in elements; that of a single token or head
+ * does not count; heads of rows that are written must not overlap).  Sequence s is the tokens
  * [cu[s], cu[s + 1]) (int32, ascending from >= 0, empty sequences allowed);
  * rows behind cu[nseq] are left as they are. */
 
 /* Waits inside the operators' kernels are bounded.  Waits for the current
  * device, then returns EC_ETIMEOUT (and clears the mark) if one of them gave
- * up since the last call, in which case that call's outputs are not valid;
- * else EC_OK. */
+ * up since the last call, in which case that call's outputs are not valid and
+ * the work of ec_attn_cached has to be zeroed again; else EC_OK. */
 int ec_op_status(void);
 
 /* frequency scalings of ec_rope_table */

@@ -93,10 +93,10 @@ int launch_flash(FlashKind kind, const CUtensorMap& q, const CUtensorMap& k, con
   return rc;
 }
 
-// How a call is cut up, from what the host knows
 // packed prompts below this many tokens on average run the kernel that leaves
 // out halves of blocks (measured beside it)
 constexpr int kHalvesBelow = 1024;
+// How a call is cut up, from what the host knows
 struct FlashPlan {
   FlashKind kind;
   int even, rows_tok;  // tokens of a tile
@@ -193,9 +193,12 @@ int run_attention(const AttnOp& op, int num_sms, cudaStream_t st) {
     a.min_chunk = 4;
     a.over = 1;
     a.part_rows = p.part_rows;
-    a.part_o = reinterpret_cast<float*>(w);
-    a.part_l = reinterpret_cast<float*>(w + part_bytes(p.part_rows, hd));
-    a.arrived = reinterpret_cast<int*>(w + part_bytes(p.part_rows, hd) + part_bytes(p.part_rows, 1));
+    // the counts, which have to be zero, lie in the same place for every kind
+    // of call that shares the workspace
+    a.arrived = reinterpret_cast<int*>(w);
+    a.part_o = reinterpret_cast<float*>(w + kMaxCtas * 4);
+    a.part_l = reinterpret_cast<float*>(w + kMaxCtas * 4 + part_bytes(p.part_rows, hd));
+    static_assert(kMaxCtas * 4 % 32 == 0, "parts are written 32 bytes at a time");
     grid = num_sms;
   }
   const int ctas = static_cast<int>(std::min<int64_t>(grid, num_sms));
@@ -208,7 +211,7 @@ int run_attention(const AttnOp& op, int num_sms, cudaStream_t st) {
 
 namespace {
 
-int check_attention(const AttnOp& op, int64_t tokens, int nseq, float scale) {
+int check_attention(AttnOp& op, int64_t tokens, int nseq, float scale) {
   if (op.dtype != EC_BF16 && op.dtype != EC_F16)
     return set_error(EC_EINVAL, "attention takes bf16 or f16, not dtype %d", op.dtype);
   if (tokens < 0 || tokens > (1 << 30) || nseq < 0 || nseq > (1 << 24))
@@ -220,6 +223,9 @@ int check_attention(const AttnOp& op, int64_t tokens, int nseq, float scale) {
   if (!std::isfinite(scale) || scale < 0.f) return set_error(EC_EINVAL, "scale must be finite and >= 0 (0: 1 / sqrt(head_dim))");
   if (int rc = op_check_rows("q", op.q, tokens, op.q_heads, op.head_dim)) return rc;
   if (int rc = op_check_rows("out", op.out, tokens, op.q_heads, op.head_dim)) return rc;
+  if (!op_rows_apart(op.out.token, op.out.head, tokens, op.q_heads, op.head_dim))
+    return set_error(EC_EINVAL, "out's tokens overlap (strides %lld / %lld)", static_cast<long long>(op.out.token),
+                     static_cast<long long>(op.out.head));
   if (!op.cu && tokens && nseq) return set_error(EC_EINVAL, "cu is NULL");
   if (!op_aligned(op.cu, 4) || !op_aligned(op.slots, 4) || !op_aligned(op.lse, 4))
     return set_error(EC_EINVAL, "cu, slots and lse must be 4-byte aligned");

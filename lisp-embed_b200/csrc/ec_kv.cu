@@ -654,14 +654,15 @@ extern "C" int ec_kv_write(int handle, int layer, const void* k, int64_t k_token
   if (!c) return EC_EINVAL;
   if (layer < 0 || layer >= c->layers) return set_error(EC_EINVAL, "layer %d of %d", layer, c->layers);
   if (tokens < 0 || tokens > INT32_MAX || nseq < 0) return set_error(EC_EINVAL, "bad token or sequence count");
-  if (int rc = op_check_rows("k", {k, k_token, k_head}, tokens, c->heads, c->head_dim)) return rc;
-  if (int rc = op_check_rows("v", {v, v_token, v_head}, tokens, c->heads, c->head_dim)) return rc;
+  OpRows kr{k, k_token, k_head}, vr{v, v_token, v_head};
+  if (int rc = op_check_rows("k", kr, tokens, c->heads, c->head_dim)) return rc;
+  if (int rc = op_check_rows("v", vr, tokens, c->heads, c->head_dim)) return rc;
   if (tokens == 0 || nseq == 0) return EC_OK;
   if (!cu || !op_aligned(cu, 4) || !op_aligned(slots, 4)) return set_error(EC_EINVAL, "cu is NULL or a list misaligned");
   OpDevice dev;
   if (int rc = dev.enter({c->refs, k, v, cu, slots})) return rc;
-  const WriteArgs a{static_cast<const uint4*>(k), static_cast<const uint4*>(v), k_token / 8, k_head / 8, v_token / 8,
-                    v_head / 8, tokens, cu, slots, nseq, layer};
+  const WriteArgs a{static_cast<const uint4*>(k), static_cast<const uint4*>(v), kr.token / 8, kr.head / 8, vr.token / 8,
+                    vr.head / 8, tokens, cu, slots, nseq, layer};
   const int64_t grid = (tokens + kWriteTokens - 1) / kWriteTokens;
   return check_cuda(launch_pdl(kv_write_kernel, dim3(static_cast<unsigned>(grid)), dim3(kWriteTokens * 32), 0,
                                static_cast<cudaStream_t>(stream), *c, a),

@@ -48,7 +48,17 @@ OpDevice::~OpDevice() {
   if (prev_ >= 0) cudaSetDevice(prev_);
 }
 
-int op_check_rows(const char* name, const OpRows& r, int64_t tokens, int heads, int head_dim) {
+bool op_rows_apart(int64_t token, int64_t head, int64_t tokens, int heads, int head_dim) {
+  if (tokens <= 1 || heads <= 1) return true;
+  // one of the two strides steps over everything of the other (in double: the
+  // products pass 64 bits where they are far apart)
+  return static_cast<double>(token) >= static_cast<double>(heads - 1) * head + head_dim ||
+         static_cast<double>(head) >= static_cast<double>(tokens - 1) * token + head_dim;
+}
+
+int op_check_rows(const char* name, OpRows& r, int64_t tokens, int heads, int head_dim) {
+  if (heads == 1) r.head = 0;
+  if (tokens <= 1) r.token = 0;
   if (!r.p && tokens > 0) return set_error(EC_EINVAL, "%s is NULL", name);
   if (!op_aligned(r.p, 16)) return set_error(EC_EINVAL, "%s must be 16-byte aligned", name);
   if (r.token % 8 || r.head % 8)

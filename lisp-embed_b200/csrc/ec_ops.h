@@ -45,8 +45,11 @@ struct OpRows {
   int64_t token, head;
 };
 // checks pointer, 16-byte base and strides (in elements of 2 bytes), and that
-// heads do not overlap
-int op_check_rows(const char* name, const OpRows& r, int64_t tokens, int heads, int head_dim);
+// heads do not overlap; the stride of a single token or head, which is never
+// used, becomes 0
+int op_check_rows(const char* name, OpRows& r, int64_t tokens, int heads, int head_dim);
+// rows that are written: no two heads of any tokens may overlap either
+bool op_rows_apart(int64_t token, int64_t head, int64_t tokens, int heads, int head_dim);
 
 // a cache as ec_kv_open describes it; the memory is the caller's
 struct KvCache {

@@ -268,9 +268,15 @@ extern "C" int ec_rope(const void* x, int64_t x_token, int64_t x_head, void* y, 
   if (!x || !y || !pos || !cos_t || !sin_t) return set_error(EC_EINVAL, "a rope buffer is NULL");
   if (!op_aligned(x, es) || !op_aligned(y, es) || !op_aligned(pos, 4) || !op_aligned(cos_t, 4) || !op_aligned(sin_t, 4))
     return set_error(EC_EINVAL, "a rope buffer is not aligned to its element");
+  // the stride of a single token or head is never used
+  if (heads == 1) x_head = y_head = 0;
+  if (tokens == 1) x_token = y_token = 0;
   if ((heads > 1 && (x_head < head_dim || y_head < head_dim)) ||
       (tokens > 1 && (x_token < head_dim || y_token < head_dim)) || x_head < 0 || y_head < 0 || x_token < 0 || y_token < 0)
     return set_error(EC_EINVAL, "rope strides overlap heads of %d", head_dim);
+  if (!op_rows_apart(y_token, y_head, tokens, heads, head_dim))
+    return set_error(EC_EINVAL, "y's tokens overlap (strides %lld / %lld)", static_cast<long long>(y_token),
+                     static_cast<long long>(y_head));
   const bool in_place = x == y;
   if (in_place && (x_token != y_token || x_head != y_head))
     return set_error(EC_EINVAL, "in place the strides of x and y must be equal");

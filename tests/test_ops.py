@@ -191,3 +191,14 @@ def test_python_layer_refusals():
     cache.close()
     with pytest.raises(_lib.EcError, match="unknown cache handle"):
         cache.compact(two, stream=0)
+
+
+def test_rows_that_are_written_must_not_overlap():
+    """A token stride that does not step over a token's heads (nor a head
+    stride over the head's tokens) would have two rows in one place."""
+    refused(rope(yt=128, yh=64), "overlap")
+    refused(prompt(qt=256, qh=64), "overlap")
+    refused(prompt(qt=64, qh=256), "overlap")
+    # the stride of a single token or head does not count: not refused for it
+    assert rope(tokens=0, heads=1, xh=3, yh=5) == 0
+    assert prompt(tokens=0, qt=3, kt=5) == 0
