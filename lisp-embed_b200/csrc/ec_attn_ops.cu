@@ -102,6 +102,14 @@ struct FlashPlan {
   int even, rows_tok;  // tokens of a tile
   int part_rows;
 };
+// Few rows (a sequence's new tokens and their heads in at most 32 rows): the
+// kernels with the operands turned round, in the smallest size that holds them;
+// always an even split (64 sequences of up to 8192 tokens: 118 us with tiles of
+// 128 rows, 106 with keys per lane, 96 in the size that fits).  More rows in
+// fewer tiles than SMs: an even split, which leaves whole what is not worth
+// cutting.  Else whole tiles, in pairs where every SM has a pair (one prompt of
+// 16384 tokens 473 us, single tiles 573); one tile at a time is better for
+// fewer, and where no sequence fills more than a tile.
 FlashPlan flash_plan(const KvCache* c, int64_t tokens, int q_heads, int kv_heads, int nseq, int max_new, int num_sms) {
   const int group = q_heads / kv_heads;
   FlashPlan p{kTiles, 0, 128 / group, 128};
@@ -116,7 +124,7 @@ FlashPlan flash_plan(const KvCache* c, int64_t tokens, int q_heads, int kv_heads
       p.part_rows = few <= 4 ? 4 : few <= 8 ? 8 : few <= 16 ? 16 : 32;
       p.rows_tok = p.part_rows / group;
       p.even = 1;
-    } else if (fits && tiles < 2 * num_sms) {
+    } else if (fits && tiles <= num_sms) {
       p.even = 1;
     }
   }

@@ -258,12 +258,14 @@ __device__ __noinline__ bool flash_slots(const FlashArgs& a, int lane, Publish p
 // Even split: every CTA takes the same share of the key blocks, in the order
 // (sequence, tile, key head, block).  A tile costs its blocks and `over` units
 // more, for its start and end, which come first.  Where there are fewer tiles
-// than CTAs and all are short, every tile has a CTA of its own instead.
+// than CTAs and the longest would not gain what a join costs (8 units, 20 with
+// 128 rows: 25 us), every tile has a CTA of its own instead: 4 texts of 200
+// tokens behind 4000 61 us, cut 84; 4 of 40 behind 2000 35 and 45; one of 40
+// behind 20000 203 and 94; 8 of 64 behind 8000 98 and 96.
 //
 // Each thread of the CTA first looks at some sequences (the loads are far
 // away, and the CTA has nothing else to do yet): units[s], and tiles | longest
 // tile << 16, with the sign bit where a tile sees no key.
-constexpr int kTileAlone = 8;  // units of a tile that is not worth cutting
 __device__ __forceinline__ void flash_measure(const FlashArgs& a, int* units, int* about) {
   for (int s = threadIdx.x; s < a.nseq; s += blockDim.x) {
     const FlashSeq q = flash_seq(a, s);
@@ -284,14 +286,17 @@ __device__ __forceinline__ void flash_measure(const FlashArgs& a, int* units, in
 template <typename Publish>
 __device__ __noinline__ bool flash_even(const FlashArgs& a, int lane, int* prefix, const int* about, Publish publish) {
   const int R = a.rows_tok, ctas = gridDim.x, me = blockIdx.x;
-  int tiles = 0, most = 0;
+  int tiles = 0, most = 0, work = 0;
   for (int s = lane; s < a.nseq; s += 32) {
+    work += prefix[s];
     tiles += about[s] & 0xffff;
     most = max(most, about[s] >> 16 & 0x7fff);
   }
   tiles = __reduce_add_sync(0xffffffffu, min(tiles, 1 << 20));
   most = __reduce_max_sync(0xffffffffu, most);
-  const bool alone = tiles <= ctas && most <= kTileAlone;  // every tile padded to the longest
+  work = __reduce_add_sync(0xffffffffu, work);
+  // every tile, padded to the longest, its own CTA
+  const bool alone = tiles <= ctas && most <= work / ctas + 8 + a.part_rows / 10;
   int total = 0;
 #pragma unroll 1
   for (int s0 = 0; s0 < a.nseq; s0 += 32) {
@@ -383,37 +388,69 @@ __device__ __noinline__ bool flash_even(const FlashArgs& a, int lane, int* prefi
   return ok;
 }
 
-// The CTA that finishes a cut tile's last part joins the parts: one warp per
-// row, in the order of the keys.
+// The CTA that finishes a cut tile's last part joins the parts, in the order of
+// the keys.  A warp has a quarter of the rows: their weights first, a row to a
+// lane, then the rows themselves, eight at a time, so that many loads are under
+// way (a row after the other, each waiting for its loads: 4 texts of 200 tokens
+// behind 4000, two parts to a tile, 121 us instead of 84).
 template <int HD, typename T>
 __device__ __noinline__ void flash_join(const FlashArgs& a, int tok0, int qv, int kvh, int c0, int parts, int warp,
                                         int lane) {
-  const int rows = qv * a.group;
+  const int rows = qv * a.group, each = (rows + 3) / 4, base = warp * each, mine = min(each, rows - base);
+  if (mine <= 0) return;
+  const int row = base + min(lane, mine - 1);
   auto part = [&](int i) { return static_cast<int64_t>(2 * (c0 + i) + (i == 0)) * a.part_rows; };
-#pragma unroll 1
-  for (int row = warp; row < rows; row += 4) {
-    float m = -INFINITY;
-    for (int i = lane; i < parts; i += 32) m = fmaxf(m, __ldcg(&a.part_l[part(i) + row]));
-#pragma unroll
-    for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-    float sum = 0.f, o[HD / 32] = {};
+  float m = -INFINITY, sum = 0.f;
 #pragma unroll 4
-    for (int i = 0; i < parts; ++i) {
-      const float l2 = __ldcg(&a.part_l[part(i) + row]);
-      const float x = l2 == -INFINITY ? 0.f : fa_exp2(l2 - m);
-      sum += x;
-#pragma unroll
-      for (int e = 0; e < HD / 32; ++e) o[e] += x * __ldcg(&a.part_o[(part(i) + row) * HD + lane + 32 * e]);
-    }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const int64_t tok = tok0 + row / a.group;
-    const int h = kvh * a.group + row % a.group;
-    uint16_t* out = static_cast<uint16_t*>(a.out) + tok * a.ot + h * a.oh;
+  for (int i = 0; i < parts; ++i) m = fmaxf(m, __ldcg(&a.part_l[part(i) + row]));
+  auto weight = [&](int i) {
+    const float l2 = __ldcg(&a.part_l[part(i) + row]);
+    return l2 == -INFINITY ? 0.f : fa_exp2(l2 - m);
+  };
+#pragma unroll 4
+  for (int i = 0; i < parts; ++i) sum += weight(i);
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  if (lane < mine && a.lse)
+    a.lse[static_cast<int64_t>(tok0 + row / a.group) * a.q_heads + kvh * a.group + row % a.group] =
+        sum == 0.f ? -INFINITY : (m + log2f(sum)) * 0.693147180559945309f;
+  auto store = [&](int at, const float* o) {
+    uint16_t* out = static_cast<uint16_t*>(a.out) + static_cast<int64_t>(tok0 + at / a.group) * a.ot +
+                    (kvh * a.group + at % a.group) * a.oh;
 #pragma unroll
     for (int e = 0; e < HD / 32; ++e)
-      if (lane + 32 * e < a.head_dim) out[lane + 32 * e] = static_cast<uint16_t>(pack2<T>(o[e] * inv, 0.f));
-    if (lane == 0 && a.lse)
-      a.lse[tok * a.q_heads + h] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * 0.693147180559945309f;
+      if (lane + 32 * e < a.head_dim) out[lane + 32 * e] = static_cast<uint16_t>(pack2<T>(o[e], 0.f));
+  };
+  if (mine < 8) {  // the parts under way together instead
+#pragma unroll 1
+    for (int r = 0; r < mine; ++r) {
+      float o[HD / 32] = {};
+#pragma unroll 4
+      for (int i = 0; i < parts; ++i) {
+        const float x = __shfl_sync(0xffffffffu, weight(i) * inv, r);
+#pragma unroll
+        for (int e = 0; e < HD / 32; ++e) o[e] += x * __ldcg(&a.part_o[(part(i) + base + r) * HD + lane + 32 * e]);
+      }
+      store(base + r, o);
+    }
+    return;
+  }
+#pragma unroll 1
+  for (int r0 = 0; r0 < mine; r0 += 8) {
+    float o[8][HD / 32] = {};
+#pragma unroll 1
+    for (int i = 0; i < parts; ++i) {
+      const float w = weight(i) * inv;
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        const int at = min(r0 + r, mine - 1);
+        const float x = __shfl_sync(0xffffffffu, w, at);
+#pragma unroll
+        for (int e = 0; e < HD / 32; ++e) o[r][e] += x * __ldcg(&a.part_o[(part(i) + base + at) * HD + lane + 32 * e]);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+      if (r0 + r < mine) store(base + r0 + r, o[r]);
   }
 }
 
