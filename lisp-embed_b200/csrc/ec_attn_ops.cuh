@@ -101,6 +101,10 @@ constexpr int kFlashRing = 3;
 // keys) only reaches rows of S and O that belong to no query.
 constexpr uint32_t kQBuf = 64 * 128;
 
+// a list of whole tiles counts its sets in this many groups of sequences, up
+// to kFlashCounted sequences
+constexpr int kFlashGroups = 128, kFlashCounted = 4096;
+
 template <int HD, int NT>
 struct FlashCfg {
   static constexpr int AT = HD / 64;                 // 64-column atoms
@@ -112,7 +116,7 @@ struct FlashCfg {
   // list, none, and four that write the results.
   static constexpr int WARPS = NT == 2 ? 16 : 7;
   static constexpr int THREADS = 32 * WARPS;
-  static constexpr uint32_t TAIL = 1536 + (NT == 1 ? 8 * MAX_SEQS : 1024);
+  static constexpr uint32_t TAIL = 1536 + (NT == 1 ? 8 * MAX_SEQS : 1024 + 4 * kFlashGroups);
   static constexpr size_t SMEM = NT * TILE + STAGES * TILE + TAIL;
   static constexpr uint32_t O_COL = 256;
   static_assert(SMEM <= 232448, "shared memory");
@@ -187,37 +191,64 @@ __device__ __forceinline__ FlashSeq flash_seq(const FlashArgs& a, int s) {
 }
 
 // ------------------------------------------------------------- work lists --
-// Without a split: slot u of the list is the tile set f(s) + i of sequence s,
-// f(s) = cu[s] / BT + s for BT tokens per set.  f leaves at least
-// ceil(len / BT) slots to every sequence and needs no prefix sum; a slot's
-// sequence is found by bisection, 32 slots at a time.  Their number (times the
-// key heads) fits 31 bits, checked on the host.  The key heads of a set and the
-// sets of a sequence follow each other, so that the CTAs read the same keys at
-// about the same time: with a run of the list for every CTA, of equal work, 256
-// prompts of 320 tokens took 383 us instead of 272.
+// Without a split: the tile sets of all sequences, the last one first, and of
+// each the key heads.  flash_count leaves the number of sets of every group of
+// sequences; a set's group is found by bisection, its sequence from there, 32
+// sets at a time.  The key heads of a set and the sets of a sequence follow
+// each other, so that the CTAs read the same keys at about the same time: with
+// a run of the list for every CTA, of equal work, 256 prompts of 320 tokens took
+// 383 us instead of 272.  With more sequences than are counted, slot u is set i
+// of sequence s for f(s) + i = u, f(s) = cu[s] / BT + s (BT tokens per set): f
+// leaves at least ceil(len / BT) slots to every sequence and needs no sums, but
+// its empty slots make the turns uneven (96 texts behind 650 cached tokens
+// 160 us instead of 141, 64 prompts of 300 147 instead of 127).  Slots times
+// key heads fit 31 bits, checked on the host.
 //
 // Up to 32 sequences go by set, the latest sets of all of them first (slot u:
 // set u / nseq of sequence u % nseq), so that a CTA's few turns cost the same:
 // 4 prompts of 2048 tokens 84 us instead of 135.  With more sequences that
-// costs the keys' reuse: 96 texts behind 650 cached tokens 182 us instead of
-// 160 (64 prompts of 300 tokens 139 instead of 153).
+// costs the keys' reuse: 96 texts behind 650 cached tokens took 182 us.
+template <int NT>
+__device__ __forceinline__ void flash_count(const FlashArgs& a, int* groups) {
+  const int size = (a.nseq + kFlashGroups - 1) / kFlashGroups, BT = NT * a.rows_tok;
+  for (int s = threadIdx.x; s < a.nseq; s += blockDim.x) {
+    const int begin = min(max(a.cu[s], 0), a.tokens), end = min(max(a.cu[s + 1], begin), a.tokens);
+    if (end > begin) atomicAdd(&groups[s / size], (end - begin + BT - 1) / BT);
+  }
+}
 template <int NT, typename Publish>
-__device__ __noinline__ bool flash_slots(const FlashArgs& a, int lane, Publish publish) {
+__device__ __noinline__ bool flash_slots(const FlashArgs& a, int lane, int* groups, Publish publish) {
   const int R = a.rows_tok, BT = NT * R;
   uint32_t slots = a.tokens / BT + a.nseq;
   const uint32_t step = gridDim.x;
-  const bool few = a.nseq <= 32;
+  bool few = a.nseq <= 32;
   if (few) {
     const FlashSeq q = flash_seq(a, min(lane, a.nseq - 1));
-    slots = __reduce_max_sync(0xffffffffu, (q.end - q.begin + BT - 1) / BT) * a.nseq;
+    const uint32_t most = __reduce_max_sync(0xffffffffu, (q.end - q.begin + BT - 1) / BT);
+    few = static_cast<uint64_t>(most) * a.nseq * a.kv_heads < (1u << 30);
+    if (few) slots = most * a.nseq;
+  }
+  const bool counted = a.nseq > 32 && a.nseq <= kFlashCounted;
+  const int size = (a.nseq + kFlashGroups - 1) / kFlashGroups;
+  if (counted) {
+    int total = 0;
+#pragma unroll 1
+    for (int g = lane; g < kFlashGroups; g += 32) {  // sets before each group
+      const int v = groups[g];
+      int x = v;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, d);
+        if (lane >= d) x += y;
+      }
+      groups[g] = total + x - v;
+      total += __shfl_sync(0xffffffffu, x, 31);
+    }
+    __syncwarp();
+    slots = total;
   }
   const uint32_t all = slots * a.kv_heads;
   bool ok = true;
-  // the offsets are far away: their lines all at once, not one after the other
-  // in the bisections
-#pragma unroll 1
-  for (int s = lane * 32; s < min(a.nseq + 1, 8192); s += 1024) asm volatile("" ::"r"(a.cu[s]));
-  __syncwarp();
 #pragma unroll 1
   for (uint32_t t0 = 0; ok && t0 < all; t0 += 32 * step) {
     // late (long) tile sets first; the order turns round every pass, so that
@@ -226,15 +257,28 @@ __device__ __noinline__ bool flash_slots(const FlashArgs& a, int lane, Publish p
     FlashEntry it{};
     if (t < all) {
       const int u = static_cast<int>(slots - 1 - t / a.kv_heads);
-      int lo = few ? u % a.nseq : 0, hi = few ? 0 : a.nseq;  // last sequence with f <= u
-      while (hi - lo > 1) {
+      int lo = few ? u % a.nseq : 0, i = few ? u / a.nseq : 0;  // sequence, set
+      int hi = few ? 0 : counted ? kFlashGroups : a.nseq;
+      while (hi - lo > 1) {  // last group that begins by u, or sequence with f <= u
         const int mid = (lo + hi) >> 1;
-        if (min(max(a.cu[mid], 0), a.tokens) / BT + mid <= u) lo = mid;
+        if ((counted ? groups[mid] : min(max(a.cu[mid], 0), a.tokens) / BT + mid) <= u) lo = mid;
         else hi = mid;
+      }
+      if (counted) {
+        i = u - groups[lo];
+        lo *= size;
+        int begin = min(max(a.cu[lo], 0), a.tokens);
+        while (lo + 1 < a.nseq) {
+          const int end = min(max(a.cu[lo + 1], begin), a.tokens), sets = (end - begin + BT - 1) / BT;
+          if (i < sets) break;
+          i -= sets;
+          ++lo;
+          begin = min(max(a.cu[lo], 0), a.tokens);
+        }
       }
       const FlashSeq q = flash_seq(a, lo);
       const int len = q.end - q.begin;
-      const int i = few ? u / a.nseq : u - (q.begin / BT + lo);  // tile set of the sequence
+      if (!few && !counted) i = u - (q.begin / BT + lo);
       if (i >= 0 && i < (len + BT - 1) / BT) {
         const int q0 = i * BT;
         it.valid = 1;
@@ -504,6 +548,7 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
   volatile int* last_part = abort_flag + 1;
   int* prefix = reinterpret_cast<int*>(tail + 1536);  // [MAX_SEQS] of an even split
   float* inverse = reinterpret_cast<float*>(tail + 1536);  // [2][128] 1 / l (NT 2)
+  int* groups = reinterpret_cast<int*>(tail + 1536 + (NT == 1 ? 0 : 1024));  // [kFlashGroups] of a list
   static_assert(8 * (4 + 2 * ST + 14 + 2 * kFlashRing) + kFlashRing * sizeof(FlashItem) + 12 <= 1536, "tail");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -539,8 +584,14 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
+  const bool count = !a.even && a.nseq > 32 && a.nseq <= kFlashCounted;
+  if (count) {
+    for (int i = threadIdx.x; i < kFlashGroups; i += blockDim.x) groups[i] = 0;
+    __syncthreads();
+  }
   pdl_wait();  // what comes before may still be running up to here
   pdl_trigger();
+  if (count) flash_count<NT>(a, groups);
   if (NT == 1 && a.even) flash_measure(a, prefix, prefix + Cfg::MAX_SEQS);
   tc_fence_before();
   __syncthreads();
@@ -651,7 +702,7 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
     if (NT == 1 && a.even) {
       ok = flash_even(a, lane, prefix, prefix + Cfg::MAX_SEQS, [&](const Entry& e) { return publish(e, 0); });
     } else {
-      ok = flash_slots<NT>(a, lane, publish);
+      ok = flash_slots<NT>(a, lane, groups, publish);
     }
     Entry end{};
     if (ok) ok = publish(end, 0);
@@ -1153,7 +1204,11 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
 // row maxima through shared memory.  One warp runs per scheduler, so a block
 // takes as long as its instructions do, one after the other: NP = 4, 8, 16 and
 // 32 rows each have their own kernel (the MMA's N is 16 at least; what the
-// columns behind NP hold reaches nothing).
+// columns behind NP hold reaches nothing).  Three contexts of 100000 to 131000
+// tokens take 230 us, at 98% of the copy rate; 64 sequences of up to 8192
+// tokens, grouped by four, 76 us at 77% (118 with tiles of 128 rows): there the
+// starts and joins of about two tiles a CTA count; one token of one sequence 12
+// us, most of them between launch and first key.
 template <int HD, int NP>
 struct TokenCfg {
   static constexpr int NR = NP < 16 ? 16 : NP;         // columns of the MMAs

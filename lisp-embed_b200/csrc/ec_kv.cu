@@ -12,6 +12,13 @@
 // does not depend on timing); what moves many bytes runs on a grid that reads
 // the plan.  A request either happens as a whole or changes nothing: status[0]
 // says which, and every index read from the device is checked before use.
+//
+// What bounds them: the plans are chains of loads that wait for one another
+// (lengths, counts, lists, tables: about 1 us each out of L2), 5 to 8 us a
+// plan, so a plan reads ahead what it will need and gives a request to a warp;
+// fork, reserve and write for 96 texts (8 layers copied) take 40 us together,
+// 12 of them for the bytes.  The copies run near the memory's rate: 4096 pages
+// compacted in 51 us, 36 for the bytes.
 #include <algorithm>
 #include <map>
 #include <mutex>

@@ -359,9 +359,12 @@ static int load_llama(Device& d, const JVal& cfg) {
       return rc;
     const Tensor* qn = find_t(d, pf + "self_attn.q_norm.weight");  // get-tensor-opt
     const Tensor* kn = find_t(d, pf + "self_attn.k_norm.weight");
-    // uploads stay: one of an earlier model is not this layer's
-    if (qn && qn->model < qw->model) qn = nullptr;
-    if (kn && kn->model < kw->model) kn = nullptr;
+    // uploads stay: a norm that was there before all the rest of the layer was
+    // uploaded again is an earlier model's
+    int since = in->model;
+    for (const Tensor* t : {post, qw, kw, vw, ow, gw, uw, dw}) since = std::min(since, t->model);
+    if (qn && qn->model < since) qn = nullptr;
+    if (kn && kn->model < since) kn = nullptr;
     if (m.hd != 128 && (qn || kn))
       return set_error(EC_EUNSUPPORTED, "q/k norm with head_dim %d (supported: 128)", m.hd);
     if ((rc = as_f32(d, in, &L.in_ln)) || (rc = as_f32(d, post, &L.post_ln)) ||

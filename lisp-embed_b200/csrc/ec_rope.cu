@@ -48,8 +48,9 @@ __device__ double rope_freq(const TableArgs& a, int i) {
 // Thread (i, r): pair i of `run` consecutive positions.  The first angle and the
 // step of one position are turned into cos and sin once; the rest follows by
 // rotating in double, which drifts by a few 2^-53 a step (run <= 64: far below
-// the fp32 result).  Computing every angle's cos and sin took 150 us for
-// 262144 x 32; this is bounded by the stores.
+// the fp32 result).  Computing every angle's cos and sin took 150 us more for
+// 262144 x 32; now the table and the turn of 9001 tokens take 41 us, 23 of them
+// for what has to be written.
 __global__ void rope_table_kernel(const TableArgs a, int run) {
   pdl_wait();
   pdl_trigger();
@@ -105,7 +106,9 @@ struct alignas(sizeof(T) * V) Vec {
 // One thread: V pairs (or V elements of the tail) of a token's heads h0 ..
 // h0 + heads_per - 1.  The angle's cos and sin are read once for them, and the
 // elements of up to four heads are under way together.  I: index type that
-// holds the number of threads.
+// holds the number of threads (64-bit divisions slow the others down).  Bounded
+// by reading and writing the rows: 65536 tokens of 24 heads of 128 in 138 us,
+// 93% of the copy rate.
 template <typename T, int V, bool INTER, typename I>
 __global__ void rope_kernel(const RopeArgs a, int per_head, int groups, int heads_per) {
   using VT = Vec<T, V>;

@@ -126,3 +126,27 @@ def test_strides_of_single_tokens_and_heads(ops):
     c.h.write(0, k[:1].as_strided((1, 1, 64), (3, 1, 1)), v[:1].as_strided((1, 1, 64), (0, 5, 1)), i32([0, 1]))
     got_k, got_v = c.rows(0)
     assert torch.equal(got_k, k[:1]) and torch.equal(got_v, v[:1])
+
+
+@pytest.mark.parametrize("n", [33, 129, 2500, 4096, 4097, 9000])
+def test_lists_of_many_sequences(ops, n):
+    """Counted in groups up to 4096 sequences, found by their offsets above;
+    runs of empty ones, and a first and last one that is empty."""
+    r = random.Random(n)
+    lens = [0 if i % 7 < 3 or i in (0, n - 1) else r.choice([1, 5, 40]) for i in range(n)]
+    lens[n // 2], lens[n // 3] = 700, 300
+    hq, hk, hd = 6, 3, 64
+    cu = offsets(lens)
+    t = cu[-1]
+    q, k, v = rnd(t, hq, hd, dt=BF16, seed=1), rnd(t, hk, hd, dt=BF16, seed=2), rnd(t, hk, hd, dt=BF16, seed=3)
+    out, intact = guarded(t, hq, hd, dt=BF16)
+    ops.attn_prompt(q, k, v, i32(cu), out)
+    intact()
+    # all rows were written; some sequences against the reference
+    assert not bool((out == 7).all(-1).any())
+    some = [n // 2, n // 3] + [i for i in range(n) if lens[i]][:: max(1, n // 40)]
+    for i in some:
+        a, b = cu[i], cu[i + 1]
+        see = torch.ones(b - a, b - a, dtype=torch.bool, device="cuda").tril()
+        o, _, tol, _ = attention_reference(q[a:b], k[a:b], v[a:b], see, 1 / 8)
+        close(out[a:b], o, tol)

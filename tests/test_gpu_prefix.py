@@ -177,3 +177,32 @@ def test_head_dim_refusals(synth_root, ec):
         with pytest.raises(RuntimeError) as e:
             model.load_model(d)
         assert "head_dim" in str(e.value)
+
+
+def test_norms_of_an_earlier_model(synth_root, ec):
+    """A Llama model without q/k norms after one with them does not take
+    theirs; weights of a layer uploaded again keep the layer's norms."""
+    import dataclasses
+    qwen = synth.with_layers(dataclasses.replace(synth.QWEN3_06B, name="qwen-norms"), 1, vocab=2048)
+    plain = dataclasses.replace(qwen, name="llama-no-norms", model_type="llama")
+    ids, offs = _batch(np.random.default_rng(4), qwen, [5, 70])
+    d = _load(synth_root, plain)
+    first = model.embed_batch(ids, offs)
+    assert _cos(first, _oracle(d, ids, offs)).min() >= COS
+    dq = _load(synth_root, qwen)
+    normed = model.embed_batch(ids, offs)
+    assert _cos(normed, _oracle(dq, ids, offs)).min() >= COS
+    # one weight again, and the model put together anew: the same model
+    w = synth.make_weights(qwen, 3)["layers.0.self_attn.q_proj.weight"]
+    dims = np.array(w[1], np.int64)
+    import ctypes as C
+    raw = np.ascontiguousarray(w[2])
+    _lib.check(_lib.lib().ec_upload_tensor(b"layers.0.self_attn.q_proj.weight", _lib.EC_BF16,
+                                           dims.ctypes.data_as(C.POINTER(C.c_int64)), 2, raw.ctypes.data, raw.nbytes))
+    with open(os.path.join(dq, "config.json")) as f:
+        cfg = f.read()
+    fam, dim = C.c_int(0), C.c_int(0)
+    _lib.check(_lib.lib().ec_load_model(cfg.encode(), None, C.byref(fam), C.byref(dim)))
+    assert np.array_equal(model.embed_batch(ids, offs), normed)
+    _load(synth_root, plain)
+    assert np.array_equal(model.embed_batch(ids, offs), first)
