@@ -40,6 +40,26 @@ bool encode_rows(CUtensorMap* tm, int dtype, const OpRows& r, int head_dim, int 
 
 using FlashFn = void (*)(CUtensorMap, CUtensorMap, CUtensorMap, FlashArgs);
 
+// Lists of pairs of tiles by sequence are launched plainly.  A CTA that starts
+// early, while the kernel before still runs, gets the SM that came free first;
+// then CTAs that read the same keys no longer run side by side.  One call after
+// the other, 256 prompts of 320 tokens took 306 us instead of 252, 1024 of 130
+// 610 instead of 550, 96 texts behind 650 cached tokens 141 instead of 134.
+// The other launches gain by it (one token 14.4 -> 11.7 us, 8 prompts of 512
+// 27.1 -> 25.5, one of 4096 75.6 -> 73.0).
+class PlainLaunch {
+ public:
+  explicit PlainLaunch(bool plain) : before_(pdl_enabled()), plain_(plain) {
+    if (plain_) pdl_set_thread(false);
+  }
+  ~PlainLaunch() {
+    if (plain_) pdl_set_thread(before_);
+  }
+
+ private:
+  bool before_, plain_;
+};
+
 // kernel `id` (its shared memory is set once per device)
 int launch_one(int id, FlashFn fn, int threads, size_t smem, const CUtensorMap& q, const CUtensorMap& k,
                const CUtensorMap& v, const FlashArgs& a, int grid, cudaStream_t st) {
@@ -210,6 +230,7 @@ int run_attention(const AttnOp& op, int num_sms, cudaStream_t st) {
     grid = num_sms;
   }
   const int ctas = static_cast<int>(std::min<int64_t>(grid, num_sms));
+  const PlainLaunch launch((p.kind == kPairs || p.kind == kHalves) && op.nseq > kFlashFew);
   if (op.dtype == EC_BF16)
     return hd == 64 ? launch_flash<64, __nv_bfloat16>(p.kind, tq, tk, tv, a, ctas, st)
                     : launch_flash<128, __nv_bfloat16>(p.kind, tq, tk, tv, a, ctas, st);

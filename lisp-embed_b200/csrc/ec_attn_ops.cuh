@@ -104,6 +104,8 @@ constexpr uint32_t kQBuf = 64 * 128;
 // a list of whole tiles counts its sets in this many groups of sequences, up
 // to kFlashCounted sequences
 constexpr int kFlashGroups = 128, kFlashCounted = 4096;
+// up to this many sequences go by set (one to a lane)
+constexpr int kFlashFew = 32;
 
 template <int HD, int NT>
 struct FlashCfg {
@@ -221,14 +223,14 @@ __device__ __noinline__ bool flash_slots(const FlashArgs& a, int lane, int* grou
   const int R = a.rows_tok, BT = NT * R;
   uint32_t slots = a.tokens / BT + a.nseq;
   const uint32_t step = gridDim.x;
-  bool few = a.nseq <= 32;
+  bool few = a.nseq <= kFlashFew;
   if (few) {
     const FlashSeq q = flash_seq(a, min(lane, a.nseq - 1));
     const uint32_t most = __reduce_max_sync(0xffffffffu, (q.end - q.begin + BT - 1) / BT);
     few = static_cast<uint64_t>(most) * a.nseq * a.kv_heads < (1u << 30);
     if (few) slots = most * a.nseq;
   }
-  const bool counted = a.nseq > 32 && a.nseq <= kFlashCounted;
+  const bool counted = a.nseq > kFlashFew && a.nseq <= kFlashCounted;
   const int size = (a.nseq + kFlashGroups - 1) / kFlashGroups;
   if (counted) {
     int total = 0;
@@ -584,7 +586,7 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
-  const bool count = !a.even && a.nseq > 32 && a.nseq <= kFlashCounted;
+  const bool count = !a.even && a.nseq > kFlashFew && a.nseq <= kFlashCounted;
   if (count) {
     for (int i = threadIdx.x; i < kFlashGroups; i += blockDim.x) groups[i] = 0;
     __syncthreads();
