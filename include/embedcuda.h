@@ -318,8 +318,8 @@ int ec_kv_free(int handle, const int32_t *slots, int n, int32_t *status, void *s
 int ec_kv_compact(int handle, int32_t *status, void *stream);
 
 /* Write the packed rows k and v into one layer: sequence s is the last
- * cu[s + 1] - cu[s] tokens of slots[s] (NULL: slot s), whose room has been
- * reserved.  A token whose page is not in the table is left out. */
+ * cu[s + 1] - cu[s] tokens of slots[s] (NULL: slot s; distinct slots), whose
+ * room has been reserved.  A token whose page is not in the table is left out. */
 int ec_kv_write(int handle, int layer, const void *k, int64_t k_token, int64_t k_head,
                 const void *v, int64_t v_token, int64_t v_head, int64_t tokens,
                 const int32_t *cu, const int32_t *slots, int nseq, void *stream);
