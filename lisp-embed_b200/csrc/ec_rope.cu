@@ -98,8 +98,10 @@ __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return
 template <>
 __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
 
+// V elements, moved in pieces of 16 bytes at most: eight entries of a table are
+// two of them, and a table need not be aligned to more
 template <typename T, int V>
-struct alignas(sizeof(T) * V) Vec {
+struct alignas(sizeof(T) * V < 16 ? sizeof(T) * V : 16) Vec {
   T e[V];
 };
 
@@ -207,11 +209,12 @@ cudaError_t launch_rope_v(const RopeArgs& a, int interleaved, int num_sms, cudaS
   // widest vector (16 bytes at most) that divides the turned half, the tail
   // and every stride, and to which the buffers are aligned
   auto fits = [&](int v) {
-    const size_t b = sizeof(T) * v;
+    const size_t b = sizeof(T) * v, tb = v > 4 ? 16 : 4 * v;
     return a.half % v == 0 && a.tail % v == 0 && a.xt % v == 0 && a.xh % v == 0 && a.yt % v == 0 && a.yh % v == 0 &&
-           op_aligned(a.x, b) && op_aligned(a.y, b) && op_aligned(a.cos_t, v > 4 ? 16 : 4 * v) &&
-           op_aligned(a.sin_t, v > 4 ? 16 : 4 * v);
+           op_aligned(a.x, b) && op_aligned(a.y, b) && op_aligned(a.cos_t, tb) && op_aligned(a.sin_t, tb);
   };
+  static_assert(alignof(Vec<float, 8>) == 16 && alignof(Vec<float, 4>) == 16 && alignof(Vec<float, 2>) == 8,
+                "tables are read through this type");
   if constexpr (sizeof(T) == 2) {
     if (fits(8)) return launch_rope<T, 8>(a, interleaved, num_sms, st);
   }

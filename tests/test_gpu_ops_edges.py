@@ -1,0 +1,29 @@
+"""Calls at the edges of what the operators on device buffers accept.
+References and tolerances are those of test_gpu_ops.py."""
+import pytest
+import torch
+
+from test_gpu_ops import (BF16, F16, F32, guarded, half_step, i32, no_wait_gave_up, ops, rnd,  # noqa: F401
+                          rope_reference)
+
+pytestmark = pytest.mark.gpu
+
+
+# -------------------------------------------------------- rotary positions --
+@pytest.mark.parametrize("dt", [BF16, F16, F32])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("shift", [1, 2, 4, 8, 12])
+def test_rope_tables_at_any_float(ops, dt, interleaved, shift):
+    """Tables that start `shift` floats behind a 32-byte boundary (4 and 12: at
+    an odd multiple of 16 bytes)."""
+    tokens, heads, hd, positions = 70, 5, 128, 40
+    n = positions * hd // 2
+    cos, sin = (torch.zeros(n + 16, device="cuda")[shift:shift + n].view(positions, hd // 2) for _ in range(2))
+    assert cos.data_ptr() % 32 == 4 * shift % 32
+    ops.rope_table(cos, sin, 1e4)
+    x, pos = rnd(tokens, heads, hd, dt=dt, seed=shift), i32([i % positions for i in range(tokens)])
+    out, intact = guarded(tokens, heads, hd, dt=dt)
+    ops.rope(x, pos, cos, sin, out=out, interleaved=interleaved)
+    ref, tol = rope_reference(x, pos, cos, sin, interleaved, False)
+    assert bool(((out.double() - ref).abs() <= tol + half_step(dt) * ref.abs() * 1.01 + torch.finfo(dt).tiny).all())
+    intact()
