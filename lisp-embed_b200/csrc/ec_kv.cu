@@ -136,8 +136,10 @@ __device__ bool find_free(const KvCache& c, int32_t* list, int64_t need, int ahe
 }
 
 // Whether slots[0..n) are slots and no two are the same.  A slot is claimed by
-// the index that names it; whoever does not find its own claim is a second.
+// the index that names it; whoever does not find its own claim is a second.  A
+// list longer than the cache has slots names one twice, and is not read.
 __device__ bool claim_slots(const KvCache& c, int32_t* claim, const int32_t* slots, int n) {
+  if (n > c.slots) return false;
   bool bad = false;
   for (int i = threadIdx.x; i < n; i += kPlanThreads) {
     const int s = slots[i];
@@ -309,8 +311,8 @@ __global__ void kv_fork_copy_kernel(const KvCache c, const int32_t* src, const i
   pdl_trigger();
   const Plan plan(c);
   const int i = blockIdx.x;
+  if (plan.scalars[0] == 0) return;  // refused: there are no copies to read
   const int4 copy = plan.copies[i];
-  if (plan.scalars[0] == 0) return;
   if (blockIdx.y == 0) {
     const int full = copy.w / c.page_size;
     const int32_t* from = c.tables + static_cast<int64_t>(src[i]) * c.width;
@@ -618,7 +620,7 @@ extern "C" int ec_kv_fork(int handle, const int32_t* src, const int32_t* dst, in
   if (int rc = check_cuda(launch_pdl(kv_fork_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, *c, src, dst, n, status),
                           "kv fork"))
     return rc;
-  if (n == 0) return EC_OK;
+  if (n == 0 || n > c->slots) return EC_OK;  // (the plan refuses the latter)
   return check_cuda(launch_pdl(kv_fork_copy_kernel, dim3(n, std::min(2 * c->layers, 65535)), dim3(256), 0, st, *c, src,
                                dst),
                     "kv fork copy");
@@ -636,7 +638,7 @@ extern "C" int ec_kv_free(int handle, const int32_t* slots, int n, int32_t* stat
   if (int rc = check_cuda(launch_pdl(kv_free_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, *c, slots, n, status, alone),
                           "kv free"))
     return rc;
-  if (alone) return EC_OK;
+  if (alone || n > c->slots) return EC_OK;
   return check_cuda(launch_pdl(kv_free_kernel, dim3(n), dim3(128), 0, st, *c, slots, status), "kv free");
 }
 

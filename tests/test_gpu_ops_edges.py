@@ -3,7 +3,7 @@ References and tolerances are those of test_gpu_ops.py."""
 import pytest
 import torch
 
-from test_gpu_ops import (BF16, F16, F32, guarded, half_step, i32, no_wait_gave_up, ops, rnd,  # noqa: F401
+from test_gpu_ops import (BF16, F16, F32, Cache, guarded, half_step, i32, no_wait_gave_up, ops, rnd,  # noqa: F401
                           rope_reference)
 
 pytestmark = pytest.mark.gpu
@@ -27,3 +27,25 @@ def test_rope_tables_at_any_float(ops, dt, interleaved, shift):
     ref, tol = rope_reference(x, pos, cos, sin, interleaved, False)
     assert bool(((out.double() - ref).abs() <= tol + half_step(dt) * ref.abs() * 1.01 + torch.finfo(dt).tiny).all())
     intact()
+
+
+# --------------------------------------------------------------------- pages --
+@pytest.mark.parametrize("slots,n", [(3, 4), (3, 5000), (1, 70000), (40, 41), (2000, 2001)])
+def test_lists_longer_than_the_cache_has_slots(ops, slots, n):
+    """They name a slot twice, whatever they hold: refused, nothing changed,
+    and what lies behind the caller's scratch is not looked at."""
+    lens = [20, 5, 0][:slots]
+    c = Cache(ops, lens, 16, 1, 16, F16, spare=4, seed=1, width=6, slots=slots)
+    before = c.state()
+    src, dst = i32([i % slots for i in range(n)]), i32([(i + 1) % slots for i in range(n)])
+    calls = (lambda: c.h.reserve(src, i32([1] * n), c.status), lambda: c.h.fork(src, dst, c.status),
+             lambda: c.h.fork(i32([0] * n), i32([slots - 1] * n), c.status), lambda: c.h.free(src, c.status))
+    for call in calls:
+        c.status.fill_(9)
+        call()
+        assert c.status.tolist() == [2, 0]
+        for a, b in zip(c.state(), before):
+            assert torch.equal(a, b)
+    if slots > 2:  # and the cache goes on as before
+        c.h.fork(i32([0]), i32([2]), c.status)
+        assert c.status.tolist() == [0, 1] and c.lens.tolist()[:3] == [20, 5, 20]
