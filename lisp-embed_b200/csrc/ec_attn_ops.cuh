@@ -301,6 +301,10 @@ __device__ __noinline__ bool flash_slots(const FlashArgs& a, int lane, int* grou
   return ok;
 }
 
+// The longest tile that flash_measure has bits for (4.19 million keys); it stands
+// for all longer ones, too, so nothing is laid out by it
+constexpr int kLongestMost = 0x7fff;
+
 // Even split: every CTA takes the same share of the key blocks, in the order
 // (sequence, tile, key head, block).  A tile costs its blocks and `over` units
 // more, for its start and end, which come first.  Where there are fewer tiles
@@ -324,7 +328,7 @@ __device__ __forceinline__ void flash_measure(const FlashArgs& a, int* units, in
       else none = 1;
     }
     units[s] = v * a.kv_heads;
-    about[s] = min(n * a.kv_heads, 0xffff) | min(most, 0x7fff) << 16 | none << 31;
+    about[s] = min(n * a.kv_heads, 0xffff) | min(most, kLongestMost) << 16 | none << 31;
   }
 }
 // (Kept out of line, as the list above: inlined into the kernels, the
@@ -336,13 +340,13 @@ __device__ __noinline__ bool flash_even(const FlashArgs& a, int lane, int* prefi
   for (int s = lane; s < a.nseq; s += 32) {
     work += prefix[s];
     tiles += about[s] & 0xffff;
-    most = max(most, about[s] >> 16 & 0x7fff);
+    most = max(most, about[s] >> 16 & kLongestMost);
   }
   tiles = __reduce_add_sync(0xffffffffu, min(tiles, 1 << 20));
   most = __reduce_max_sync(0xffffffffu, most);
   work = __reduce_add_sync(0xffffffffu, work);
   // every tile, padded to the longest, its own CTA
-  const bool alone = tiles <= ctas && most <= work / ctas + 8 + a.part_rows / 10;
+  const bool alone = tiles <= ctas && most < kLongestMost && most <= work / ctas + 8 + a.part_rows / 10;
   int total = 0;
 #pragma unroll 1
   for (int s0 = 0; s0 < a.nseq; s0 += 32) {

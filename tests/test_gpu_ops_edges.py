@@ -49,3 +49,32 @@ def test_lists_longer_than_the_cache_has_slots(ops, slots, n):
     if slots > 2:  # and the cache goes on as before
         c.h.fork(i32([0]), i32([2]), c.status)
         assert c.status.tolist() == [0, 1] and c.lens.tolist()[:3] == [20, 5, 20]
+
+
+# ----------------------------------------------------------- cached attention --
+@pytest.mark.parametrize("keys,sequences", [(4_193_920 - 128, 148), (4_193_920, 148), (4_200_005, 148), (8_400_001, 74)])
+def test_a_tile_for_every_cta_behind_millions_of_keys(ops, keys, sequences):
+    """The last key takes all the weight: the others' scores are 56 below it,
+    4e6 e^-56 < 2^-56.  Left out, the result would be the others' mean."""
+    page, hd = 128, 8
+    pages = -(-keys // page)
+    k = torch.zeros(1, pages, page, 1, hd, device="cuda", dtype=BF16)
+    v = rnd(1, pages, page, 1, hd, dt=BF16, seed=1)
+    at = (0, (keys - 1) // page, (keys - 1) % page)
+    k[at][0, 0] = 20.0
+    tables = torch.arange(pages, device="cuda", dtype=torch.int32)[None]
+    h = ops.KvCache(k, v, tables, i32([keys]), torch.ones(pages, device="cuda", dtype=torch.int32))
+    q = torch.zeros(sequences, 1, hd, device="cuda", dtype=BF16)
+    q[..., 0] = 8.0
+    cu, slots = i32(range(sequences + 1)), i32([0] * sequences)
+    work = torch.zeros(h.attention_workspace(q, cu, 1), dtype=torch.uint8, device="cuda")
+    for _ in range(2):
+        out, intact = guarded(sequences, 1, hd, dt=BF16)
+        h.attention(0, q, cu, out, 1, work, slots=slots)
+        assert bool((out[:, 0] == v[at][0]).all())
+        intact()
+    # the workspace is left ready for a call that is cut
+    out, intact = guarded(3, 1, hd, dt=BF16)
+    h.attention(0, q[:3], cu[:4], out, 1, work, slots=slots[:3])
+    assert bool((out[:, 0] == v[at][0]).all())
+    intact()
