@@ -223,7 +223,8 @@ int ec_flat_search_noalloc(const float *d_x, int64_t n, int d, const float *d_q,
  * h * head_stride + i] (strides in elements; that of a single token or head
  * does not count; heads of rows that are written must not overlap).  Sequence s is the tokens
  * [cu[s], cu[s + 1]) (int32, ascending from >= 0, empty sequences allowed);
- * rows behind cu[nseq] are left as they are. */
+ * rows behind cu[nseq] are left as they are.  What the attentions leave in the
+ * rows of a call whose offsets descend is not defined. */
 
 /* Waits inside the operators' kernels are bounded.  Waits for the current
  * device, then returns EC_ETIMEOUT (and clears the mark) if one of them gave

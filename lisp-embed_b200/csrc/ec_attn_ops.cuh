@@ -210,13 +210,22 @@ __device__ __forceinline__ FlashSeq flash_seq(const FlashArgs& a, int s) {
 // set u / nseq of sequence u % nseq), so that a CTA's few turns cost the same:
 // 4 prompts of 2048 tokens 84 us instead of 135.  With more sequences that
 // costs the keys' reuse: 96 texts behind 650 cached tokens took 182 us.
+//
+// Sums over the sequences are bounded by the tokens of the call as long as the
+// offsets ascend.  flash_count and flash_measure tell where they do not; then
+// the list stays empty (the sums could pass 32 bits, and what is laid out by
+// them the buffers).
 template <int NT>
-__device__ __forceinline__ void flash_count(const FlashArgs& a, int* groups) {
+__device__ __forceinline__ bool flash_count(const FlashArgs& a, int* groups) {
   const int size = (a.nseq + kFlashGroups - 1) / kFlashGroups, BT = NT * a.rows_tok;
+  bool descend = false;
   for (int s = threadIdx.x; s < a.nseq; s += blockDim.x) {
-    const int begin = min(max(a.cu[s], 0), a.tokens), end = min(max(a.cu[s + 1], begin), a.tokens);
+    const int c0 = a.cu[s], c1 = a.cu[s + 1];
+    const int begin = min(max(c0, 0), a.tokens), end = min(max(c1, begin), a.tokens);
+    descend |= c1 < c0;
     if (end > begin) atomicAdd(&groups[s / size], (end - begin + BT - 1) / BT);
   }
+  return descend;
 }
 template <int NT, typename Publish>
 __device__ __noinline__ bool flash_slots(const FlashArgs& a, int lane, int* groups, Publish publish) {
@@ -316,7 +325,8 @@ constexpr int kLongestMost = 0x7fff;
 // Each thread of the CTA first looks at some sequences (the loads are far
 // away, and the CTA has nothing else to do yet): units[s], and tiles | longest
 // tile << 16, with the sign bit where a tile sees no key.
-__device__ __forceinline__ void flash_measure(const FlashArgs& a, int* units, int* about) {
+__device__ __forceinline__ bool flash_measure(const FlashArgs& a, int* units, int* about) {
+  bool descend = false;
   for (int s = threadIdx.x; s < a.nseq; s += blockDim.x) {
     const FlashSeq q = flash_seq(a, s);
     const int len = q.end - q.begin, R = a.rows_tok;
@@ -329,7 +339,9 @@ __device__ __forceinline__ void flash_measure(const FlashArgs& a, int* units, in
     }
     units[s] = v * a.kv_heads;
     about[s] = min(n * a.kv_heads, 0xffff) | min(most, kLongestMost) << 16 | none << 31;
+    descend |= a.cu[s + 1] < a.cu[s];
   }
+  return descend;
 }
 // (Kept out of line, as the list above: inlined into the kernels, the
 // optimiser dropped an iteration of the sequence loop.)
@@ -597,10 +609,11 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
   }
   pdl_wait();  // what comes before may still be running up to here
   pdl_trigger();
-  if (count) flash_count<NT>(a, groups);
-  if (NT == 1 && a.even) flash_measure(a, prefix, prefix + Cfg::MAX_SEQS);
+  bool descend = false;
+  if (count) descend = flash_count<NT>(a, groups);
+  if (NT == 1 && a.even) descend = flash_measure(a, prefix, prefix + Cfg::MAX_SEQS);
   tc_fence_before();
-  __syncthreads();
+  descend = __syncthreads_or(descend);
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const int R = a.rows_tok, G = a.group;
@@ -705,7 +718,8 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
       ++n;
       return true;
     };
-    if (NT == 1 && a.even) {
+    if (descend) {
+    } else if (NT == 1 && a.even) {
       ok = flash_even(a, lane, prefix, prefix + Cfg::MAX_SEQS, [&](const Entry& e) { return publish(e, 0); });
     } else {
       ok = flash_slots<NT>(a, lane, groups, publish);
@@ -1345,9 +1359,9 @@ __global__ void __launch_bounds__(TokenCfg<HD, NP>::THREADS, 1)
   }
   pdl_wait();
   pdl_trigger();
-  flash_measure(a, prefix, prefix + Cfg::MAX_SEQS);
+  bool descend = flash_measure(a, prefix, prefix + Cfg::MAX_SEQS);
   tc_fence_before();
-  __syncthreads();
+  descend = __syncthreads_or(descend);
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const int R = a.rows_tok, G = a.group;
@@ -1384,7 +1398,7 @@ __global__ void __launch_bounds__(TokenCfg<HD, NP>::THREADS, 1)
       ++n;
       return true;
     };
-    ok = flash_even(a, lane, prefix, prefix + Cfg::MAX_SEQS, publish);
+    if (!descend) ok = flash_even(a, lane, prefix, prefix + Cfg::MAX_SEQS, publish);
     FlashEntry end{};
     if (ok) ok = publish(end);
   } else if (warp == W_LOAD) {

@@ -78,3 +78,39 @@ def test_a_tile_for_every_cta_behind_millions_of_keys(ops, keys, sequences):
     h.attention(0, q[:3], cu[:4], out, 1, work, slots=slots[:3])
     assert bool((out[:, 0] == v[at][0]).all())
     intact()
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_offsets_that_descend_again_and_again(ops, new):
+    """Every other sequence is all the tokens of the call (here 1024 times, with
+    more units of work than 32 bits hold): nothing outside the rows is written,
+    and the workspace is left ready."""
+    t, hk, hd, page, pages = 4096, 8, 8, 128, 512
+    k, v = (rnd(1, pages, page, hk, hd, dt=BF16, seed=i) for i in (1, 2))
+    tables = torch.arange(pages, device="cuda", dtype=torch.int32)[None]
+    h = ops.KvCache(k, v, tables, i32([page * pages]), torch.ones(pages, device="cuda", dtype=torch.int32))
+    q = rnd(t, hk, hd, dt=BF16, seed=3)
+    cu, slots = i32([0, t] * 1024 + [0]), i32([0] * 2048)
+    good = i32([0, 5])
+    work = torch.zeros(max(h.attention_workspace(q, cu, new), h.attention_workspace(q[:5], good, 5)), dtype=torch.uint8,
+                       device="cuda")
+    want, out = (torch.empty_like(q[:5]) for _ in range(2))
+    h.attention(0, q[:5], good, want, 5, work.clone(), slots=slots[:1])
+    rows, intact = guarded(t, hk, hd, dt=BF16)
+    lse, intact_l = guarded(t, hk, dt=F32)
+    h.attention(0, q, cu, rows, new, work, slots=slots, lse=lse)
+    h.attention(0, q[:5], good, out, 5, work, slots=slots[:1])
+    torch.cuda.synchronize()
+    intact(), intact_l()
+    assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("n", [33, 400, 4096, 4097])
+def test_prompt_offsets_that_descend_again_and_again(ops, n):
+    t, hd = 3000, 64
+    q, k, v = (rnd(t, 2, hd, dt=BF16, seed=h) for h in range(3))
+    out, intact = guarded(t, 2, hd, dt=BF16)
+    lse, intact_l = guarded(t, 2, dt=F32)
+    ops.attn_prompt(q, k, v, i32([t * (i & 1) for i in range(n + 1)]), out, lse=lse)
+    torch.cuda.synchronize()
+    intact(), intact_l()
