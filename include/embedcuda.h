@@ -290,6 +290,7 @@ int64_t ec_kv_work_size(int pages, int slots);
  * 16, 32, 64 or 128), tables[slots][table_width] (page of tokens
  * [j * page_size, (j + 1) * page_size) of a slot), lens[slots], refs[pages]
  * (slots that hold a page, 0 = free).  An empty cache has lens and refs 0.
+ * All of it lies on one device (EC_EINVAL by the first call that would use it).
  * The handle keeps the description only; calls on one cache are ordered by
  * the caller's streams. */
 int ec_kv_open(void *k, void *v, int dtype, int layers, int pages, int page_size, int heads,

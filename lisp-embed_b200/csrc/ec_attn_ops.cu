@@ -329,6 +329,6 @@ extern "C" int ec_attn_cached(int handle, int layer, const void* q, int64_t q_to
   op.work = work, op.work_bytes = static_cast<size_t>(work_bytes);
   op.scale = scale > 0.f ? scale : 1.f / std::sqrt(static_cast<float>(c->head_dim));
   OpDevice dev;
-  if (int rc = dev.enter({c->refs, q, out, lse, cu, slots, work})) return rc;
+  if (int rc = kv_enter(dev, *c, {q, out, lse, cu, slots, work})) return rc;
   return run_attention(op, dev.num_sms(), static_cast<cudaStream_t>(stream));
 }

@@ -29,11 +29,11 @@ namespace ec {
 
 namespace {
 std::mutex g_kv_mu;
-std::map<int, std::shared_ptr<const KvCache>> g_kv;
+std::map<int, std::shared_ptr<const KvOpen>> g_kv;
 int g_kv_next = 1;
 }  // namespace
 
-std::shared_ptr<const KvCache> kv_find(int handle) {
+std::shared_ptr<const KvOpen> kv_find(int handle) {
   std::lock_guard<std::mutex> lk(g_kv_mu);
   auto it = g_kv.find(handle);
   if (it == g_kv.end()) {
@@ -580,8 +580,8 @@ extern "C" int ec_kv_open(void* k, void* v, int dtype, int layers, int pages, in
   if (work_bytes < ec_kv_work_size(pages, slots))
     return set_error(EC_EINVAL, "work holds %lld bytes, the cache needs %lld", static_cast<long long>(work_bytes),
                      static_cast<long long>(ec_kv_work_size(pages, slots)));
-  auto c = std::make_shared<KvCache>(KvCache{k, v, dtype, layers, pages, page_size, heads, head_dim, tables, slots,
-                                             table_width, lens, refs, static_cast<int32_t*>(work)});
+  auto c = std::make_shared<KvOpen>(KvCache{k, v, dtype, layers, pages, page_size, heads, head_dim, tables, slots,
+                                            table_width, lens, refs, static_cast<int32_t*>(work)});
   std::lock_guard<std::mutex> lk(g_kv_mu);
   *handle = g_kv_next++;
   g_kv[*handle] = std::move(c);
@@ -603,7 +603,7 @@ extern "C" int ec_kv_reserve(int handle, const int32_t* slots, const int32_t* ad
   if (!c) return EC_EINVAL;
   if (int rc = check_lists(slots, add, n, status)) return rc;
   OpDevice dev;
-  if (int rc = dev.enter({c->refs, slots, add, status})) return rc;
+  if (int rc = kv_enter(dev, *c, {slots, add, status})) return rc;
   return check_cuda(launch_pdl(kv_reserve_kernel, dim3(1), dim3(kPlanThreads), 0, static_cast<cudaStream_t>(stream), *c,
                                slots, add, n, status),
                     "kv reserve");
@@ -615,7 +615,7 @@ extern "C" int ec_kv_fork(int handle, const int32_t* src, const int32_t* dst, in
   if (!c) return EC_EINVAL;
   if (int rc = check_lists(src, dst, n, status)) return rc;
   OpDevice dev;
-  if (int rc = dev.enter({c->refs, src, dst, status})) return rc;
+  if (int rc = kv_enter(dev, *c, {src, dst, status})) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (int rc = check_cuda(launch_pdl(kv_fork_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, *c, src, dst, n, status),
                           "kv fork"))
@@ -632,7 +632,7 @@ extern "C" int ec_kv_free(int handle, const int32_t* slots, int n, int32_t* stat
   if (!c) return EC_EINVAL;
   if (int rc = check_lists(slots, slots, n, status)) return rc;
   OpDevice dev;
-  if (int rc = dev.enter({c->refs, slots, status})) return rc;
+  if (int rc = kv_enter(dev, *c, {slots, status})) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int alone = static_cast<int64_t>(n) * c->width <= kFreeAlone;
   if (int rc = check_cuda(launch_pdl(kv_free_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, *c, slots, n, status, alone),
@@ -648,7 +648,7 @@ extern "C" int ec_kv_compact(int handle, int32_t* status, void* stream) {
   if (!c) return EC_EINVAL;
   if (int rc = check_lists(status, status, 0, status)) return rc;
   OpDevice dev;
-  if (int rc = dev.enter({c->refs, status})) return rc;
+  if (int rc = kv_enter(dev, *c, {status})) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (int rc = check_cuda(launch_pdl(kv_compact_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, *c, status), "kv compact"))
     return rc;
@@ -669,7 +669,7 @@ extern "C" int ec_kv_write(int handle, int layer, const void* k, int64_t k_token
   if (tokens == 0 || nseq == 0) return EC_OK;
   if (!cu || !op_aligned(cu, 4) || !op_aligned(slots, 4)) return set_error(EC_EINVAL, "cu is NULL or a list misaligned");
   OpDevice dev;
-  if (int rc = dev.enter({c->refs, k, v, cu, slots})) return rc;
+  if (int rc = kv_enter(dev, *c, {k, v, cu, slots})) return rc;
   const WriteArgs a{static_cast<const uint4*>(k), static_cast<const uint4*>(v), kr.token / 8, kr.head / 8, vr.token / 8,
                     vr.head / 8, tokens, cu, slots, nseq, layer};
   const int64_t grid = (tokens + kWriteTokens - 1) / kWriteTokens;

@@ -5,8 +5,7 @@
 
 namespace ec {
 
-int OpDevice::enter(std::initializer_list<const void*> ptrs) {
-  int dev = -1;
+int OpDevice::enter(std::initializer_list<const void*> ptrs, int dev) {
   for (const void* p : ptrs) {
     if (!p) continue;
     cudaPointerAttributes a;
@@ -42,6 +41,18 @@ int OpDevice::enter(std::initializer_list<const void*> ptrs) {
   }
   sms_ = sms[dev];
   return EC_OK;
+}
+
+int kv_enter(OpDevice& dev, const KvOpen& c, std::initializer_list<const void*> ptrs) {
+  int on = c.device.load(std::memory_order_relaxed);
+  if (on < 0) {
+    if (int rc = dev.enter({c.k, c.v, c.tables, c.lens, c.refs, c.work})) {
+      const std::string why = ec_last_error();
+      return set_error(rc, "the cache's memory: %s", why.c_str());
+    }
+    c.device.store(on = dev.ordinal(), std::memory_order_relaxed);
+  }
+  return dev.enter(ptrs, on);
 }
 
 OpDevice::~OpDevice() {

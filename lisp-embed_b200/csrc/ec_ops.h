@@ -9,6 +9,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <initializer_list>
 #include <memory>
 
@@ -22,8 +23,8 @@ namespace ec {
 class OpDevice {
  public:
   // EC_OK, or an error when one of the non-null pointers is not device memory
-  // or lies on another device than the first
-  int enter(std::initializer_list<const void*> ptrs);
+  // or lies on another device than the first (or than `dev`)
+  int enter(std::initializer_list<const void*> ptrs, int dev = -1);
   ~OpDevice();
   int num_sms() const { return sms_; }
   int ordinal() const { return dev_; }
@@ -61,9 +62,17 @@ struct KvCache {
   int32_t* refs;       // [pages]
   int32_t* work;       // scratch of the page operations
 };
+struct KvOpen : KvCache {
+  explicit KvOpen(const KvCache& c) : KvCache(c) {}
+  // the device that all its buffers were found on, by the first call that
+  // launches anything (a handle's pointers never change); -1: not looked at
+  mutable std::atomic<int> device{-1};
+};
 // the cache behind a handle (held until the pointer goes away), or nullptr
 // with the error set
-std::shared_ptr<const KvCache> kv_find(int handle);
+std::shared_ptr<const KvOpen> kv_find(int handle);
+// dev.enter for a call on cache c with these buffers
+int kv_enter(OpDevice& dev, const KvOpen& c, std::initializer_list<const void*> ptrs);
 
 // ---- attention over packed queries (ec_attn_ops.cu) --------------------------
 struct AttnOp {

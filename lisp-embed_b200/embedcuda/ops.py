@@ -178,6 +178,9 @@ class KvCache:
             work = refs.new_zeros((size + 3) // 4)
         if not work.is_contiguous():
             raise ValueError("work must be contiguous")
+        for t, what in ((v, "v"), (tables, "tables"), (lens, "lens"), (refs, "refs"), (work, "work")):
+            if t.device != k.device:
+                raise ValueError(f"{what} is on {t.device}, k is on {k.device}")
         h = C.c_int()
         _lib.check(_lib.lib().ec_kv_open(k.data_ptr(), v.data_ptr(), code, layers, pages, page, heads, hd,
                                          tables.data_ptr(), slots, width, lens_p, refs_p, work.data_ptr(),

@@ -114,3 +114,50 @@ def test_prompt_offsets_that_descend_again_and_again(ops, n):
     ops.attn_prompt(q, k, v, i32([t * (i & 1) for i in range(n + 1)]), out, lse=lse)
     torch.cuda.synchronize()
     intact(), intact_l()
+
+
+# -------------------------------------------------------------- where it lies --
+@pytest.mark.parametrize("which", range(6))
+def test_cache_memory_of_the_host_is_refused(ops, which):
+    """Any of the six buffers of a cache, by every call that would launch."""
+    import ctypes as C
+    from embedcuda import _lib
+    L = _lib.lib()
+    k, v = (torch.zeros(1, 8, 16, 1, 64, dtype=BF16) for _ in range(2))
+    tables, lens, refs = torch.zeros(2, 3, dtype=torch.int32), i32([0, 0]).cpu(), torch.zeros(8, dtype=torch.int32)
+    work = torch.zeros(L.ec_kv_work_size(8, 2), dtype=torch.uint8)
+    bufs = [t if i == which else t.cuda() for i, t in enumerate((k, v, tables, lens, refs, work))]
+    k, v, tables, lens, refs, work = (t.data_ptr() for t in bufs)
+    h = C.c_int()
+    assert L.ec_kv_open(k, v, _lib.EC_BF16, 1, 8, 16, 1, 64, tables, 2, 3, lens, refs, work, bufs[5].numel(),
+                        C.byref(h)) == 0
+    one, status, cu = i32([0]), i32([9, 9]), i32([0, 1])
+    x = torch.zeros(1, 1, 64, device="cuda", dtype=BF16)
+    scratch = torch.zeros(L.ec_attn_cached_work_size(h.value, 1, 1, 1, 1), dtype=torch.uint8, device="cuda")
+    st = torch.cuda.current_stream().cuda_stream
+    p = lambda t: t.data_ptr()  # noqa: E731
+    calls = (lambda: L.ec_kv_reserve(h, p(one), p(one), 1, p(status), st),
+             lambda: L.ec_kv_fork(h, p(one), p(one), 1, p(status), st),
+             lambda: L.ec_kv_free(h, p(one), 1, p(status), st),
+             lambda: L.ec_kv_compact(h, p(status), st),
+             lambda: L.ec_kv_write(h, 0, p(x), 64, 64, p(x), 64, 64, 1, p(cu), None, 1, st),
+             lambda: L.ec_attn_cached(h, 0, p(x), 64, 64, p(x), 64, 64, None, 1, 1, p(cu), None, 1, 1, 0.0,
+                                      p(scratch), scratch.numel(), st))
+    for call in calls:
+        for _ in range(2):
+            assert call() == _lib.EC_EINVAL
+            assert "the cache's memory" in _lib.last_error() and "device memory" in _lib.last_error()
+    assert status.tolist() == [9, 9]
+    assert L.ec_kv_close(h) == 0
+
+
+def test_cache_lists_of_the_host_are_refused(ops):
+    from embedcuda import _lib
+    c = Cache(ops, [5, 0], 16, 1, 64, BF16)
+    for _ in range(2):  # before and after a call that was right
+        with pytest.raises(_lib.EcError, match="device memory"):
+            c.h.reserve(i32([0]).cpu(), i32([1]), c.status)
+        c.h.reserve(i32([0]), i32([1]), c.status)
+        assert c.status.tolist() == [0, 0]
+    with pytest.raises(ValueError, match="tables is on cpu"):
+        ops.KvCache(c.k, c.v, c.tables.cpu(), c.lens, c.refs)
