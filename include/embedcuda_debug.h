@@ -81,6 +81,10 @@ int ecdbg_tensor_read(const char *name, void *host, size_t nbytes, int *dtype);
  * returns EC_ETIMEOUT with the context still usable. */
 int ecdbg_wait_timeout(int limit_ms);
 
+/* Leave the current device as if a wait of a caller's own operator had given
+ * up: the next ec_op_status returns EC_ETIMEOUT. */
+int ecdbg_op_timeout(void);
+
 #ifdef __cplusplus
 }
 #endif

@@ -164,10 +164,14 @@ size_t attention_work_bytes(const KvCache& c, int64_t tokens, int q_heads, int n
   return part_bytes(p.part_rows, c.head_dim <= 64 ? 64 : 128) + part_bytes(p.part_rows, 1) + kMaxCtas * 4;
 }
 
-int op_status_fetch(unsigned* host, cudaStream_t st) {
-  void* p = nullptr;
-  if (int rc = check_cuda(cudaGetSymbolAddress(&p, g_op_status), "operator status")) return rc;
-  return check_cuda(cudaMemcpyAsync(host, p, sizeof(unsigned), cudaMemcpyDeviceToHost, st), "operator status");
+namespace {
+thread_local unsigned* t_status_word = nullptr;
+}
+OpStatusWord::OpStatusWord(unsigned* word) { t_status_word = word; }
+OpStatusWord::~OpStatusWord() { t_status_word = nullptr; }
+
+int op_status_mark(unsigned code) {
+  return check_cuda(cudaMemcpyToSymbol(g_op_status, &code, sizeof code), "operator status");
 }
 
 size_t attention_work_most(int head_dim) {
@@ -198,6 +202,7 @@ int run_attention(const AttnOp& op, int num_sms, cudaStream_t st) {
   a.out = const_cast<void*>(op.out.p), a.ot = op.out.token, a.oh = op.out.head;
   a.wide = op_aligned(a.out, 32) && a.ot % 16 == 0 && a.oh % 16 == 0 && op.head_dim % 16 == 0;
   a.lse = op.lse;
+  a.status = t_status_word;
   a.cu = op.cu, a.slots = op.slots;
   a.tokens = static_cast<int>(op.tokens), a.nseq = op.nseq;
   a.group = group, a.rows_tok = p.rows_tok, a.q_heads = op.q_heads, a.kv_heads = op.kv_heads;

@@ -71,6 +71,7 @@ struct FlashArgs {
   float* part_o;           // [2 * CTAs][part_rows][HD] partial results of cut tiles
   float* part_l;           // [2 * CTAs][part_rows] their log2-sum-exp2
   int* arrived;            // [CTAs] parts done of the tile whose first part is the CTA's; 0 between calls
+  unsigned* status;        // marked by a wait that gives up; nullptr: g_op_status
 };
 
 // a tile set that one CTA works on
@@ -124,8 +125,10 @@ struct FlashCfg {
   static_assert(SMEM <= 232448, "shared memory");
 };
 
-// first wait that gave up on this device since ec_op_status last asked
+// first wait of a caller's own call that gave up on this device since
+// ec_op_status last asked
 static __device__ unsigned g_op_status;
+__device__ __forceinline__ unsigned* status_word(const FlashArgs& a) { return a.status ? a.status : &g_op_status; }
 
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float a, float b);
@@ -541,7 +544,7 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
 
   extern __shared__ __align__(1024) uint8_t smem[];
   if (smem_u32(smem) & 1023u) {  // swizzled tiles need 1024-byte alignment
-    if (threadIdx.x == 0) report(&g_op_status, kDevBadArg);
+    if (threadIdx.x == 0) report(status_word(a), kDevBadArg);
     return;
   }
   uint8_t* sQ = smem;
@@ -972,7 +975,7 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
         if (!ok) break;
       }
       if (!ok) {
-        report(&g_op_status, code);
+        report(status_word(a), code);
         *abort_flag = 1;
       }
     }
@@ -1198,7 +1201,7 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
     }
   }
   if (!ok) {
-    report(&g_op_status, code);
+    report(status_word(a), code);
     *abort_flag = 1;
   }
   tc_fence_before();
@@ -1303,7 +1306,7 @@ __global__ void __launch_bounds__(TokenCfg<HD, NP>::THREADS, 1)
 
   extern __shared__ __align__(1024) uint8_t smem[];
   if (smem_u32(smem) & 1023u) {
-    if (threadIdx.x == 0) report(&g_op_status, kDevBadArg);
+    if (threadIdx.x == 0) report(status_word(a), kDevBadArg);
     return;
   }
   uint8_t* sKV = smem;
@@ -1539,7 +1542,7 @@ __global__ void __launch_bounds__(TokenCfg<HD, NP>::THREADS, 1)
         if (!ok) break;
       }
       if (!ok) {
-        report(&g_op_status, code);
+        report(status_word(a), code);
         *abort_flag = 1;
       }
     }
@@ -1713,7 +1716,7 @@ __global__ void __launch_bounds__(TokenCfg<HD, NP>::THREADS, 1)
     }
   }
   if (!ok) {
-    report(&g_op_status, code);
+    report(status_word(a), code);
     *abort_flag = 1;
   }
   tc_fence_before();

@@ -4,6 +4,7 @@
 #include <vector>
 
 #include "../../include/embedcuda_debug.h"
+#include "ec_ops.h"
 #include "ec_ptx.cuh"
 #include "ec_state.h"
 
@@ -256,6 +257,12 @@ int ecdbg_wait_timeout(int limit_ms) {
   rc = check_cuda(cudaGetLastError(), "wait kernel");
   if (rc) return rc;
   return sync_and_check(d, "bounded wait");
+}
+
+int ecdbg_op_timeout(void) {
+  clear_error();
+  int rc = check_cuda(cudaDeviceSynchronize(), "operators");
+  return rc ? rc : op_status_mark(kDevTimeoutOther);
 }
 
 long long ecdbg_launches(void) {

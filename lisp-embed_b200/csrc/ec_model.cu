@@ -809,6 +809,7 @@ static int forward_packed(Device& d, const WsLayout& L, int T, int nseq, const A
   at.num_sms = d.num_sms;
   auto attention = [&](int layer) -> int {
     const int e0 = prof_begin(d);
+    const OpStatusWord word(d.status);  // what sync_and_check looks at
     if (px) {
       // the texts' keys and values go behind the prefix's, into pages of the
       // pool; the queries read both
@@ -1306,8 +1307,6 @@ int embed_on_device(Device& d, const int32_t* ids_host, const int32_t* ids_dev,
     for (int k = 0; k < nseq; ++k)
       pairs += m.family == EC_FAMILY_LLAMA ? lens[k] * (0.5 * (lens[k] + 1.0) + first)
                                            : static_cast<double>(lens[k]) * lens[k];
-    // the attention operators' bounded waits have a status word of their own
-    const bool operators = pool || (m.family == EC_FAMILY_LLAMA && m.hd != 128);
     PrefixRun run{};
     int* hadd = hid + T + 8;  // lengths of the sequences, behind the ids
     if (pool) {
@@ -1334,7 +1333,6 @@ int embed_on_device(Device& d, const int32_t* ids_host, const int32_t* ids_dev,
                                           dout, obytes, cudaMemcpyDeviceToHost, d.stream),
                           "output download"));
       if (pool) EC_TRY(prefix_fetch(d, *pool));
-      if (operators && d.status_host) EC_TRY(op_status_fetch(d.status_host + 4, d.stream));
       return EC_OK;
     };
     fill_tables(d, lens, &tb);
@@ -1388,7 +1386,6 @@ int embed_on_device(Device& d, const int32_t* ids_host, const int32_t* ids_dev,
     tmark(g ? "graph launch" : "enqueue");
     EC_TRY(sync_and_check(d, "forward"));
     if (pool) EC_TRY(prefix_check(*pool));
-    if (operators && (!d.status_host || d.status_host[4])) EC_TRY(ec_op_status());
     tmark("device (wait)");
     prof_collect(d);
     if (!out_dev && !direct_out)

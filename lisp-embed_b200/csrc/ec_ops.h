@@ -93,8 +93,16 @@ struct AttnOp {
 };
 int run_attention(const AttnOp& op, int num_sms, cudaStream_t st);
 size_t attention_work_bytes(const KvCache& c, int64_t tokens, int q_heads, int nseq, int max_new);
-// copies the mark of a wait that gave up (0: none) to `host`, in stream order
-int op_status_fetch(unsigned* host, cudaStream_t st);
+// While one lives, this thread's attention calls mark `word` (of the call's
+// device) when a wait gives up, not the word that ec_op_status asks: a forward
+// of the library and a caller's own calls do not hear of each other's.
+class OpStatusWord {
+ public:
+  explicit OpStatusWord(unsigned* word);
+  ~OpStatusWord();
+};
+// marks the word that ec_op_status asks, on the current device (for tests)
+int op_status_mark(unsigned code);
 // enough for every call on a cache of this head size
 size_t attention_work_most(int head_dim);
 
