@@ -85,6 +85,12 @@ int ecdbg_wait_timeout(int limit_ms);
  * up: the next ec_op_status returns EC_ETIMEOUT. */
 int ecdbg_op_timeout(void);
 
+/* Leave device 0 as if a wait of the cached attention had given up in a
+ * forward behind an open prefix: the status word is set and the workspace's
+ * counts are not zero, so the next forward of the library returns
+ * EC_ETIMEOUT. */
+int ecdbg_prefix_timeout(void);
+
 #ifdef __cplusplus
 }
 #endif

@@ -178,6 +178,8 @@ size_t attention_work_most(int head_dim) {
   return part_bytes(128, head_dim <= 64 ? 64 : 128) + part_bytes(128, 1) + kMaxCtas * 4;
 }
 
+int attention_counts() { return kMaxCtas; }
+
 int run_attention(const AttnOp& op, int num_sms, cudaStream_t st) {
   const KvCache* c = op.cache;
   num_sms = std::min(num_sms, kMaxCtas);

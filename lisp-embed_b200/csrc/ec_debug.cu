@@ -5,6 +5,7 @@
 
 #include "../../include/embedcuda_debug.h"
 #include "ec_ops.h"
+#include "ec_prefix.h"
 #include "ec_ptx.cuh"
 #include "ec_state.h"
 
@@ -263,6 +264,20 @@ int ecdbg_op_timeout(void) {
   clear_error();
   int rc = check_cuda(cudaDeviceSynchronize(), "operators");
   return rc ? rc : op_status_mark(kDevTimeoutOther);
+}
+
+int ecdbg_prefix_timeout(void) {
+  std::lock_guard<std::mutex> lk(G().mu);
+  clear_error();
+  if (!G().inited) return set_error(EC_ESTATE, "ec_init first");
+  Device& d = *G().devs[0];
+  if (!d.prefixes) return set_error(EC_ESTATE, "no prefix is open");
+  int rc = check_cuda(cudaSetDevice(d.ordinal), "cudaSetDevice");
+  const std::vector<int> counts(attention_counts(), 1);
+  const unsigned code = kDevTimeoutOther;
+  if (!rc) rc = check_cuda(cudaStreamSynchronize(d.stream), "prefix");
+  if (!rc) rc = check_cuda(cudaMemcpy(d.prefixes->work, counts.data(), counts.size() * 4, cudaMemcpyHostToDevice), "counts");
+  return rc ? rc : check_cuda(cudaMemcpy(d.status, &code, sizeof code, cudaMemcpyHostToDevice), "status");
 }
 
 long long ecdbg_launches(void) {

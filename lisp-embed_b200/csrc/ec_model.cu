@@ -1384,7 +1384,10 @@ int embed_on_device(Device& d, const int32_t* ids_host, const int32_t* ids_dev,
       EC_TRY(enqueue());
     }
     tmark(g ? "graph launch" : "enqueue");
-    EC_TRY(sync_and_check(d, "forward"));
+    if (const int rc = sync_and_check(d, "forward")) {
+      if (pool) prefix_failed(d, *pool);
+      return rc;
+    }
     if (pool) EC_TRY(prefix_check(*pool));
     tmark("device (wait)");
     prof_collect(d);

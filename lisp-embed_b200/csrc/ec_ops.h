@@ -105,5 +105,7 @@ class OpStatusWord {
 int op_status_mark(unsigned code);
 // enough for every call on a cache of this head size
 size_t attention_work_most(int head_dim);
+// the int32 counts at the start of a workspace, zero between calls
+int attention_counts();
 
 }  // namespace ec

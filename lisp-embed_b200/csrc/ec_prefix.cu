@@ -120,6 +120,13 @@ int prefix_check(const PrefixPool& p) {
   return EC_OK;
 }
 
+// A wait that gave up may have left tiles of the cached attention half counted:
+// the next forward would join their parts too early, or never.
+void prefix_failed(Device& d, PrefixPool& p) {
+  cudaMemsetAsync(p.work, 0, p.work_bytes, d.stream);
+  cudaStreamSynchronize(d.stream);
+}
+
 // the slot of a prefix id, or -1 with the error set
 static int prefix_slot(int id) {
   const PrefixPool* p = G().devs[0]->prefixes;

@@ -48,5 +48,6 @@ PrefixRun prefix_run(const PrefixPool& p, int slot, bool fill, int longest);
 int prefix_plan(Device& d, PrefixPool& p, int slot, bool fill, const int* lens, int nseq);
 int prefix_fetch(Device& d, PrefixPool& p);  // enqueue the download of the page operations' status
 int prefix_check(const PrefixPool& p);       // after the stream was waited for
+void prefix_failed(Device& d, PrefixPool& p);  // after a forward that gave up
 
 }  // namespace ec

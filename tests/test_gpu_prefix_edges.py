@@ -29,3 +29,22 @@ def test_a_callers_time_out_is_not_the_librarys(synth_root, ec, shape):
         assert L.ec_op_status() == _lib.EC_ETIMEOUT
         assert L.ec_op_status() == 0
         assert np.array_equal(p.embed_batch(ids, offs), want)
+
+
+def test_a_forward_that_timed_out_leaves_the_next_ones_right(synth_root, ec):
+    """Texts of few tokens behind a long prefix: more tiles than SMs, so some
+    are cut and joined by the workspace's counts."""
+    _load(synth_root, QWEN)
+    rng = np.random.default_rng(8)
+    batches = [_batch(rng, QWEN, rng.integers(1, 9, 120)) for _ in range(2)]
+    with model.Prefix(_ids(rng, QWEN, 1000)) as p, model.Prefix(_ids(rng, QWEN, 900)) as other:
+        want = [x.embed_batch(*b) for x in (p, other) for b in batches]
+        for _ in range(2):
+            assert ec.lib().ecdbg_prefix_timeout() == 0
+            with pytest.raises(_lib.EcError) as e:
+                p.embed_batch(*batches[1])
+            assert e.value.code == _lib.EC_ETIMEOUT
+            for _ in range(2):
+                got = [x.embed_batch(*b) for x in (p, other) for b in batches]
+                for g, w in zip(got, want):
+                    assert np.array_equal(g, w)
