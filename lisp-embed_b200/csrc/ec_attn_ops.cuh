@@ -521,8 +521,10 @@ __device__ __noinline__ void flash_join(const FlashArgs& a, int tok0, int qv, in
 
 // Counts a finished part; true in the CTA that finished the last one, which
 // leaves the count at 0 for the next call.  By one thread, after all threads
-// have written the part and fenced.
+// have written the part and fenced: what they wrote is released by this
+// thread's fence between meeting them and counting.
 __device__ __forceinline__ bool flash_arrive(const FlashArgs& a, const FlashEntry& it) {
+  __threadfence();
   const bool last = atomicAdd(&a.arrived[it.c0], 1) == it.parts - 1;
   if (last) a.arrived[it.c0] = 0;
   __threadfence();
