@@ -4,6 +4,7 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <mutex>
 
@@ -166,7 +167,20 @@ size_t attention_work_bytes(const KvCache& c, int64_t tokens, int q_heads, int n
 
 namespace {
 thread_local unsigned* t_status_word = nullptr;
+
+// the current device's word that ec_op_status asks
+int caller_status_word(unsigned** word) {
+  static std::atomic<unsigned*> words[64] = {};
+  int dev = 0;
+  if (int rc = check_cuda(cudaGetDevice(&dev), "cudaGetDevice")) return rc;
+  *word = words[dev].load(std::memory_order_relaxed);
+  if (*word) return EC_OK;
+  void* p = nullptr;
+  if (int rc = check_cuda(cudaGetSymbolAddress(&p, g_op_status), "operator status")) return rc;
+  words[dev].store(*word = static_cast<unsigned*>(p), std::memory_order_relaxed);
+  return EC_OK;
 }
+}  // namespace
 OpStatusWord::OpStatusWord(unsigned* word) { t_status_word = word; }
 OpStatusWord::~OpStatusWord() { t_status_word = nullptr; }
 
@@ -205,6 +219,8 @@ int run_attention(const AttnOp& op, int num_sms, cudaStream_t st) {
   a.wide = op_aligned(a.out, 32) && a.ot % 16 == 0 && a.oh % 16 == 0 && op.head_dim % 16 == 0;
   a.lse = op.lse;
   a.status = t_status_word;
+  if (!a.status)
+    if (int rc = caller_status_word(&a.status)) return rc;
   a.cu = op.cu, a.slots = op.slots;
   a.tokens = static_cast<int>(op.tokens), a.nseq = op.nseq;
   a.group = group, a.rows_tok = p.rows_tok, a.q_heads = op.q_heads, a.kv_heads = op.kv_heads;

@@ -71,7 +71,7 @@ struct FlashArgs {
   float* part_o;           // [2 * CTAs][part_rows][HD] partial results of cut tiles
   float* part_l;           // [2 * CTAs][part_rows] their log2-sum-exp2
   int* arrived;            // [CTAs] parts done of the tile whose first part is the CTA's; 0 between calls
-  unsigned* status;        // marked by a wait that gives up; nullptr: g_op_status
+  unsigned* status;        // marked by a wait that gives up
 };
 
 // a tile set that one CTA works on
@@ -128,7 +128,6 @@ struct FlashCfg {
 // first wait of a caller's own call that gave up on this device since
 // ec_op_status last asked
 static __device__ unsigned g_op_status;
-__device__ __forceinline__ unsigned* status_word(const FlashArgs& a) { return a.status ? a.status : &g_op_status; }
 
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float a, float b);
@@ -215,20 +214,19 @@ __device__ __forceinline__ FlashSeq flash_seq(const FlashArgs& a, int s) {
 // costs the keys' reuse: 96 texts behind 650 cached tokens took 182 us.
 //
 // Sums over the sequences are bounded by the tokens of the call as long as the
-// offsets ascend.  flash_count and flash_measure tell where they do not; then
+// offsets ascend.  flash_count and flash_measure mark where they do not; then
 // the list stays empty (the sums could pass 32 bits, and what is laid out by
-// them the buffers).
+// them the buffers).  The mark lies in shared memory: in a register it cost the
+// pairs' kernels spills (256 prompts, 71060 tokens: 281 -> 294 us).
 template <int NT>
-__device__ __forceinline__ bool flash_count(const FlashArgs& a, int* groups) {
+__device__ __forceinline__ void flash_count(const FlashArgs& a, int* groups, volatile int* descend) {
   const int size = (a.nseq + kFlashGroups - 1) / kFlashGroups, BT = NT * a.rows_tok;
-  bool descend = false;
   for (int s = threadIdx.x; s < a.nseq; s += blockDim.x) {
     const int c0 = a.cu[s], c1 = a.cu[s + 1];
     const int begin = min(max(c0, 0), a.tokens), end = min(max(c1, begin), a.tokens);
-    descend |= c1 < c0;
+    if (c1 < c0) *descend = 1;
     if (end > begin) atomicAdd(&groups[s / size], (end - begin + BT - 1) / BT);
   }
-  return descend;
 }
 template <int NT, typename Publish>
 __device__ __noinline__ bool flash_slots(const FlashArgs& a, int lane, int* groups, Publish publish) {
@@ -326,10 +324,10 @@ constexpr int kLongestMost = 0x7fff;
 // behind 20000 203 and 94; 8 of 64 behind 8000 98 and 96.
 //
 // Each thread of the CTA first looks at some sequences (the loads are far
-// away, and the CTA has nothing else to do yet): units[s], and tiles | longest
-// tile << 16, with the sign bit where a tile sees no key.
-__device__ __forceinline__ bool flash_measure(const FlashArgs& a, int* units, int* about) {
-  bool descend = false;
+// away, and the CTA has nothing else to do yet): units[s] (-1: its offsets
+// descend), and tiles | longest tile << 16, with the sign bit where a tile sees
+// no key.
+__device__ __forceinline__ void flash_measure(const FlashArgs& a, int* units, int* about) {
   for (int s = threadIdx.x; s < a.nseq; s += blockDim.x) {
     const FlashSeq q = flash_seq(a, s);
     const int len = q.end - q.begin, R = a.rows_tok;
@@ -340,11 +338,9 @@ __device__ __forceinline__ bool flash_measure(const FlashArgs& a, int* units, in
       if (nb) v += nb + a.over, ++n, most = nb + a.over;
       else none = 1;
     }
-    units[s] = v * a.kv_heads;
+    units[s] = a.cu[s + 1] < a.cu[s] ? -1 : v * a.kv_heads;
     about[s] = min(n * a.kv_heads, 0xffff) | min(most, kLongestMost) << 16 | none << 31;
-    descend |= a.cu[s + 1] < a.cu[s];
   }
-  return descend;
 }
 // (Kept out of line, as the list above: inlined into the kernels, the
 // optimiser dropped an iteration of the sequence loop.)
@@ -352,14 +348,17 @@ template <typename Publish>
 __device__ __noinline__ bool flash_even(const FlashArgs& a, int lane, int* prefix, const int* about, Publish publish) {
   const int R = a.rows_tok, ctas = gridDim.x, me = blockIdx.x;
   int tiles = 0, most = 0, work = 0;
+  bool descend = false;
   for (int s = lane; s < a.nseq; s += 32) {
     work += prefix[s];
+    descend |= prefix[s] < 0;
     tiles += about[s] & 0xffff;
     most = max(most, about[s] >> 16 & kLongestMost);
   }
   tiles = __reduce_add_sync(0xffffffffu, min(tiles, 1 << 20));
   most = __reduce_max_sync(0xffffffffu, most);
   work = __reduce_add_sync(0xffffffffu, work);
+  if (__any_sync(0xffffffffu, descend)) return true;
   // every tile, padded to the longest, its own CTA
   const bool alone = tiles <= ctas && most < kLongestMost && most <= work / ctas + 8 + a.part_rows / 10;
   int total = 0;
@@ -546,7 +545,7 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
 
   extern __shared__ __align__(1024) uint8_t smem[];
   if (smem_u32(smem) & 1023u) {  // swizzled tiles need 1024-byte alignment
-    if (threadIdx.x == 0) report(status_word(a), kDevBadArg);
+    if (threadIdx.x == 0) report(a.status, kDevBadArg);
     return;
   }
   uint8_t* sQ = smem;
@@ -569,10 +568,11 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(items + kFlashRing);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* last_part = abort_flag + 1;
+  volatile int* descend = last_part + 1;
   int* prefix = reinterpret_cast<int*>(tail + 1536);  // [MAX_SEQS] of an even split
   float* inverse = reinterpret_cast<float*>(tail + 1536);  // [2][128] 1 / l (NT 2)
   int* groups = reinterpret_cast<int*>(tail + 1536 + (NT == 1 ? 0 : 1024));  // [kFlashGroups] of a list
-  static_assert(8 * (4 + 2 * ST + 14 + 2 * kFlashRing) + kFlashRing * sizeof(FlashItem) + 12 <= 1536, "tail");
+  static_assert(8 * (4 + 2 * ST + 14 + 2 * kFlashRing) + kFlashRing * sizeof(FlashItem) + 16 <= 1536, "tail");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -596,6 +596,7 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
       mbar_init(&i_empty[i], READERS);
     }
     *abort_flag = 0;
+    *descend = 0;
     fence_barrier_init();
   }
   if (warp == W_LOAD && lane == 0) {
@@ -614,11 +615,10 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
   }
   pdl_wait();  // what comes before may still be running up to here
   pdl_trigger();
-  bool descend = false;
-  if (count) descend = flash_count<NT>(a, groups);
-  if (NT == 1 && a.even) descend = flash_measure(a, prefix, prefix + Cfg::MAX_SEQS);
+  if (count) flash_count<NT>(a, groups, descend);
+  if (NT == 1 && a.even) flash_measure(a, prefix, prefix + Cfg::MAX_SEQS);
   tc_fence_before();
-  descend = __syncthreads_or(descend);
+  __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const int R = a.rows_tok, G = a.group;
@@ -723,7 +723,7 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
       ++n;
       return true;
     };
-    if (descend) {
+    if (*descend) {
     } else if (NT == 1 && a.even) {
       ok = flash_even(a, lane, prefix, prefix + Cfg::MAX_SEQS, [&](const Entry& e) { return publish(e, 0); });
     } else {
@@ -977,7 +977,7 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
         if (!ok) break;
       }
       if (!ok) {
-        report(status_word(a), code);
+        report(a.status, code);
         *abort_flag = 1;
       }
     }
@@ -1203,7 +1203,7 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
     }
   }
   if (!ok) {
-    report(status_word(a), code);
+    report(a.status, code);
     *abort_flag = 1;
   }
   tc_fence_before();
@@ -1308,7 +1308,7 @@ __global__ void __launch_bounds__(TokenCfg<HD, NP>::THREADS, 1)
 
   extern __shared__ __align__(1024) uint8_t smem[];
   if (smem_u32(smem) & 1023u) {
-    if (threadIdx.x == 0) report(status_word(a), kDevBadArg);
+    if (threadIdx.x == 0) report(a.status, kDevBadArg);
     return;
   }
   uint8_t* sKV = smem;
@@ -1364,9 +1364,9 @@ __global__ void __launch_bounds__(TokenCfg<HD, NP>::THREADS, 1)
   }
   pdl_wait();
   pdl_trigger();
-  bool descend = flash_measure(a, prefix, prefix + Cfg::MAX_SEQS);
+  flash_measure(a, prefix, prefix + Cfg::MAX_SEQS);
   tc_fence_before();
-  descend = __syncthreads_or(descend);
+  __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const int R = a.rows_tok, G = a.group;
@@ -1403,7 +1403,7 @@ __global__ void __launch_bounds__(TokenCfg<HD, NP>::THREADS, 1)
       ++n;
       return true;
     };
-    if (!descend) ok = flash_even(a, lane, prefix, prefix + Cfg::MAX_SEQS, publish);
+    ok = flash_even(a, lane, prefix, prefix + Cfg::MAX_SEQS, publish);
     FlashEntry end{};
     if (ok) ok = publish(end);
   } else if (warp == W_LOAD) {
@@ -1544,7 +1544,7 @@ __global__ void __launch_bounds__(TokenCfg<HD, NP>::THREADS, 1)
         if (!ok) break;
       }
       if (!ok) {
-        report(status_word(a), code);
+        report(a.status, code);
         *abort_flag = 1;
       }
     }
@@ -1718,7 +1718,7 @@ __global__ void __launch_bounds__(TokenCfg<HD, NP>::THREADS, 1)
     }
   }
   if (!ok) {
-    report(status_word(a), code);
+    report(a.status, code);
     *abort_flag = 1;
   }
   tc_fence_before();
