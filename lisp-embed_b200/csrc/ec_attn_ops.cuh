@@ -519,9 +519,9 @@ __device__ __noinline__ void flash_join(const FlashArgs& a, int tok0, int qv, in
 }
 
 // Counts a finished part; true in the CTA that finished the last one, which
-// leaves the count at 0 for the next call.  By one thread, after all threads
-// have written the part and fenced: what they wrote is released by this
-// thread's fence between meeting them and counting.
+// leaves the count at 0 for the next call.  By one thread, once it has met all
+// threads that wrote the part: its fence between the meeting and the count
+// releases what they wrote.
 __device__ __forceinline__ bool flash_arrive(const FlashArgs& a, const FlashEntry& it) {
   __threadfence();
   const bool last = atomicAdd(&a.arrived[it.c0], 1) == it.parts - 1;
@@ -1185,7 +1185,6 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
         __syncwarp();
       }
       if (NT == 1 && it.part >= 0) {
-        __threadfence();
         auto meet = [&]() -> bool {  // the four warps
           __syncwarp();
           if (lane == 0) mbar_arrive(&x_bar[x & 1]);
@@ -1707,7 +1706,6 @@ __global__ void __launch_bounds__(TokenCfg<HD, NP>::THREADS, 1)
       }
       __syncwarp();
       if (it.part >= 0) {
-        __threadfence();
         exchange(0.f, all);  // every warp has written its share
         if (!ok) break;
         exchange(warp == 0 && lane == 0 && flash_arrive(a, it) ? 1.f : 0.f, all);
