@@ -263,6 +263,12 @@ int run_attention(const AttnOp& op, int num_sms, cudaStream_t st) {
 
 namespace {
 
+int check_heads(int q_heads, int kv_heads) {
+  if (q_heads < 1 || kv_heads < 1 || q_heads > 1024 || q_heads % kv_heads || q_heads / kv_heads > 128)
+    return set_error(EC_EINVAL, "%d query heads over %d key heads (a multiple of at most 128)", q_heads, kv_heads);
+  return EC_OK;
+}
+
 int check_attention(AttnOp& op, int64_t tokens, int nseq, float scale) {
   if (op.dtype != EC_BF16 && op.dtype != EC_F16)
     return set_error(EC_EINVAL, "attention takes bf16 or f16, not dtype %d", op.dtype);
@@ -270,8 +276,7 @@ int check_attention(AttnOp& op, int64_t tokens, int nseq, float scale) {
     return set_error(EC_EINVAL, "bad token or sequence count");
   if (op.head_dim < 8 || op.head_dim > 128 || op.head_dim % 8)
     return set_error(EC_EINVAL, "head_dim %d (supported: multiples of 8 up to 128)", op.head_dim);
-  if (op.q_heads < 1 || op.kv_heads < 1 || op.q_heads > 1024 || op.q_heads % op.kv_heads || op.q_heads / op.kv_heads > 128)
-    return set_error(EC_EINVAL, "%d query heads over %d key heads (a multiple of at most 128)", op.q_heads, op.kv_heads);
+  if (int rc = check_heads(op.q_heads, op.kv_heads)) return rc;
   if (!std::isfinite(scale) || scale < 0.f) return set_error(EC_EINVAL, "scale must be finite and >= 0 (0: 1 / sqrt(head_dim))");
   if (int rc = op_check_rows("q", op.q, tokens, op.q_heads, op.head_dim)) return rc;
   if (int rc = op_check_rows("out", op.out, tokens, op.q_heads, op.head_dim)) return rc;
@@ -324,8 +329,9 @@ extern "C" int64_t ec_attn_cached_work_size(int handle, int64_t tokens, int q_he
   clear_error();
   auto c = kv_find(handle);
   if (!c) return EC_EINVAL;
-  if (tokens < 0 || tokens > (1 << 30) || nseq < 0 || nseq > (1 << 24) || max_new < 0 || q_heads < 1 || q_heads % c->heads)
+  if (tokens < 0 || tokens > (1 << 30) || nseq < 0 || nseq > (1 << 24) || max_new < 0)
     return set_error(EC_EINVAL, "bad attention shape");
+  if (int rc = check_heads(q_heads, c->heads)) return rc;
   return static_cast<int64_t>(attention_work_bytes(*c, tokens, q_heads, nseq, max_new));
 }
 

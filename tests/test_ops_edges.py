@@ -1,0 +1,36 @@
+"""Refusals of the operators on device buffers at the edges of their ranges;
+none of these calls needs a GPU (pointers are never followed)."""
+import os
+import subprocess
+import sys
+
+import pytest
+import torch
+
+from conftest import REPO
+from embedcuda import _lib, ops
+from test_ops import L, open_, refused
+
+
+def test_work_size_of_more_heads_than_a_tile_has_rows():
+    """In a process of its own: a division by zero would end this one."""
+    code = ("import sys, os, ctypes as C; sys.path[:0] = [%r, os.path.join(%r, 'lisp-embed_b200'), %r];"
+            "from test_ops import L, open_; rc, h = open_(heads=1); assert rc == 0;"
+            "print([L().ec_attn_cached_work_size(h, 4, q, 1, 4) for q in (129, 256, 1024, 2048, 1 << 30)])"
+            ) % (REPO, REPO, os.path.join(REPO, "tests"))
+    out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0, (out.returncode, out.stderr)
+    assert out.stdout.strip() == str([_lib.EC_EINVAL] * 5)
+
+
+def test_work_size_takes_what_the_call_takes():
+    for heads, most in ((1, 128), (4, 512), (16, 1024)):
+        rc, h = open_(heads=heads)
+        assert rc == 0
+        assert L().ec_attn_cached_work_size(h, 4, most, 1, 4) > 0
+        refused(L().ec_attn_cached_work_size(h, 4, most + heads, 1, 4), "query heads")
+        refused(L().ec_attn_cached_work_size(h, 4, 0, 1, 4), "query heads")
+        if heads > 1:
+            refused(L().ec_attn_cached_work_size(h, 4, most - 1, 1, 4), "query heads")
+        refused(L().ec_attn_cached_work_size(h, -1, most, 1, 4), "shape")
+        assert L().ec_kv_close(h) == 0
