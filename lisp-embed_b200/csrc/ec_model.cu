@@ -283,7 +283,8 @@ static int load_bert(Device& d, const JVal& cfg, const std::string& mt, int pool
   return EC_OK;
 }
 
-static int load_llama(Device& d, const JVal& cfg) {
+// q/k norms belong to qwen3 (`normed`); other types take what was uploaded with them
+static int load_llama(Device& d, const JVal& cfg, bool normed) {
   ModelW& m = d.model;
   int rc;
   if ((rc = cfg_int(cfg, "hidden_size", &m.H)) || (rc = cfg_int(cfg, "num_hidden_layers", &m.layers)) ||
@@ -359,9 +360,9 @@ static int load_llama(Device& d, const JVal& cfg) {
       return rc;
     const Tensor* qn = find_t(d, pf + "self_attn.q_norm.weight");  // get-tensor-opt
     const Tensor* kn = find_t(d, pf + "self_attn.k_norm.weight");
-    // uploads stay: a norm that was there before all the rest of the layer was
-    // uploaded again is an earlier model's
-    int since = in->model;
+    // uploads stay: of another type than qwen3, a norm that was there before all
+    // the rest of the layer was uploaded again is an earlier model's
+    int since = normed ? 0 : in->model;
     for (const Tensor* t : {post, qw, kw, vw, ow, gw, uw, dw}) since = std::min(since, t->model);
     if (qn && qn->model < since) qn = nullptr;
     if (kn && kn->model < since) kn = nullptr;
@@ -561,7 +562,7 @@ int load_model_on(Device& d, const JVal& cfg, const JVal* pool) {
     rc = load_bert(d, cfg, mt, pooling);
   } else if (mt == "llama" || mt == "qwen2" || mt == "qwen3" || mt == "mistral" || mt == "gemma" ||
              mt == "gemma2") {
-    rc = load_llama(d, cfg);
+    rc = load_llama(d, cfg, mt == "qwen3");
   } else if (mt == "embedding_gemma2" || mt == "embedding_gemma2_text") {
     rc = load_gemma(d, tc && tc->kind == JVal::Obj ? *tc : cfg);  // model.lisp:41-43
   } else {
