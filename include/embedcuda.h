@@ -70,6 +70,10 @@ int ec_upload_tensor(const char *name, int dtype, const int64_t *shape, int ndim
  * model:load-model's dispatch (model.lisp:28-46) plus bert:load-model
  * (bert.lisp:55-129, 343-389), llama:load-model (llama.lisp:172-220) and
  * gemma:load-model (gemma.lisp:140-212).
+ * Llama models have heads of 128, or of another multiple of 8 up to 128 and no
+ * q/k norms.  With heads of 128 a rope_scaling in config.json is not read, as
+ * in llama.lisp:124-135; with others it is (linear, llama3, yarn; dynamic
+ * changes nothing within the positions; EC_EUNSUPPORTED for another type).
  * Writes the family (EC_FAMILY_*) and the embedding dimension. */
 int ec_load_model(const char *config_json, const char *pooling_json, int *family,
                   int *dim);

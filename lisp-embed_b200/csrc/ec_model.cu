@@ -283,6 +283,47 @@ static int load_bert(Device& d, const JVal& cfg, const std::string& mt, int pool
   return EC_OK;
 }
 
+// rope_scaling of config.json as ec_rope_table takes it, which refuses what is
+// missing or out of range
+struct RopeScaling {
+  int code = EC_ROPE_NONE;
+  double factor = 1.0, p0 = 0.0, p1 = 0.0, original = 0.0, amplitude = 0.0;
+};
+static int cfg_rope_scaling(const JVal& cfg, int max_pos, RopeScaling* out) {
+  const JVal* r = cfg.get("rope_scaling");
+  if (!r || !r->truthy()) return EC_OK;
+  const JVal* ty = r->get("rope_type") ? r->get("rope_type") : r->get("type");
+  if (!ty || ty->kind != JVal::Str) return set_error(EC_EINVAL, "rope_scaling has no rope_type");
+  auto num = [](const JVal& in, const char* key, double missing) {
+    const JVal* v = in.get(key);
+    return v && v->is_num() ? v->num() : missing;
+  };
+  const double positions = num(cfg, "max_position_embeddings", 0.0);
+  const std::string& type = ty->s;
+  if (type == "default") return EC_OK;
+  if (type == "dynamic" && positions >= max_pos) return EC_OK;  // scales only behind those positions
+  out->factor = num(*r, "factor", 0.0);
+  out->original = num(*r, "original_max_position_embeddings", type == "yarn" ? positions : 0.0);
+  if (type == "linear") {
+    out->code = EC_ROPE_LINEAR;
+  } else if (type == "llama3") {
+    out->code = EC_ROPE_LLAMA3;
+    out->p0 = num(*r, "low_freq_factor", 0.0);
+    out->p1 = num(*r, "high_freq_factor", 0.0);
+  } else if (type == "yarn") {
+    const JVal* whole = r->get("truncate");  // the pairs' range in whole pairs
+    if ((whole && !whole->truthy()) || num(*r, "mscale", 0.0) != 0.0 || num(*r, "mscale_all_dim", 0.0) != 0.0)
+      return set_error(EC_EUNSUPPORTED, "rope_scaling yarn with truncate false or mscale");
+    out->code = EC_ROPE_YARN;
+    out->p0 = num(*r, "beta_fast", 32.0);
+    out->p1 = num(*r, "beta_slow", 1.0);
+    out->amplitude = num(*r, "attention_factor", 0.0);
+  } else {
+    return set_error(EC_EUNSUPPORTED, "rope_scaling of type %s", type.c_str());
+  }
+  return EC_OK;
+}
+
 // q/k norms belong to qwen3 (`normed`); other types take what was uploaded with them
 static int load_llama(Device& d, const JVal& cfg, bool normed) {
   ModelW& m = d.model;
@@ -343,6 +384,14 @@ static int load_llama(Device& d, const JVal& cfg, bool normed) {
     return rc;
   m.cos_t = static_cast<float*>(dc);
   m.sin_t = static_cast<float*>(ds);
+  // llama.lisp knows no scaled frequencies, and head dim 128 stays with its
+  // table; models of other head dims are what their config.json says
+  RopeScaling rs;
+  if (m.hd != 128 && (rc = cfg_rope_scaling(cfg, m.max_pos, &rs))) return rc;
+  if (rs.code != EC_ROPE_NONE &&
+      (rc = ec_rope_table(m.cos_t, m.sin_t, m.max_pos, m.hd, m.theta, rs.code, rs.factor, rs.p0, rs.p1, rs.original,
+                          rs.amplitude, d.stream)))
+    return rc;
   m.ll.resize(m.layers);
   for (int li = 0; li < m.layers; ++li) {
     const std::string pf = "layers." + std::to_string(li) + ".";
