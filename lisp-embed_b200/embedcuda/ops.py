@@ -93,13 +93,27 @@ def _tables(cos, sin):
     return shape
 
 
+# keys of rope_scaling that a table is made by (a type has no use for the others'
+# keys), and those that say nothing about it (how much of a head is turned is
+# the tables' width)
+_SCALING = {"rope_type", "type", "factor", "low_freq_factor", "high_freq_factor", "beta_fast", "beta_slow",
+            "attention_factor", "original_max_position_embeddings", "finetuned", "partial_rotary_factor"}
+
+
 def rope_table(cos, sin, theta, scaling=None, stream=None):
     """Fill cos and sin float32[positions, rot_dim / 2].  ``scaling`` is
     config.json's rope_scaling (None, or rope_type linear / llama3 / yarn with
-    their keys)."""
+    their keys); a key that would change the table in another way is an error."""
     positions, half = _tables(cos, sin)
-    s = dict(scaling or {})
+    s = {k: v for k, v in (scaling or {}).items() if v is not None}
     kind = s.get("rope_type", s.get("type", "default" if not s else None))
+    if s.pop("rope_theta", theta) != theta:
+        raise ValueError(f"rope_scaling has another rope_theta than {theta}")
+    if s.get("truncate") is True:  # yarn's range in whole pairs
+        del s["truncate"]
+    unknown = [k for k in s if k not in _SCALING]
+    if unknown and kind in ("linear", "llama3", "yarn"):
+        raise ValueError(f"rope_scaling {kind} with {', '.join(unknown)}")
     factor, p0, p1, original, amp = 1.0, 0.0, 0.0, 0.0, 0.0
     if kind == "default":
         code = ROPE_NONE

@@ -34,3 +34,30 @@ def test_work_size_takes_what_the_call_takes():
             refused(L().ec_attn_cached_work_size(h, 4, most - 1, 1, 4), "query heads")
         refused(L().ec_attn_cached_work_size(h, -1, most, 1, 4), "shape")
         assert L().ec_kv_close(h) == 0
+
+
+@pytest.mark.parametrize("scaling,text", [
+    ({"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 4096, "truncate": False}, "truncate"),
+    ({"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 4096, "mscale": 0.707,
+      "mscale_all_dim": 0.7}, "mscale, mscale_all_dim"),
+    ({"rope_type": "llama3", "factor": 8.0, "low_freq_factor": 1.0, "high_freq_factor": 4.0,
+      "original_max_position_embeddings": 8192, "short_factor": [1.0]}, "short_factor"),
+    ({"rope_type": "linear", "factor": 4.0, "rope_theta": 1e6}, "rope_theta"),
+])
+def test_rope_scaling_that_would_be_dropped(scaling, text):
+    cos = torch.zeros(16, 32)
+    with pytest.raises(ValueError, match=text):
+        ops.rope_table(cos, cos, 1e4, scaling, stream=0)
+
+
+@pytest.mark.parametrize("scaling", [
+    {"rope_type": "default", "rope_theta": 1e4, "factor": 4.0}, {"rope_type": "linear", "factor": 4.0, "beta_fast": 32},
+    {"type": "yarn", "factor": 4.0, "original_max_position_embeddings": 4096, "finetuned": True, "truncate": True,
+     "attention_factor": None},
+    {"type": "linear", "factor": 4.0, "original_max_position_embeddings": 4096, "partial_rotary_factor": 0.5}])
+def test_rope_scaling_that_says_nothing_more(scaling):
+    """Taken: what refuses the call is that the tables are in host memory (or
+    that there is no GPU to ask)."""
+    cos = torch.zeros(16, 32)
+    with pytest.raises(_lib.EcError):
+        ops.rope_table(cos, cos, 1e4, scaling, stream=0)
