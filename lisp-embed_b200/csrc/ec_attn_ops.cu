@@ -232,7 +232,6 @@ int run_attention(const AttnOp& op, int num_sms, cudaStream_t st) {
     a.pages = c->pages, a.page_size = c->page_size;
     a.page0 = op.layer * c->pages, a.page_end = c->layers * c->pages;
   }
-  a.q_bufs = p.kind == kTiles && group * p.rows_tok <= 64 ? 2 : 1;
   const int sets = p.rows_tok * (p.kind == kPairs || p.kind == kHalves ? 2 : 1);
   int64_t grid = (op.tokens / sets + op.nseq) * op.kv_heads;
   if (grid >= INT32_MAX / 2)

@@ -63,7 +63,6 @@ struct FlashArgs {
   float scale_log2;
   int paged;
   int wide;                // out rows in 32-byte pieces
-  int q_bufs;              // 2: queries are double-buffered (NT 1, at most 64 rows)
   int even;                // 1: the blocks are split evenly over the CTAs
   int min_chunk;           // units a CTA takes at least
   int over;                // units of a tile besides its blocks
@@ -97,10 +96,6 @@ constexpr int kFmaEvery = 4;
 
 // work-list entries in flight
 constexpr int kFlashRing = 3;
-// Second query buffer of NT 1: 64 rows of 128 bytes after the first.  A tile's
-// operand is 128 rows all the same; what the rest reads (the other buffer, or
-// keys) only reaches rows of S and O that belong to no query.
-constexpr uint32_t kQBuf = 64 * 128;
 
 // a list of whole tiles counts its sets in this many groups of sequences, up
 // to kFlashCounted sequences
@@ -551,9 +546,9 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
   uint8_t* sQ = smem;
   uint8_t* sKV = sQ + NT * Cfg::TILE;
   uint8_t* tail = sKV + ST * Cfg::TILE;
-  uint64_t* q_full = reinterpret_cast<uint64_t*>(tail);  // [2]
-  uint64_t* q_empty = q_full + 2;     // [2]
-  uint64_t* kv_full = q_empty + 2;
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(tail);
+  uint64_t* q_empty = q_full + 1;
+  uint64_t* kv_full = q_empty + 1;
   uint64_t* kv_empty = kv_full + ST;
   uint64_t* s_full = kv_empty + ST;   // [2] tile (NT 2) or buffer (NT 1)
   uint64_t* p_full = s_full + 2;      // [2]
@@ -572,7 +567,7 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
   int* prefix = reinterpret_cast<int*>(tail + 1536);  // [MAX_SEQS] of an even split
   float* inverse = reinterpret_cast<float*>(tail + 1536);  // [2][128] 1 / l (NT 2)
   int* groups = reinterpret_cast<int*>(tail + 1536 + (NT == 1 ? 0 : 1024));  // [kFlashGroups] of a list
-  static_assert(8 * (4 + 2 * ST + 14 + 2 * kFlashRing) + kFlashRing * sizeof(FlashItem) + 16 <= 1536, "tail");
+  static_assert(8 * (2 + 2 * ST + 14 + 2 * kFlashRing) + kFlashRing * sizeof(FlashItem) + 16 <= 1536, "tail");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -580,9 +575,9 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
       mbar_init(&kv_full[i], 1);
       mbar_init(&kv_empty[i], 1);
     }
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&q_full[i], 1);
-      mbar_init(&q_empty[i], 1);
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
       mbar_init(&p_half[i], 4);
@@ -793,20 +788,18 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
           if (j == kb0 && kv == 0) {
             // the queries, once the tiles before have no more use for theirs;
             // rows past the tokens of the call are filled with zeros
-            const int qb = a.q_bufs == 2 ? qi & 1 : 0;
-            const uint32_t qp = (a.q_bufs == 2 ? qi >> 1 : qi) & 1;
+            if (!(ok = mbar_wait_warp(q_empty, (qi & 1) ^ 1, abort_flag))) break;
             ++qi;
-            if (!(ok = mbar_wait_warp(&q_empty[qb], qp ^ 1, abort_flag))) break;
             if (elect_one()) {
-              mbar_arrive_expect_tx(&q_full[qb], NT * AT * static_cast<uint32_t>(G * R) * 128u);
+              mbar_arrive_expect_tx(q_full, NT * AT * static_cast<uint32_t>(G * R) * 128u);
 #pragma unroll
               for (int t = 0; t < NT; ++t)
 #pragma unroll
                 for (int c = 0; c < AT; ++c)
                   asm volatile(
                       "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], "
-                      "[%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(sQ + qb * kQBuf + t * Cfg::TILE + c * Cfg::ATOM)),
-                      "l"(reinterpret_cast<uint64_t>(&tm_q)), "r"(smem_u32(&q_full[qb])), "r"(c * 64), "r"(kvh * G),
+                      "[%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(sQ + t * Cfg::TILE + c * Cfg::ATOM)),
+                      "l"(reinterpret_cast<uint64_t>(&tm_q)), "r"(smem_u32(q_full)), "r"(c * 64), "r"(kvh * G),
                       "r"(tok0 + t * R)
                       : "memory");
             }
@@ -842,8 +835,8 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
           ph ^= 1;
         }
       };
-      auto mma_s = [&](int qb, int t, int stage, uint32_t d, bool half) {
-        const uint64_t q = dq + qb * (kQBuf >> 4) + t * (Cfg::TILE >> 4), k = dk + stage * (Cfg::TILE >> 4);
+      auto mma_s = [&](int t, int stage, uint32_t d, bool half) {
+        const uint64_t q = dq + t * (Cfg::TILE >> 4), k = dk + stage * (Cfg::TILE >> 4);
 #pragma unroll
         for (int kk = 0; kk < HD / 16; ++kk) {
           const uint32_t off = ((kk >> 2) * Cfg::ATOM + (kk & 3) * 32) >> 4;
@@ -877,16 +870,16 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
         // the first scores of the item taken last, tile t
         auto begin = [&](int t) -> bool {
           if (t == 0) {
-            if (!wait(&q_full[0], qi & 1) || !wait(&kv_full[st], ph)) return false;
+            if (!wait(q_full, qi & 1) || !wait(&kv_full[st], ph)) return false;
             ++qi;
           }
           if ((t ? n1 : n0) > 0) {
-            mma_s(0, t, st, tmem + t * 128, one_half(t ? k1 : k0, 0));
+            mma_s(t, st, tmem + t * 128, one_half(t ? k1 : k0, 0));
             umma_commit(&s_full[t]);
           }
           if (t == 1) {
             umma_commit(&kv_empty[st]);
-            if (max(n0, n1) == 1) umma_commit(&q_empty[0]);
+            if (max(n0, n1) == 1) umma_commit(q_empty);
             advance();
           }
           return true;
@@ -923,7 +916,7 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
               if (j + 1 < nt) {
                 if (!have_k && !(ok = wait(&kv_full[st], ph))) continue;
                 have_k = true;
-                mma_s(0, t, st, tmem + t * 128, one_half(t ? e1 : e0, j + 1));
+                mma_s(t, st, tmem + t * 128, one_half(t ? e1 : e0, j + 1));
                 umma_commit(&s_full[t]);
               }
               if (j + 1 == n) {
@@ -936,7 +929,7 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
             if (!ok) break;
             if (j + 1 < n) {
               umma_commit(&kv_empty[st]);
-              if (j + 2 == n) umma_commit(&q_empty[0]);
+              if (j + 2 == n) umma_commit(q_empty);
               advance();
             }
           }
@@ -944,14 +937,14 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
       }
       while (NT == 1) {
         if (!(ok = take()) || !more) break;
-        const int n = n0, qb = a.q_bufs == 2 ? qi & 1 : 0;
-        if (!(ok = wait(&q_full[qb], (a.q_bufs == 2 ? qi >> 1 : qi) & 1)) || !(ok = wait(&kv_full[st], ph))) break;
+        const int n = n0;
+        if (!(ok = wait(q_full, qi & 1)) || !(ok = wait(&kv_full[st], ph))) break;
         ++qi;
         {
-          mma_s(qb, 0, st, tmem + (g & 1) * 128, one_half(k0, 0));
+          mma_s(0, st, tmem + (g & 1) * 128, one_half(k0, 0));
           umma_commit(&s_full[g & 1]);
           umma_commit(&kv_empty[st]);
-          if (n == 1) umma_commit(&q_empty[qb]);
+          if (n == 1) umma_commit(q_empty);
           advance();
 #pragma unroll 1
           for (int j = 0; j < n; ++j, ++g) {
@@ -960,10 +953,10 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
             advance();
             if (j + 1 < n) {
               if (!(ok = wait(&kv_full[st], ph))) break;
-              mma_s(qb, 0, st, tmem + ((g + 1) & 1) * 128, one_half(k0, j + 1));
+              mma_s(0, st, tmem + ((g + 1) & 1) * 128, one_half(k0, j + 1));
               umma_commit(&s_full[(g + 1) & 1]);
               umma_commit(&kv_empty[st]);
-              if (j + 2 == n) umma_commit(&q_empty[qb]);
+              if (j + 2 == n) umma_commit(q_empty);
               advance();
             }
             if (!(ok = wait(&kv_full[sv], phv)) || !(ok = wait(&p_half[g & 1], (g >> 1) & 1))) break;
