@@ -61,13 +61,11 @@ class PlainLaunch {
   bool before_, plain_;
 };
 
-// kernel `id` (its shared memory is set once per device)
-int launch_one(int id, FlashFn fn, int threads, size_t smem, const CUtensorMap& q, const CUtensorMap& k,
+// kernel `id` on device `dev` (its shared memory is set once per device)
+int launch_one(int dev, int id, FlashFn fn, int threads, size_t smem, const CUtensorMap& q, const CUtensorMap& k,
                const CUtensorMap& v, const FlashArgs& a, int grid, cudaStream_t st) {
   static std::mutex mu;
   static uint32_t set[64] = {};
-  int dev = 0;
-  if (int rc = check_cuda(cudaGetDevice(&dev), "cudaGetDevice")) return rc;
   {
     std::lock_guard<std::mutex> lk(mu);
     if (!(set[dev] >> id & 1)) {
@@ -85,31 +83,31 @@ int launch_one(int id, FlashFn fn, int threads, size_t smem, const CUtensorMap& 
 enum FlashKind { kPairs, kHalves, kTiles, kFew32, kFew16, kFew8, kFew4 };
 
 template <int HD, int NP, typename T>
-int launch_token(int id, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const FlashArgs& a, int grid,
+int launch_token(int dev, int id, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const FlashArgs& a, int grid,
                  cudaStream_t st) {
   using Cfg = TokenCfg<HD, NP>;
-  return launch_one(id, flash_token_kernel<HD, NP, T>, Cfg::THREADS, Cfg::SMEM, q, k, v, a, grid, st);
+  return launch_one(dev, id, flash_token_kernel<HD, NP, T>, Cfg::THREADS, Cfg::SMEM, q, k, v, a, grid, st);
 }
 
 template <int HD, typename T>
-int launch_flash(FlashKind kind, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const FlashArgs& a,
+int launch_flash(int dev, FlashKind kind, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const FlashArgs& a,
                  int grid, cudaStream_t st) {
   const int id = (HD == 64 ? 0 : 16) + (std::is_same<T, __half>::value ? 8 : 0) + kind;
   int rc;
   switch (kind) {
     case kPairs:
-      rc = launch_one(id, flash_kernel<HD, 2, false, T>, FlashCfg<HD, 2>::THREADS, FlashCfg<HD, 2>::SMEM, q, k, v, a, grid, st);
+      rc = launch_one(dev, id, flash_kernel<HD, 2, false, T>, FlashCfg<HD, 2>::THREADS, FlashCfg<HD, 2>::SMEM, q, k, v, a, grid, st);
       break;
     case kHalves:
-      rc = launch_one(id, flash_kernel<HD, 2, true, T>, FlashCfg<HD, 2>::THREADS, FlashCfg<HD, 2>::SMEM, q, k, v, a, grid, st);
+      rc = launch_one(dev, id, flash_kernel<HD, 2, true, T>, FlashCfg<HD, 2>::THREADS, FlashCfg<HD, 2>::SMEM, q, k, v, a, grid, st);
       break;
     case kTiles:
-      rc = launch_one(id, flash_kernel<HD, 1, true, T>, FlashCfg<HD, 1>::THREADS, FlashCfg<HD, 1>::SMEM, q, k, v, a, grid, st);
+      rc = launch_one(dev, id, flash_kernel<HD, 1, true, T>, FlashCfg<HD, 1>::THREADS, FlashCfg<HD, 1>::SMEM, q, k, v, a, grid, st);
       break;
-    case kFew32: rc = launch_token<HD, 32, T>(id, q, k, v, a, grid, st); break;
-    case kFew16: rc = launch_token<HD, 16, T>(id, q, k, v, a, grid, st); break;
-    case kFew8: rc = launch_token<HD, 8, T>(id, q, k, v, a, grid, st); break;
-    default: rc = launch_token<HD, 4, T>(id, q, k, v, a, grid, st);
+    case kFew32: rc = launch_token<HD, 32, T>(dev, id, q, k, v, a, grid, st); break;
+    case kFew16: rc = launch_token<HD, 16, T>(dev, id, q, k, v, a, grid, st); break;
+    case kFew8: rc = launch_token<HD, 8, T>(dev, id, q, k, v, a, grid, st); break;
+    default: rc = launch_token<HD, 4, T>(dev, id, q, k, v, a, grid, st);
   }
   return rc;
 }
@@ -168,11 +166,9 @@ size_t attention_work_bytes(const KvCache& c, int64_t tokens, int q_heads, int n
 namespace {
 thread_local unsigned* t_status_word = nullptr;
 
-// the current device's word that ec_op_status asks
-int caller_status_word(unsigned** word) {
+// the word that ec_op_status asks on device `dev`, the current one
+int caller_status_word(int dev, unsigned** word) {
   static std::atomic<unsigned*> words[64] = {};
-  int dev = 0;
-  if (int rc = check_cuda(cudaGetDevice(&dev), "cudaGetDevice")) return rc;
   *word = words[dev].load(std::memory_order_relaxed);
   if (*word) return EC_OK;
   void* p = nullptr;
@@ -194,9 +190,9 @@ size_t attention_work_most(int head_dim) {
 
 int attention_counts() { return kMaxCtas; }
 
-int run_attention(const AttnOp& op, int num_sms, cudaStream_t st) {
+int run_attention(const AttnOp& op, cudaStream_t st) {
   const KvCache* c = op.cache;
-  num_sms = std::min(num_sms, kMaxCtas);
+  const int num_sms = std::min(op.num_sms, kMaxCtas);
   const FlashPlan p = flash_plan(c, op.tokens, op.q_heads, op.kv_heads, op.nseq, op.max_new, num_sms);
   const int group = op.q_heads / op.kv_heads, hd = op.head_dim <= 64 ? 64 : 128;
   CUtensorMap tq, tk, tv;
@@ -220,7 +216,7 @@ int run_attention(const AttnOp& op, int num_sms, cudaStream_t st) {
   a.lse = op.lse;
   a.status = t_status_word;
   if (!a.status)
-    if (int rc = caller_status_word(&a.status)) return rc;
+    if (int rc = caller_status_word(op.device, &a.status)) return rc;
   a.cu = op.cu, a.slots = op.slots;
   a.tokens = static_cast<int>(op.tokens), a.nseq = op.nseq;
   a.group = group, a.rows_tok = p.rows_tok, a.q_heads = op.q_heads, a.kv_heads = op.kv_heads;
@@ -254,10 +250,10 @@ int run_attention(const AttnOp& op, int num_sms, cudaStream_t st) {
   const int ctas = static_cast<int>(std::min<int64_t>(grid, num_sms));
   const PlainLaunch launch((p.kind == kPairs || p.kind == kHalves) && op.nseq > kFlashFew);
   if (op.dtype == EC_BF16)
-    return hd == 64 ? launch_flash<64, __nv_bfloat16>(p.kind, tq, tk, tv, a, ctas, st)
-                    : launch_flash<128, __nv_bfloat16>(p.kind, tq, tk, tv, a, ctas, st);
-  return hd == 64 ? launch_flash<64, __half>(p.kind, tq, tk, tv, a, ctas, st)
-                  : launch_flash<128, __half>(p.kind, tq, tk, tv, a, ctas, st);
+    return hd == 64 ? launch_flash<64, __nv_bfloat16>(op.device, p.kind, tq, tk, tv, a, ctas, st)
+                    : launch_flash<128, __nv_bfloat16>(op.device, p.kind, tq, tk, tv, a, ctas, st);
+  return hd == 64 ? launch_flash<64, __half>(op.device, p.kind, tq, tk, tv, a, ctas, st)
+                  : launch_flash<128, __half>(op.device, p.kind, tq, tk, tv, a, ctas, st);
 }
 
 namespace {
@@ -321,7 +317,8 @@ extern "C" int ec_attn_prompt(const void* q, int64_t q_token, int64_t q_head, co
   op.scale = scale > 0.f ? scale : 1.f / std::sqrt(static_cast<float>(head_dim));
   OpDevice dev;
   if (int rc = dev.enter({q, k, v, out, lse, cu})) return rc;
-  return run_attention(op, dev.num_sms(), static_cast<cudaStream_t>(stream));
+  op.device = dev.ordinal(), op.num_sms = dev.num_sms();
+  return run_attention(op, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int64_t ec_attn_cached_work_size(int handle, int64_t tokens, int q_heads, int nseq, int max_new) {
@@ -358,5 +355,6 @@ extern "C" int ec_attn_cached(int handle, int layer, const void* q, int64_t q_to
   op.scale = scale > 0.f ? scale : 1.f / std::sqrt(static_cast<float>(c->head_dim));
   OpDevice dev;
   if (int rc = kv_enter(dev, *c, {q, out, lse, cu, slots, work})) return rc;
-  return run_attention(op, dev.num_sms(), static_cast<cudaStream_t>(stream));
+  op.device = dev.ordinal(), op.num_sms = dev.num_sms();
+  return run_attention(op, static_cast<cudaStream_t>(stream));
 }

@@ -41,6 +41,8 @@
 
 #include <cuda_fp16.h>
 
+#include <climits>
+
 #include "ec_fa.cuh"
 #include "ec_ops.h"
 #include "ec_ptx.cuh"
@@ -343,17 +345,15 @@ template <typename Publish>
 __device__ __noinline__ bool flash_even(const FlashArgs& a, int lane, int* prefix, const int* about, Publish publish) {
   const int R = a.rows_tok, ctas = gridDim.x, me = blockIdx.x;
   int tiles = 0, most = 0, work = 0;
-  bool descend = false;
   for (int s = lane; s < a.nseq; s += 32) {
     work += prefix[s];
-    descend |= prefix[s] < 0;
     tiles += about[s] & 0xffff;
-    most = max(most, about[s] >> 16 & kLongestMost);
+    most = max(most, prefix[s] < 0 ? INT_MAX : about[s] >> 16 & kLongestMost);
   }
   tiles = __reduce_add_sync(0xffffffffu, min(tiles, 1 << 20));
   most = __reduce_max_sync(0xffffffffu, most);
   work = __reduce_add_sync(0xffffffffu, work);
-  if (__any_sync(0xffffffffu, descend)) return true;
+  if (most == INT_MAX) return true;  // offsets that descend
   // every tile, padded to the longest, its own CTA
   const bool alone = tiles <= ctas && most < kLongestMost && most <= work / ctas + 8 + a.part_rows / 10;
   int total = 0;

@@ -90,8 +90,9 @@ struct AttnOp {
   int max_new;
   void* work;
   size_t work_bytes;
+  int device, num_sms;  // of the call (OpDevice)
 };
-int run_attention(const AttnOp& op, int num_sms, cudaStream_t st);
+int run_attention(const AttnOp& op, cudaStream_t st);
 size_t attention_work_bytes(const KvCache& c, int64_t tokens, int q_heads, int nseq, int max_new);
 // While one lives, this thread's attention calls mark `word` (of the call's
 // device) when a wait gives up, not the word that ec_op_status asks: a forward
