@@ -662,7 +662,8 @@ extern "C" int ec_kv_write(int handle, int layer, const void* k, int64_t k_token
   auto c = kv_find(handle);
   if (!c) return EC_EINVAL;
   if (layer < 0 || layer >= c->layers) return set_error(EC_EINVAL, "layer %d of %d", layer, c->layers);
-  if (tokens < 0 || tokens > INT32_MAX || nseq < 0) return set_error(EC_EINVAL, "bad token or sequence count");
+  // (more sequences than any cache has slots; the search adds such counts)
+  if (tokens < 0 || tokens > INT32_MAX || nseq < 0 || nseq > (1 << 30)) return set_error(EC_EINVAL, "bad token or sequence count");
   OpRows kr{k, k_token, k_head}, vr{v, v_token, v_head};
   if (int rc = op_check_rows("k", kr, tokens, c->heads, c->head_dim)) return rc;
   if (int rc = op_check_rows("v", vr, tokens, c->heads, c->head_dim)) return rc;

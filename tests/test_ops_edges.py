@@ -61,3 +61,12 @@ def test_rope_scaling_that_says_nothing_more(scaling):
     cos = torch.zeros(16, 32)
     with pytest.raises(_lib.EcError):
         ops.rope_table(cos, cos, 1e4, scaling, stream=0)
+
+
+def test_write_of_more_sequences_than_the_search_counts():
+    rc, h = open_()
+    assert rc == 0
+    for nseq in (-1, (1 << 30) + 1, (1 << 31) - 1):
+        refused(L().ec_kv_write(h, 0, 1 << 20, 256, 64, 1 << 20, 256, 64, 4, None, None, nseq, None), "count")
+    refused(L().ec_kv_write(h, 0, 1 << 20, 256, 64, 1 << 20, 256, 64, 4, None, None, 1 << 30, None), "cu is NULL")
+    assert L().ec_kv_close(h) == 0
