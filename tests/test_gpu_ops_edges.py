@@ -161,3 +161,25 @@ def test_cache_lists_of_the_host_are_refused(ops):
         assert c.status.tolist() == [0, 0]
     with pytest.raises(ValueError, match="tables is on cpu"):
         ops.KvCache(c.k, c.v, c.tables.cpu(), c.lens, c.refs)
+
+
+def test_compaction_past_32_bits(ops):
+    """The r-th page in use at or above their number goes to the r-th hole below
+    it: 9, 16500, 17000 and 17999 to 0, 1, 2 and 3, contents and table."""
+    layers, pages, page, hk, hd = 2, 18000, 128, 8, 128  # 2.36e9 elements a layer
+    k, v = (torch.empty(layers, pages, page, hk, hd, device="cuda", dtype=BF16) for _ in range(2))
+    mine = [17999, 16500, 9, 17000]
+    for x, s in ((k, 1), (v, 2)):
+        x[:, mine] = rnd(layers, 4, page, hk, hd, dt=BF16, seed=s)
+    want = [x[:, mine].clone() for x in (k, v)]
+    tables, lens, refs = i32([mine + [-1]]), i32([450]), torch.zeros(pages, dtype=torch.int32, device="cuda")
+    refs[mine] = 1
+    h, status = ops.KvCache(k, v, tables, lens, refs), i32([9, 9])
+    h.compact(status)
+    assert status.tolist() == [0, 4]
+    assert tables.tolist() == [[3, 1, 0, 2, -1]] and lens.tolist() == [450]
+    assert refs.nonzero()[:, 0].tolist() == [0, 1, 2, 3] and refs[:4].tolist() == [1] * 4
+    for x, w in zip((k, v), want):
+        assert torch.equal(x[:, [3, 1, 0, 2]], w)
+    h.compact(status)
+    assert status.tolist() == [0, 0] and tables.tolist() == [[3, 1, 0, 2, -1]]
