@@ -213,6 +213,9 @@ int run_attention(const AttnOp& op, cudaStream_t st) {
   FlashArgs a{};
   a.out = const_cast<void*>(op.out.p), a.ot = op.out.token, a.oh = op.out.head;
   a.wide = op_aligned(a.out, 32) && a.ot % 16 == 0 && a.oh % 16 == 0 && op.head_dim % 16 == 0;
+  a.q = op.q.p, a.qt = op.q.token, a.qh = op.q.head;
+  a.k = c ? c->k : op.k.p, a.kt = op.k.token, a.kh = op.k.head;
+  a.v = c ? c->v : op.v.p, a.vt = op.v.token, a.vh = op.v.head;
   a.lse = op.lse;
   a.status = t_status_word;
   if (!a.status)

@@ -53,6 +53,8 @@ namespace ec {
 constexpr int kMaxCtas = 160;
 
 struct FlashArgs {
+  const void *q, *k, *v;   // rows, or the cache's pools: for rows that are computed again
+  int64_t qt, qh, kt, kh, vt, vh;  // their strides in elements
   void* out;
   float* lse;
   int64_t ot, oh;          // out strides in elements
@@ -157,6 +159,14 @@ __device__ __forceinline__ float2 exp2_fma(float2 x) {
                                    __uint_as_float(__float_as_uint(t.y) << 23)));
 }
 
+// acc + 0 * v, both halves: NaN once a value is not finite
+template <typename T>
+__device__ __forceinline__ uint32_t times_zero(uint32_t v, uint32_t acc) {
+  if constexpr (std::is_same<T, __half>::value) asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(acc) : "r"(v), "r"(0));
+  else asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(acc) : "r"(v), "r"(0));
+  return acc;
+}
+
 // 32 bytes to a 32-byte aligned address
 __device__ __forceinline__ void store32(void* p, const uint32_t* v) {
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
@@ -225,8 +235,9 @@ __device__ __forceinline__ void flash_count(const FlashArgs& a, int* groups, vol
     if (end > begin) atomicAdd(&groups[s / size], (end - begin + BT - 1) / BT);
   }
 }
+// (`summed`: the groups' sums are there already, their total in *sets)
 template <int NT, typename Publish>
-__device__ __noinline__ bool flash_slots(const FlashArgs& a, int lane, int* groups, Publish publish) {
+__device__ __noinline__ bool flash_slots(const FlashArgs& a, int lane, int* groups, int* sets, bool summed, const Publish& publish) {
   const int R = a.rows_tok, BT = NT * R;
   uint32_t slots = a.tokens / BT + a.nseq;
   const uint32_t step = gridDim.x;
@@ -239,7 +250,9 @@ __device__ __noinline__ bool flash_slots(const FlashArgs& a, int lane, int* grou
   }
   const bool counted = a.nseq > kFlashFew && a.nseq <= kFlashCounted;
   const int size = (a.nseq + kFlashGroups - 1) / kFlashGroups;
-  if (counted) {
+  if (counted && summed) {
+    slots = *sets;
+  } else if (counted) {
     int total = 0;
 #pragma unroll 1
     for (int g = lane; g < kFlashGroups; g += 32) {  // sets before each group
@@ -254,7 +267,7 @@ __device__ __noinline__ bool flash_slots(const FlashArgs& a, int lane, int* grou
       total += __shfl_sync(0xffffffffu, x, 31);
     }
     __syncwarp();
-    slots = total;
+    slots = *sets = total;
   }
   const uint32_t all = slots * a.kv_heads;
   bool ok = true;
@@ -513,6 +526,162 @@ __device__ __noinline__ void flash_join(const FlashArgs& a, int tok0, int qv, in
   }
 }
 
+// -------------------------------------------------- rows computed again --
+// A key that a row does not see has the probability 0, and 0 times an infinity
+// or a NaN among its values is NaN.  It can only lie in the blocks that the
+// row's tile cuts, at most 255 keys behind the row.  So a row whose result is
+// not finite, although its sum is, looks there; if such a value is found, the
+// row is computed again from the keys that it sees alone, by one warp, in fp32.
+// Finite inputs cost the look at the result, which no time shows.
+
+// row j of the keys (kv 0) or values (kv 1) of a packed sequence that starts at
+// kbase or of slot kbase; nullptr: a page that is none, which reads as zeros
+template <typename T>
+__device__ __forceinline__ const T* flash_key(const FlashArgs& a, int kv, int kbase, int kvh, int j) {
+  const T* base = static_cast<const T*>(kv ? a.v : a.k);
+  if (!a.paged) return base + static_cast<int64_t>(kbase + j) * (kv ? a.vt : a.kt) + kvh * (kv ? a.vh : a.kh);
+  const int p = a.tables[static_cast<int64_t>(kbase) * a.width + j / a.page_size];
+  if (p < 0 || p >= a.pages) return nullptr;
+  return base + ((static_cast<int64_t>(a.page0 + p) * a.page_size + j % a.page_size) * a.kv_heads + kvh) * a.head_dim;
+}
+__device__ __forceinline__ float2 unpack2(__nv_bfloat16, uint32_t v) {
+  return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
+}
+__device__ __forceinline__ float2 unpack2(__half, uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
+
+// Row of token `tok` and query head `head` over the keys [first, vis): elements
+// d0 + 32 e + lane, e < E, divided by the sum, to out (this lane's addresses
+// for e = 0 are out and part; part: a part of a cut tile).
+template <int E, typename T>
+__device__ __noinline__ void flash_row(const FlashArgs& a, int tok, int head, int kvh, int kbase, int first, int vis,
+                                       int d0, int lane, T* out, float* part) {
+  const uint4* q = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + tok * a.qt + head * a.qh);
+  float m = -INFINITY, l = 0.f, o[E] = {};
+#pragma unroll 1
+  for (int j0 = first; j0 < vis; j0 += 32) {
+    float s = -INFINITY;
+    if (j0 + lane < vis) {
+      const uint4* k = reinterpret_cast<const uint4*>(flash_key<T>(a, 0, kbase, kvh, j0 + lane));
+      s = 0.f;
+#pragma unroll 1
+      for (int i = 0; k && i < a.head_dim / 8; ++i) {
+        const uint4 x = q[i], y = k[i];
+        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const float2 f = unpack2(T(), xs[c]), g = unpack2(T(), ys[c]);
+          s = fmaf(f.x, g.x, fmaf(f.y, g.y, s));
+        }
+      }
+      s *= a.scale_log2;
+    }
+    float top = s;
+#pragma unroll
+    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    const float mn = fmaxf(m, top), base = mn == -INFINITY ? 0.f : mn, corr = exp2f(m - base);
+    float p = exp2f(s - base), sum = p;
+#pragma unroll
+    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    l = l * corr + sum;
+    m = mn;
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] *= corr;
+#pragma unroll 4
+    for (int i = 0; i < min(32, vis - j0); ++i) {
+      const T* v = flash_key<T>(a, 1, kbase, kvh, j0 + i);
+      const float w = __shfl_sync(0xffffffffu, p, i);
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (v && d0 + 32 * e + lane < a.head_dim) o[e] = fmaf(w, static_cast<float>(v[d0 + 32 * e + lane]), o[e]);
+    }
+    bool any = false;  // a row of which nothing is finite stays so
+#pragma unroll
+    for (int e = 0; e < E; ++e) any |= d0 + 32 * e + lane < a.head_dim && !isnan(o[e]);
+    if (!__any_sync(0xffffffffu, any)) break;
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const float v = l == 0.f ? 0.f : o[e] / l;
+    if (part) part[32 * e] = v;
+    else if (d0 + 32 * e + lane < a.head_dim) out[32 * e] = static_cast<T>(v);
+  }
+}
+
+// the last of the keys [from, to) with a value that is not finite, or -1
+template <typename T>
+__device__ __forceinline__ int flash_last_odd(const FlashArgs& a, int kbase, int kvh, int from, int to, int lane) {
+  constexpr uint32_t EXP = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+  int last = -1;
+#pragma unroll 1
+  for (int j = from + lane; j < to; j += 32) {
+    const uint4* v = reinterpret_cast<const uint4*>(flash_key<T>(a, 1, kbase, kvh, j));
+#pragma unroll 1
+    for (int i = 0; v && i < a.head_dim / 8; ++i) {
+      const uint4 x = v[i];
+      const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        if ((xs[c] & EXP) == EXP || (xs[c] >> 16 & EXP) == EXP) last = j;
+    }
+  }
+  return __reduce_max_sync(0xffffffffu, last);
+}
+
+// Rows base .. base + 31 of a tile of rows (token, head) whose first token is
+// tok0, at position pos: those of the lanes with `odd` are looked at, by the
+// whole warp.  Keys [first, end) of the slot or sequence; row: of the tile's
+// part, -1: whole.  Elements from d0 on, 32 E of them.
+template <int HD, int E, typename T>
+__device__ __noinline__ void flash_again(const FlashArgs& a, int tok0, int pos, int kvh, int kbase, int first, int end,
+                                         int base, bool odd, int part, int d0, int lane) {
+  const int vis = min(end, pos + (base + lane) / a.group + 1);
+  odd &= vis < end;
+  if (!__any_sync(0xffffffffu, odd)) return;
+  const int from = __reduce_min_sync(0xffffffffu, odd ? vis : end);
+  odd &= flash_last_odd<T>(a, kbase, kvh, from, end, lane) >= vis;
+  __syncwarp();  // the rows have been written
+#pragma unroll 1
+  for (unsigned rest = __ballot_sync(0xffffffffu, odd); rest; rest &= rest - 1) {
+    const int i = __ffs(rest) - 1, r = base + i, tok = tok0 + r / a.group, head = kvh * a.group + r % a.group;
+    T* out = static_cast<T*>(a.out) + tok * a.ot + head * a.oh + d0 + lane;
+    float* po = part < 0 ? nullptr : a.part_o + (static_cast<int64_t>(part) * a.part_rows + r) * HD + d0 + lane;
+    flash_row<E, T>(a, tok, head, kvh, kbase, first, __shfl_sync(0xffffffffu, vis, i), d0, lane, out, po);
+  }
+}
+
+// The list of pairs of tiles.  `finish` ends it and waits for the results; where
+// it says that one of them is not finite, the list's warp goes through the list
+// again and looks at them.  (The closures that go into functions out of line hold
+// copies: kernel variables that they held by reference lay in local memory for
+// all warps, 256 prompts of 71060 tokens 316 us instead of 280, one token of one
+// sequence 11.7 instead of 11.3.)
+template <int HD, typename T, typename Publish, typename Finish>
+__device__ __forceinline__ bool flash_pairs(const FlashArgs& a, int lane, int* groups, int* sets, bool empty,
+                                            const Publish& publish, Finish finish) {
+  bool ok = empty || flash_slots<2>(a, lane, groups, sets, false, publish);
+  if (!finish(ok)) return ok;
+  const int R = a.rows_tok;
+  return flash_slots<2>(a, lane, groups, sets, true, [&](const FlashEntry& mine, int from) -> bool {
+    auto of = [&](int v) { return __shfl_sync(0xffffffffu, v, from); };
+    const int tok0 = of(mine.tok0), qv = of(mine.qv), kvh = of(mine.kvh), pos0 = of(mine.pos0), kv_len = of(mine.kv_len);
+    const int kbase = of(mine.kbase), nb0 = of(mine.nb[0]), nb1 = of(mine.nb[1]);
+#pragma unroll 1
+    for (int r = 0; r < qv * a.group; ++r) {
+      const int tok = r / a.group, end = min(kv_len, (tok < R ? nb0 : nb1) * 128), vis = min(end, pos0 + tok + 1);
+      if (vis >= end) continue;
+      const int head = kvh * a.group + r % a.group;
+      T* out = static_cast<T*>(a.out) + (tok0 + tok) * a.ot + head * a.oh + lane;
+      bool odd = false;
+#pragma unroll
+      for (int e = 0; e < HD / 32; ++e)
+        if (32 * e + lane < a.head_dim) odd |= !(fabsf(static_cast<float>(out[32 * e])) < INFINITY);
+      if (__any_sync(0xffffffffu, odd) && flash_last_odd<T>(a, kbase, kvh, vis, end, lane) >= 0)
+        flash_row<HD / 32, T>(a, tok0 + tok, head, kvh, kbase, 0, vis, 0, lane, out, nullptr);
+    }
+    return true;
+  });
+}
+
 // Counts a finished part; true in the CTA that finished the last one, which
 // leaves the count at 0 for the next call.  By one thread, once it has met all
 // threads that wrote the part: its fence between the meeting and the count
@@ -523,6 +692,15 @@ __device__ __forceinline__ bool flash_arrive(const FlashArgs& a, const FlashEntr
   if (last) a.arrived[it.c0] = 0;
   __threadfence();
   return last;
+}
+
+// The end of the results (NT 2): the four warps that write them arrive, whether a
+// wait of theirs gave up or not, and the list's warp waits (in hardware: a warp
+// that polls takes turns from the softmax warps, 16384 tokens 534 -> 546 us).
+__device__ __forceinline__ void results_done(bool wait) {
+  __syncwarp();
+  if (wait) asm volatile("barrier.cta.sync 1, 160;" ::: "memory");
+  else asm volatile("barrier.cta.arrive 1, 160;" ::: "memory");
 }
 
 template <int HD, int NT, bool HALF, typename T>
@@ -564,10 +742,12 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* last_part = abort_flag + 1;
   volatile int* descend = last_part + 1;
+  volatile int* odd_rows = descend + 1;  // some result is not finite (NT 2)
+  int* sets = reinterpret_cast<int*>(tmem_slot + 5);  // of a counted list
   int* prefix = reinterpret_cast<int*>(tail + 1536);  // [MAX_SEQS] of an even split
   float* inverse = reinterpret_cast<float*>(tail + 1536);  // [2][128] 1 / l (NT 2)
   int* groups = reinterpret_cast<int*>(tail + 1536 + (NT == 1 ? 0 : 1024));  // [kFlashGroups] of a list
-  static_assert(8 * (2 + 2 * ST + 14 + 2 * kFlashRing) + kFlashRing * sizeof(FlashItem) + 16 <= 1536, "tail");
+  static_assert(8 * (2 + 2 * ST + 14 + 2 * kFlashRing) + kFlashRing * sizeof(FlashItem) + 24 <= 1536, "tail");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -592,6 +772,7 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
     }
     *abort_flag = 0;
     *descend = 0;
+    *odd_rows = 0;
     fence_barrier_init();
   }
   if (warp == W_LOAD && lane == 0) {
@@ -660,6 +841,8 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
     const int64_t row = it.tok0 + t * R + tok;
     T* o = static_cast<T*>(a.out) + row * a.ot + (it.kvh * G + r - tok * G) * a.oh;
     float* po = a.part_o + (static_cast<int64_t>(max(it.part, 0)) * a.part_rows + r) * HD;
+    float2 sum = make_float2(0.f, 0.f);  // finite if the row is (NT 1)
+    uint32_t zero = 0;                   // 0 if it is (NT 2)
 #pragma unroll 1
     for (int c = 0; c < HD / 32; ++c) {
       uint32_t v[32];
@@ -673,6 +856,11 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
         if (lane == 0) mbar_arrive(&o_free[t]);
       }
       if (live) {
+        if constexpr (NT == 1) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 2)
+            sum = __fadd2_rn(sum, make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])));
+        }
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = inv == 0.f ? 0u : __float_as_uint(__uint_as_float(v[i]) * inv);
         if (NT == 1 && it.part >= 0) {
@@ -681,6 +869,10 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
         } else {
 #pragma unroll
           for (int i = 0; i < 16; ++i) v[i] = pack2<T>(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+          if constexpr (NT == 2) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) zero = times_zero<T>(v[i], zero);
+          }
           if (a.wide) {
             if (c * 32 < a.head_dim) store32(o + c * 32, v);
             if (c * 32 + 16 < a.head_dim) store32(o + c * 32 + 16, v + 8);
@@ -694,6 +886,14 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
       }
       __syncwarp();  // the loads from TMEM are the whole warp's
     }
+    if constexpr (NT == 2) {
+      if (zero & 0x7fff7fffu) *odd_rows = 1;  // looked at by the list's warp, at the end
+    } else {
+      const bool odd = live && n > 0 && !(fabsf(sum.x + sum.y) < INFINITY);
+      if (__any_sync(0xffffffffu, odd))
+        flash_again<HD, HD / 32, T>(a, it.tok0, it.pos0, it.kvh, it.kbase, it.kb0 * 128, min(it.kv_len, it.nb[0] * 128),
+                                    (warp & 3) * 32, odd, it.part, 0, lane);
+    }
   };
 
   if constexpr (NT == 2) {
@@ -704,7 +904,7 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
     using Entry = FlashEntry;
     // ------------------------------------------------------------ work list
     int n = 0;
-    auto publish = [&](const Entry& it, int from) -> bool {  // lane `from`'s entry
+    auto publish = [=, &a, &n](const Entry& it, int from) -> bool {  // lane `from`'s entry
       const int b = n % kFlashRing;
       if (!mbar_wait_warp(&i_empty[b], ((n / kFlashRing) & 1) ^ 1, abort_flag)) return false;
       if (a.paged && __shfl_sync(0xffffffffu, it.valid, from)) {
@@ -718,14 +918,17 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
       ++n;
       return true;
     };
-    if (*descend) {
-    } else if (NT == 1 && a.even) {
-      ok = flash_even(a, lane, prefix, prefix + Cfg::MAX_SEQS, [&](const Entry& e) { return publish(e, 0); });
+    if constexpr (NT == 2) {
+      ok = flash_pairs<HD, T>(a, lane, groups, sets, *descend, publish, [=](bool& fine) -> bool {
+        fine = fine && publish(Entry{}, 0);
+        results_done(true);
+        return fine && *odd_rows && !*abort_flag;
+      });
     } else {
-      ok = flash_slots<NT>(a, lane, groups, publish);
+      if (a.even) ok = flash_even(a, lane, prefix, prefix + Cfg::MAX_SEQS, [=](const Entry& e) { return publish(e, 0); });
+      else if (!*descend) ok = flash_slots<NT>(a, lane, groups, sets, false, publish);
+      if (ok) ok = publish(Entry{}, 0);
     }
-    Entry end{};
-    if (ok) ok = publish(end, 0);
   } else if (warp == W_LOAD) {
     // ---------------------------------------------------------------- loads
     code = kDevTimeoutProducer;
@@ -1003,6 +1206,7 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
       }
       if (!ok) break;
     }
+    if (warp >= W_EPI) results_done(false);
   } else {
     // -------------------------------------------------------------- softmax
     if constexpr (NT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
@@ -1384,7 +1588,7 @@ __global__ void __launch_bounds__(TokenCfg<HD, NP>::THREADS, 1)
 
   if (warp == W_LIST) {
     int n = 0;
-    auto publish = [&](const FlashEntry& it) -> bool {
+    auto publish = [=, &a, &n](const FlashEntry& it) -> bool {
       const int b = n % kFlashRing;
       if (!mbar_wait_warp(&i_empty[b], ((n / kFlashRing) & 1) ^ 1, abort_flag)) return false;
       if (it.valid)
@@ -1696,6 +1900,18 @@ __global__ void __launch_bounds__(TokenCfg<HD, NP>::THREADS, 1)
         }
         to += a.oh;
         if (++head == G) head = 0, to += a.ot - G * a.oh;
+      }
+      const int keys = min(it.kv_len, it.nb[0] * 128);
+      if (it.pos0 + 1 < keys) {  // some keys are not seen by some rows
+        unsigned odd = 0;
+#pragma unroll
+        for (int i = 0; i < NP; ++i)
+          if (!(fabsf(__uint_as_float(o[i])) < INFINITY)) odd |= 1u << i;
+        odd = __reduce_or_sync(0xffffffffu, key < HD && n > 0 ? odd : 0u);
+        if (rows < 32) odd &= (1u << rows) - 1u;
+        if (odd)
+          flash_again<HD, 1, T>(a, it.tok0, it.pos0, it.kvh, it.kbase, it.kb0 * 128, keys, 0, odd >> lane & 1, it.part,
+                                warp * 32, lane);
       }
       __syncwarp();
       if (it.part >= 0) {

@@ -1,10 +1,13 @@
 """Calls at the edges of what the operators on device buffers accept.
 References and tolerances are those of test_gpu_ops.py."""
+import math
+import random
+
 import pytest
 import torch
 
-from test_gpu_ops import (BF16, F16, F32, Cache, guarded, half_step, i32, no_wait_gave_up, ops, rnd,  # noqa: F401
-                          rope_reference)
+from test_gpu_ops import (BF16, F16, F32, Cache, attention_reference, close, guarded, half_step, i32,  # noqa: F401
+                          no_wait_gave_up, offsets, ops, rnd, rope_reference)
 
 pytestmark = pytest.mark.gpu
 
@@ -183,3 +186,96 @@ def test_compaction_past_32_bits(ops):
         assert torch.equal(x[:, [3, 1, 0, 2]], w)
     h.compact(status)
     assert status.tolist() == [0, 0] and tables.tolist() == [[3, 1, 0, 2, -1]]
+
+
+# ------------------------------------- infinities and NaN that are not seen --
+def _poisoned(t, hk, hd, dt, seed, places):
+    """Values [t, hk, hd] with NaN and infinities at (token, head, element)."""
+    v = rnd(t, hk, hd, dt=dt, seed=seed)
+    for i, (tok, h, e) in enumerate(places):
+        v[tok, h, e] = (math.nan, math.inf, -math.inf)[i % 3]
+    return v
+
+
+def _seen(v, see):
+    """[m, hk, hd]: what a row gets where it sees a value that is not finite
+    (NaN, or an infinity of one sign); 0 where all that it sees is finite."""
+    see, v = see[:, :, None, None], v.double()[None]
+    nan = (see & v.isnan()).any(1)
+    up, down = (see & (v == math.inf)).any(1), (see & (v == -math.inf)).any(1)
+    r = torch.zeros_like(nan, dtype=torch.float64)
+    r[up], r[down], r[nan | (up & down)] = math.inf, -math.inf, math.nan
+    return r
+
+
+def _check_unseen(out, lse, q, k, v, see, scale):
+    """Rows are right wherever they see finite values only; where they see an
+    infinity or a NaN they are not finite, as the definition has it."""
+    bad = _seen(v, see).repeat_interleave(q.shape[1] // k.shape[1], 1)
+    o, z, tol, tol_z = attention_reference(q, k, v.nan_to_num(0, 0, 0), see, scale)
+    fine = bad == 0
+    assert bool(fine.any()) and not bool(fine.all())
+    close(out[fine], o[fine], tol[fine])
+    assert not bool(out[~fine].isfinite().any())
+    close(lse, z, tol_z)
+
+
+@pytest.mark.parametrize("dt", [BF16, F16])
+@pytest.mark.parametrize("hq,hk,hd", [(16, 8, 128), (4, 1, 64), (6, 2, 96), (14, 2, 128), (2, 2, 8), (128, 1, 64)])
+@pytest.mark.parametrize("lens", [[300], [90, 40, 257], [200] * 40])
+def test_prompt_values_that_are_not_seen(ops, dt, hq, hk, hd, lens):
+    r = random.Random(hq + len(lens))
+    cu = offsets(lens)
+    places = []
+    for a, b in zip(cu, cu[1:]):
+        places += [(r.randrange(a, b), r.randrange(hk), r.randrange(hd)) for _ in range(r.choice([1, 2]))]
+        places.append((b - 1, r.randrange(hk), r.randrange(hd)))
+    t = cu[-1]
+    q, k = rnd(t, hq, hd, dt=dt, seed=1), rnd(t, hk, hd, dt=dt, seed=2)
+    v = _poisoned(t, hk, hd, dt, 3, places)
+    out, intact = guarded(t, hq, hd, dt=dt)
+    lse, intact_l = guarded(t, hq, dt=F32)
+    ops.attn_prompt(q, k, v, i32(cu), out, lse=lse)
+    intact(), intact_l()
+    for a, b in list(zip(cu, cu[1:]))[:3]:
+        see = torch.ones(b - a, b - a, dtype=torch.bool, device="cuda").tril()
+        _check_unseen(out[a:b], lse[a:b], q[a:b], k[a:b], v[a:b], see, hd ** -0.5)
+
+
+@pytest.mark.parametrize("hq,hk,hd,page", [(8, 2, 128, 32), (4, 4, 64, 16), (6, 2, 96, 128), (3, 1, 40, 64)])
+@pytest.mark.parametrize("new,past", [([4], [700]), ([2, 3, 1], [40, 127, 0]), ([16, 5], [3000, 64]), ([200], [5000]),
+                                      ([300, 77], [0, 900]), ([60] * 30, [90] * 30), ([2] * 40, [900] * 40)])
+def test_cached_values_that_are_not_seen(ops, hq, hk, hd, page, new, past):
+    """Few rows, cut tiles and whole ones: a value among the new tokens reaches
+    only those behind it."""
+    r = random.Random(sum(new) + hq)
+    kv = [a + b for a, b in zip(new, past)]
+    c = Cache(ops, kv, page, hk, hd, BF16, seed=4, layers=2)
+    for s, (n, m) in enumerate(zip(new, kv)):
+        for i in range(2):
+            tok = m - 1 if i == 0 else r.randrange(m - n, m)
+            c.v[1, int(c.tables[s, tok // page]), tok % page, r.randrange(hk), r.randrange(hd)] = (math.nan, math.inf)[i]
+    cu = offsets(new)
+    q = rnd(cu[-1], hq, hd, dt=BF16, seed=5)
+    out, lse = c.attend(q, cu, layer=1)
+    for s in range(min(3, len(new))):
+        a, b = cu[s], cu[s + 1]
+        k, v = c.rows(s, 1)
+        pos = torch.arange(b - a, device="cuda")[:, None] + kv[s] - (b - a)
+        see = torch.arange(kv[s], device="cuda") <= pos
+        if b - a > 1:
+            _check_unseen(out[a:b], lse[a:b], q[a:b], k, v, see, hd ** -0.5)
+
+
+def test_all_values_nan(ops):
+    """Nothing to compute again that would be finite, and in no time that the
+    waits would notice."""
+    for hq, hk, t in ((8, 8, 6000), (4, 1, 3000)):
+        q, k = rnd(t, hq, 128, dt=BF16, seed=1), rnd(t, hk, 128, dt=BF16, seed=2)
+        v = torch.full((t, hk, 128), math.nan, device="cuda", dtype=BF16)
+        out = torch.zeros_like(q)
+        ops.attn_prompt(q, k, v, i32([0, t // 2, t]), out)
+        assert bool(out.isnan().all())
+        v[:, :, 1:] = 0
+        ops.attn_prompt(q, k, v, i32([0, t // 2, t]), out)
+        assert bool(out[..., 0].isnan().all()) and bool((out[..., 1:] == 0).all())
