@@ -33,7 +33,11 @@ int set_error(int code, const char* fmt, ...) {
   va_start(ap, fmt);
   vsnprintf(buf, sizeof(buf), fmt, ap);
   va_end(ap);
-  t_err = buf;
+  try {
+    t_err = buf;
+  } catch (const std::bad_alloc&) {  // the code says enough
+    t_err.clear();
+  }
   return code;
 }
 

@@ -580,12 +580,14 @@ extern "C" int ec_kv_open(void* k, void* v, int dtype, int layers, int pages, in
   if (work_bytes < ec_kv_work_size(pages, slots))
     return set_error(EC_EINVAL, "work holds %lld bytes, the cache needs %lld", static_cast<long long>(work_bytes),
                      static_cast<long long>(ec_kv_work_size(pages, slots)));
-  auto c = std::make_shared<KvOpen>(KvCache{k, v, dtype, layers, pages, page_size, heads, head_dim, tables, slots,
-                                            table_width, lens, refs, static_cast<int32_t*>(work)});
-  std::lock_guard<std::mutex> lk(g_kv_mu);
-  *handle = g_kv_next++;
-  g_kv[*handle] = std::move(c);
-  return EC_OK;
+  return guarded("kv open", [&] {
+    auto c = std::make_shared<KvOpen>(KvCache{k, v, dtype, layers, pages, page_size, heads, head_dim, tables, slots,
+                                              table_width, lens, refs, static_cast<int32_t*>(work)});
+    std::lock_guard<std::mutex> lk(g_kv_mu);
+    g_kv.emplace(g_kv_next, std::move(c));
+    *handle = g_kv_next++;
+    return EC_OK;
+  });
 }
 
 extern "C" int ec_kv_close(int handle) {

@@ -12,6 +12,7 @@
 #include <atomic>
 #include <initializer_list>
 #include <memory>
+#include <new>
 
 #include "ec_state.h"
 
@@ -32,6 +33,18 @@ class OpDevice {
  private:
   int prev_ = -1, dev_ = -1, sms_ = 0;
 };
+
+// No C++ exception leaves the C ABI: a host allocation that fails is EC_ENOMEM.
+template <class F>
+int guarded(const char* what, F&& f) {
+  try {
+    return f();
+  } catch (const std::bad_alloc&) {
+    return set_error(EC_ENOMEM, "%s: out of host memory", what);
+  } catch (const std::exception& e) {
+    return set_error(EC_EINVAL, "%s: %s", what, e.what());
+  }
+}
 
 // element size of EC_F32 / EC_BF16 / EC_F16, 0 for another code
 inline int op_elem_size(int dtype) {

@@ -154,9 +154,7 @@ static void prefix_forget(int slot) {
 
 using namespace ec;
 
-extern "C" int ec_prefix_open(const int32_t* ids, int n, int* prefix) {
-  std::lock_guard<std::mutex> lk(G().mu);
-  clear_error();
+static int prefix_open(const int32_t* ids, int n, int* prefix) {
   if (!G().inited) return set_error(EC_ESTATE, "ec_init first");
   if (!ids || !prefix) return set_error(EC_EINVAL, "ids and prefix must not be NULL");
   const ModelW& m = G().devs[0]->model;
@@ -189,6 +187,12 @@ extern "C" int ec_prefix_open(const int32_t* ids, int n, int* prefix) {
   return EC_OK;
 }
 
+extern "C" int ec_prefix_open(const int32_t* ids, int n, int* prefix) {
+  std::lock_guard<std::mutex> lk(G().mu);
+  clear_error();
+  return guarded("prefix", [&] { return prefix_open(ids, n, prefix); });
+}
+
 extern "C" int ec_prefix_close(int prefix) {
   std::lock_guard<std::mutex> lk(G().mu);
   clear_error();
@@ -206,5 +210,5 @@ extern "C" int ec_embed_batch_prefix(int prefix, const int32_t* ids, const int64
   if (!G().inited) return set_error(EC_ESTATE, "ec_init first");
   const int slot = prefix_slot(prefix);
   if (slot < 0) return EC_EINVAL;
-  return embed_batch_split(ids, offsets, nseq, out, out_stride, slot);
+  return guarded("batch", [&] { return embed_batch_split(ids, offsets, nseq, out, out_stride, slot); });
 }

@@ -70,3 +70,22 @@ def test_write_of_more_sequences_than_the_search_counts():
         refused(L().ec_kv_write(h, 0, 1 << 20, 256, 64, 1 << 20, 256, 64, 4, None, None, nseq, None), "count")
     refused(L().ec_kv_write(h, 0, 1 << 20, 256, 64, 1 << 20, 256, 64, 4, None, None, 1 << 30, None), "cu is NULL")
     assert L().ec_kv_close(h) == 0
+
+
+def test_handles_until_memory_is_out():
+    """A host allocation that fails is an error code; the process goes on."""
+    code = ("import sys, os, resource, ctypes as C; sys.path[:0] = [%r, os.path.join(%r, 'lisp-embed_b200'), %r];"
+            "from test_ops import L, FAKE; from embedcuda import _lib\n"
+            "l, h = L(), C.c_int()\n"
+            "size = l.ec_kv_work_size(10, 3)\n"
+            "used = int(open('/proc/self/statm').read().split()[0]) * os.sysconf('SC_PAGE_SIZE')\n"
+            "resource.setrlimit(resource.RLIMIT_AS, (used + (20 << 20), resource.RLIM_INFINITY))\n"
+            "rc, n, ref = 0, 0, C.byref(h)\n"
+            "while rc == 0 and n < 4000000:\n"
+            "    rc = l.ec_kv_open(FAKE, FAKE, 1, 2, 10, 16, 4, 64, FAKE, 3, 5, FAKE, FAKE, FAKE, size, ref); n += 1\n"
+            "resource.setrlimit(resource.RLIMIT_AS, (resource.RLIM_INFINITY, resource.RLIM_INFINITY))\n"
+            "assert l.ec_kv_close(h) == 0\n"
+            "print(rc, n > 1000, flush=True)\n") % (REPO, REPO, os.path.join(REPO, "tests"))
+    out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=600)
+    assert out.returncode == 0, (out.returncode, out.stderr[-500:])
+    assert out.stdout.split() == [str(_lib.EC_ENOMEM), "True"]
