@@ -311,8 +311,8 @@ __global__ void kv_fork_copy_kernel(const KvCache c, const int32_t* src, const i
   pdl_trigger();
   const Plan plan(c);
   const int i = blockIdx.x;
-  if (plan.scalars[0] == 0) return;  // refused: there are no copies to read
-  const int4 copy = plan.copies[i];
+  const int4 copy = plan.copies[i];  // there is one for every slot, and no more blocks than that
+  if (plan.scalars[0] == 0) return;
   if (blockIdx.y == 0) {
     const int full = copy.w / c.page_size;
     const int32_t* from = c.tables + static_cast<int64_t>(src[i]) * c.width;
@@ -622,7 +622,7 @@ extern "C" int ec_kv_fork(int handle, const int32_t* src, const int32_t* dst, in
   if (int rc = check_cuda(launch_pdl(kv_fork_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, *c, src, dst, n, status),
                           "kv fork"))
     return rc;
-  if (n == 0 || n > c->slots) return EC_OK;  // (the plan refuses the latter)
+  if (n == 0 || n > c->slots) return EC_OK;  // the plan refuses the latter; its scratch has `slots` copies
   return check_cuda(launch_pdl(kv_fork_copy_kernel, dim3(n, std::min(2 * c->layers, 65535)), dim3(256), 0, st, *c, src,
                                dst),
                     "kv fork copy");
