@@ -44,10 +44,10 @@ using FlashFn = void (*)(CUtensorMap, CUtensorMap, CUtensorMap, FlashArgs);
 // Lists of pairs of tiles by sequence are launched plainly.  A CTA that starts
 // early, while the kernel before still runs, gets the SM that came free first;
 // then CTAs that read the same keys no longer run side by side.  One call after
-// the other, 256 prompts of 320 tokens took 306 us instead of 252, 1024 of 130
-// 610 instead of 550, 96 texts behind 650 cached tokens 141 instead of 134.
-// The other launches gain by it (one token 14.4 -> 11.7 us, 8 prompts of 512
-// 27.1 -> 25.5, one of 4096 75.6 -> 73.0).
+// the other on the same buffers, 256 prompts of 320 tokens take 255 us (with early
+// starts 1.2), 1024 of 130 553 (1.11), 96 texts behind 650 cached tokens 133
+// (1.05).  The other launches gain by it (one token 11.3 us, without it 1.2; 8
+// prompts of 512 24 us, 1.06; one of 4096 72 us, 1.04).
 class PlainLaunch {
  public:
   explicit PlainLaunch(bool plain) : before_(pdl_enabled()), plain_(plain) {
@@ -123,12 +123,21 @@ struct FlashPlan {
 };
 // Few rows (a sequence's new tokens and their heads in at most 32 rows): the
 // kernels with the operands turned round, in the smallest size that holds them;
-// always an even split (64 sequences of up to 8192 tokens: 118 us with tiles of
-// 128 rows, 106 with keys per lane, 96 in the size that fits).  More rows in
-// fewer tiles than SMs: an even split, which leaves whole what is not worth
-// cutting.  Else whole tiles, in pairs where every SM has a pair (one prompt of
-// 16384 tokens 473 us, single tiles 573); one tile at a time is better for
-// fewer, and where no sequence fills more than a tile.
+// always an even split (64 sequences of up to 8192 tokens 94 us; in 32 rows
+// whatever they need 1.1, in tiles of 128 rows 1.23).  More rows in fewer tiles
+// than SMs: an even split, which leaves whole what is not worth cutting.  Else
+// whole tiles, in pairs where every SM has a pair (one prompt of 16384 tokens 477
+// us, in single tiles 1.2); one tile at a time is better for fewer, and where no
+// sequence fills more than a tile.
+//
+// The kind goes by the call's longest sequence and their count.  One call after
+// the other, 64 single tokens behind up to 8192 keys take 108 us, with a text of 9 tokens or more among them 160 to
+// 170 (its rows pass 32: tiles of 128 rows for all), of 8 tokens 236 (32 rows for
+// all); 2048 single tokens behind 500 keys 664, 2049 837 (more than the even
+// split's prefix sums hold).  Heads other than 64 and 128 run padded to those, in
+// MMAs and shared memory (the bytes from memory are their own): 256 prompts of
+// 128 to 512 tokens take 217, 217 and 219 us with heads of 16, 32 and 64, 242
+// with 80 and 96, 246 with 128.
 FlashPlan flash_plan(const KvCache* c, int64_t tokens, int q_heads, int kv_heads, int nseq, int max_new, int num_sms) {
   const int group = q_heads / kv_heads;
   FlashPlan p{kTiles, 0, 128 / group, 128};

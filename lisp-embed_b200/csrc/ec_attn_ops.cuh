@@ -26,17 +26,26 @@
 // work list.  NT = 2 has four more that divide O by the row sums and write it,
 // and the MMA warp issues a tile's first scores of the next tile set as soon as
 // the tile is through: a softmax warp has nothing to wait for between two sets
-// (256 prompts of 320 tokens: 305 -> 276 us; a trace had shown 35% of the
-// softmax warps' time between their last exponentials and the next scores).
-// All waits are bounded.
+// (a trace had shown 35% of its time between its last exponentials and the next
+// scores).  All waits are bounded.
 //
-// What bounds it: the exponentials.  16384 tokens of 8 heads of 128 take 473
-// us; the MMAs alone 344 (the peak rate 328), the softmax warps alone 426.  A
-// block costs a warp 128 exponentials (three of four on the special-function
-// unit, 16 a cycle and SM, every fourth on the FMA units: all on the former 522
-// us, every third on the FMA units 490), the scale, sum and packing two values
-// an instruction, the maximum three, and two reads of the scores from TMEM,
-// which keep a thread within 168 registers.
+// Times here are of one pass by itself with cold caches (a graph replayed after a
+// write larger than L2) where nothing else is said.  "The corpus" is 256 prompts
+// of 128 to 512 tokens (71060 in all) of 16 query and 8 key heads of 128; what an
+// alternative cost is said as a factor of the time without it.
+//
+// What bounds it: the chain of a block.  16384 tokens of 8 heads of 128 take 477
+// us; the MMAs alone took 344 (the peak rate 328), the softmax warps alone 426,
+// and no unit is full then (tensor pipe 53%, special functions 40%, issue 42%).
+// A block costs a warp 128 exponentials (three of four on the special-function
+// unit, 16 a cycle and SM, every fourth on the FMA units; all on the former
+// 1.10, every third on the FMA units 1.04), the scale, sum and packing two
+// values an instruction, the maximum three, two reads of the scores from TMEM,
+// which keep a thread within 168 registers, and the rescaling of O.  In short
+// tile sets (the corpus 252 us, 134 for its bytes) each set's start counts: its
+// queries have one buffer and are asked for within the key stream, once the last
+// scores of the set before are done; and a set of one tile runs its scores,
+// exponentials and P V one after the other.
 #pragma once
 
 #include <cuda_fp16.h>
@@ -139,8 +148,9 @@ __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
 }
 
 // 2^x for two values on the FMA units: x = n + f with n the nearest integer,
-// 2^f by a minimax polynomial of degree 5 on [-1/2, 1/2] (Remez; 7.5e-8 from
-// the truth, 2.4e-7 with the roundings of its evaluation), 2^n put together as
+// 2^f by a minimax polynomial of degree 5 on [-1/2, 1/2] (Remez; with its
+// coefficients rounded to fp32 1.6e-7 from the truth, 2.4e-7 with the roundings
+// of its evaluation, both relative), 2^n put together as
 // an exponent.  x <= -127 gives 0; NaN stays NaN.  For x < 128.
 __device__ __forceinline__ float2 exp2_fma(float2 x) {
   const float2 magic = make_float2(12582912.f + 127.f, 12582912.f + 127.f);  // 1.5 * 2^23: n + 127 in the low bits
@@ -206,25 +216,25 @@ __device__ __forceinline__ FlashSeq flash_seq(const FlashArgs& a, int s) {
 // each the key heads.  flash_count leaves the number of sets of every group of
 // sequences; a set's group is found by bisection, its sequence from there, 32
 // sets at a time.  The key heads of a set and the sets of a sequence follow
-// each other, so that the CTAs read the same keys at about the same time: with
-// a run of the list for every CTA, of equal work, 256 prompts of 320 tokens took
-// 383 us instead of 272.  With more sequences than are counted, slot u is set i
+// each other, so that the CTAs read the same keys at about the same time (a run
+// of the list for every CTA, of equal work: the corpus 1.41).  With more
+// sequences than are counted, slot u is set i
 // of sequence s for f(s) + i = u, f(s) = cu[s] / BT + s (BT tokens per set): f
 // leaves at least ceil(len / BT) slots to every sequence and needs no sums, but
-// its empty slots make the turns uneven (96 texts behind 650 cached tokens
-// 160 us instead of 141, 64 prompts of 300 147 instead of 127).  Slots times
-// key heads fit 31 bits, checked on the host.
+// its empty slots make the turns uneven (96 texts behind 650 cached tokens 1.13,
+// 64 prompts of 300 1.16).  Slots times key heads fit 31 bits, checked on the
+// host.
 //
 // Up to 32 sequences go by set, the latest sets of all of them first (slot u:
 // set u / nseq of sequence u % nseq), so that a CTA's few turns cost the same:
-// 4 prompts of 2048 tokens 84 us instead of 135.  With more sequences that
-// costs the keys' reuse: 96 texts behind 650 cached tokens took 182 us.
+// 4 prompts of 2048 tokens 86 us (by sequence 1.6).  With more sequences that
+// costs the keys' reuse: 96 texts behind 650 cached tokens 1.29.
 //
 // Sums over the sequences are bounded by the tokens of the call as long as the
 // offsets ascend.  flash_count and flash_measure mark where they do not; then
 // the list stays empty (the sums could pass 32 bits, and what is laid out by
 // them the buffers).  The mark lies in shared memory: in a register it cost the
-// pairs' kernels spills (256 prompts, 71060 tokens: 281 -> 294 us).
+// pairs' kernels spills (the corpus 1.05).
 template <int NT>
 __device__ __forceinline__ void flash_count(const FlashArgs& a, int* groups, volatile int* descend) {
   const int size = (a.nseq + kFlashGroups - 1) / kFlashGroups, BT = NT * a.rows_tok;
@@ -330,8 +340,9 @@ constexpr int kLongestMost = 0x7fff;
 // more, for its start and end, which come first.  Where there are fewer tiles
 // than CTAs and the longest would not gain what a join costs (8 units, 20 with
 // 128 rows: 25 us), every tile has a CTA of its own instead: 4 texts of 200
-// tokens behind 4000 61 us, cut 84; 4 of 40 behind 2000 35 and 45; one of 40
-// behind 20000 203 and 94; 8 of 64 behind 8000 98 and 96.
+// tokens behind 4000 59 us (cut 1.4), 4 of 40 behind 2000 35 (cut 1.3); cut are
+// one of 40 behind 20000, 98 us (whole 2.1), and 8 of 64 behind 8000, 96 us
+// (whole 1.02).
 //
 // Each thread of the CTA first looks at some sequences (the loads are far
 // away, and the CTA has nothing else to do yet): units[s] (-1: its offsets
@@ -464,7 +475,7 @@ __device__ __noinline__ bool flash_even(const FlashArgs& a, int lane, int* prefi
 // the keys.  A warp has a quarter of the rows: their weights first, a row to a
 // lane, then the rows themselves, eight at a time, so that many loads are under
 // way (a row after the other, each waiting for its loads: 4 texts of 200 tokens
-// behind 4000, two parts to a tile, 121 us instead of 84).
+// behind 4000, two parts to a tile, 1.44).
 template <int HD, typename T>
 __device__ __noinline__ void flash_join(const FlashArgs& a, int tok0, int qv, int kvh, int c0, int parts, int warp,
                                         int lane) {
@@ -653,8 +664,7 @@ __device__ __noinline__ void flash_again(const FlashArgs& a, int tok0, int pos, 
 // it says that one of them is not finite, the list's warp goes through the list
 // again and looks at them.  (The closures that go into functions out of line hold
 // copies: kernel variables that they held by reference lay in local memory for
-// all warps, 256 prompts of 71060 tokens 316 us instead of 280, one token of one
-// sequence 11.7 instead of 11.3.)
+// all warps: the corpus 1.13, one token of one sequence 1.04.)
 template <int HD, typename T, typename Publish, typename Finish>
 __device__ __forceinline__ bool flash_pairs(const FlashArgs& a, int lane, int* groups, int* sets, bool empty,
                                             const Publish& publish, Finish finish) {
@@ -696,7 +706,7 @@ __device__ __forceinline__ bool flash_arrive(const FlashArgs& a, const FlashEntr
 
 // The end of the results (NT 2): the four warps that write them arrive, whether a
 // wait of theirs gave up or not, and the list's warp waits (in hardware: a warp
-// that polls takes turns from the softmax warps, 16384 tokens 534 -> 546 us).
+// that polls takes turns from the softmax warps, 16384 tokens 1.01).
 __device__ __forceinline__ void results_done(bool wait) {
   __syncwarp();
   if (wait) asm volatile("barrier.cta.sync 1, 160;" ::: "memory");
@@ -817,9 +827,9 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
   // Keys that the last query of tile t sees, from the block `at` on.  HALF: in
   // a block where that is 64 or less, the other half takes no part in anything.
   // It pays with short sequences, whose last blocks are many (1024 prompts of
-  // 130 tokens 590 -> 545 us, 256 of 320 279 -> 273); elsewhere the loops of one
-  // or two halves slow the others down (one of 16384 481 -> 496, of 4096 82 ->
-  // 86, 32 of 1024 190 -> 188).
+  // 130 tokens 559 us, without it 1.08; 256 of 320 262 us, 1.02); elsewhere the
+  // loops of one or two halves slow the others down (one of 16384 with it 1.03,
+  // of 4096 1.05, 32 of 1024 0.99).
   auto tile_sees = [&](const FlashEntry& it, int t, int at) {
     return HALF ? min(it.kv_len, it.pos0 + min((t + 1) * R, it.qv)) - at * 128 : 128;
   };
@@ -1425,11 +1435,11 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
 // row maxima through shared memory.  One warp runs per scheduler, so a block
 // takes as long as its instructions do, one after the other: NP = 4, 8, 16 and
 // 32 rows each have their own kernel (the MMA's N is 16 at least; what the
-// columns behind NP hold reaches nothing).  Three contexts of 100000 to 131000
-// tokens take 230 us, at 98% of the copy rate; 64 sequences of up to 8192
-// tokens, grouped by four, 76 us at 77% (118 with tiles of 128 rows): there the
-// starts and joins of about two tiles a CTA count; one token of one sequence 12
-// us, most of them between launch and first key.
+// columns behind NP hold reaches nothing).  One call after the other, three
+// contexts of 100000 to 131000 tokens take 223 us, at the copy rate; 64 sequences
+// of up to 8192 tokens, grouped by four, 74 us at 79% of it (tiles of 128 rows
+// 1.5): there the starts and joins of about two tiles a CTA count; one token of
+// one sequence 11 us, most of them between launch and first key.
 template <int HD, int NP>
 struct TokenCfg {
   static constexpr int NR = NP < 16 ? 16 : NP;         // columns of the MMAs

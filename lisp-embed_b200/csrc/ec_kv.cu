@@ -14,11 +14,13 @@
 // says which, and every index read from the device is checked before use.
 //
 // What bounds them: the plans are chains of loads that wait for one another
-// (lengths, counts, lists, tables: about 1 us each out of L2), 5 to 8 us a
-// plan, so a plan reads ahead what it will need and gives a request to a warp;
-// fork, reserve and write for 96 texts (8 layers copied) take 40 us together,
-// 12 of them for the bytes.  The copies run near the memory's rate: 4096 pages
-// compacted in 51 us, 36 for the bytes.
+// (lengths, counts, lists, tables: about 1 us each out of L2), 7 to 11 us a
+// plan, so a plan reads ahead what it will need and gives a request to a warp.
+// Reserve and fork pass over their lists more than once (claims, checks, sums,
+// hand-out) and read lists and lengths again each time, which makes part of that
+// chain.  Free, fork, reserve and write for 96 texts (8 layers copied) take 41 us
+// together, 12 of them for the bytes.  The copies run near the memory's rate:
+// 4096 pages compacted in 51 us, 36 for the bytes.
 #include <algorithm>
 #include <map>
 #include <mutex>
