@@ -273,7 +273,8 @@ int ec_rope(const void *x, int64_t x_token, int64_t x_head, void *y, int64_t y_t
  * 1 / sqrt(head_dim).  lse (NULL or [tokens][q_heads]) receives the natural
  * log of the softmax's denominator.  Sums and statistics are fp32,
  * probabilities are rounded to the inputs' type for the product with v.  A
- * NaN or infinity in a key or value reaches the tokens that see it, no others. */
+ * NaN or infinity in a key or value reaches the tokens that see it, no others.
+ * out and lse overlap none of the inputs. */
 int ec_attn_prompt(const void *q, int64_t q_token, int64_t q_head, const void *k,
                    int64_t k_token, int64_t k_head, const void *v, int64_t v_token,
                    int64_t v_head, void *out, int64_t o_token, int64_t o_head, float *lse,

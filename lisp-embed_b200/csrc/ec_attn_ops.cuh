@@ -218,12 +218,11 @@ __device__ __forceinline__ FlashSeq flash_seq(const FlashArgs& a, int s) {
 // sets at a time.  The key heads of a set and the sets of a sequence follow
 // each other, so that the CTAs read the same keys at about the same time (a run
 // of the list for every CTA, of equal work: the corpus 1.41).  With more
-// sequences than are counted, slot u is set i
-// of sequence s for f(s) + i = u, f(s) = cu[s] / BT + s (BT tokens per set): f
-// leaves at least ceil(len / BT) slots to every sequence and needs no sums, but
-// its empty slots make the turns uneven (96 texts behind 650 cached tokens 1.13,
-// 64 prompts of 300 1.16).  Slots times key heads fit 31 bits, checked on the
-// host.
+// sequences than are counted, slot u is set i of sequence s for f(s) + i = u,
+// f(s) = cu[s] / BT + s (BT tokens per set): f leaves at least ceil(len / BT)
+// slots to every sequence and needs no sums, but its empty slots make the turns
+// uneven (96 texts behind 650 cached tokens 1.13, 64 prompts of 300 1.16).  Slots
+// times key heads fit 31 bits, checked on the host.
 //
 // Up to 32 sequences go by set, the latest sets of all of them first (slot u:
 // set u / nseq of sequence u % nseq), so that a CTA's few turns cost the same:
@@ -247,7 +246,8 @@ __device__ __forceinline__ void flash_count(const FlashArgs& a, int* groups, vol
 }
 // (`summed`: the groups' sums are there already, their total in *sets)
 template <int NT, typename Publish>
-__device__ __noinline__ bool flash_slots(const FlashArgs& a, int lane, int* groups, int* sets, bool summed, const Publish& publish) {
+__device__ __noinline__ bool flash_slots(const FlashArgs& a, int lane, int* groups, int* sets, bool summed,
+                                         const Publish& publish) {
   const int R = a.rows_tok, BT = NT * R;
   uint32_t slots = a.tokens / BT + a.nseq;
   const uint32_t step = gridDim.x;
@@ -558,7 +558,9 @@ __device__ __forceinline__ const T* flash_key(const FlashArgs& a, int kv, int kb
 __device__ __forceinline__ float2 unpack2(__nv_bfloat16, uint32_t v) {
   return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
 }
-__device__ __forceinline__ float2 unpack2(__half, uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
+__device__ __forceinline__ float2 unpack2(__half, uint32_t v) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&v));
+}
 
 // Row of token `tok` and query head `head` over the keys [first, vis): elements
 // d0 + 32 e + lane, e < E, divided by the sum, to out (this lane's addresses
@@ -640,8 +642,8 @@ __device__ __forceinline__ int flash_last_odd(const FlashArgs& a, int kbase, int
 
 // Rows base .. base + 31 of a tile of rows (token, head) whose first token is
 // tok0, at position pos: those of the lanes with `odd` are looked at, by the
-// whole warp.  Keys [first, end) of the slot or sequence; row: of the tile's
-// part, -1: whole.  Elements from d0 on, 32 E of them.
+// whole warp.  Keys [first, end) of the slot or sequence; part: of a cut tile,
+// -1: whole.  Elements from d0 on, 32 E of them.
 template <int HD, int E, typename T>
 __device__ __noinline__ void flash_again(const FlashArgs& a, int tok0, int pos, int kvh, int kbase, int first, int end,
                                          int base, bool odd, int part, int d0, int lane) {
@@ -935,7 +937,8 @@ __global__ void __launch_bounds__(FlashCfg<HD, NT>::THREADS, 1)
         return fine && *odd_rows && !*abort_flag;
       });
     } else {
-      if (a.even) ok = flash_even(a, lane, prefix, prefix + Cfg::MAX_SEQS, [=](const Entry& e) { return publish(e, 0); });
+      if (a.even)
+        ok = flash_even(a, lane, prefix, prefix + Cfg::MAX_SEQS, [=](const Entry& e) { return publish(e, 0); });
       else if (!*descend) ok = flash_slots<NT>(a, lane, groups, sets, false, publish);
       if (ok) ok = publish(Entry{}, 0);
     }
